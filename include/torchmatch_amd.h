@@ -332,6 +332,80 @@ int tm_sinkhorn_form_f64(const double *cost, const double *a, const double *b, i
                          double *log_v, void *workspace, size_t workspace_bytes,
                          hipStream_t stream);
 
+/* ---- attention and rotation ---------------------------------------------
+ * What produces the scores the solvers above work on: attention within and
+ * between point sets, and the rotation of feature pairs by positions.  The
+ * reference has no counterpart.  Nothing here reads anything back, so every
+ * call may be captured into a graph. */
+
+/* Element types of features, and of positions. */
+enum { TM_BF16 = 0, TM_F16 = 1, TM_F32 = 2 };
+enum { TM_POS_F32 = 0, TM_POS_I32 = 1, TM_POS_I64 = 2 };
+
+/* One attention problem.  q is (B, Lq, H, D), k and v are (B, Lk, Hkv, D), Hkv
+ * dividing H: query head h reads key head h / (H / Hkv).  They may be strided
+ * (strides in elements, D contiguous); addresses and strides must be multiples
+ * of 16 bytes and so must D (TM_ERR_INVALID_ARGUMENT, TM_ERR_UNSUPPORTED_SHAPE),
+ * D at most tm_attention_max_head_dim().
+ *
+ *   s_ij = scale * q_i . k_j
+ *   s_ij = cap * tanh(s_ij / cap)                       where cap > 0
+ *   s_ij = s_ij - slopes[h] * |q_positions_i - k_positions_j|   (sum over axes)
+ *   out_i = sum_j softmax_j(s_ij) v_j  over the j that query i sees
+ *
+ * Without positions the distance is that of indices, query i standing at
+ * i + length - Lq.  Query i of batch row b sees key j where
+ *   j < lengths[b] (Lk without lengths), and
+ *   if causal: j <= i + length - Lq, or j < prefix[b], and
+ *   with documents: q_docs_i == k_docs_j >= 0.
+ * A query that sees nothing gets zeros, lse = -inf and no gradient.  Keys past
+ * every limit and rows of negative documents may hold anything, NaN included. */
+typedef struct tm_attention {
+    const void *q, *k, *v;
+    int64_t q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h;
+    const float *slopes;                    /* (H) or NULL: no bias */
+    const float *q_positions, *k_positions; /* (B, L, axes) or NULL; need slopes */
+    const int32_t *q_docs, *k_docs;         /* (B, L) or NULL */
+    const int32_t *prefix, *lengths;        /* (B) or NULL */
+    int32_t dtype, B, Lq, Lk, H, Hkv, D, axes, causal;
+    float scale, cap;
+} tm_attention;
+
+int32_t tm_attention_max_head_dim(void);
+
+/* out: (B, Lq, H, D) contiguous, the inputs' type; lse: (B, H, Lq) float32, the
+ * natural logarithm of each row's sum, or NULL.  workspace: device, at least
+ * tm_attention_workspace_bytes(a), 16-byte aligned, any contents. */
+size_t tm_attention_workspace_bytes(const tm_attention *a);
+int tm_attention_forward(const tm_attention *a, void *out, float *lse, void *workspace,
+                         size_t workspace_bytes, hipStream_t stream);
+
+/* Gradients of q, k and v (contiguous, the inputs' type) from out and lse of the
+ * forward call and the output's gradient, (B, Lq, H, D) with its own strides.
+ * The same call gives the same bits: nothing is added by atomics. */
+size_t tm_attention_backward_workspace_bytes(const tm_attention *a);
+int tm_attention_backward(const tm_attention *a, const void *out, const float *lse,
+                          const void *dout, int64_t do_b, int64_t do_l, int64_t do_h, void *dq,
+                          void *dk, void *dv, void *workspace, size_t workspace_bytes,
+                          hipStream_t stream);
+
+/* Rotation of feature pairs.  x is (B, L, H, D) of `dtype` with strides in
+ * elements (D contiguous); out is (B, L, H, D), contiguous.  positions are
+ * (B, L, axes) of `pos_type`, batch rows pos_b elements apart (0: shared).
+ * sections[a] pairs turn by axis a: pair p of a token by the angle
+ * positions[axis(p)] * freqs[p] (the opposite angle with `inverse`, which is the
+ * gradient).  Pair p is features p and P + p, or 2p and 2p + 1 where
+ * interleaved, P the number of pairs; the features past 2 P are copied. */
+enum { TM_ROTATE_MAX_AXES = 4 };
+typedef struct tm_rotation {
+    const void *x, *positions;
+    const float *freqs; /* (P) */
+    int64_t x_b, x_l, x_h, pos_b;
+    int32_t dtype, pos_type, B, L, H, D, axes, interleaved, inverse;
+    int32_t sections[4];
+} tm_rotation;
+int tm_rotate(const tm_rotation *r, void *out, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

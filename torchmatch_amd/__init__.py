@@ -10,6 +10,8 @@ and schemas:
 
 ``torchmatch_amd.assignment.solve`` and ``torchmatch_amd.transport.matrix.solve``
 mirror ``torchmatch.assignment.solve`` and ``torchmatch.transport.matrix.solve``.
+``torchmatch_amd.attention`` adds what matching networks compute their scores with:
+attention with capped and biased scores and masks, and rotation by positions.
 The C ABI underneath is declared in ``include/torchmatch_amd.h``.
 """
 
@@ -19,6 +21,6 @@ from torchmatch_amd._loader import ExtensionMissingError, load
 
 load()
 
-from torchmatch_amd import assignment, transport  # noqa: E402
+from torchmatch_amd import assignment, attention, transport  # noqa: E402
 
-__all__ = ["ExtensionMissingError", "assignment", "load", "transport"]
+__all__ = ["ExtensionMissingError", "assignment", "attention", "load", "transport"]

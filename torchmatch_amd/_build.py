@@ -4,7 +4,7 @@ Produces, next to this file:
 
 * ``lib/libtorchmatch_amd.so`` -- the C-ABI library (``include/torchmatch_amd.h``):
   the HIP kernels in ``csrc/*.hip``, compiled by ``hipcc --offload-arch=gfx950``;
-* ``_C.so`` -- torch dispatcher registrations (``csrc/torch_ops.cpp``) linked
+* ``_C.so`` -- torch dispatcher registrations (``csrc/torch_*.cpp``) linked
   against the C-ABI library; loaded with ``torch.ops.load_library``;
 * ``bench_probes.so`` at the repository root -- the microbenchmarks
   ``bench.py`` prices the JV kernels against (``bench_probes.hip``: LDS read
@@ -36,7 +36,10 @@ PROBE_SO = PKG.parent / "bench_probes.so"
 
 HIP_SOURCES = ["jv_batch.hip", "jv_large.hip", "jv_unpack.hip", "sinkhorn.hip", "sinkhorn64.hip",
                "sinkhorn_resident.hip", "sk_tiles_narrow.hip", "sk_tiles_wide.hip",
-               "sk_tiles_f64.hip"]
+               "sk_tiles_f64.hip", "attention.hip", "attn_forward_bf16.hip",
+               "attn_forward_f16.hip", "attn_forward_f32.hip", "attn_backward_bf16.hip",
+               "attn_backward_f16.hip", "attn_backward_f32.hip", "rotate.hip"]
+OPS_SOURCES = ["torch_ops.cpp", "torch_attention.cpp"]
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = "gfx950"
 
@@ -75,7 +78,7 @@ def build_cabi(verbose: bool = True) -> Path:
              verbose)
         return str(obj)
 
-    with ThreadPoolExecutor(max_workers=4) as pool:
+    with ThreadPoolExecutor(max_workers=8) as pool:
         objs = list(pool.map(compile_one, HIP_SOURCES))
     tmp = CABI_SO.with_suffix(".so.tmp")
     _run(["hipcc", f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *objs,
@@ -110,7 +113,7 @@ def build_ops(verbose: bool = True) -> Path:
         *[f"-I{p}" for p in includes],
         f"-I{INCLUDE}",
         f"-I{sysconfig.get_paths()['include']}",
-        str(CSRC / "torch_ops.cpp"),
+        *[str(CSRC / src) for src in OPS_SOURCES],
         "-o", str(OPS_SO.with_suffix(".so.tmp")),
         *[f"-L{p}" for p in libdirs],
         f"-L{LIB_DIR}",

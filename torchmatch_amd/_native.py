@@ -29,6 +29,37 @@ TM_JV_FLAG_ANY_FINITE = 8
 TM_JV_FLAG_NEG_ZERO = 16
 TM_JV_FLAG_DONE = 0x80000000
 
+TM_BF16, TM_F16, TM_F32 = 0, 1, 2
+TM_POS_F32, TM_POS_I32, TM_POS_I64 = 0, 1, 2
+
+
+class Attention(ctypes.Structure):
+    """``tm_attention``: one attention problem (device pointers, strides in elements)."""
+
+    _fields_ = [
+        *((n, ctypes.c_void_p) for n in ("q", "k", "v")),
+        *((n, ctypes.c_int64) for n in ("q_b", "q_l", "q_h", "k_b", "k_l", "k_h", "v_b", "v_l",
+                                        "v_h")),
+        *((n, ctypes.c_void_p) for n in ("slopes", "q_positions", "k_positions", "q_docs",
+                                         "k_docs", "prefix", "lengths")),
+        *((n, ctypes.c_int32) for n in ("dtype", "B", "Lq", "Lk", "H", "Hkv", "D", "axes",
+                                        "causal")),
+        ("scale", ctypes.c_float), ("cap", ctypes.c_float),
+    ]
+
+
+class Rotation(ctypes.Structure):
+    """``tm_rotation``: feature pairs to turn by positions."""
+
+    _fields_ = [
+        *((n, ctypes.c_void_p) for n in ("x", "positions", "freqs")),
+        *((n, ctypes.c_int64) for n in ("x_b", "x_l", "x_h", "pos_b")),
+        *((n, ctypes.c_int32) for n in ("dtype", "pos_type", "B", "L", "H", "D", "axes",
+                                        "interleaved", "inverse")),
+        ("sections", ctypes.c_int32 * 4),
+    ]
+
+
 # symbol -> (restype, argtypes); the declarations of include/torchmatch_amd.h
 _VP = ctypes.c_void_p
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -141,6 +172,20 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _VP, _VP, _VP, _VP, ctypes.c_size_t, _VP,
         ],
     ),
+    "tm_attention_max_head_dim": (ctypes.c_int32, []),
+    "tm_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Attention)]),
+    "tm_attention_forward": (
+        ctypes.c_int, [ctypes.POINTER(Attention), _VP, _VP, _VP, ctypes.c_size_t, _VP]
+    ),
+    "tm_attention_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Attention)]),
+    "tm_attention_backward": (
+        ctypes.c_int,
+        [
+            ctypes.POINTER(Attention), _VP, _VP, _VP, ctypes.c_int64, ctypes.c_int64,
+            ctypes.c_int64, _VP, _VP, _VP, _VP, ctypes.c_size_t, _VP,
+        ],
+    ),
+    "tm_rotate": (ctypes.c_int, [ctypes.POINTER(Rotation), _VP, _VP]),
 }
 
 

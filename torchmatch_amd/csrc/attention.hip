@@ -1,0 +1,223 @@
+// attention.hip -- the C entries of the attention operators: checks, workspace, launches.
+#include <algorithm>
+
+#include "../../include/torchmatch_amd.h"
+#include "attn.h"
+
+namespace {
+
+using attn::Args;
+
+// Summaries of the documents of 64 rows each: the smallest and the largest id that is not
+// negative (INT_MAX, -1 without one), and whether one is negative.  A wave for each.
+__global__ __launch_bounds__(256) void attend_docs(const int32_t *q_docs, const int32_t *k_docs,
+                                                   int B, int Lq, int Lk, int4 *q_tiles,
+                                                   int4 *k_tiles) {
+    const int64_t nq = (Lq + 63) / 64, nk = (Lk + 63) / 64;
+    int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (t >= B * (nq + nk))
+        return;
+    const bool keys = t >= B * nq;
+    if (keys)
+        t -= B * nq;
+    const int64_t n = keys ? nk : nq, len = keys ? Lk : Lq;
+    const int64_t b = t / n, i = t % n * 64 + lane;
+    const int id = i < len ? (keys ? k_docs : q_docs)[b * len + i] : -1;
+    int lo = id < 0 ? 0x7fffffff : id, hi = id < 0 ? -1 : id;
+    const bool hidden = __any(i < len && id < 0);
+#pragma unroll
+    for (int x = 32; x; x >>= 1) {
+        lo = min(lo, __shfl_xor(lo, x));
+        hi = max(hi, __shfl_xor(hi, x));
+    }
+    if (!lane)
+        (keys ? k_tiles : q_tiles)[t] = make_int4(lo, hi, hidden, 0);
+}
+
+int padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : 256; }
+
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+size_t docs_bytes(const tm_attention *a) {
+    if (!a->q_docs)
+        return 0;
+    const size_t tiles = (size_t)a->B * ((a->Lq + 63) / 64 + (a->Lk + 63) / 64);
+    return align256(tiles * sizeof(int4));
+}
+
+// Keys are split over blocks when there are too few rows to fill the chip with whole ones.
+// At least four tiles of 64 keys a split, so that its start and the join are worth it.
+struct Splits {
+    int n, tiles;
+};
+Splits splits_of(const tm_attention *a) {
+    const int64_t blocks = (int64_t)((a->Lq + 127) / 128) * a->H * a->B;
+    const int tiles = (a->Lk + 63) / 64;
+    if (blocks >= 256 || tiles < 8)
+        return {1, std::max(tiles, 1)};
+    const int want = (int)std::min<int64_t>((512 + blocks - 1) / blocks, tiles / 4);
+    const int per = (tiles + want - 1) / want;
+    return {(tiles + per - 1) / per, per};
+}
+
+// What every call must hold; sizes of zero are the callers' to answer.
+int check(const tm_attention *a) {
+    if (!a || a->B < 0 || a->Lq < 0 || a->Lk < 0 || a->H < 1 || a->Hkv < 1 || a->H % a->Hkv ||
+        a->D < 1)
+        return TM_ERR_INVALID_ARGUMENT;
+    if (a->dtype < TM_BF16 || a->dtype > TM_F32)
+        return TM_ERR_INVALID_ARGUMENT;
+    const int unit = a->dtype == TM_F32 ? 4 : 8;
+    if (a->D > tm_attention_max_head_dim() || a->D % unit)
+        return TM_ERR_UNSUPPORTED_SHAPE;
+    if ((int64_t)a->B * ((a->Lq + 63) / 64 + (a->Lk + 63) / 64 + 1) * a->H >= INT32_MAX)
+        return TM_ERR_UNSUPPORTED_SHAPE;
+    if (!(a->scale == a->scale) || !(a->cap >= 0.f) || (!a->q_docs != !a->k_docs) ||
+        (!a->q_positions != !a->k_positions) || (a->q_positions && !a->slopes))
+        return TM_ERR_INVALID_ARGUMENT;
+    if (a->q_positions && (a->axes < 1 || a->axes > 3))
+        return TM_ERR_UNSUPPORTED_SHAPE;
+    const int64_t strides[] = {a->q_b, a->q_l, a->q_h, a->k_b, a->k_l, a->k_h,
+                               a->v_b, a->v_l, a->v_h};
+    for (int64_t s : strides)
+        if (s % unit)
+            return TM_ERR_INVALID_ARGUMENT;
+    if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) % 16)
+        return TM_ERR_INVALID_ARGUMENT;
+    return TM_OK;
+}
+
+Args args_of(const tm_attention *a) {
+    Args p = {};
+    p.q = a->q;
+    p.k = a->k;
+    p.v = a->v;
+    p.slopes = a->slopes;
+    p.q_pos = a->q_positions;
+    p.k_pos = a->k_positions;
+    p.q_docs = a->q_docs;
+    p.k_docs = a->k_docs;
+    p.prefix = a->causal ? a->prefix : nullptr;
+    p.lengths = a->lengths;
+    p.q_b = a->q_b, p.q_l = a->q_l, p.q_h = a->q_h;
+    p.k_b = a->k_b, p.k_l = a->k_l, p.k_h = a->k_h;
+    p.v_b = a->v_b, p.v_l = a->v_l, p.v_h = a->v_h;
+    p.B = a->B, p.Lq = a->Lq, p.Lk = a->Lk, p.H = a->H, p.Hkv = a->Hkv, p.D = a->D;
+    p.axes = a->axes, p.causal = a->causal ? 1 : 0;
+    p.scale = a->scale, p.cap = a->cap;
+    p.splits = 1;
+    return p;
+}
+
+#define ATTN_BY_TYPE(call, ...)                                                                   \
+    (a->dtype == TM_BF16  ? attn::call##_bf16(__VA_ARGS__)                                        \
+     : a->dtype == TM_F16 ? attn::call##_f16(__VA_ARGS__)                                         \
+                          : attn::call##_f32(__VA_ARGS__))
+
+int summarise_docs(const tm_attention *a, Args &p, char *ws, hipStream_t stream) {
+    if (!a->q_docs)
+        return 0;
+    const int64_t nq = (a->Lq + 63) / 64, nk = (a->Lk + 63) / 64;
+    int4 *q_tiles = (int4 *)ws, *k_tiles = q_tiles + a->B * nq;
+    p.q_tiles = q_tiles;
+    p.k_tiles = k_tiles;
+    attend_docs<<<dim3((unsigned)((a->B * (nq + nk) + 3) / 4)), 256, 0, stream>>>(
+        a->q_docs, a->k_docs, a->B, a->Lq, a->Lk, q_tiles, k_tiles);
+    return hipGetLastError() == hipSuccess ? 0 : 1;
+}
+
+} // namespace
+
+extern "C" int32_t tm_attention_max_head_dim(void) { return 256; }
+
+extern "C" size_t tm_attention_workspace_bytes(const tm_attention *a) {
+    if (check(a) != TM_OK)
+        return 0;
+    size_t n = docs_bytes(a);
+    const Splits s = splits_of(a);
+    if (s.n > 1) {
+        const size_t rows = (size_t)s.n * a->B * a->H * a->Lq;
+        n += align256(rows * padded(a->D) * sizeof(float)) + align256(rows * sizeof(float2));
+    }
+    return n;
+}
+
+extern "C" int tm_attention_forward(const tm_attention *a, void *out, float *lse, void *workspace,
+                                    size_t workspace_bytes, hipStream_t stream) {
+    const int rc = check(a);
+    if (rc != TM_OK)
+        return rc;
+    if (a->B == 0 || a->Lq == 0)
+        return TM_OK;
+    if (!a->q || !out || (a->Lk && (!a->k || !a->v)))
+        return TM_ERR_INVALID_ARGUMENT;
+    const size_t need = tm_attention_workspace_bytes(a);
+    if (workspace_bytes < need || (need && !workspace))
+        return TM_ERR_WORKSPACE;
+    Args p = args_of(a);
+    p.out = out;
+    p.lse = lse;
+    char *ws = (char *)workspace;
+    if (summarise_docs(a, p, ws, stream))
+        return TM_ERR_LAUNCH;
+    ws += docs_bytes(a);
+    const Splits s = splits_of(a);
+    const int dp = padded(a->D);
+    p.splits = s.n;
+    p.tiles_per_split = s.tiles;
+    if (s.n > 1) {
+        const size_t rows = (size_t)s.n * a->B * a->H * a->Lq;
+        p.part_o = (float *)ws;
+        p.part_ml = (float2 *)(ws + align256(rows * dp * sizeof(float)));
+    }
+    if (ATTN_BY_TYPE(forward, p, dp, stream))
+        return TM_ERR_LAUNCH;
+    if (s.n > 1 && ATTN_BY_TYPE(join, p, dp, stream))
+        return TM_ERR_LAUNCH;
+    return TM_OK;
+}
+
+extern "C" size_t tm_attention_backward_workspace_bytes(const tm_attention *a) {
+    if (check(a) != TM_OK)
+        return 0;
+    return docs_bytes(a) + align256((size_t)a->B * a->H * a->Lq * sizeof(float));
+}
+
+extern "C" int tm_attention_backward(const tm_attention *a, const void *out, const float *lse,
+                                     const void *dout, int64_t do_b, int64_t do_l, int64_t do_h,
+                                     void *dq, void *dk, void *dv, void *workspace,
+                                     size_t workspace_bytes, hipStream_t stream) {
+    const int rc = check(a);
+    if (rc != TM_OK)
+        return rc;
+    if (a->B == 0 || (a->Lq == 0 && a->Lk == 0))
+        return TM_OK;
+    const int unit = a->dtype == TM_F32 ? 4 : 8;
+    if ((a->Lq && (!a->q || !out || !lse || !dout || !dq)) ||
+        (a->Lk && (!a->k || !a->v || !dk || !dv)) || (uintptr_t)dout % 16 || do_b % unit ||
+        do_l % unit || do_h % unit)
+        return TM_ERR_INVALID_ARGUMENT;
+    const size_t need = tm_attention_backward_workspace_bytes(a);
+    if (workspace_bytes < need || (need && !workspace))
+        return TM_ERR_WORKSPACE;
+    Args p = args_of(a);
+    p.out = const_cast<void *>(out);
+    p.lse = const_cast<float *>(lse);
+    p.dout = dout;
+    p.do_b = do_b, p.do_l = do_l, p.do_h = do_h;
+    p.dq = dq, p.dk = dk, p.dv = dv;
+    char *ws = (char *)workspace;
+    if (summarise_docs(a, p, ws, stream))
+        return TM_ERR_LAUNCH;
+    float *delta = (float *)(ws + docs_bytes(a));
+    p.delta = delta;
+    const int dp = padded(a->D);
+    if (a->Lq && ATTN_BY_TYPE(delta, p, delta, stream))
+        return TM_ERR_LAUNCH;
+    if (a->Lk && ATTN_BY_TYPE(backward_kv, p, dp, stream))
+        return TM_ERR_LAUNCH;
+    if (a->Lq && ATTN_BY_TYPE(backward_q, p, dp, stream))
+        return TM_ERR_LAUNCH;
+    return TM_OK;
+}

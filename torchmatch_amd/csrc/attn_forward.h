@@ -1,0 +1,299 @@
+// attn_forward.h -- attention forward: out = softmax(scores) v in one pass over
+// the keys.
+//
+// A wave owns 32 queries.  It forms the transposed scores, keys by queries
+// (k q^T), so that a lane holds scores of one query only: the running maximum
+// and sum need one exchange between the two halves of the wave, the rescaling
+// of the output is by a scalar per lane, and the weights lie as the next product
+// (v^T p^T) wants them.  q stays in registers; tiles of 64 keys pass through LDS,
+// brought by all four waves and the next one loaded while this one is used.
+//
+// Weights are rounded to the inputs' type for the second product, as they lie
+// between 0 and 2^8 and every weight of a row errs by as much, relatively, as an
+// input does; scores, maxima, sums and the output accumulate in float32.
+#ifndef TORCHMATCH_AMD_ATTN_FORWARD_H
+#define TORCHMATCH_AMD_ATTN_FORWARD_H
+
+#include "attn_tile.h"
+
+namespace attn {
+
+template <typename T, int DP> struct ForwardShape {
+    // float32 rows of 256: 32 keys at a time, so that both tiles fit in LDS
+    static constexpr int kKeys = sizeof(T) == 4 && DP == 256 ? 32 : 64;
+    static constexpr int kWaves = 4;
+    static constexpr int kQueries = 32 * kWaves;
+    static constexpr int kOccupancy = sizeof(T) * DP <= 256 ? 2 : 1;
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, (ForwardShape<T, DP>::kOccupancy)) void
+attend_forward(const Args p) {
+    using S = ForwardShape<T, DP>;
+    using L = Tile<T, DP>;
+    constexpr int KT = S::kKeys, KB = KT / 32, QT = S::kQueries, C = DP / 16, DB = DP / 32;
+    __shared__ u32x4 sk[KT * L::U];
+    __shared__ u32x4 sv[KT * L::U];
+    __shared__ __attribute__((aligned(16))) int s_docs[KT];
+    __shared__ __attribute__((aligned(16))) float s_pos[3][KT];
+
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q_blocks = (p.Lq + QT - 1) / QT;
+    const int group = p.H / p.Hkv;
+    // the queries of a key head together; long causal rows first
+    int id = xcd_order(blockIdx.x, gridDim.x);
+    const int qb = q_blocks - 1 - id % q_blocks;
+    id /= q_blocks;
+    const int split = id % p.splits;
+    id /= p.splits;
+    const int head = id % p.H, b = id / p.H;
+    const int kvh = head / group;
+
+    const int q0 = qb * QT, qw = q0 + 32 * wave, qi = qw + (lane & 31);
+    const bool q_real = qi < p.Lq;
+    const Limits lim(p, b);
+    const int block_limit = lim.of(min(q0 + QT, p.Lq) - 1);
+    const int wave_limit = qw < p.Lq ? lim.of(min(qw + 32, p.Lq) - 1) : 0;
+    const int full_limit = qw < p.Lq ? lim.of(qw) : 0; // keys that all of the wave see
+
+    const T *q = (const T *)p.q + b * p.q_b + head * p.q_h;
+    const T *k = (const T *)p.k + b * p.k_b + kvh * p.k_h;
+    const T *v = (const T *)p.v + b * p.v_b + kvh * p.v_h;
+    const int32_t *k_docs = p.k_docs ? p.k_docs + (int64_t)b * p.Lk : nullptr;
+    const float *k_pos = p.k_pos ? p.k_pos + (int64_t)b * p.Lk * p.axes : nullptr;
+    const QueryLane<T> rows(p, lim, b, head, qi);
+
+    x8<T> qf[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+        qf[c] = global8<T>(q + (int64_t)(q_real ? qi : 0) * p.q_l, 16 * c + 8 * half, p.D, q_real);
+    // documents: of the block (which tiles to visit) and of the wave (which to use)
+    constexpr int per64 = 64 / KT; // key tiles to a summary
+    int4 wave_docs = {0, 0, 0, 0};
+    TileWalk walk;
+    const int t_end = min((block_limit + 63) / 64, (split + 1) * p.tiles_per_split);
+    {
+        const int64_t nk = (p.Lk + 63) / 64, nq = (p.Lq + 63) / 64;
+        int4 mine = {0, 0, 0, 0};
+        if (p.q_tiles) {
+            const int4 *t = p.q_tiles + b * nq;
+            mine = t[q0 / 64];
+            if (q0 / 64 + 1 < nq) {
+                const int4 o = t[q0 / 64 + 1];
+                mine.x = min(mine.x, o.x);
+                mine.y = max(mine.y, o.y);
+            }
+            wave_docs = qw < p.Lq ? t[qw / 64] : (int4){0x7fffffff, -1, 0, 0};
+        }
+        walk.start(p.k_tiles ? p.k_tiles + b * nk : nullptr, mine, split * p.tiles_per_split,
+                   t_end, lane);
+    }
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+        o[i] = f32x16{};
+    float top = -kInf, sum = 0.f; // of this lane's query; the sum of this half's keys
+
+    Stage<T, DP, KT, 256> gk, gv;
+    int g_doc = -1;
+    float g_pos[3];
+    const int seen = min(block_limit, p.Lk); // keys past it may hold anything
+    auto fetch = [&](int k0) {
+        gk.load(k, p.k_l, k0, seen, p.D, k_docs, tid);
+        gv.load(v, p.v_l, k0, seen, p.D, k_docs, tid);
+        if (k_docs && tid < KT)
+            g_doc = k0 + tid < seen ? k_docs[k0 + tid] : -1;
+        if (k_pos && tid < KT)
+#pragma unroll
+            for (int a = 0; a < 3; ++a)
+                if (a < p.axes)
+                    g_pos[a] = k0 + tid < seen ? k_pos[(int64_t)(k0 + tid) * p.axes + a] : 0.f;
+    };
+
+    int t64 = walk.next(lane), sub = 0;
+    if (t64 < t_end)
+        fetch(t64 * 64);
+    while (t64 < t_end) {
+        const int k0 = t64 * 64 + sub * KT;
+        __syncthreads();
+        gk.store(sk, tid);
+        gv.store(sv, tid);
+        if (k_docs && tid < KT)
+            s_docs[tid] = g_doc;
+        if (k_pos && tid < KT)
+#pragma unroll
+            for (int a = 0; a < 3; ++a)
+                if (a < p.axes)
+                    s_pos[a][tid] = g_pos[a];
+        __syncthreads();
+        const int this64 = t64;
+        if (++sub == per64) {
+            sub = 0;
+            t64 = walk.next(lane);
+        }
+        if (t64 < t_end)
+            fetch(t64 * 64 + sub * KT);
+
+        bool use = k0 < wave_limit, masked = k0 + KT > full_limit;
+        if (k_docs) {
+            const int4 kd = p.k_tiles[(int64_t)b * ((p.Lk + 63) / 64) + this64];
+            use = use && docs_meet(kd, wave_docs);
+            masked = masked || !docs_same(kd, wave_docs);
+        }
+        if (!use)
+            continue;
+
+        // scores: keys by queries
+        f32x16 s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            s[kb] = f32x16{};
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                s[kb] = mma32(L::row8(sk, 32 * kb + (lane & 31), 2 * c + half), qf[c], s[kb]);
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+            rows.score(p, s[kb], nullptr, k0 + 32 * kb, half, &s_pos[0][32 * kb], KT);
+        if (masked) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+                rows.hide(p, s[kb], -kInf, k0 + 32 * kb, half, s_docs + 32 * kb);
+        }
+
+        // the running maximum moves only when it would grow by more than 2^8: weights up
+        // to 2^8 cost no precision, and the output is rarely rescaled
+        float m = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                m = fmaxf(m, s[kb][i]);
+        m = fmaxf(m, __shfl_xor(m, 32));
+        if (__any(m > top + 8.f)) {
+            const float now = fmaxf(m, top);
+            const float r = now == -kInf ? 1.f : __builtin_amdgcn_exp2f(top - now);
+            top = now;
+            sum *= r;
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    o[i][e] *= r;
+        }
+        const float from = top == -kInf ? 0.f : top;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[kb][i] = __builtin_amdgcn_exp2f(s[kb][i] - from);
+                sum += s[kb][i];
+            }
+
+        // output, transposed: v^T p^T
+#pragma unroll
+        for (int t = 0; t < KT / 16; ++t) {
+            const x8<T> w = pack8<T>(s[t / 2], t % 2);
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+                o[i] = mma32(L::col8(sv, 16 * t, i, lane), w, o[i]);
+        }
+    }
+
+    sum += __shfl_xor(sum, 32);
+    if (!q_real)
+        return;
+    const int64_t row = ((int64_t)b * p.H + head) * p.Lq + qi;
+    if (p.splits > 1) {
+        const int64_t at = (int64_t)split * p.B * p.H * p.Lq + row;
+        float *dst = p.part_o + at * DP;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *(f32x4 *)(dst + 32 * i + 2 * e + 4 * half) =
+                    (f32x4){o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+        if (!half)
+            p.part_ml[at] = make_float2(top, sum);
+        return;
+    }
+    const float r = sum == 0.f ? 0.f : 1.f / sum;
+    T *dst = (T *)p.out + (((int64_t)b * p.Lq + qi) * p.H + head) * p.D;
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int d = 32 * i + 2 * e + 4 * half;
+            if (d < p.D) {
+                x4<T> y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    y[j] = (T)(o[i][e + j] * r);
+                *(x4<T> *)(dst + d) = y;
+            }
+        }
+    if (!half && p.lse)
+        p.lse[row] = sum == 0.f ? -kInf : kLn2 * (top + __builtin_amdgcn_logf(sum));
+}
+
+// Joins the partial results of a split over keys: a wave for each query.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attend_join(const Args p) {
+    const int64_t rows = (int64_t)p.B * p.H * p.Lq;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= rows)
+        return;
+    float top = -kInf;
+    for (int s = lane; s < p.splits; s += 64)
+        top = fmaxf(top, p.part_ml[s * rows + row].x);
+#pragma unroll
+    for (int x = 32; x; x >>= 1)
+        top = fmaxf(top, __shfl_xor(top, x));
+    const float from = top == -kInf ? 0.f : top;
+    constexpr int N = (DP + 63) / 64;
+    float sum = 0.f, o[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+        o[n] = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+        const int64_t at = s * rows + row;
+        const float2 ml = p.part_ml[at];
+        const float w = __builtin_amdgcn_exp2f(ml.x - from);
+        sum += ml.y * w;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (lane + 64 * n < DP)
+                o[n] = fmaf(w, p.part_o[at * DP + lane + 64 * n], o[n]);
+    }
+    const int i = (int)(row % p.Lq), head = (int)(row / p.Lq % p.H);
+    const int64_t b = row / p.Lq / p.H;
+    const float r = sum == 0.f ? 0.f : 1.f / sum;
+    T *dst = (T *)p.out + ((b * p.Lq + i) * p.H + head) * p.D;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+        if (lane + 64 * n < p.D)
+            dst[lane + 64 * n] = (T)(o[n] * r);
+    if (!lane && p.lse)
+        p.lse[row] = sum == 0.f ? -kInf : kLn2 * (top + __builtin_amdgcn_logf(sum));
+}
+
+template <typename T, int DP> int run_forward(const Args &a, hipStream_t s) {
+    const int64_t blocks = (int64_t)((a.Lq + ForwardShape<T, DP>::kQueries - 1) /
+                                     ForwardShape<T, DP>::kQueries) *
+                           a.splits * a.H * a.B;
+    attend_forward<T, DP><<<dim3((unsigned)blocks), 256, 0, s>>>(a);
+    return hipGetLastError() == hipSuccess ? 0 : 1;
+}
+
+template <typename T, int DP> int run_join(const Args &a, hipStream_t s) {
+    const int64_t rows = (int64_t)a.B * a.H * a.Lq;
+    attend_join<T, DP><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, s>>>(a);
+    return hipGetLastError() == hipSuccess ? 0 : 1;
+}
+
+} // namespace attn
+
+#endif

@@ -1,0 +1,371 @@
+// attn_tile.h -- the pieces the attention kernels share: matrix-core steps on
+// 32 x 32 tiles, tiles in LDS that are read by rows and by columns without
+// bank conflicts, and the scores' cap, bias and masks.
+//
+// Register layouts of one wave (lane l, half h = l / 32):
+//   operand   8 elements of row l % 32, contraction indices 8h .. 8h + 7
+//   result    16 floats of column l % 32, element i is row 8(i/4) + 4h + i%4
+// A contraction may take its indices in any order as long as both operands
+// agree, so elements 8t .. 8t + 7 of a result serve, as they lie, as an operand
+// of the next product over rows 16t + 8(j/4) + 4h + j%4 (j = 0..7): scores go
+// from one product to the next without leaving the registers.
+#ifndef TORCHMATCH_AMD_ATTN_TILE_H
+#define TORCHMATCH_AMD_ATTN_TILE_H
+
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "attn.h"
+
+namespace attn {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+constexpr float kInf = __builtin_inff();
+
+template <typename T> struct Vec;
+template <> struct Vec<__bf16> {
+    using x4 = b16x4;
+    using x8 = b16x8;
+};
+template <> struct Vec<_Float16> {
+    using x4 = h16x4;
+    using x8 = h16x8;
+};
+template <> struct Vec<float> {
+    using x4 = f32x4;
+    using x8 = f32x8;
+};
+template <typename T> using x4 = typename Vec<T>::x4;
+template <typename T> using x8 = typename Vec<T>::x8;
+
+// c += a b over 16 contraction indices
+__device__ inline f32x16 mma32(b16x8 a, b16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x16 mma32(h16x8 a, h16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+// float32: the step takes two indices, one per half; element i of both halves
+__device__ inline f32x16 mma32(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+}
+
+template <typename T> __device__ inline x8<T> pack8(const f32x16 &c, int t) {
+    x8<T> r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        r[j] = (T)c[8 * t + j];
+    return r;
+}
+
+// A tile of ROWS x DP elements in LDS, in units of 16 bytes.  Rows are padded
+// to a power of two (U units) and a row's units are permuted by an exclusive
+// or with a function of the row, so that both ways of reading spread over all
+// banks: 8 consecutive rows at one unit (row operands), and 4 consecutive rows
+// over 4 aligned units (column operands).
+template <typename T, int DP> struct Tile {
+    static constexpr int E = 16 / (int)sizeof(T); // elements a unit
+    static constexpr int U0 = DP / E;
+    static constexpr int U = U0 <= 4 ? 4 : U0 <= 8 ? 8 : U0 <= 16 ? 16 : U0 <= 32 ? 32 : 64;
+
+    __device__ static inline int swz(int row) {
+        if constexpr (U == 4)
+            return (row >> 2) & 3;
+        else if constexpr (U == 8)
+            return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+        else
+            return ((row & 3) << 2) | ((row >> 2) & 3);
+    }
+    __device__ static inline int at(int row, int unit) { return row * U + (unit ^ swz(row)); }
+
+    // 8 elements of `row` from element 8 c
+    __device__ static inline x8<T> row8(const u32x4 *t, int row, int c) {
+        if constexpr (sizeof(T) == 2) {
+            return __builtin_bit_cast(x8<T>, t[at(row, c)]);
+        } else {
+            const f32x4 lo = __builtin_bit_cast(f32x4, t[at(row, 2 * c)]);
+            const f32x4 hi = __builtin_bit_cast(f32x4, t[at(row, 2 * c + 1)]);
+            return (x8<T>){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        }
+    }
+
+    // column 32 db + l % 32, rows r0 + 8(j/4) + 4h + j%4: an operand whose rows
+    // are the tile's columns
+    __device__ static inline x8<T> col8(const u32x4 *t, int r0, int db, int lane) {
+        if constexpr (sizeof(T) == 2) {
+            // the transposed read: each 16 lanes load 4 rows of 16 elements (4 a
+            // lane) and each lane gets one column of them
+            const int row = r0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
+            const int d = 32 * db + (lane & 16) + 4 * (lane & 3);
+            x8<T> r;
+#pragma unroll
+            for (int jj = 0; jj < 2; ++jj) {
+                const u32x4 *u = t + at(row + 8 * jj, d >> 3);
+                const auto *p = (__attribute__((address_space(3))) s16x4 *)((const s16x4 *)u +
+                                                                          ((d >> 2) & 1));
+                const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s16x4 *)p);
+                const x4<T> y = __builtin_bit_cast(x4<T>, x);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    r[4 * jj + j] = y[j];
+            }
+            return r;
+        } else {
+            const int d = 32 * db + (lane & 31);
+            x8<T> r;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int row = r0 + 8 * (j >> 2) + 4 * (lane >> 5) + (j & 3);
+                r[j] = ((const T *)(t + at(row, d / E)))[d % E];
+            }
+            return r;
+        }
+    }
+};
+
+// The part of a tile that each of NT threads brings from memory: loaded into
+// registers early, written to LDS when the tile before it is done with.
+template <typename T, int DP, int ROWS, int NT> struct Stage {
+    using L = Tile<T, DP>;
+    static constexpr int N = (ROWS * L::U0 + NT - 1) / NT;
+    u32x4 r[N];
+
+    // rows row0 + 0 .. ROWS - 1 of a matrix of `rows` rows (stride elements
+    // apart, d of them real); what lies outside is zero, and so are rows whose
+    // id is negative (ids may be null): they may hold anything
+    __device__ inline void load(const T *base, int64_t stride, int row0, int rows, int d,
+                                const int32_t *ids, int tid) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = tid + n * NT;
+            const int row = i / L::U0, u = i % L::U0;
+            const int at = row0 + row;
+            u32x4 x = {0u, 0u, 0u, 0u};
+            if ((ROWS * L::U0 % NT == 0 || row < ROWS) && at < rows && u * L::E < d &&
+                !(ids && ids[at] < 0))
+                x = *(const u32x4 *)(base + (int64_t)at * stride + u * L::E);
+            r[n] = x;
+        }
+    }
+    __device__ inline void store(u32x4 *t, int tid) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int i = tid + n * NT;
+            const int row = i / L::U0, u = i % L::U0;
+            if (ROWS * L::U0 % NT == 0 || row < ROWS)
+                t[L::at(row, u)] = r[n];
+        }
+    }
+};
+
+// 8 elements of a row in memory (a row operand that stays in registers)
+template <typename T>
+__device__ inline x8<T> global8(const T *row, int e, int d, bool valid) {
+    x8<T> r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        r[j] = (T)0.f;
+    if constexpr (sizeof(T) == 2) {
+        if (valid && e < d)
+            r = *(const x8<T> *)(row + e);
+    } else {
+        if (valid && e < d) {
+            const f32x4 a = *(const f32x4 *)(row + e);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                r[j] = a[j];
+        }
+        if (valid && e + 4 < d) {
+            const f32x4 a = *(const f32x4 *)(row + e + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                r[4 + j] = a[j];
+        }
+    }
+    return r;
+}
+
+// How many leading keys query i of batch row b may see, masks by document aside.
+struct Limits {
+    int length, offset, prefix, causal;
+    __device__ inline Limits(const Args &p, int b) {
+        length = p.lengths ? min(max(p.lengths[b], 0), p.Lk) : p.Lk;
+        offset = length - p.Lq;
+        prefix = p.prefix ? min(max(p.prefix[b], 0), length) : 0;
+        causal = p.causal;
+    }
+    __device__ inline int of(int i) const {
+        return causal ? min(length, max(max(i + offset + 1, prefix), 0)) : length;
+    }
+};
+
+// tanh(y) by exp and a reciprocal: the error, 2e-7, is absolute, and what it
+// multiplies is a score.  float32 products leave the time for the library's.
+template <typename T> __device__ inline float cap_tanh(float y) {
+    if constexpr (sizeof(T) == 4)
+        return tanhf(y);
+    const float e = __builtin_amdgcn_exp2f(y * (2.f * kLog2e));
+    return fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
+}
+
+__device__ inline f32x4 away(f32x4 a, float b) {
+    return (f32x4){fabsf(a[0] - b), fabsf(a[1] - b), fabsf(a[2] - b), fabsf(a[3] - b)};
+}
+
+// One lane's query against results of k q^T, 32 keys a block: the scores in base 2, what the
+// lane may see.
+template <typename T> struct QueryLane {
+    int limit, doc, at;
+    float slope, pos[3];
+
+    __device__ inline QueryLane(const Args &p, const Limits &lim, int b, int head, int i) {
+        const bool real = i < p.Lq;
+        limit = real ? lim.of(i) : 0;
+        doc = p.q_docs && real ? p.q_docs[(int64_t)b * p.Lq + i] : -1;
+        at = i + lim.offset;
+        slope = p.slopes ? p.slopes[head] * kLog2e : 0.f;
+        pos[0] = pos[1] = pos[2] = 0.f;
+        if (p.q_pos && real)
+#pragma unroll
+            for (int a = 0; a < 3; ++a)
+                if (a < p.axes)
+                    pos[a] = p.q_pos[((int64_t)b * p.Lq + i) * p.axes + a];
+    }
+
+    // s: products with keys k0 ..; to scores times log2 e.  With `grad`, the derivative of
+    // the cap too.  k_pos: the block's positions in LDS, `axis` apart.
+    __device__ inline void score(const Args &p, f32x16 &s, f32x16 *grad, int k0, int half,
+                                 const float *k_pos, int axis) const {
+        if (p.cap > 0.f) {
+            const float in = p.scale / p.cap, out = p.cap * kLog2e;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float t = cap_tanh<T>(s[i] * in);
+                if (grad)
+                    (*grad)[i] = fmaf(-t, t, 1.f);
+                s[i] = out * t;
+            }
+        } else {
+            const float m = p.scale * kLog2e;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                s[i] *= m;
+        }
+        if (p.q_pos) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const int j = 8 * n + 4 * half;
+                f32x4 dist = away(*(const f32x4 *)(k_pos + j), pos[0]);
+                if (p.axes > 1)
+                    dist += away(*(const f32x4 *)(k_pos + axis + j), pos[1]);
+                if (p.axes > 2)
+                    dist += away(*(const f32x4 *)(k_pos + 2 * axis + j), pos[2]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    s[4 * n + e] = fmaf(-slope, dist[e], s[4 * n + e]);
+            }
+        } else if (p.slopes) {
+            const float from = (float)(at - k0 - 4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                s[i] = fmaf(-slope, fabsf(from - (float)(8 * (i / 4) + i % 4)), s[i]);
+        }
+    }
+    // x where the lane does not see the key; docs: the block's documents in LDS
+    __device__ inline void hide(const Args &p, f32x16 &s, float x, int k0, int half,
+                                const int *docs) const {
+        const int last = limit - k0 - 4 * half;
+        if (p.k_docs) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const i32x4 d = *(const i32x4 *)(docs + 8 * n + 4 * half);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool see = (8 * n + e < last) & (d[e] == doc) & (doc >= 0);
+                    s[4 * n + e] = see ? s[4 * n + e] : x;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                s[i] = 8 * (i / 4) + i % 4 < last ? s[i] : x;
+        }
+    }
+};
+
+// Documents of 64 consecutive keys or queries: the smallest and the largest id
+// that is not negative, and whether any is negative.
+__device__ inline bool docs_meet(int4 a, int4 b) { return a.x <= b.y && b.x <= a.y; }
+__device__ inline bool docs_same(int4 a, int4 b) {
+    return a.x == a.y && b.x == b.y && a.x == b.x && !a.z && !b.z;
+}
+
+// Walks the tiles of 64 rows in [t, end) that can hold something to see: all of them, or
+// those whose documents meet `mine`.
+struct TileWalk {
+    const int4 *tiles;
+    int4 mine;
+    int base, end;
+    uint64_t left;
+
+    __device__ inline void start(const int4 *tiles_, int4 mine_, int t, int end_, int lane) {
+        tiles = tiles_;
+        mine = mine_;
+        base = t;
+        end = end_;
+        left = 0;
+        if (tiles)
+            fill(lane);
+    }
+    __device__ inline void fill(int lane) {
+        for (left = 0; base < end; base += 64) {
+            const int i = base + lane;
+            left = __ballot(i < end && docs_meet(tiles[min(i, end - 1)], mine));
+            if (left)
+                return;
+        }
+    }
+    // the next tile, or `end`
+    __device__ inline int next(int lane) {
+        if (!tiles)
+            return base < end ? base++ : end;
+        if (!left)
+            return end;
+        const int t = base + __builtin_ctzll(left);
+        left &= left - 1;
+        if (!left) {
+            base += 64;
+            fill(lane);
+        }
+        return t;
+    }
+};
+
+// Blocks are dealt to the 8 XCDs in turn; each has its own L2.  Gives every XCD a
+// run of consecutive work items, so that those which read the same keys meet.
+__device__ inline int xcd_order(int id, int n) {
+    const int per = n >> 3, rest = n & 7, x = id & 7;
+    return x * per + min(x, rest) + (id >> 3);
+}
+
+} // namespace attn
+
+#endif
