@@ -373,20 +373,22 @@ typedef struct tm_attention {
 
 int32_t tm_attention_max_head_dim(void);
 
-/* out: (B, Lq, H, D) contiguous, the inputs' type; lse: (B, H, Lq) float32, the
+/* out: (B, Lq, H, D) contiguous, the inputs' type; out_low: what rounding took off
+ * it, of the same shape and type, or NULL (16-bit types; the gradients are the
+ * better for it); lse: (B, H, Lq) float32, the
  * natural logarithm of each row's sum, or NULL.  workspace: device, at least
  * tm_attention_workspace_bytes(a), 16-byte aligned, any contents. */
 size_t tm_attention_workspace_bytes(const tm_attention *a);
-int tm_attention_forward(const tm_attention *a, void *out, float *lse, void *workspace,
-                         size_t workspace_bytes, hipStream_t stream);
+int tm_attention_forward(const tm_attention *a, void *out, void *out_low, float *lse,
+                         void *workspace, size_t workspace_bytes, hipStream_t stream);
 
-/* Gradients of q, k and v (contiguous, the inputs' type) from out and lse of the
- * forward call and the output's gradient, (B, Lq, H, D) with its own strides.
+/* Gradients of q, k and v (contiguous, the inputs' type) from out, out_low
+ * (or NULL) and lse of the forward call and the output's gradient, (B, Lq, H, D) with its own strides.
  * The same call gives the same bits: nothing is added by atomics. */
 size_t tm_attention_backward_workspace_bytes(const tm_attention *a);
-int tm_attention_backward(const tm_attention *a, const void *out, const float *lse,
-                          const void *dout, int64_t do_b, int64_t do_l, int64_t do_h, void *dq,
-                          void *dk, void *dv, void *workspace, size_t workspace_bytes,
+int tm_attention_backward(const tm_attention *a, const void *out, const void *out_low,
+                          const float *lse, const void *dout, int64_t do_b, int64_t do_l,
+                          int64_t do_h, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
                           hipStream_t stream);
 
 /* Rotation of feature pairs.  x is (B, L, H, D) of `dtype` with strides in

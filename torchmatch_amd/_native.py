@@ -175,13 +175,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tm_attention_max_head_dim": (ctypes.c_int32, []),
     "tm_attention_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Attention)]),
     "tm_attention_forward": (
-        ctypes.c_int, [ctypes.POINTER(Attention), _VP, _VP, _VP, ctypes.c_size_t, _VP]
+        ctypes.c_int, [ctypes.POINTER(Attention), _VP, _VP, _VP, _VP, ctypes.c_size_t, _VP]
     ),
     "tm_attention_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Attention)]),
     "tm_attention_backward": (
         ctypes.c_int,
         [
-            ctypes.POINTER(Attention), _VP, _VP, _VP, ctypes.c_int64, ctypes.c_int64,
+            ctypes.POINTER(Attention), _VP, _VP, _VP, _VP, ctypes.c_int64, ctypes.c_int64,
             ctypes.c_int64, _VP, _VP, _VP, _VP, ctypes.c_size_t, _VP,
         ],
     ),

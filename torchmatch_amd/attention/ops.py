@@ -23,6 +23,13 @@ def _attend_fake(q, k, v, *masks, scale, cap=0.0, causal=False):  # noqa: ANN002
             q.new_empty(b, heads, length, dtype=torch.float32))
 
 
+@torch.library.register_fake("attention::attend_forward")
+def _attend_forward_fake(q, k, v, *masks, scale, cap=0.0, causal=False):  # noqa: ANN002
+    out, lse = _attend_fake(q, k, v, *masks, scale=scale, cap=cap, causal=causal)
+    low = q.new_empty(0) if q.dtype == torch.float32 else torch.empty_like(out)
+    return out, low, lse
+
+
 @torch.library.register_fake("attention::attend_backward")
 def _attend_backward_fake(dout, q, k, v, *rest, scale, cap=0.0, causal=False):  # noqa: ANN002
     del dout, rest, scale, cap, causal

@@ -46,18 +46,31 @@ size_t docs_bytes(const tm_attention *a) {
     return align256(tiles * sizeof(int4));
 }
 
-// Keys are split over blocks when there are too few rows to fill the chip with whole ones.
-// At least four tiles of 64 keys a split, so that its start and the join are worth it.
+// Few queries: the kernel that packs the queries of a key head's group into 32 rows.
+// Above 32 queries the other kernel's 128 rows a block are no longer mostly empty.
+bool few(const tm_attention *a) { return a->Lq <= 32; }
+
+// Keys are split over blocks when there are too few rows to fill the chip.  Few queries are
+// bound by reading the keys: about four blocks for each of the 256 compute units keep them
+// busy whatever the rows' lengths, with a tile of 64 keys or more for each of a block's
+// 8 waves.  Else a block needs at least four tiles, so that its start and the join are worth it.
 struct Splits {
     int n, tiles;
 };
 Splits splits_of(const tm_attention *a) {
-    const int64_t blocks = (int64_t)((a->Lq + 127) / 128) * a->H * a->B;
-    const int tiles = (a->Lk + 63) / 64;
-    if (blocks >= 256 || tiles < 8)
-        return {1, std::max(tiles, 1)};
-    const int want = (int)std::min<int64_t>((512 + blocks - 1) / blocks, tiles / 4);
-    const int per = (tiles + want - 1) / want;
+    const int tiles = std::max((a->Lk + 63) / 64, 1);
+    int64_t blocks, want, most;
+    if (few(a)) {
+        blocks = (int64_t)((a->H / a->Hkv * a->Lq + 31) / 32) * a->Hkv * a->B;
+        want = (1024 + blocks - 1) / blocks;
+        most = tiles / 8;
+    } else {
+        blocks = (int64_t)((a->Lq + 127) / 128) * a->H * a->B;
+        want = blocks >= 256 ? 1 : (512 + blocks - 1) / blocks;
+        most = tiles / 4;
+    }
+    const int n = (int)std::max<int64_t>(1, std::min(want, most));
+    const int per = (tiles + n - 1) / n;
     return {(tiles + per - 1) / per, per};
 }
 
@@ -143,8 +156,9 @@ extern "C" size_t tm_attention_workspace_bytes(const tm_attention *a) {
     return n;
 }
 
-extern "C" int tm_attention_forward(const tm_attention *a, void *out, float *lse, void *workspace,
-                                    size_t workspace_bytes, hipStream_t stream) {
+extern "C" int tm_attention_forward(const tm_attention *a, void *out, void *out_low,
+                                    float *lse, void *workspace, size_t workspace_bytes,
+                                    hipStream_t stream) {
     const int rc = check(a);
     if (rc != TM_OK)
         return rc;
@@ -157,6 +171,7 @@ extern "C" int tm_attention_forward(const tm_attention *a, void *out, float *lse
         return TM_ERR_WORKSPACE;
     Args p = args_of(a);
     p.out = out;
+    p.out_low = a->dtype == TM_F32 ? nullptr : out_low;
     p.lse = lse;
     char *ws = (char *)workspace;
     if (summarise_docs(a, p, ws, stream))
@@ -171,7 +186,7 @@ extern "C" int tm_attention_forward(const tm_attention *a, void *out, float *lse
         p.part_o = (float *)ws;
         p.part_ml = (float2 *)(ws + align256(rows * dp * sizeof(float)));
     }
-    if (ATTN_BY_TYPE(forward, p, dp, stream))
+    if (few(a) ? ATTN_BY_TYPE(tokens, p, dp, stream) : ATTN_BY_TYPE(forward, p, dp, stream))
         return TM_ERR_LAUNCH;
     if (s.n > 1 && ATTN_BY_TYPE(join, p, dp, stream))
         return TM_ERR_LAUNCH;
@@ -184,9 +199,9 @@ extern "C" size_t tm_attention_backward_workspace_bytes(const tm_attention *a) {
     return docs_bytes(a) + align256((size_t)a->B * a->H * a->Lq * sizeof(float));
 }
 
-extern "C" int tm_attention_backward(const tm_attention *a, const void *out, const float *lse,
-                                     const void *dout, int64_t do_b, int64_t do_l, int64_t do_h,
-                                     void *dq, void *dk, void *dv, void *workspace,
+extern "C" int tm_attention_backward(const tm_attention *a, const void *out,
+                                     const void *out_low, const float *lse, const void *dout,
+                                     int64_t do_b, int64_t do_l, int64_t do_h, void *dq, void *dk, void *dv, void *workspace,
                                      size_t workspace_bytes, hipStream_t stream) {
     const int rc = check(a);
     if (rc != TM_OK)
@@ -203,6 +218,7 @@ extern "C" int tm_attention_backward(const tm_attention *a, const void *out, con
         return TM_ERR_WORKSPACE;
     Args p = args_of(a);
     p.out = const_cast<void *>(out);
+    p.out_low = a->dtype == TM_F32 ? nullptr : const_cast<void *>(out_low);
     p.lse = const_cast<float *>(lse);
     p.dout = dout;
     p.do_b = do_b, p.do_l = do_l, p.do_h = do_h;

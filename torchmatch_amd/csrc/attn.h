@@ -10,7 +10,7 @@ namespace attn {
 
 struct Args {
     const void *q, *k, *v, *dout;
-    void *out, *dq, *dk, *dv; // contiguous (B, L, heads, D)
+    void *out, *out_low, *dq, *dk, *dv; // contiguous (B, L, heads, D); out_low may be null
     float *lse;               // (B, H, Lq), natural logarithm, -inf for empty rows
     const float *delta;       // (B, H, Lq): sum over d of out * dout
     const float *slopes;      // (H) or null
@@ -20,7 +20,7 @@ struct Args {
     const int32_t *prefix, *lengths; // (B) or null
     // partial results of a split over keys
     float *part_o;  // (splits, B, H, Lq, DP)
-    float2 *part_ml; // (splits, B, H, Lq): largest score (base 2), sum
+    float2 *part_ml; // (splits, B, H, Lq): what weights are relative to (base 2), their sum
     // strides in elements
     int64_t q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h, do_b, do_l, do_h;
     int32_t B, Lq, Lk, H, Hkv, D;
@@ -31,6 +31,7 @@ struct Args {
 // One file per type; dp is D padded to 32, 64, 96, 128 or 256.  Non-zero: a launch failed.
 #define ATTN_DECLARE(type)                                                                        \
     int forward_##type(const Args &, int dp, hipStream_t);                                        \
+    int tokens_##type(const Args &, int dp, hipStream_t);                                         \
     int join_##type(const Args &, int dp, hipStream_t);                                           \
     int backward_kv_##type(const Args &, int dp, hipStream_t);                                    \
     int backward_q_##type(const Args &, int dp, hipStream_t);                                     \

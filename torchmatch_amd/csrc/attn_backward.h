@@ -448,7 +448,8 @@ __global__ __launch_bounds__(256, 1) void attend_backward_q(const Args p) {
         }
 }
 
-// delta: a wave for each query and head
+// delta: a wave for each query and head.  From the output as it was before it was rounded,
+// in two parts: the rounding alone would add as much error to dq and dk as that of ds does.
 template <typename T>
 __global__ __launch_bounds__(256) void attend_delta(const Args p, float *delta) {
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -457,7 +458,7 @@ __global__ __launch_bounds__(256) void attend_delta(const Args p, float *delta) 
         return;
     const int head = (int)(row % p.H), i = (int)(row / p.H % p.Lq);
     const int64_t b = row / p.H / p.Lq;
-    const T *o = (const T *)p.out + row * p.D;
+    const T *o = (const T *)p.out + row * p.D, *low = (const T *)p.out_low + row * p.D;
     const T *dout = (const T *)p.dout + b * p.do_b + i * p.do_l + head * p.do_h;
     float x = 0.f;
     for (int d = 4 * lane; d < p.D; d += 256) {
@@ -465,6 +466,12 @@ __global__ __launch_bounds__(256) void attend_delta(const Args p, float *delta) 
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             x = fmaf((float)u[j], (float)w[j], x);
+        if (p.out_low) {
+            const x4<T> r = *(const x4<T> *)(low + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                x = fmaf((float)r[j], (float)w[j], x);
+        }
     }
 #pragma unroll
     for (int n = 32; n; n >>= 1)

@@ -163,34 +163,7 @@ attend_forward(const Args p) {
                 rows.hide(p, s[kb], -kInf, k0 + 32 * kb, half, s_docs + 32 * kb);
         }
 
-        // the running maximum moves only when it would grow by more than 2^8: weights up
-        // to 2^8 cost no precision, and the output is rarely rescaled
-        float m = s[0][0];
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                m = fmaxf(m, s[kb][i]);
-        m = fmaxf(m, __shfl_xor(m, 32));
-        if (__any(m > top + 8.f)) {
-            const float now = fmaxf(m, top);
-            const float r = now == -kInf ? 1.f : __builtin_amdgcn_exp2f(top - now);
-            top = now;
-            sum *= r;
-#pragma unroll
-            for (int i = 0; i < DB; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    o[i][e] *= r;
-        }
-        const float from = top == -kInf ? 0.f : top;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[kb][i] = __builtin_amdgcn_exp2f(s[kb][i] - from);
-                sum += s[kb][i];
-            }
+        soften<T>(s, o, top, sum);
 
         // output, transposed: v^T p^T
 #pragma unroll
@@ -220,27 +193,26 @@ attend_forward(const Args p) {
         return;
     }
     const float r = sum == 0.f ? 0.f : 1.f / sum;
-    T *dst = (T *)p.out + (((int64_t)b * p.Lq + qi) * p.H + head) * p.D;
+    const int64_t at = (((int64_t)b * p.Lq + qi) * p.H + head) * p.D;
 #pragma unroll
     for (int i = 0; i < DB; ++i)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             const int d = 32 * i + 2 * e + 4 * half;
             if (d < p.D) {
-                x4<T> y;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    y[j] = (T)(o[i][e + j] * r);
-                *(x4<T> *)(dst + d) = y;
+                const f32x4 x = {o[i][e] * r, o[i][e + 1] * r, o[i][e + 2] * r, o[i][e + 3] * r};
+                put<T>(p, at + d, __builtin_convertvector(x, x4<T>), x);
             }
         }
     if (!half && p.lse)
         p.lse[row] = sum == 0.f ? -kInf : kLn2 * (top + __builtin_amdgcn_logf(sum));
 }
 
-// Joins the partial results of a split over keys: a wave for each query.
+// Joins the partial results of a split over keys: 64 threads for each query, 4 features each
+// thread; where a row has fewer than 256, the rest of them take other splits.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void attend_join(const Args p) {
+    constexpr int N = DP / 4, P = 64 / N; // threads of a part's row, parts at a time
     const int64_t rows = (int64_t)p.B * p.H * p.Lq;
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
@@ -253,29 +225,38 @@ __global__ __launch_bounds__(256) void attend_join(const Args p) {
     for (int x = 32; x; x >>= 1)
         top = fmaxf(top, __shfl_xor(top, x));
     const float from = top == -kInf ? 0.f : top;
-    constexpr int N = (DP + 63) / 64;
-    float sum = 0.f, o[N];
+    const int part = lane / N, d = 4 * (lane % N);
+    float sum = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (part < P) {
+#pragma unroll 4
+        for (int s = part; s < p.splits; s += P) {
+            const int64_t at = s * rows + row;
+            const float2 ml = p.part_ml[at];
+            const float w = __builtin_amdgcn_exp2f(ml.x - from);
+            const f32x4 x = *(const f32x4 *)(p.part_o + at * DP + d);
+            sum = fmaf(ml.y, w, sum);
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-        o[n] = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-        const int64_t at = s * rows + row;
-        const float2 ml = p.part_ml[at];
-        const float w = __builtin_amdgcn_exp2f(ml.x - from);
-        sum += ml.y * w;
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-            if (lane + 64 * n < DP)
-                o[n] = fmaf(w, p.part_o[at * DP + lane + 64 * n], o[n]);
+            for (int j = 0; j < 4; ++j)
+                o[j] = fmaf(w, x[j], o[j]);
+        }
     }
-    const int i = (int)(row % p.Lq), head = (int)(row / p.Lq % p.H);
-    const int64_t b = row / p.Lq / p.H;
-    const float r = sum == 0.f ? 0.f : 1.f / sum;
-    T *dst = (T *)p.out + ((b * p.Lq + i) * p.H + head) * p.D;
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-        if (lane + 64 * n < p.D)
-            dst[lane + 64 * n] = (T)(o[n] * r);
+    for (int x = 1; x < P; ++x) {
+        const float more = __shfl(sum, lane % N + x * N);
+        sum = part == 0 ? sum + more : sum;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float y = __shfl(o[j], lane % N + x * N);
+            o[j] = part == 0 ? o[j] + y : o[j];
+        }
+    }
+    if (part == 0 && d < p.D) {
+        const int i = (int)(row % p.Lq), head = (int)(row / p.Lq % p.H);
+        const int64_t b = row / p.Lq / p.H;
+        o *= sum == 0.f ? 0.f : 1.f / sum;
+        put<T>(p, ((b * p.Lq + i) * p.H + head) * p.D + d, __builtin_convertvector(o, x4<T>), o);
+    }
     if (!lane && p.lse)
         p.lse[row] = sum == 0.f ? -kInf : kLn2 * (top + __builtin_amdgcn_logf(sum));
 }

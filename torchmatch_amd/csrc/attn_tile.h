@@ -311,6 +311,58 @@ template <typename T> struct QueryLane {
     }
 };
 
+// Weights of half precision are held 2^7 up: its smallest normal number is 2^-14, and weights
+// below it lose bits that count where many keys share a row.  At most 2^(8 + 7) then.
+template <typename T> constexpr float weight_shift() {
+    return __is_same(T, _Float16) ? 7.f : 0.f;
+}
+
+// One step of the running softmax: scores s (base 2, keys by queries) become weights
+// 2^(s - top).  `top` follows the largest score seen only when that grew by more than
+// 2^8: weights up to 2^8 cost no precision in float32 sums, and the output is rarely rescaled.
+// `sum` adds this lane's half of the keys.
+template <typename T, int KB, int DB>
+__device__ inline void soften(f32x16 (&s)[KB], f32x16 (&o)[DB], float &top, float &sum) {
+    float m = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            m = fmaxf(m, s[kb][i]);
+    m = fmaxf(m, __shfl_xor(m, 32)) - weight_shift<T>();
+    if (__any(m > top + 8.f)) {
+        const float now = fmaxf(m, top);
+        const float r = now == -kInf ? 1.f : __builtin_amdgcn_exp2f(top - now);
+        top = now;
+        sum *= r;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                o[i][e] *= r;
+    }
+    const float from = top == -kInf ? 0.f : top;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[kb][i] = __builtin_amdgcn_exp2f(s[kb][i] - from);
+            sum += s[kb][i];
+        }
+}
+
+// A result in the outputs' type, and what the rounding took off (for the gradient)
+template <typename T> __device__ inline void put(const Args &p, int64_t at, x4<T> y, f32x4 x) {
+    *(x4<T> *)((T *)p.out + at) = y;
+    if (sizeof(T) == 2 && p.out_low) {
+        x4<T> z;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            z[j] = (T)(x[j] - (float)y[j]);
+        *(x4<T> *)((T *)p.out_low + at) = z;
+    }
+}
+
 // Documents of 64 consecutive keys or queries: the smallest and the largest id
 // that is not negative, and whether any is negative.
 __device__ inline bool docs_meet(int4 a, int4 b) { return a.x <= b.y && b.x <= a.y; }

@@ -161,35 +161,60 @@ Tensor narrowed(const Tensor &t, int64_t d) {
     return t.size(3) == d ? t : t.narrow(3, 0, d).contiguous();
 }
 
+// `with_low`: also what rounding took off the output (empty for float32)
+std::tuple<Tensor, Tensor, Tensor>
+forward(const Tensor &q, const Tensor &k, const Tensor &v, const OptTensor &slopes,
+        const OptTensor &q_pos, const OptTensor &k_pos, const OptTensor &q_docs,
+        const OptTensor &k_docs, const OptTensor &prefix, const OptTensor &lengths, double scale,
+        double cap, bool causal, bool with_low) {
+    const c10::DeviceGuard guard(q.device());
+    const Problem p = problem(q, k, v, slopes, q_pos, k_pos, q_docs, k_docs, prefix, lengths,
+                              scale, cap, causal);
+    Tensor out = at::empty({p.a.B, p.a.Lq, p.a.H, p.a.D}, q.options());
+    Tensor lse = at::empty({p.a.B, p.a.H, p.a.Lq}, q.options().dtype(at::kFloat)), low;
+    with_low = with_low && p.a.dtype != TM_F32;
+    if (with_low)
+        low = at::empty_like(out);
+    if (out.numel()) {
+        const size_t bytes = tm_attention_workspace_bytes(&p.a);
+        Tensor ws;
+        if (bytes)
+            ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+        check_rc(tm_attention_forward(&p.a, out.data_ptr(), with_low ? low.data_ptr() : nullptr,
+                                      lse.data_ptr<float>(), bytes ? ws.data_ptr() : nullptr,
+                                      bytes, current_stream(q)),
+                 "attend");
+    }
+    return {narrowed(out, p.d), with_low ? narrowed(low, p.d) : low, lse};
+}
+
 std::tuple<Tensor, Tensor> attend_hip(const Tensor &q, const Tensor &k, const Tensor &v,
                                       const OptTensor &slopes, const OptTensor &q_pos,
                                       const OptTensor &k_pos, const OptTensor &q_docs,
                                       const OptTensor &k_docs, const OptTensor &prefix,
                                       const OptTensor &lengths, double scale, double cap,
                                       bool causal) {
-    const c10::DeviceGuard guard(q.device());
-    const Problem p = problem(q, k, v, slopes, q_pos, k_pos, q_docs, k_docs, prefix, lengths,
-                              scale, cap, causal);
-    Tensor out = at::empty({p.a.B, p.a.Lq, p.a.H, p.a.D}, q.options());
-    Tensor lse = at::empty({p.a.B, p.a.H, p.a.Lq}, q.options().dtype(at::kFloat));
-    if (out.numel()) {
-        const size_t bytes = tm_attention_workspace_bytes(&p.a);
-        Tensor ws;
-        if (bytes)
-            ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
-        check_rc(tm_attention_forward(&p.a, out.data_ptr(), lse.data_ptr<float>(),
-                                      bytes ? ws.data_ptr() : nullptr, bytes, current_stream(q)),
-                 "attend");
-    }
-    return {narrowed(out, p.d), lse};
+    auto [out, low, lse] = forward(q, k, v, slopes, q_pos, k_pos, q_docs, k_docs, prefix,
+                                   lengths, scale, cap, causal, false);
+    return {out, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor>
+attend_forward_hip(const Tensor &q, const Tensor &k, const Tensor &v, const OptTensor &slopes,
+                   const OptTensor &q_pos, const OptTensor &k_pos, const OptTensor &q_docs,
+                   const OptTensor &k_docs, const OptTensor &prefix, const OptTensor &lengths,
+                   double scale, double cap, bool causal) {
+    auto [out, low, lse] = forward(q, k, v, slopes, q_pos, k_pos, q_docs, k_docs, prefix,
+                                   lengths, scale, cap, causal, true);
+    return {out, low.defined() ? low : at::empty({0}, q.options()), lse};
 }
 
 std::tuple<Tensor, Tensor, Tensor>
 attend_backward_hip(const Tensor &dout, const Tensor &q, const Tensor &k, const Tensor &v,
-                    const Tensor &out, const Tensor &lse, const OptTensor &slopes,
-                    const OptTensor &q_pos, const OptTensor &k_pos, const OptTensor &q_docs,
-                    const OptTensor &k_docs, const OptTensor &prefix, const OptTensor &lengths,
-                    double scale, double cap, bool causal) {
+                    const Tensor &out, const Tensor &out_low, const Tensor &lse,
+                    const OptTensor &slopes, const OptTensor &q_pos, const OptTensor &k_pos,
+                    const OptTensor &q_docs, const OptTensor &k_docs, const OptTensor &prefix,
+                    const OptTensor &lengths, double scale, double cap, bool causal) {
     const c10::DeviceGuard guard(q.device());
     const Problem p = problem(q, k, v, slopes, q_pos, k_pos, q_docs, k_docs, prefix, lengths,
                               scale, cap, causal);
@@ -204,14 +229,21 @@ attend_backward_hip(const Tensor &dout, const Tensor &q, const Tensor &k, const 
     TORCH_CHECK_VALUE(lse.dim() == 3 && lse.size(0) == q.size(0) && lse.size(1) == q.size(2) &&
                           lse.size(2) == q.size(1) && lse.is_contiguous(),
                       "attend_backward: lse must be a contiguous (B, H, Lq)");
+    const bool has_low = out_low.numel() && p.a.dtype != TM_F32;
+    TORCH_CHECK_VALUE(!has_low || (out_low.sizes() == q.sizes() &&
+                                   out_low.device() == q.device() &&
+                                   out_low.scalar_type() == q.scalar_type()),
+                      "attend_backward: out_low must be as out, or empty");
     const Tensor o = readable(out).contiguous(), g = readable(dout);
+    const Tensor low = has_low ? readable(out_low).contiguous() : out_low;
     Tensor dq = at::empty(p.q.sizes(), q.options()), dk = at::empty(p.k.sizes(), q.options()),
            dv = at::empty(p.k.sizes(), q.options());
     if (dq.numel() || dk.numel()) {
         const size_t bytes = tm_attention_backward_workspace_bytes(&p.a);
         Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
-        check_rc(tm_attention_backward(&p.a, o.const_data_ptr(), lse.const_data_ptr<float>(),
-                                       g.const_data_ptr(), step_of(g, 0), step_of(g, 1),
+        check_rc(tm_attention_backward(&p.a, o.const_data_ptr(),
+                                       has_low ? low.const_data_ptr() : nullptr,
+                                       lse.const_data_ptr<float>(), g.const_data_ptr(), step_of(g, 0), step_of(g, 1),
                                        step_of(g, 2), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                        ws.data_ptr(), bytes, current_stream(q)),
                  "attend_backward");
@@ -287,28 +319,23 @@ void constant(const OptTensor &t, const char *op, const char *name) {
                                 name);
 }
 
-using AttendOp = std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &,
-                                            const OptTensor &, const OptTensor &,
-                                            const OptTensor &, const OptTensor &,
-                                            const OptTensor &, const OptTensor &,
-                                            const OptTensor &, double, double, bool);
-
-std::tuple<Tensor, Tensor> call_attend(const Tensor &q, const Tensor &k, const Tensor &v,
-                                       const std::vector<OptTensor> &m, double scale, double cap,
-                                       bool causal) {
-    static auto op = c10::Dispatcher::singleton()
-                         .findSchemaOrThrow("attention::attend", "")
-                         .typed<AttendOp>();
-    return op.call(q, k, v, m[0], m[1], m[2], m[3], m[4], m[5], m[6], scale, cap, causal);
-}
+template <typename... R>
+using AttendOp = std::tuple<R...>(const Tensor &, const Tensor &, const Tensor &,
+                                  const OptTensor &, const OptTensor &, const OptTensor &,
+                                  const OptTensor &, const OptTensor &, const OptTensor &,
+                                  const OptTensor &, double, double, bool);
 
 struct AttendFunction : torch::autograd::Function<AttendFunction> {
     static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k,
                                  const Tensor &v, const std::vector<OptTensor> &masks,
                                  double scale, double cap, bool causal) {
         at::AutoDispatchBelowADInplaceOrView below;
-        auto [out, lse] = call_attend(q, k, v, masks, scale, cap, causal);
-        variable_list saved = {q, k, v, out, lse};
+        static auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("attention::attend_forward", "")
+                             .typed<AttendOp<Tensor, Tensor, Tensor>>();
+        auto [out, low, lse] = op.call(q, k, v, masks[0], masks[1], masks[2], masks[3], masks[4],
+                                       masks[5], masks[6], scale, cap, causal);
+        variable_list saved = {q, k, v, out, low, lse};
         for (const auto &m : masks)
             saved.push_back(m.has_value() ? *m : Tensor());
         ctx->save_for_backward(saved);
@@ -329,12 +356,12 @@ struct AttendFunction : torch::autograd::Function<AttendFunction> {
                 .findSchemaOrThrow("attention::attend_backward", "")
                 .typed<std::tuple<Tensor, Tensor, Tensor>(
                     const Tensor &, const Tensor &, const Tensor &, const Tensor &,
-                    const Tensor &, const Tensor &, const OptTensor &, const OptTensor &,
+                    const Tensor &, const Tensor &, const Tensor &, const OptTensor &,
                     const OptTensor &, const OptTensor &, const OptTensor &, const OptTensor &,
-                    const OptTensor &, double, double, bool)>();
+                    const OptTensor &, const OptTensor &, double, double, bool)>();
         auto [dq, dk, dv] =
-            op.call(grads[0], s[0], s[1], s[2], s[3], s[4], opt(5), opt(6), opt(7), opt(8),
-                    opt(9), opt(10), opt(11), ctx->saved_data["scale"].toDouble(),
+            op.call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], opt(6), opt(7), opt(8),
+                    opt(9), opt(10), opt(11), opt(12), ctx->saved_data["scale"].toDouble(),
                     ctx->saved_data["cap"].toDouble(), ctx->saved_data["causal"].toBool());
         result[0] = dq;
         result[1] = dk;
@@ -360,7 +387,11 @@ std::tuple<Tensor, Tensor> attend_autograd(const Tensor &q, const Tensor &k, con
         }
     }
     at::AutoDispatchBelowADInplaceOrView below;
-    return call_attend(q, k, v, masks, scale, cap, causal);
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("attention::attend", "")
+                         .typed<AttendOp<Tensor, Tensor>>();
+    return op.call(q, k, v, slopes, q_pos, k_pos, q_docs, k_docs, prefix, lengths, scale, cap,
+                   causal);
 }
 
 Tensor call_rotate(const Tensor &x, const Tensor &positions, const Tensor &freqs,
@@ -415,7 +446,13 @@ TORCH_LIBRARY(attention, m) {
           "Tensor? k_positions=None, Tensor? q_docs=None, Tensor? k_docs=None, "
           "Tensor? prefix=None, Tensor? lengths=None, *, float scale, float cap=0., "
           "bool causal=False) -> (Tensor, Tensor)");
-    m.def("attend_backward(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, "
+    // the same with what rounding took off the output, for attend_backward
+    m.def("attend_forward(Tensor q, Tensor k, Tensor v, Tensor? slopes=None, "
+          "Tensor? q_positions=None, Tensor? k_positions=None, Tensor? q_docs=None, "
+          "Tensor? k_docs=None, Tensor? prefix=None, Tensor? lengths=None, *, float scale, "
+          "float cap=0., bool causal=False) -> (Tensor, Tensor, Tensor)");
+    m.def("attend_backward(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, "
+          "Tensor out_low, Tensor lse, "
           "Tensor? slopes=None, Tensor? q_positions=None, Tensor? k_positions=None, "
           "Tensor? q_docs=None, Tensor? k_docs=None, Tensor? prefix=None, "
           "Tensor? lengths=None, *, float scale, float cap=0., bool causal=False) "
@@ -426,12 +463,14 @@ TORCH_LIBRARY(attention, m) {
 
 TORCH_LIBRARY_IMPL(attention, CUDA, m) {
     m.impl("attend", &attend_hip);
+    m.impl("attend_forward", &attend_forward_hip);
     m.impl("attend_backward", &attend_backward_hip);
     m.impl("rotate", &rotate_hip);
 }
 
 TORCH_LIBRARY_IMPL(attention, Autograd, m) {
     m.impl("attend", &attend_autograd);
+    m.impl("attend_forward", torch::autograd::autogradNotImplementedFallback());
     m.impl("attend_backward", torch::autograd::autogradNotImplementedFallback());
     m.impl("rotate", &rotate_autograd);
 }
