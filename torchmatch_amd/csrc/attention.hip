@@ -96,6 +96,11 @@ int check(const tm_attention *a) {
     for (int64_t s : strides)
         if (s % unit)
             return TM_ERR_INVALID_ARGUMENT;
+    // a tile's rows are reached by 32 bits from its first
+    const int64_t size = a->dtype == TM_F32 ? 4 : 2;
+    if (a->q_l < 0 || a->k_l < 0 || a->v_l < 0 ||
+        std::max({a->q_l, a->k_l, a->v_l}) * size >= TM_ATTENTION_MAX_ROW_BYTES)
+        return TM_ERR_UNSUPPORTED_SHAPE;
     if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) % 16)
         return TM_ERR_INVALID_ARGUMENT;
     return TM_OK;
@@ -213,6 +218,8 @@ extern "C" int tm_attention_backward(const tm_attention *a, const void *out,
         (a->Lk && (!a->k || !a->v || !dk || !dv)) || (uintptr_t)dout % 16 || do_b % unit ||
         do_l % unit || do_h % unit)
         return TM_ERR_INVALID_ARGUMENT;
+    if (do_l < 0 || do_l * (a->dtype == TM_F32 ? 4 : 2) >= TM_ATTENTION_MAX_ROW_BYTES)
+        return TM_ERR_UNSUPPORTED_SHAPE;
     const size_t need = tm_attention_backward_workspace_bytes(a);
     if (workspace_bytes < need || (need && !workspace))
         return TM_ERR_WORKSPACE;

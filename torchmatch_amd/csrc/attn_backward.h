@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256, 1) void attend_backward_q(const Args p) {
     const int block_limit = lim.of(min(q0 + 128, p.Lq) - 1);
     const int wave_limit = qw < p.Lq ? lim.of(min(qw + 32, p.Lq) - 1) : 0;
     const int full_limit = qw < p.Lq ? lim.of(qw) : 0;
-    const QueryLane<T> rows(p, lim, b, head, qi);
+    const QueryLane<T, true> rows(p, lim, b, head, qi);
     const bool q_real = qi < p.Lq && !(p.q_docs && rows.doc < 0);
 
     const T *q = (const T *)p.q + b * p.q_b + head * p.q_h + (q_real ? qi : 0) * p.q_l;
@@ -327,6 +327,7 @@ __global__ __launch_bounds__(256, 1) void attend_backward_q(const Args p) {
     float lse = qi < p.Lq ? p.lse[row] * kLog2e : kInf;
     lse = lse == -kInf ? kInf : lse; // an empty row: every weight 2^-inf
     const float delta = qi < p.Lq ? p.delta[row] : 0.f;
+    const float mul = rows.factor(p);
 
     constexpr int per64 = 64 / KT;
     int4 wave_docs = {0, 0, 0, 0};
@@ -412,7 +413,7 @@ __global__ __launch_bounds__(256, 1) void attend_backward_q(const Args p) {
             rows.score(p, s, &slant, k0 + 32 * kb, half, &s_pos[0][32 * kb], KT);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                ds[i] = __builtin_amdgcn_exp2f(s[i] - lse) * (ds[i] - delta);
+                ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], mul, -lse)) * (ds[i] - delta);
             if (p.cap > 0.f) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)

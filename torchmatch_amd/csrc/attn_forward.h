@@ -5,8 +5,8 @@
 // (k q^T), so that a lane holds scores of one query only: the running maximum
 // and sum need one exchange between the two halves of the wave, the rescaling
 // of the output is by a scalar per lane, and the weights lie as the next product
-// (v^T p^T) wants them.  q stays in registers; tiles of 64 keys pass through LDS,
-// brought by all four waves and the next one loaded while this one is used.
+// (v^T p^T) wants them.  q stays in registers; tiles of 64 keys pass through LDS in two
+// buffers, brought by all four waves, one on its way while the other is used.
 //
 // Weights are rounded to the inputs' type for the second product, as they lie
 // between 0 and 2^8 and every weight of a row errs by as much, relatively, as an
@@ -26,16 +26,16 @@ template <typename T, int DP> struct ForwardShape {
     static constexpr int kOccupancy = sizeof(T) * DP <= 256 ? 2 : 1;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool SIDE>
 __global__ __launch_bounds__(256, (ForwardShape<T, DP>::kOccupancy)) void
 attend_forward(const Args p) {
     using S = ForwardShape<T, DP>;
     using L = Tile<T, DP>;
     constexpr int KT = S::kKeys, KB = KT / 32, QT = S::kQueries, C = DP / 16, DB = DP / 32;
-    __shared__ u32x4 sk[KT * L::U];
-    __shared__ u32x4 sv[KT * L::U];
-    __shared__ __attribute__((aligned(16))) int s_docs[KT];
-    __shared__ __attribute__((aligned(16))) float s_pos[3][KT];
+    __shared__ u32x4 sk0[KT * L::U], sk1[KT * L::U];
+    __shared__ u32x4 sv0[KT * L::U], sv1[KT * L::U];
+    __shared__ __attribute__((aligned(16))) int s_docs0[64], s_docs1[64];
+    __shared__ __attribute__((aligned(16))) float s_pos0[3][64], s_pos1[3][64];
 
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -60,9 +60,9 @@ attend_forward(const Args p) {
     const T *q = (const T *)p.q + b * p.q_b + head * p.q_h;
     const T *k = (const T *)p.k + b * p.k_b + kvh * p.k_h;
     const T *v = (const T *)p.v + b * p.v_b + kvh * p.v_h;
-    const int32_t *k_docs = p.k_docs ? p.k_docs + (int64_t)b * p.Lk : nullptr;
-    const float *k_pos = p.k_pos ? p.k_pos + (int64_t)b * p.Lk * p.axes : nullptr;
-    const QueryLane<T> rows(p, lim, b, head, qi);
+    const int32_t *k_docs = SIDE && p.k_docs ? p.k_docs + (int64_t)b * p.Lk : nullptr;
+    const float *k_pos = SIDE && p.k_pos ? p.k_pos + (int64_t)b * p.Lk * p.axes : nullptr;
+    const QueryLane<T, SIDE> rows(p, lim, b, head, qi);
 
     x8<T> qf[C];
 #pragma unroll
@@ -76,7 +76,7 @@ attend_forward(const Args p) {
     {
         const int64_t nk = (p.Lk + 63) / 64, nq = (p.Lq + 63) / 64;
         int4 mine = {0, 0, 0, 0};
-        if (p.q_tiles) {
+        if (SIDE && p.q_tiles) {
             const int4 *t = p.q_tiles + b * nq;
             mine = t[q0 / 64];
             if (q0 / 64 + 1 < nq) {
@@ -86,7 +86,7 @@ attend_forward(const Args p) {
             }
             wave_docs = qw < p.Lq ? t[qw / 64] : (int4){0x7fffffff, -1, 0, 0};
         }
-        walk.start(p.k_tiles ? p.k_tiles + b * nk : nullptr, mine, split * p.tiles_per_split,
+        walk.start(SIDE && p.k_tiles ? p.k_tiles + b * nk : nullptr, mine, split * p.tiles_per_split,
                    t_end, lane);
     }
 
@@ -96,74 +96,73 @@ attend_forward(const Args p) {
         o[i] = f32x16{};
     float top = -kInf, sum = 0.f; // of this lane's query; the sum of this half's keys
 
-    Stage<T, DP, KT, 256> gk, gv;
-    int g_doc = -1;
-    float g_pos[3];
+    using B = Bring<T, DP, KT, 256>;
     const int seen = min(block_limit, p.Lk); // keys past it may hold anything
-    auto fetch = [&](int k0) {
-        gk.load(k, p.k_l, k0, seen, p.D, k_docs, tid);
-        gv.load(v, p.v_l, k0, seen, p.D, k_docs, tid);
-        if (k_docs && tid < KT)
-            g_doc = k0 + tid < seen ? k_docs[k0 + tid] : -1;
-        if (k_pos && tid < KT)
-#pragma unroll
-            for (int a = 0; a < 3; ++a)
-                if (a < p.axes)
-                    g_pos[a] = k0 + tid < seen ? k_pos[(int64_t)(k0 + tid) * p.axes + a] : 0.f;
-    };
-
+    const float mul = rows.factor(p);
     int t64 = walk.next(lane), sub = 0;
-    if (t64 < t_end)
-        fetch(t64 * 64);
-    while (t64 < t_end) {
-        const int k0 = t64 * 64 + sub * KT;
-        __syncthreads();
-        gk.store(sk, tid);
-        gv.store(sv, tid);
-        if (k_docs && tid < KT)
-            s_docs[tid] = g_doc;
-        if (k_pos && tid < KT)
+
+    // The tile from key k0 on into a buffer.
+    auto fetch = [&](int k0, u32x4 *sk, u32x4 *sv, int *s_docs, float (*s_pos)[64]) {
+        B::load(sk, k, p.k_l, k0, seen, p.D, tid);
+        B::load(sv, v, p.v_l, k0, seen, p.D, tid);
+        if (SIDE && wave == 0) {
+            const int64_t j = min(k0 + lane, seen - 1);
+            if (k_docs)
+                bring_word(s_docs, k_docs + j);
+            if (k_pos) {
 #pragma unroll
-            for (int a = 0; a < 3; ++a)
-                if (a < p.axes)
-                    s_pos[a][tid] = g_pos[a];
-        __syncthreads();
-        const int this64 = t64;
-        if (++sub == per64) {
+                for (int a = 0; a < 3; ++a)
+                    if (a < p.axes)
+                        bring_word(s_pos[a], k_pos + j * p.axes + a);
+            }
+        }
+    };
+    // One tile from its buffer while the next one is on its way into the other.
+    auto step = [&](u32x4 *sk, u32x4 *sv, int *s_docs, float (*s_pos)[64], u32x4 *next_k,
+                    u32x4 *next_v, int *next_docs, float (*next_pos)[64]) {
+        const int k0 = t64 * 64 + sub * KT;
+        const int4 kd = walk.docs;
+        arrived();
+        __syncthreads(); // this tile is here, and the other buffer is done with
+        if (++sub == per64 || k0 + KT >= seen) { // no row of the second half may be there
             sub = 0;
             t64 = walk.next(lane);
         }
         if (t64 < t_end)
-            fetch(t64 * 64 + sub * KT);
+            fetch(t64 * 64 + sub * KT, next_k, next_v, next_docs, next_pos);
 
-        bool use = k0 < wave_limit, masked = k0 + KT > full_limit;
+        bool use = k0 < wave_limit, masked = k0 + KT > full_limit, dirty = k0 + KT > seen;
         if (k_docs) {
-            const int4 kd = p.k_tiles[(int64_t)b * ((p.Lk + 63) / 64) + this64];
             use = use && docs_meet(kd, wave_docs);
             masked = masked || !docs_same(kd, wave_docs);
+            dirty = dirty || kd.z;
+        }
+        if (dirty) { // the same for all waves
+            B::clear(sv, k0, seen, k_docs, s_docs, tid);
+            __syncthreads();
         }
         if (!use)
-            continue;
+            return;
 
         // scores: keys by queries
         f32x16 s[KB];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
+        for (int kb = 0; kb < KB; ++kb)
             s[kb] = f32x16{};
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
                 s[kb] = mma32(L::row8(sk, 32 * kb + (lane & 31), 2 * c + half), qf[c], s[kb]);
-        }
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
-            rows.score(p, s[kb], nullptr, k0 + 32 * kb, half, &s_pos[0][32 * kb], KT);
+            rows.score(p, s[kb], nullptr, k0 + 32 * kb, half, &s_pos[0][32 * kb], 64);
         if (masked) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
                 rows.hide(p, s[kb], -kInf, k0 + 32 * kb, half, s_docs + 32 * kb);
         }
-
-        soften<T>(s, o, top, sum);
+        soften<T>(s, o, mul, top, sum);
 
         // output, transposed: v^T p^T
 #pragma unroll
@@ -173,6 +172,21 @@ attend_forward(const Args p) {
             for (int i = 0; i < DB; ++i)
                 o[i] = mma32(L::col8(sv, 16 * t, i, lane), w, o[i]);
         }
+    };
+
+    B::pad(sk0, p.D, tid);
+    B::pad(sk1, p.D, tid);
+    B::pad(sv0, p.D, tid);
+    B::pad(sv1, p.D, tid);
+    if (p.D < DP)
+        __syncthreads();
+    if (t64 < t_end)
+        fetch(t64 * 64, sk0, sv0, s_docs0, s_pos0);
+    while (t64 < t_end) {
+        step(sk0, sv0, s_docs0, s_pos0, sk1, sv1, s_docs1, s_pos1);
+        if (t64 >= t_end)
+            break;
+        step(sk1, sv1, s_docs1, s_pos1, sk0, sv0, s_docs0, s_pos0);
     }
 
     sum += __shfl_xor(sum, 32);
@@ -265,7 +279,10 @@ template <typename T, int DP> int run_forward(const Args &a, hipStream_t s) {
     const int64_t blocks = (int64_t)((a.Lq + ForwardShape<T, DP>::kQueries - 1) /
                                      ForwardShape<T, DP>::kQueries) *
                            a.splits * a.H * a.B;
-    attend_forward<T, DP><<<dim3((unsigned)blocks), 256, 0, s>>>(a);
+    if (a.q_docs || a.q_pos)
+        attend_forward<T, DP, true><<<dim3((unsigned)blocks), 256, 0, s>>>(a);
+    else
+        attend_forward<T, DP, false><<<dim3((unsigned)blocks), 256, 0, s>>>(a);
     return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 

@@ -176,6 +176,68 @@ template <typename T, int DP, int ROWS, int NT> struct Stage {
     }
 };
 
+// A tile brought from memory straight into LDS by NT threads, without passing through
+// registers.  A wave's 64 units land next to each other, so the permutation of a row's units
+// is made on the side of the addresses: a scalar row and 32 bits a lane.  Features past the
+// d real ones are not brought: pad() zeroes their place once.  arrived() before the barrier
+// that lets others read.
+template <typename T, int DP, int ROWS, int NT> struct Bring {
+    using L = Tile<T, DP>;
+    static constexpr int N = ROWS * L::U / NT, STEP = NT / L::U; // rows from load to load
+    static_assert(ROWS * L::U % NT == 0 && NT % L::U == 0);
+
+    // rows row0 + 0 .. ROWS - 1 of a matrix of `rows` > row0 rows; those past the last repeat it
+    __device__ static inline void load(u32x4 *t, const T *base, int64_t stride, int row0, int rows,
+                                       int d, int tid) {
+        const int row = tid / L::U, pos = tid % L::U;
+        const int left = rows - row0;
+        u32x4 *to = t + __builtin_amdgcn_readfirstlane(tid & ~63);
+        const char *from = (const char *)(base + (int64_t)row0 * stride);
+        const uint32_t bytes = (uint32_t)stride * (uint32_t)sizeof(T);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int u = pos ^ L::swz(row + n * STEP);
+            const char *s = from;
+            uint32_t off;
+            if (left >= ROWS) {
+                s += (int64_t)n * STEP * stride * (int)sizeof(T);
+                off = (uint32_t)row * bytes + 16u * u;
+            } else {
+                off = (uint32_t)max(min(row + n * STEP, left - 1), 0) * bytes + 16u * u;
+            }
+            if ((L::U == L::U0 && d == DP) || u * L::E < d)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void *)(s + off),
+                    (__attribute__((address_space(3))) void *)(to + n * NT), 16, 0, 0);
+        }
+    }
+    __device__ static inline void pad(u32x4 *t, int d, int tid) {
+        if (d < DP) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                t[tid + n * NT] = u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+    // zeros in the rows that nobody may see: past `rows`, or of a negative document
+    __device__ static inline void clear(u32x4 *t, int row0, int rows, bool by_doc, const int *docs,
+                                        int tid) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int r = tid / L::U + n * STEP;
+            if (row0 + r >= rows || (by_doc && docs[r] < 0))
+                t[tid + n * NT] = u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+};
+
+// 64 words from memory into LDS by one wave, a word each lane
+__device__ inline void bring_word(void *to, const void *from) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                     (__attribute__((address_space(3))) void *)to, 4, 0, 0);
+}
+
+__device__ inline void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // 8 elements of a row in memory (a row operand that stays in registers)
 template <typename T>
 __device__ inline x8<T> global8(const T *row, int e, int d, bool valid) {
@@ -232,26 +294,32 @@ __device__ inline f32x4 away(f32x4 a, float b) {
 
 // One lane's query against results of k q^T, 32 keys a block: the scores in base 2, what the
 // lane may see.
-template <typename T> struct QueryLane {
+// SIDE: there may be documents or positions (without them a kernel needs fewer registers).
+template <typename T, bool SIDE> struct QueryLane {
     int limit, doc, at;
     float slope, pos[3];
 
     __device__ inline QueryLane(const Args &p, const Limits &lim, int b, int head, int i) {
         const bool real = i < p.Lq;
         limit = real ? lim.of(i) : 0;
-        doc = p.q_docs && real ? p.q_docs[(int64_t)b * p.Lq + i] : -1;
+        doc = SIDE && p.q_docs && real ? p.q_docs[(int64_t)b * p.Lq + i] : -1;
         at = i + lim.offset;
         slope = p.slopes ? p.slopes[head] * kLog2e : 0.f;
         pos[0] = pos[1] = pos[2] = 0.f;
-        if (p.q_pos && real)
+        if (SIDE && p.q_pos && real)
 #pragma unroll
             for (int a = 0; a < 3; ++a)
                 if (a < p.axes)
                     pos[a] = p.q_pos[((int64_t)b * p.Lq + i) * p.axes + a];
     }
 
-    // s: products with keys k0 ..; to scores times log2 e.  With `grad`, the derivative of
-    // the cap too.  k_pos: the block's positions in LDS, `axis` apart.
+    // What scores must be multiplied with after score(): plain products wait for the
+    // exponential, which takes the factor along.
+    __device__ static inline float factor(const Args &p) {
+        return p.cap > 0.f || p.slopes || p.scale < 0.f ? 1.f : p.scale * kLog2e;
+    }
+    // s: products with keys k0 ..; to scores times log2 e but for factor().  With `grad`, the
+    // derivative of the cap too.  k_pos: the block's positions in LDS, `axis` apart.
     __device__ inline void score(const Args &p, f32x16 &s, f32x16 *grad, int k0, int half,
                                  const float *k_pos, int axis) const {
         if (p.cap > 0.f) {
@@ -263,13 +331,13 @@ template <typename T> struct QueryLane {
                     (*grad)[i] = fmaf(-t, t, 1.f);
                 s[i] = out * t;
             }
-        } else {
+        } else if (p.slopes || p.scale < 0.f) {
             const float m = p.scale * kLog2e;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 s[i] *= m;
         }
-        if (p.q_pos) {
+        if (SIDE && p.q_pos) {
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 const int j = 8 * n + 4 * half;
@@ -293,7 +361,7 @@ template <typename T> struct QueryLane {
     __device__ inline void hide(const Args &p, f32x16 &s, float x, int k0, int half,
                                 const int *docs) const {
         const int last = limit - k0 - 4 * half;
-        if (p.k_docs) {
+        if (SIDE && p.k_docs) {
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 const i32x4 d = *(const i32x4 *)(docs + 8 * n + 4 * half);
@@ -317,19 +385,33 @@ template <typename T> constexpr float weight_shift() {
     return __is_same(T, _Float16) ? 7.f : 0.f;
 }
 
-// One step of the running softmax: scores s (base 2, keys by queries) become weights
-// 2^(s - top).  `top` follows the largest score seen only when that grew by more than
-// 2^8: weights up to 2^8 cost no precision in float32 sums, and the output is rarely rescaled.
-// `sum` adds this lane's half of the keys.
+// One step of the running softmax: scores s (keys by queries), which times mul >= 0 are in
+// base 2, become weights 2^(s mul - top).  `top` follows the largest score seen only when that
+// grew by more than 2^8: weights up to 2^8 cost no precision in float32 sums, and the output
+// is rarely rescaled.  `sum` adds this lane's half of the keys.
 template <typename T, int KB, int DB>
-__device__ inline void soften(f32x16 (&s)[KB], f32x16 (&o)[DB], float &top, float &sum) {
+__device__ inline void soften(f32x16 (&s)[KB], f32x16 (&o)[DB], float mul, float &top,
+                              float &sum) {
     float m = s[0][0];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             m = fmaxf(m, s[kb][i]);
-    m = fmaxf(m, __shfl_xor(m, 32)) - weight_shift<T>();
+    m = fmaxf(m, __shfl_xor(m, 32));
+    // s mul - top in one rounding leaves the rounding of top in the weights, all of a row by
+    // the same factor; past 2^11 that would show in 16 bits, so there products come first and
+    // the largest weight stays a power of two
+    if (__any(fabsf(m) * mul > 2048.f)) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                s[kb][i] *= mul;
+        m *= mul;
+        mul = 1.f;
+    }
+    m = m == -kInf ? m : fmaf(m, mul, -weight_shift<T>());
     if (__any(m > top + 8.f)) {
         const float now = fmaxf(m, top);
         const float r = now == -kInf ? 1.f : __builtin_amdgcn_exp2f(top - now);
@@ -342,13 +424,15 @@ __device__ inline void soften(f32x16 (&s)[KB], f32x16 (&o)[DB], float &top, floa
                 o[i][e] *= r;
     }
     const float from = top == -kInf ? 0.f : top;
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            s[kb][i] = __builtin_amdgcn_exp2f(s[kb][i] - from);
-            sum += s[kb][i];
+            s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], mul, -from));
+            part[i % 4] += s[kb][i];
         }
+    sum += (part[0] + part[1]) + (part[2] + part[3]);
 }
 
 // A result in the outputs' type, and what the rounding took off (for the gradient)
@@ -371,12 +455,13 @@ __device__ inline bool docs_same(int4 a, int4 b) {
 }
 
 // Walks the tiles of 64 rows in [t, end) that can hold something to see: all of them, or
-// those whose documents meet `mine`.
+// those whose documents meet `mine`.  A lane holds the summary of one tile of 64.
 struct TileWalk {
     const int4 *tiles;
     int4 mine;
     int base, end;
     uint64_t left;
+    int4 held, docs; // docs: of the tile that next() gave
 
     __device__ inline void start(const int4 *tiles_, int4 mine_, int t, int end_, int lane) {
         tiles = tiles_;
@@ -384,13 +469,15 @@ struct TileWalk {
         base = t;
         end = end_;
         left = 0;
+        held = docs = int4{0, 0, 0, 0};
         if (tiles)
             fill(lane);
     }
     __device__ inline void fill(int lane) {
         for (left = 0; base < end; base += 64) {
             const int i = base + lane;
-            left = __ballot(i < end && docs_meet(tiles[min(i, end - 1)], mine));
+            held = tiles[min(i, end - 1)];
+            left = __ballot(i < end && docs_meet(held, mine));
             if (left)
                 return;
         }
@@ -401,7 +488,10 @@ struct TileWalk {
             return base < end ? base++ : end;
         if (!left)
             return end;
-        const int t = base + __builtin_ctzll(left);
+        const int i = __builtin_ctzll(left), t = base + i;
+        docs.x = __builtin_amdgcn_readlane(held.x, i);
+        docs.y = __builtin_amdgcn_readlane(held.y, i);
+        docs.z = __builtin_amdgcn_readlane(held.z, i);
         left &= left - 1;
         if (!left) {
             base += 64;

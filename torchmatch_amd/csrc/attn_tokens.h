@@ -61,7 +61,7 @@ attend_tokens(const Args p) {
     const int head = kvh * group + (q_real ? r / p.Lq : 0);
     const Limits lim(p, b);
     const int all_limit = lim.of(p.Lq - 1), full_limit = lim.of(0);
-    const QueryLane<T> rows(p, lim, b, head, qi);
+    const QueryLane<T, true> rows(p, lim, b, head, qi);
 
     const T *q = (const T *)p.q + b * p.q_b + head * p.q_h;
     const T *k = (const T *)p.k + b * p.k_b + kvh * p.k_h;
@@ -143,7 +143,7 @@ attend_tokens(const Args p) {
         wave_fence();
         bool masked = k0 + 32 > full_limit;
         if (k_tiles)
-            masked = masked || !docs_same(k_tiles[t64], mine);
+            masked = masked || !docs_same(walk.docs, mine);
         sub ^= 1;
         if (!sub || k0 + 32 >= seen) {
             sub = 0;
@@ -159,7 +159,7 @@ attend_tokens(const Args p) {
         rows.score(p, s[0], nullptr, k0, half, &s_pos[wave][0][0], 32);
         if (masked)
             rows.hide(p, s[0], -kInf, k0, half, s_docs[wave]);
-        soften<T>(s, o, top, sum);
+        soften<T>(s, o, rows.factor(p), top, sum);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const x8<T> w = pack8<T>(s[0], t);

@@ -53,7 +53,8 @@ Tensor readable(const Tensor &t) {
     if (d % unit)
         return at::constant_pad_nd(t, {0, unit - d % unit}).contiguous();
     const bool ok = (d == 1 || t.stride(3) == 1) && step_of(t, 0) % unit == 0 &&
-                    step_of(t, 1) % unit == 0 && step_of(t, 2) % unit == 0 &&
+                    step_of(t, 1) % unit == 0 &&
+                    step_of(t, 1) * t.element_size() < TM_ATTENTION_MAX_ROW_BYTES && step_of(t, 2) % unit == 0 &&
                     reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
     return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
