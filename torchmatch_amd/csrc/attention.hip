@@ -201,7 +201,7 @@ extern "C" int tm_attention_forward(const tm_attention *a, void *out, void *out_
 extern "C" size_t tm_attention_backward_workspace_bytes(const tm_attention *a) {
     if (check(a) != TM_OK)
         return 0;
-    return docs_bytes(a) + align256((size_t)a->B * a->H * a->Lq * sizeof(float));
+    return docs_bytes(a) + 2 * align256((size_t)a->B * a->H * a->Lq * sizeof(float));
 }
 
 extern "C" int tm_attention_backward(const tm_attention *a, const void *out,
@@ -226,7 +226,6 @@ extern "C" int tm_attention_backward(const tm_attention *a, const void *out,
     Args p = args_of(a);
     p.out = const_cast<void *>(out);
     p.out_low = a->dtype == TM_F32 ? nullptr : const_cast<void *>(out_low);
-    p.lse = const_cast<float *>(lse);
     p.dout = dout;
     p.do_b = do_b, p.do_l = do_l, p.do_h = do_h;
     p.dq = dq, p.dk = dk, p.dv = dv;
@@ -234,9 +233,12 @@ extern "C" int tm_attention_backward(const tm_attention *a, const void *out,
     if (summarise_docs(a, p, ws, stream))
         return TM_ERR_LAUNCH;
     float *delta = (float *)(ws + docs_bytes(a));
+    float *base2 = (float *)((char *)delta +
+                             align256((size_t)a->B * a->H * a->Lq * sizeof(float)));
     p.delta = delta;
+    p.lse = base2;
     const int dp = padded(a->D);
-    if (a->Lq && ATTN_BY_TYPE(delta, p, delta, stream))
+    if (a->Lq && ATTN_BY_TYPE(delta, p, lse, base2, delta, stream))
         return TM_ERR_LAUNCH;
     if (a->Lk && ATTN_BY_TYPE(backward_kv, p, dp, stream))
         return TM_ERR_LAUNCH;

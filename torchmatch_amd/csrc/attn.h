@@ -11,7 +11,7 @@ namespace attn {
 struct Args {
     const void *q, *k, *v, *dout;
     void *out, *out_low, *dq, *dk, *dv; // contiguous (B, L, heads, D); out_low may be null
-    float *lse;               // (B, H, Lq), natural logarithm, -inf for empty rows
+    float *lse; // (B, H, Lq), natural logarithm, -inf for empty rows; backward: base 2, +inf
     const float *delta;       // (B, H, Lq): sum over d of out * dout
     const float *slopes;      // (H) or null
     const float *q_pos, *k_pos; // (B, L, axes), or null: distance of indices
@@ -35,7 +35,7 @@ struct Args {
     int join_##type(const Args &, int dp, hipStream_t);                                           \
     int backward_kv_##type(const Args &, int dp, hipStream_t);                                    \
     int backward_q_##type(const Args &, int dp, hipStream_t);                                     \
-    int delta_##type(const Args &, float *delta, hipStream_t);
+    int delta_##type(const Args &, const float *lse, float *base2, float *delta, hipStream_t);
 ATTN_DECLARE(bf16)
 ATTN_DECLARE(f16)
 ATTN_DECLARE(f32)

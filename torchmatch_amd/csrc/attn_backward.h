@@ -22,18 +22,21 @@ template <typename T, int DP> struct BackwardShape {
     static constexpr int kRows = sizeof(T) == 4 && DP == 256 ? 32 : 64; // rows of a tile in LDS
     // float32 rows of 256: dk and dv by a pass each, the registers hold one of them
     static constexpr bool kTwoPasses = sizeof(T) == 4 && DP == 256;
+    static constexpr int kOccupancy = sizeof(T) * DP <= 256 ? 2 : 1;
 };
 
 // WHICH: 1 dv, 2 dk, 3 both
-template <typename T, int DP, int WHICH>
+template <typename T, int DP, bool SIDE, int WHICH>
 __global__ __launch_bounds__(256, 1) void attend_backward_kv(const Args p) {
     using L = Tile<T, DP>;
     constexpr int QT = BackwardShape<T, DP>::kRows, QB = QT / 32, C = DP / 16, DB = DP / 32;
     constexpr bool DV = WHICH & 1, DK = WHICH & 2;
-    __shared__ u32x4 sq[QT * L::U];
-    __shared__ u32x4 sdo[QT * L::U];
-    __shared__ __attribute__((aligned(16))) float s_lse[QT], s_delta[QT], s_pos[3][QT];
-    __shared__ __attribute__((aligned(16))) int s_limit[QT], s_doc[QT];
+    using B = Bring<T, DP, QT, 256>;
+    __shared__ u32x4 sq0[QT * L::U], sq1[QT * L::U];
+    __shared__ u32x4 so0[QT * L::U], so1[QT * L::U];
+    // of the tile's queries: the log of the sum (base 2), delta, positions; documents
+    __shared__ __attribute__((aligned(16))) float s_row0[5][64], s_row1[5][64];
+    __shared__ __attribute__((aligned(16))) int s_docs0[64], s_docs1[64];
 
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -45,8 +48,12 @@ __global__ __launch_bounds__(256, 1) void attend_backward_kv(const Args p) {
     const int kvh = id % p.Hkv, b = id / p.Hkv;
     const int k0 = 128 * kb, kw = k0 + 32 * wave, kj = kw + (lane & 31);
     const Limits lim(p, b);
-    const int my_doc = p.k_docs && kj < p.Lk ? p.k_docs[(int64_t)b * p.Lk + kj] : -1;
-    const bool k_real = kj < lim.length && !(p.k_docs && my_doc < 0);
+    const int my_doc = SIDE && p.k_docs && kj < p.Lk ? p.k_docs[(int64_t)b * p.Lk + kj] : -1;
+    const bool k_real = kj < lim.length && !(SIDE && p.k_docs && my_doc < 0);
+    // the first query that sees this lane's key; the last that must be asked for
+    const int my_first = !k_real ? 0x7fffffff
+                         : lim.causal && kj >= lim.prefix ? max(0, kj - lim.offset)
+                                                          : 0;
 
     const T *k = (const T *)p.k + b * p.k_b + kvh * p.k_h + (k_real ? kj : 0) * p.k_l;
     const T *v = (const T *)p.v + b * p.v_b + kvh * p.v_h + (k_real ? kj : 0) * p.v_l;
@@ -58,7 +65,7 @@ __global__ __launch_bounds__(256, 1) void attend_backward_kv(const Args p) {
             vf[c] = global8<T>(v, 16 * c + 8 * half, p.D, k_real);
     }
     float my_pos[3] = {0.f, 0.f, 0.f};
-    if (p.k_pos && kj < p.Lk)
+    if (SIDE && p.k_pos && kj < p.Lk)
 #pragma unroll
         for (int a = 0; a < 3; ++a)
             if (a < p.axes)
@@ -72,9 +79,11 @@ __global__ __launch_bounds__(256, 1) void attend_backward_kv(const Args p) {
         first = min(p.Lq, max(0, k0 - lim.offset));
     const int nq = (p.Lq + 63) / 64, nk = (p.Lk + 63) / 64;
     const int t_end = first < p.Lq ? nq : 0;
-    const int4 *q_tiles = p.q_tiles ? p.q_tiles + (int64_t)b * nq : nullptr;
+    const int4 *q_tiles = SIDE && p.q_tiles ? p.q_tiles + (int64_t)b * nq : nullptr;
+    const int32_t *q_docs = SIDE && p.q_docs ? p.q_docs + (int64_t)b * p.Lq : nullptr;
+    const float *q_pos = SIDE && p.q_pos ? p.q_pos + (int64_t)b * p.Lq * p.axes : nullptr;
     int4 mine = {0, 0, 0, 0}, wave_docs = {0, 0, 0, 0};
-    if (p.k_tiles) {
+    if (SIDE && p.k_tiles) {
         const int4 *t = p.k_tiles + (int64_t)b * nk;
         mine = t[k0 / 64];
         if (k0 / 64 + 1 < nk) {
@@ -84,6 +93,7 @@ __global__ __launch_bounds__(256, 1) void attend_backward_kv(const Args p) {
         }
         wave_docs = kw < p.Lk ? t[kw / 64] : (int4){0x7fffffff, -1, 0, 0};
     }
+    const float factor = QueryLane<T, SIDE>::factor(p);
 
     f32x16 dk[DB], dv[DB];
 #pragma unroll
@@ -92,173 +102,179 @@ __global__ __launch_bounds__(256, 1) void attend_backward_kv(const Args p) {
         dv[i] = f32x16{};
     }
 
-    for (int g = 0; g < group; ++g) {
-        const int head = kvh * group + g;
-        const T *q = (const T *)p.q + b * p.q_b + head * p.q_h;
-        const T *dout = (const T *)p.dout + b * p.do_b + head * p.do_h;
-        const int64_t row = ((int64_t)b * p.H + head) * p.Lq;
-        const int32_t *q_docs = p.q_docs ? p.q_docs + (int64_t)b * p.Lq : nullptr;
+    // the tiles of one query head after the other's: at head g, tile (t64, sub)
+    int g = 0, t64, sub = 0;
+    TileWalk walk;
+    auto advance = [&]() {
+        t64 = walk.next(lane);
+        while (t64 >= t_end && g + 1 < group) {
+            ++g;
+            walk.start(q_tiles, mine, first / 64, t_end, lane);
+            t64 = walk.next(lane);
+        }
+    };
+    auto fetch = [&](u32x4 *sq, u32x4 *so, float (*s_row)[64], int *s_docs) {
+        const int q0 = t64 * 64 + sub * QT, head = kvh * group + g;
+        B::load(sq, (const T *)p.q + b * p.q_b + head * p.q_h, p.q_l, q0, p.Lq, p.D, tid);
+        B::load(so, (const T *)p.dout + b * p.do_b + head * p.do_h, p.do_l, q0, p.Lq, p.D, tid);
+        const int i = min(q0 + lane, p.Lq - 1);
+        const int64_t row = ((int64_t)b * p.H + head) * p.Lq + i;
+        if (wave == 0) {
+            bring_word(s_row[0], p.lse + row);
+            if (DK)
+                bring_word(s_row[1], p.delta + row);
+        } else if (SIDE && wave == 1) {
+            if (q_docs)
+                bring_word(s_docs, q_docs + i);
+            if (q_pos) {
+#pragma unroll
+                for (int a = 0; a < 3; ++a)
+                    if (a < p.axes)
+                        bring_word(s_row[2 + a], q_pos + (int64_t)i * p.axes + a);
+            }
+        }
+    };
+    auto step = [&](u32x4 *sq, u32x4 *so, float (*s_row)[64], int *s_docs, u32x4 *next_q,
+                    u32x4 *next_o, float (*next_row)[64], int *next_docs) {
+        const int q0 = t64 * 64 + sub * QT, head = kvh * group + g;
+        const int4 qd = walk.docs;
+        arrived();
+        __syncthreads(); // this tile is here, and the other buffer is done with
+        if (++sub == 64 / QT || q0 + QT >= p.Lq) {
+            sub = 0;
+            advance();
+        }
+        if (t64 < t_end)
+            fetch(next_q, next_o, next_row, next_docs);
+
+        const int last = min(q0 + QT, p.Lq) - 1;
+        bool use = kw < lim.of(last), dirty = q0 + QT > p.Lq;
+        bool masked = kw + 32 > lim.of(q0) || q0 + QT > p.Lq;
+        if (q_docs) {
+            use = use && docs_meet(qd, wave_docs);
+            masked = masked || !docs_same(qd, wave_docs);
+            dirty = dirty || qd.z;
+        }
+        if (dirty) { // the same for all waves
+            B::clear(sq, q0, p.Lq, q_docs, s_docs, tid);
+            B::clear(so, q0, p.Lq, q_docs, s_docs, tid);
+            __syncthreads();
+        }
+        if (!use)
+            return;
         const float slope = p.slopes ? p.slopes[head] * kLog2e : 0.f;
 
-        Stage<T, DP, QT, 256> gq, gdo;
-        float g_lse = 0.f, g_delta = 0.f, g_pos[3];
-        int g_doc = -1;
-        auto fetch = [&](int q0) {
-            gq.load(q, p.q_l, q0, p.Lq, p.D, q_docs, tid);
-            gdo.load(dout, p.do_l, q0, p.Lq, p.D, q_docs, tid);
-            if (tid < QT) {
-                const int i = q0 + tid;
-                const bool real = i < p.Lq;
-                g_lse = real ? p.lse[row + i] * kLog2e : -kInf;
-                g_delta = real ? p.delta[row + i] : 0.f;
-                g_doc = q_docs && real ? q_docs[i] : -1;
-                if (p.q_pos)
-#pragma unroll
-                    for (int a = 0; a < 3; ++a)
-                        if (a < p.axes)
-                            g_pos[a] = real ? p.q_pos[((int64_t)b * p.Lq + i) * p.axes + a] : 0.f;
-            }
-        };
-
-        TileWalk walk;
-        walk.start(q_tiles, mine, first / 64, t_end, lane);
-        constexpr int per64 = 64 / QT;
-        int t64 = walk.next(lane), sub = 0;
-        if (t64 < t_end)
-            fetch(t64 * 64);
-        while (t64 < t_end) {
-            const int q0 = t64 * 64 + sub * QT;
-            __syncthreads();
-            gq.store(sq, tid);
-            gdo.store(sdo, tid);
-            if (tid < QT) {
-                // an empty row: every weight 2^-inf
-                s_lse[tid] = g_lse == -kInf ? kInf : g_lse;
-                s_delta[tid] = g_delta;
-                s_limit[tid] = q0 + tid < p.Lq ? lim.of(q0 + tid) : 0;
-                s_doc[tid] = g_doc;
-                if (p.q_pos)
-#pragma unroll
-                    for (int a = 0; a < 3; ++a)
-                        if (a < p.axes)
-                            s_pos[a][tid] = g_pos[a];
-            }
-            __syncthreads();
-            const int this64 = t64;
-            if (++sub == per64) {
-                sub = 0;
-                t64 = walk.next(lane);
-            }
-            if (t64 < t_end)
-                fetch(t64 * 64 + sub * QT);
-
-            const int last = min(q0 + QT, p.Lq) - 1;
-            if (last < q0)
-                continue;
-            bool use = kw < lim.of(last);
-            bool masked = kw + 32 > lim.of(q0) || q0 + QT > p.Lq;
-            if (q_tiles) {
-                use = use && docs_meet(q_tiles[this64], wave_docs);
-                masked = masked || !docs_same(q_tiles[this64], wave_docs);
-            }
-            if (!use)
-                continue;
-
 #pragma unroll 1
-            for (int qb = 0; qb < QB; ++qb) {
-                f32x16 s = {}, ds = {};
+        for (int qb = 0; qb < QB; ++qb) {
+            f32x16 s = {}, ds = {};
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    s = mma32(L::row8(sq, 32 * qb + (lane & 31), 2 * c + half), kf[c], s);
-                    if constexpr (DK)
-                        ds = mma32(L::row8(sdo, 32 * qb + (lane & 31), 2 * c + half), vf[c], ds);
+            for (int c = 0; c < C; ++c) {
+                s = mma32(L::row8(sq, 32 * qb + (lane & 31), 2 * c + half), kf[c], s);
+                if constexpr (DK)
+                    ds = mma32(L::row8(so, 32 * qb + (lane & 31), 2 * c + half), vf[c], ds);
+            }
+            f32x16 slant;
+            if (p.cap > 0.f) {
+                const float in = p.scale / p.cap, out = p.cap * kLog2e;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float t = cap_tanh<T>(s[i] * in);
+                    slant[i] = fmaf(-t, t, 1.f);
+                    s[i] = out * t;
                 }
-                f32x16 slant;
-                if (p.cap > 0.f) {
-                    const float in = p.scale / p.cap, out = p.cap * kLog2e;
+            } else if (factor == 1.f) {
+                const float m = p.scale * kLog2e;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float t = cap_tanh<T>(s[i] * in);
-                        slant[i] = fmaf(-t, t, 1.f);
-                        s[i] = out * t;
-                    }
-                } else {
-                    const float m = p.scale * kLog2e;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[i] *= m;
-                }
-                if (p.q_pos) {
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const int j = 32 * qb + 8 * n + 4 * half;
-                        f32x4 dist = away(*(const f32x4 *)(s_pos[0] + j), my_pos[0]);
-                        if (p.axes > 1)
-                            dist += away(*(const f32x4 *)(s_pos[1] + j), my_pos[1]);
-                        if (p.axes > 2)
-                            dist += away(*(const f32x4 *)(s_pos[2] + j), my_pos[2]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            s[4 * n + e] = fmaf(-slope, dist[e], s[4 * n + e]);
-                    }
-                } else if (p.slopes) {
-                    const float from = (float)(q0 + 32 * qb + 4 * half + lim.offset - kj);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[i] = fmaf(-slope, fabsf(from + (float)(8 * (i / 4) + i % 4)), s[i]);
-                }
+                for (int i = 0; i < 16; ++i)
+                    s[i] *= m;
+            }
+            if (SIDE && q_pos) {
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
                     const int j = 32 * qb + 8 * n + 4 * half;
-                    const f32x4 lse = *(const f32x4 *)(s_lse + j);
-                    const f32x4 delta = *(const f32x4 *)(s_delta + j);
+                    f32x4 dist = away(*(const f32x4 *)(s_row[2] + j), my_pos[0]);
+                    if (p.axes > 1)
+                        dist += away(*(const f32x4 *)(s_row[3] + j), my_pos[1]);
+                    if (p.axes > 2)
+                        dist += away(*(const f32x4 *)(s_row[4] + j), my_pos[2]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[4 * n + e] = fmaf(-slope, dist[e], s[4 * n + e]);
+                }
+            } else if (p.slopes) {
+                const float from = (float)(q0 + 32 * qb + 4 * half + lim.offset - kj);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[i] = fmaf(-slope, fabsf(from + (float)(8 * (i / 4) + i % 4)), s[i]);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const int j = 32 * qb + 8 * n + 4 * half;
+                const f32x4 lse = *(const f32x4 *)(s_row[0] + j);
+                const f32x4 delta = *(const f32x4 *)(s_row[1] + j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 4 * n + e;
+                    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], factor, -lse[e]));
+                    if constexpr (DK)
+                        ds[i] = s[i] * (ds[i] - delta[e]);
+                }
+            }
+            if (DK && p.cap > 0.f) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    ds[i] *= slant[i];
+            }
+            if (masked) {
+                const int row0 = q0 + 32 * qb + 4 * half;
+                const int from = my_first - row0, to = p.Lq - row0;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    i32x4 doc = {my_doc, my_doc, my_doc, my_doc};
+                    if (SIDE && q_docs)
+                        doc = *(const i32x4 *)(s_docs + 32 * qb + 8 * n + 4 * half);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int i = 4 * n + e;
-                        s[i] = __builtin_amdgcn_exp2f(s[i] - lse[e]);
-                        if constexpr (DK)
-                            ds[i] = s[i] * (ds[i] - delta[e]);
-                    }
-                }
-                if (DK && p.cap > 0.f) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        ds[i] *= slant[i];
-                }
-                if (masked) {
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const int j = 32 * qb + 8 * n + 4 * half;
-                        const i32x4 limit = *(const i32x4 *)(s_limit + j);
-                        i32x4 doc = {my_doc, my_doc, my_doc, my_doc};
-                        if (q_docs)
-                            doc = *(const i32x4 *)(s_doc + j);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const bool see = (kj < limit[e]) & (doc[e] == my_doc) &
-                                             (my_doc >= 0 || !q_docs);
-                            s[4 * n + e] = see ? s[4 * n + e] : 0.f;
-                            ds[4 * n + e] = see ? ds[4 * n + e] : 0.f;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if constexpr (DV) {
-                        const x8<T> w = pack8<T>(s, t);
-#pragma unroll
-                        for (int i = 0; i < DB; ++i)
-                            dv[i] = mma32(L::col8(sdo, 32 * qb + 16 * t, i, lane), w, dv[i]);
-                    }
-                    if constexpr (DK) {
-                        const x8<T> w = pack8<T>(ds, t);
-#pragma unroll
-                        for (int i = 0; i < DB; ++i)
-                            dk[i] = mma32(L::col8(sq, 32 * qb + 16 * t, i, lane), w, dk[i]);
+                        const bool see =
+                            (8 * n + e >= from) & (8 * n + e < to) & (doc[e] == my_doc);
+                        s[4 * n + e] = see ? s[4 * n + e] : 0.f;
+                        ds[4 * n + e] = see ? ds[4 * n + e] : 0.f;
                     }
                 }
             }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if constexpr (DV) {
+                    const x8<T> w = pack8<T>(s, t);
+#pragma unroll
+                    for (int i = 0; i < DB; ++i)
+                        dv[i] = mma32(L::col8(so, 32 * qb + 16 * t, i, lane), w, dv[i]);
+                }
+                if constexpr (DK) {
+                    const x8<T> w = pack8<T>(ds, t);
+#pragma unroll
+                    for (int i = 0; i < DB; ++i)
+                        dk[i] = mma32(L::col8(sq, 32 * qb + 16 * t, i, lane), w, dk[i]);
+                }
+            }
         }
+    };
+
+    B::pad(sq0, p.D, tid);
+    B::pad(sq1, p.D, tid);
+    B::pad(so0, p.D, tid);
+    B::pad(so1, p.D, tid);
+    if (p.D < DP)
+        __syncthreads();
+    walk.start(q_tiles, mine, first / 64, t_end, lane);
+    advance();
+    if (t64 < t_end)
+        fetch(sq0, so0, s_row0, s_docs0);
+    while (t64 < t_end) {
+        step(sq0, so0, s_row0, s_docs0, sq1, so1, s_row1, s_docs1);
+        if (t64 >= t_end)
+            break;
+        step(sq1, so1, s_row1, s_docs1, sq0, so0, s_row0, s_docs0);
     }
 
     if (kj >= p.Lk)
@@ -284,14 +300,16 @@ __global__ __launch_bounds__(256, 1) void attend_backward_kv(const Args p) {
         }
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(256, 1) void attend_backward_q(const Args p) {
+template <typename T, int DP, bool SIDE>
+__global__ __launch_bounds__(256, (BackwardShape<T, DP>::kOccupancy)) void
+attend_backward_q(const Args p) {
     using L = Tile<T, DP>;
     constexpr int KT = BackwardShape<T, DP>::kRows, KB = KT / 32, C = DP / 16, DB = DP / 32;
-    __shared__ u32x4 sk[KT * L::U];
-    __shared__ u32x4 sv[KT * L::U];
-    __shared__ __attribute__((aligned(16))) int s_docs[KT];
-    __shared__ __attribute__((aligned(16))) float s_pos[3][KT];
+    using B = Bring<T, DP, KT, 256>;
+    __shared__ u32x4 sk0[KT * L::U], sk1[KT * L::U];
+    __shared__ u32x4 sv0[KT * L::U], sv1[KT * L::U];
+    __shared__ __attribute__((aligned(16))) int s_docs0[64], s_docs1[64];
+    __shared__ __attribute__((aligned(16))) float s_pos0[3][64], s_pos1[3][64];
 
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -307,15 +325,15 @@ __global__ __launch_bounds__(256, 1) void attend_backward_q(const Args p) {
     const int block_limit = lim.of(min(q0 + 128, p.Lq) - 1);
     const int wave_limit = qw < p.Lq ? lim.of(min(qw + 32, p.Lq) - 1) : 0;
     const int full_limit = qw < p.Lq ? lim.of(qw) : 0;
-    const QueryLane<T, true> rows(p, lim, b, head, qi);
-    const bool q_real = qi < p.Lq && !(p.q_docs && rows.doc < 0);
+    const QueryLane<T, SIDE> rows(p, lim, b, head, qi);
+    const bool q_real = qi < p.Lq && !(SIDE && p.q_docs && rows.doc < 0);
 
     const T *q = (const T *)p.q + b * p.q_b + head * p.q_h + (q_real ? qi : 0) * p.q_l;
     const T *dout = (const T *)p.dout + b * p.do_b + head * p.do_h + (q_real ? qi : 0) * p.do_l;
     const T *k = (const T *)p.k + b * p.k_b + kvh * p.k_h;
     const T *v = (const T *)p.v + b * p.v_b + kvh * p.v_h;
-    const int32_t *k_docs = p.k_docs ? p.k_docs + (int64_t)b * p.Lk : nullptr;
-    const float *k_pos = p.k_pos ? p.k_pos + (int64_t)b * p.Lk * p.axes : nullptr;
+    const int32_t *k_docs = SIDE && p.k_docs ? p.k_docs + (int64_t)b * p.Lk : nullptr;
+    const float *k_pos = SIDE && p.k_pos ? p.k_pos + (int64_t)b * p.Lk * p.axes : nullptr;
 
     x8<T> qf[C], of[C];
 #pragma unroll
@@ -324,20 +342,18 @@ __global__ __launch_bounds__(256, 1) void attend_backward_q(const Args p) {
         of[c] = global8<T>(dout, 16 * c + 8 * half, p.D, q_real);
     }
     const int64_t row = ((int64_t)b * p.H + head) * p.Lq + qi;
-    float lse = qi < p.Lq ? p.lse[row] * kLog2e : kInf;
-    lse = lse == -kInf ? kInf : lse; // an empty row: every weight 2^-inf
+    const float lse = qi < p.Lq ? p.lse[row] : kInf;
     const float delta = qi < p.Lq ? p.delta[row] : 0.f;
     const float mul = rows.factor(p);
 
     constexpr int per64 = 64 / KT;
     int4 wave_docs = {0, 0, 0, 0};
     const int64_t nk = (p.Lk + 63) / 64, nq = (p.Lq + 63) / 64;
-    const int4 *k_tiles = p.k_tiles ? p.k_tiles + b * nk : nullptr;
     const int t_end = (block_limit + 63) / 64;
     TileWalk walk;
     {
         int4 mine = {0, 0, 0, 0};
-        if (p.q_tiles) {
+        if (SIDE && p.q_tiles) {
             const int4 *t = p.q_tiles + b * nq;
             mine = t[q0 / 64];
             if (q0 / 64 + 1 < nq) {
@@ -347,7 +363,7 @@ __global__ __launch_bounds__(256, 1) void attend_backward_q(const Args p) {
             }
             wave_docs = qw < p.Lq ? t[qw / 64] : (int4){0x7fffffff, -1, 0, 0};
         }
-        walk.start(k_tiles, mine, 0, t_end, lane);
+        walk.start(SIDE && p.k_tiles ? p.k_tiles + b * nk : nullptr, mine, 0, t_end, lane);
     }
 
     f32x16 dq[DB];
@@ -355,52 +371,48 @@ __global__ __launch_bounds__(256, 1) void attend_backward_q(const Args p) {
     for (int i = 0; i < DB; ++i)
         dq[i] = f32x16{};
 
-    Stage<T, DP, KT, 256> gk, gv;
-    int g_doc = -1;
-    float g_pos[3];
-    const int seen = min(block_limit, p.Lk);
-    auto fetch = [&](int k0) {
-        gk.load(k, p.k_l, k0, seen, p.D, k_docs, tid);
-        gv.load(v, p.v_l, k0, seen, p.D, k_docs, tid);
-        if (k_docs && tid < KT)
-            g_doc = k0 + tid < seen ? k_docs[k0 + tid] : -1;
-        if (k_pos && tid < KT)
-#pragma unroll
-            for (int a = 0; a < 3; ++a)
-                if (a < p.axes)
-                    g_pos[a] = k0 + tid < seen ? k_pos[(int64_t)(k0 + tid) * p.axes + a] : 0.f;
-    };
+    const int seen = min(block_limit, p.Lk); // keys past it may hold anything
     int t64 = walk.next(lane), sub = 0;
-    if (t64 < t_end)
-        fetch(t64 * 64);
-    while (t64 < t_end) {
-        const int k0 = t64 * 64 + sub * KT;
-        __syncthreads();
-        gk.store(sk, tid);
-        gv.store(sv, tid);
-        if (k_docs && tid < KT)
-            s_docs[tid] = g_doc;
-        if (k_pos && tid < KT)
+    auto fetch = [&](int k0, u32x4 *sk, u32x4 *sv, int *s_docs, float (*s_pos)[64]) {
+        B::load(sk, k, p.k_l, k0, seen, p.D, tid);
+        B::load(sv, v, p.v_l, k0, seen, p.D, tid);
+        if (SIDE && wave == 0) {
+            const int64_t j = min(k0 + lane, seen - 1);
+            if (k_docs)
+                bring_word(s_docs, k_docs + j);
+            if (k_pos) {
 #pragma unroll
-            for (int a = 0; a < 3; ++a)
-                if (a < p.axes)
-                    s_pos[a][tid] = g_pos[a];
-        __syncthreads();
-        const int this64 = t64;
-        if (++sub == per64) {
+                for (int a = 0; a < 3; ++a)
+                    if (a < p.axes)
+                        bring_word(s_pos[a], k_pos + j * p.axes + a);
+            }
+        }
+    };
+    auto step = [&](u32x4 *sk, u32x4 *sv, int *s_docs, float (*s_pos)[64], u32x4 *next_k,
+                    u32x4 *next_v, int *next_docs, float (*next_pos)[64]) {
+        const int k0 = t64 * 64 + sub * KT;
+        const int4 kd = walk.docs;
+        arrived();
+        __syncthreads(); // this tile is here, and the other buffer is done with
+        if (++sub == per64 || k0 + KT >= seen) { // no row of the second half may be there
             sub = 0;
             t64 = walk.next(lane);
         }
         if (t64 < t_end)
-            fetch(t64 * 64 + sub * KT);
+            fetch(t64 * 64 + sub * KT, next_k, next_v, next_docs, next_pos);
 
-        bool use = k0 < wave_limit, masked = k0 + KT > full_limit;
+        bool use = k0 < wave_limit, masked = k0 + KT > full_limit, dirty = k0 + KT > seen;
         if (k_docs) {
-            use = use && docs_meet(k_tiles[this64], wave_docs);
-            masked = masked || !docs_same(k_tiles[this64], wave_docs);
+            use = use && docs_meet(kd, wave_docs);
+            masked = masked || !docs_same(kd, wave_docs);
+            dirty = dirty || kd.z;
+        }
+        if (dirty) { // the same for all waves
+            B::clear(sk, k0, seen, k_docs, s_docs, tid);
+            __syncthreads();
         }
         if (!use)
-            continue;
+            return;
 
 #pragma unroll 1
         for (int kb = 0; kb < KB; ++kb) {
@@ -410,7 +422,7 @@ __global__ __launch_bounds__(256, 1) void attend_backward_q(const Args p) {
                 s = mma32(L::row8(sk, 32 * kb + (lane & 31), 2 * c + half), qf[c], s);
                 ds = mma32(L::row8(sv, 32 * kb + (lane & 31), 2 * c + half), of[c], ds);
             }
-            rows.score(p, s, &slant, k0 + 32 * kb, half, &s_pos[0][32 * kb], KT);
+            rows.score(p, s, &slant, k0 + 32 * kb, half, &s_pos[0][32 * kb], 64);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], mul, -lse)) * (ds[i] - delta);
@@ -429,6 +441,21 @@ __global__ __launch_bounds__(256, 1) void attend_backward_q(const Args p) {
                     dq[i] = mma32(L::col8(sk, 32 * kb + 16 * t, i, lane), w, dq[i]);
             }
         }
+    };
+
+    B::pad(sk0, p.D, tid);
+    B::pad(sk1, p.D, tid);
+    B::pad(sv0, p.D, tid);
+    B::pad(sv1, p.D, tid);
+    if (p.D < DP)
+        __syncthreads();
+    if (t64 < t_end)
+        fetch(t64 * 64, sk0, sv0, s_docs0, s_pos0);
+    while (t64 < t_end) {
+        step(sk0, sv0, s_docs0, s_pos0, sk1, sv1, s_docs1, s_pos1);
+        if (t64 >= t_end)
+            break;
+        step(sk1, sv1, s_docs1, s_pos1, sk0, sv0, s_docs0, s_pos0);
     }
 
     if (qi >= p.Lq)
@@ -449,58 +476,81 @@ __global__ __launch_bounds__(256, 1) void attend_backward_q(const Args p) {
         }
 }
 
-// delta: a wave for each query and head.  From the output as it was before it was rounded,
-// in two parts: the rounding alone would add as much error to dq and dk as that of ds does.
-template <typename T>
-__global__ __launch_bounds__(256) void attend_delta(const Args p, float *delta) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (row >= (int64_t)p.B * p.Lq * p.H)
-        return;
+// delta of each query and head, and the log of its sum in base 2 (+inf for an empty row, which
+// makes all its weights zero).  16 bytes a thread, DP / E threads a row.  From the output as
+// it was before it was rounded, in two parts: the rounding alone would add as much error to dq
+// and dk as that of ds does.
+template <typename T, int N> // N threads a row: a power of two, N * E >= D
+__global__ __launch_bounds__(256) void attend_delta(const Args p, const float *lse,
+                                                    float *base2, float *delta) {
+    constexpr int E = 16 / (int)sizeof(T);
+    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / N;
+    const int d = (int)threadIdx.x % N * E;
+    const bool real = row < (int64_t)p.B * p.Lq * p.H;
     const int head = (int)(row % p.H), i = (int)(row / p.H % p.Lq);
     const int64_t b = row / p.H / p.Lq;
-    const T *o = (const T *)p.out + row * p.D, *low = (const T *)p.out_low + row * p.D;
-    const T *dout = (const T *)p.dout + b * p.do_b + i * p.do_l + head * p.do_h;
     float x = 0.f;
-    for (int d = 4 * lane; d < p.D; d += 256) {
-        const x4<T> u = *(const x4<T> *)(o + d), w = *(const x4<T> *)(dout + d);
+    if (real && d < p.D) {
+        typedef T unit __attribute__((ext_vector_type(E)));
+        const unit u = *(const unit *)((const T *)p.out + row * p.D + d);
+        const unit w =
+            *(const unit *)((const T *)p.dout + b * p.do_b + i * p.do_l + head * p.do_h + d);
+        unit r = u;
+        if (p.out_low)
+            r = *(const unit *)((const T *)p.out_low + row * p.D + d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            x = fmaf((float)u[j], (float)w[j], x);
-        if (p.out_low) {
-            const x4<T> r = *(const x4<T> *)(low + d);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                x = fmaf((float)r[j], (float)w[j], x);
-        }
+        for (int j = 0; j < E; ++j)
+            x = fmaf((float)u[j] + (p.out_low ? (float)r[j] : 0.f), (float)w[j], x);
     }
 #pragma unroll
-    for (int n = 32; n; n >>= 1)
+    for (int n = N / 2; n; n >>= 1)
         x += __shfl_xor(x, n);
-    if (!lane)
-        delta[(b * p.H + head) * p.Lq + i] = x;
+    if (real && d == 0) {
+        const int64_t at = (b * p.H + head) * p.Lq + i;
+        const float l = lse[at];
+        delta[at] = x;
+        base2[at] = l == -kInf ? kInf : l * kLog2e;
+    }
 }
 
-template <typename T> int run_delta(const Args &a, float *delta, hipStream_t s) {
+template <typename T>
+int run_delta(const Args &a, const float *lse, float *base2, float *delta, hipStream_t s) {
     const int64_t rows = (int64_t)a.B * a.Lq * a.H;
-    attend_delta<T><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, s>>>(a, delta);
+    const int units = a.D * (int)sizeof(T) / 16;
+    const auto grid = [&](int n) { return dim3((unsigned)((rows * n + 255) / 256)); };
+    if (units <= 8)
+        attend_delta<T, 8><<<grid(8), 256, 0, s>>>(a, lse, base2, delta);
+    else if (units <= 16)
+        attend_delta<T, 16><<<grid(16), 256, 0, s>>>(a, lse, base2, delta);
+    else
+        attend_delta<T, 64><<<grid(64), 256, 0, s>>>(a, lse, base2, delta);
     return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 
-template <typename T, int DP> int run_backward_kv(const Args &a, hipStream_t s) {
+template <typename T, int DP, bool SIDE> void start_backward_kv(const Args &a, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)((a.Lk + 127) / 128) * a.Hkv * a.B));
     if constexpr (BackwardShape<T, DP>::kTwoPasses) {
-        attend_backward_kv<T, DP, 1><<<grid, 256, 0, s>>>(a);
-        attend_backward_kv<T, DP, 2><<<grid, 256, 0, s>>>(a);
+        attend_backward_kv<T, DP, SIDE, 1><<<grid, 256, 0, s>>>(a);
+        attend_backward_kv<T, DP, SIDE, 2><<<grid, 256, 0, s>>>(a);
     } else {
-        attend_backward_kv<T, DP, 3><<<grid, 256, 0, s>>>(a);
+        attend_backward_kv<T, DP, SIDE, 3><<<grid, 256, 0, s>>>(a);
     }
+}
+
+template <typename T, int DP> int run_backward_kv(const Args &a, hipStream_t s) {
+    if (a.q_docs || a.q_pos)
+        start_backward_kv<T, DP, true>(a, s);
+    else
+        start_backward_kv<T, DP, false>(a, s);
     return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 
 template <typename T, int DP> int run_backward_q(const Args &a, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)((a.Lq + 127) / 128) * a.H * a.B));
-    attend_backward_q<T, DP><<<grid, 256, 0, s>>>(a);
+    if (a.q_docs || a.q_pos)
+        attend_backward_q<T, DP, true><<<grid, 256, 0, s>>>(a);
+    else
+        attend_backward_q<T, DP, false><<<grid, 256, 0, s>>>(a);
     return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 

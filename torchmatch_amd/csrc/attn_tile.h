@@ -402,7 +402,7 @@ __device__ inline void soften(f32x16 (&s)[KB], f32x16 (&o)[DB], float mul, float
     // s mul - top in one rounding leaves the rounding of top in the weights, all of a row by
     // the same factor; past 2^11 that would show in 16 bits, so there products come first and
     // the largest weight stays a power of two
-    if (__any(fabsf(m) * mul > 2048.f)) {
+    if (__any(fabsf(m) * mul > 2048.f && m != -kInf)) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
