@@ -20,14 +20,20 @@ namespace attn {
 
 template <typename T, int DP> struct BackwardShape {
     static constexpr int kRows = sizeof(T) == 4 && DP == 256 ? 32 : 64; // rows of a tile in LDS
-    // float32 rows of 256: dk and dv by a pass each, the registers hold one of them
-    static constexpr bool kTwoPasses = sizeof(T) == 4 && DP == 256;
+    // The kernel over keys holds k, v, dk and dv of 32 keys a wave.  Where that leaves no
+    // registers for two waves a SIMD (128 features of 16 bits; any 256), dk and dv take a pass
+    // each: one product of five is made twice, but two waves hide each other's waits.
+    static constexpr bool kTwoPasses = (sizeof(T) == 2 && DP >= 128) || DP == 256;
     static constexpr int kOccupancy = sizeof(T) * DP <= 256 ? 2 : 1;
+    static constexpr int kKvOccupancy = sizeof(T) * DP <= 192 || (sizeof(T) == 2 && DP == 128)
+                                            ? 2
+                                            : 1;
 };
 
 // WHICH: 1 dv, 2 dk, 3 both
 template <typename T, int DP, bool SIDE, int WHICH>
-__global__ __launch_bounds__(256, 1) void attend_backward_kv(const Args p) {
+__global__ __launch_bounds__(256, (BackwardShape<T, DP>::kKvOccupancy)) void
+attend_backward_kv(const Args p) {
     using L = Tile<T, DP>;
     constexpr int QT = BackwardShape<T, DP>::kRows, QB = QT / 32, C = DP / 16, DB = DP / 32;
     constexpr bool DV = WHICH & 1, DK = WHICH & 2;
@@ -48,6 +54,7 @@ __global__ __launch_bounds__(256, 1) void attend_backward_kv(const Args p) {
     const int kvh = id % p.Hkv, b = id / p.Hkv;
     const int k0 = 128 * kb, kw = k0 + 32 * wave, kj = kw + (lane & 31);
     const Limits lim(p, b);
+    const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
     const int my_doc = SIDE && p.k_docs && kj < p.Lk ? p.k_docs[(int64_t)b * p.Lk + kj] : -1;
     const bool k_real = kj < lim.length && !(SIDE && p.k_docs && my_doc < 0);
     // the first query that sees this lane's key; the last that must be asked for
@@ -86,14 +93,12 @@ __global__ __launch_bounds__(256, 1) void attend_backward_kv(const Args p) {
     if (SIDE && p.k_tiles) {
         const int4 *t = p.k_tiles + (int64_t)b * nk;
         mine = t[k0 / 64];
-        if (k0 / 64 + 1 < nk) {
-            const int4 o = t[k0 / 64 + 1];
-            mine.x = min(mine.x, o.x);
-            mine.y = max(mine.y, o.y);
+        for (int n = k0 / 64 + 1; n < min(nk, (k0 + 128) / 64); ++n) {
+            mine.x = min(mine.x, t[n].x);
+            mine.y = max(mine.y, t[n].y);
         }
         wave_docs = kw < p.Lk ? t[kw / 64] : (int4){0x7fffffff, -1, 0, 0};
     }
-    const float factor = QueryLane<T, SIDE>::factor(p);
 
     f32x16 dk[DB], dv[DB];
 #pragma unroll
@@ -169,62 +174,30 @@ __global__ __launch_bounds__(256, 1) void attend_backward_kv(const Args p) {
             f32x16 s = {}, ds = {};
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                s = mma32(L::row8(sq, 32 * qb + (lane & 31), 2 * c + half), kf[c], s);
+                s = mma32(L::row8(sq, row_at, 32 * qb, c), kf[c], s);
                 if constexpr (DK)
-                    ds = mma32(L::row8(so, 32 * qb + (lane & 31), 2 * c + half), vf[c], ds);
+                    ds = mma32(L::row8(so, row_at, 32 * qb, c), vf[c], ds);
             }
-            f32x16 slant;
-            if (p.cap > 0.f) {
-                const float in = p.scale / p.cap, out = p.cap * kLog2e;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float t = cap_tanh<T>(s[i] * in);
-                    slant[i] = fmaf(-t, t, 1.f);
-                    s[i] = out * t;
-                }
-            } else if (factor == 1.f) {
-                const float m = p.scale * kLog2e;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[i] *= m;
-            }
-            if (SIDE && q_pos) {
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
+            const float from = (float)(kj - q0 - 32 * qb - 4 * half - lim.offset);
+            weigh<T, DK>(
+                p, s, ds,
+                [&](int n) -> f32x4 {
                     const int j = 32 * qb + 8 * n + 4 * half;
-                    f32x4 dist = away(*(const f32x4 *)(s_row[2] + j), my_pos[0]);
-                    if (p.axes > 1)
-                        dist += away(*(const f32x4 *)(s_row[3] + j), my_pos[1]);
-                    if (p.axes > 2)
-                        dist += away(*(const f32x4 *)(s_row[4] + j), my_pos[2]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[4 * n + e] = fmaf(-slope, dist[e], s[4 * n + e]);
-                }
-            } else if (p.slopes) {
-                const float from = (float)(q0 + 32 * qb + 4 * half + lim.offset - kj);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    s[i] = fmaf(-slope, fabsf(from + (float)(8 * (i / 4) + i % 4)), s[i]);
-            }
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const int j = 32 * qb + 8 * n + 4 * half;
-                const f32x4 lse = *(const f32x4 *)(s_row[0] + j);
-                const f32x4 delta = *(const f32x4 *)(s_row[1] + j);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = 4 * n + e;
-                    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], factor, -lse[e]));
-                    if constexpr (DK)
-                        ds[i] = s[i] * (ds[i] - delta[e]);
-                }
-            }
-            if (DK && p.cap > 0.f) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    ds[i] *= slant[i];
-            }
+                    f32x4 d;
+                    if (SIDE && q_pos) {
+                        d = away(*(const f32x4 *)(s_row[2] + j), my_pos[0]);
+                        if (p.axes > 1)
+                            d += away(*(const f32x4 *)(s_row[3] + j), my_pos[1]);
+                        if (p.axes > 2)
+                            d += away(*(const f32x4 *)(s_row[4] + j), my_pos[2]);
+                    } else {
+                        d = away(f32x4{8.f * n, 8.f * n + 1.f, 8.f * n + 2.f, 8.f * n + 3.f},
+                                 from);
+                    }
+                    return d * slope;
+                },
+                [&](int n) { return *(const f32x4 *)(s_row[0] + 32 * qb + 8 * n + 4 * half); },
+                [&](int n) { return *(const f32x4 *)(s_row[1] + 32 * qb + 8 * n + 4 * half); });
             if (masked) {
                 const int row0 = q0 + 32 * qb + 4 * half;
                 const int from = my_first - row0, to = p.Lq - row0;
@@ -248,13 +221,13 @@ __global__ __launch_bounds__(256, 1) void attend_backward_kv(const Args p) {
                     const x8<T> w = pack8<T>(s, t);
 #pragma unroll
                     for (int i = 0; i < DB; ++i)
-                        dv[i] = mma32(L::col8(so, 32 * qb + 16 * t, i, lane), w, dv[i]);
+                        dv[i] = mma32(L::col8(so, col_at, 32 * qb + 16 * t, i), w, dv[i]);
                 }
                 if constexpr (DK) {
                     const x8<T> w = pack8<T>(ds, t);
 #pragma unroll
                     for (int i = 0; i < DB; ++i)
-                        dk[i] = mma32(L::col8(sq, 32 * qb + 16 * t, i, lane), w, dk[i]);
+                        dk[i] = mma32(L::col8(sq, col_at, 32 * qb + 16 * t, i), w, dk[i]);
                 }
             }
         }
@@ -322,6 +295,7 @@ attend_backward_q(const Args p) {
 
     const int q0 = qb * 128, qw = q0 + 32 * wave, qi = qw + (lane & 31);
     const Limits lim(p, b);
+    const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
     const int block_limit = lim.of(min(q0 + 128, p.Lq) - 1);
     const int wave_limit = qw < p.Lq ? lim.of(min(qw + 32, p.Lq) - 1) : 0;
     const int full_limit = qw < p.Lq ? lim.of(qw) : 0;
@@ -344,7 +318,6 @@ attend_backward_q(const Args p) {
     const int64_t row = ((int64_t)b * p.H + head) * p.Lq + qi;
     const float lse = qi < p.Lq ? p.lse[row] : kInf;
     const float delta = qi < p.Lq ? p.delta[row] : 0.f;
-    const float mul = rows.factor(p);
 
     constexpr int per64 = 64 / KT;
     int4 wave_docs = {0, 0, 0, 0};
@@ -416,21 +389,20 @@ attend_backward_q(const Args p) {
 
 #pragma unroll 1
         for (int kb = 0; kb < KB; ++kb) {
-            f32x16 s = {}, ds = {}, slant;
+            f32x16 s = {}, ds = {};
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                s = mma32(L::row8(sk, 32 * kb + (lane & 31), 2 * c + half), qf[c], s);
-                ds = mma32(L::row8(sv, 32 * kb + (lane & 31), 2 * c + half), of[c], ds);
+                s = mma32(L::row8(sk, row_at, 32 * kb, c), qf[c], s);
+                ds = mma32(L::row8(sv, row_at, 32 * kb, c), of[c], ds);
             }
-            rows.score(p, s, &slant, k0 + 32 * kb, half, &s_pos[0][32 * kb], 64);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                ds[i] = __builtin_amdgcn_exp2f(fmaf(s[i], mul, -lse)) * (ds[i] - delta);
-            if (p.cap > 0.f) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    ds[i] *= slant[i];
-            }
+            weigh<T, true>(
+                p, s, ds,
+                [&](int n) {
+                    return rows.distance(p, n, k0 + 32 * kb, half, &s_pos[0][32 * kb], 64) *
+                           rows.slope;
+                },
+                [&](int) { return f32x4{lse, lse, lse, lse}; },
+                [&](int) { return f32x4{delta, delta, delta, delta}; });
             if (masked)
                 rows.hide(p, ds, 0.f, k0 + 32 * kb, half, s_docs + 32 * kb);
 #pragma unroll
@@ -438,7 +410,7 @@ attend_backward_q(const Args p) {
                 const x8<T> w = pack8<T>(ds, t);
 #pragma unroll
                 for (int i = 0; i < DB; ++i)
-                    dq[i] = mma32(L::col8(sk, 32 * kb + 16 * t, i, lane), w, dq[i]);
+                    dq[i] = mma32(L::col8(sk, col_at, 32 * kb + 16 * t, i), w, dq[i]);
             }
         }
     };

@@ -53,6 +53,7 @@ attend_forward(const Args p) {
     const int q0 = qb * QT, qw = q0 + 32 * wave, qi = qw + (lane & 31);
     const bool q_real = qi < p.Lq;
     const Limits lim(p, b);
+    const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
     const int block_limit = lim.of(min(q0 + QT, p.Lq) - 1);
     const int wave_limit = qw < p.Lq ? lim.of(min(qw + 32, p.Lq) - 1) : 0;
     const int full_limit = qw < p.Lq ? lim.of(qw) : 0; // keys that all of the wave see
@@ -153,10 +154,10 @@ attend_forward(const Args p) {
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
-                s[kb] = mma32(L::row8(sk, 32 * kb + (lane & 31), 2 * c + half), qf[c], s[kb]);
+                s[kb] = mma32(L::row8(sk, row_at, 32 * kb, c), qf[c], s[kb]);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
-            rows.score(p, s[kb], nullptr, k0 + 32 * kb, half, &s_pos[0][32 * kb], 64);
+            rows.score(p, s[kb], k0 + 32 * kb, half, &s_pos[0][32 * kb], 64);
         if (masked) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
@@ -170,7 +171,7 @@ attend_forward(const Args p) {
             const x8<T> w = pack8<T>(s[t / 2], t % 2);
 #pragma unroll
             for (int i = 0; i < DB; ++i)
-                o[i] = mma32(L::col8(sv, 16 * t, i, lane), w, o[i]);
+                o[i] = mma32(L::col8(sv, col_at, 16 * t, i), w, o[i]);
         }
     };
 

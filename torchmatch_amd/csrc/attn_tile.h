@@ -95,49 +95,60 @@ template <typename T, int DP> struct Tile {
     }
     __device__ static inline int at(int row, int unit) { return row * U + (unit ^ swz(row)); }
 
-    // 8 elements of `row` from element 8 c
-    __device__ static inline x8<T> row8(const u32x4 *t, int row, int c) {
+    // Where a lane reads: a byte offset from which every read of one kind differs by an
+    // exclusive or with a constant and a constant number of rows, so that few registers
+    // hold addresses.  Rows r0 are multiples of 16, over which swz() repeats.
+    __device__ static inline uint32_t row_lane(int lane) {
+        const int row = lane & 31, half = lane >> 5;
+        return 16u * at(row, sizeof(T) == 2 ? half : 2 * half);
+    }
+    __device__ static inline uint32_t col_lane(int lane) {
         if constexpr (sizeof(T) == 2) {
-            return __builtin_bit_cast(x8<T>, t[at(row, c)]);
+            const int d = (lane & 16) + 4 * (lane & 3);
+            return 16u * at(4 * (lane >> 5) + ((lane & 15) >> 2), d >> 3) + 2u * (d & 7);
         } else {
-            const f32x4 lo = __builtin_bit_cast(f32x4, t[at(row, 2 * c)]);
-            const f32x4 hi = __builtin_bit_cast(f32x4, t[at(row, 2 * c + 1)]);
+            return 16u * at(4 * (lane >> 5), (lane & 31) / E) + 4u * (lane & 3);
+        }
+    }
+
+    // row operand: row r0 + lane % 32, elements 16 c + 8 (lane / 32) + 0 .. 7
+    __device__ static inline x8<T> row8(const u32x4 *t, uint32_t row, int r0, int c) {
+        const char *from = (const char *)t + r0 * U * 16;
+        if constexpr (sizeof(T) == 2) {
+            return *(const x8<T> *)(from + (row ^ (32u * c)));
+        } else {
+            const f32x4 lo = *(const f32x4 *)(from + (row ^ (64u * c)));
+            const f32x4 hi = *(const f32x4 *)(from + (row ^ (64u * c + 16u)));
             return (x8<T>){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         }
     }
 
-    // column 32 db + l % 32, rows r0 + 8(j/4) + 4h + j%4: an operand whose rows
-    // are the tile's columns
-    __device__ static inline x8<T> col8(const u32x4 *t, int r0, int db, int lane) {
+    // column operand: column 32 db + lane % 32, rows r0 + 8(j/4) + 4(lane / 32) + j%4
+    __device__ static inline x8<T> col8(const u32x4 *t, uint32_t col, int r0, int db) {
+        const char *from = (const char *)t + r0 * U * 16;
+        x8<T> r;
         if constexpr (sizeof(T) == 2) {
             // the transposed read: each 16 lanes load 4 rows of 16 elements (4 a
             // lane) and each lane gets one column of them
-            const int row = r0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
-            const int d = 32 * db + (lane & 16) + 4 * (lane & 3);
-            x8<T> r;
 #pragma unroll
             for (int jj = 0; jj < 2; ++jj) {
-                const u32x4 *u = t + at(row + 8 * jj, d >> 3);
-                const auto *p = (__attribute__((address_space(3))) s16x4 *)((const s16x4 *)u +
-                                                                          ((d >> 2) & 1));
+                const char *at = from + 8 * jj * U * 16 + (col ^ (64u * db + 32u * jj));
                 const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4 *)p);
+                    (__attribute__((address_space(3))) s16x4 *)at);
                 const x4<T> y = __builtin_bit_cast(x4<T>, x);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     r[4 * jj + j] = y[j];
             }
-            return r;
         } else {
-            const int d = 32 * db + (lane & 31);
-            x8<T> r;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int row = r0 + 8 * (j >> 2) + 4 * (lane >> 5) + (j & 3);
-                r[j] = ((const T *)(t + at(row, d / E)))[d % E];
+                const int row = 8 * (j >> 2) + (j & 3);
+                r[j] = *(const float *)(from + row * U * 16 +
+                                        (col ^ (16u * (8 * db ^ swz(row)))));
             }
-            return r;
         }
+        return r;
     }
 };
 
@@ -318,44 +329,45 @@ template <typename T, bool SIDE> struct QueryLane {
     __device__ static inline float factor(const Args &p) {
         return p.cap > 0.f || p.slopes || p.scale < 0.f ? 1.f : p.scale * kLog2e;
     }
-    // s: products with keys k0 ..; to scores times log2 e but for factor().  With `grad`, the
-    // derivative of the cap too.  k_pos: the block's positions in LDS, `axis` apart.
-    __device__ inline void score(const Args &p, f32x16 &s, f32x16 *grad, int k0, int half,
-                                 const float *k_pos, int axis) const {
+    // s: products with keys k0 ..; to scores times log2 e but for factor().  k_pos: the block's
+    // positions in LDS, `axis` apart.
+    __device__ inline void score(const Args &p, f32x16 &s, int k0, int half, const float *k_pos,
+                                 int axis) const {
         if (p.cap > 0.f) {
             const float in = p.scale / p.cap, out = p.cap * kLog2e;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float t = cap_tanh<T>(s[i] * in);
-                if (grad)
-                    (*grad)[i] = fmaf(-t, t, 1.f);
-                s[i] = out * t;
-            }
+            for (int i = 0; i < 16; ++i)
+                s[i] = out * cap_tanh<T>(s[i] * in);
         } else if (p.slopes || p.scale < 0.f) {
             const float m = p.scale * kLog2e;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 s[i] *= m;
         }
-        if (SIDE && p.q_pos) {
+        if (p.slopes) {
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
-                const int j = 8 * n + 4 * half;
-                f32x4 dist = away(*(const f32x4 *)(k_pos + j), pos[0]);
-                if (p.axes > 1)
-                    dist += away(*(const f32x4 *)(k_pos + axis + j), pos[1]);
-                if (p.axes > 2)
-                    dist += away(*(const f32x4 *)(k_pos + 2 * axis + j), pos[2]);
+                const f32x4 d = distance(p, n, k0, half, k_pos, axis);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    s[4 * n + e] = fmaf(-slope, dist[e], s[4 * n + e]);
+                    s[4 * n + e] = fmaf(-slope, d[e], s[4 * n + e]);
             }
-        } else if (p.slopes) {
-            const float from = (float)(at - k0 - 4 * half);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                s[i] = fmaf(-slope, fabsf(from - (float)(8 * (i / 4) + i % 4)), s[i]);
         }
+    }
+    // to keys k0 + 8 n + 4 half + 0 .. 3
+    __device__ inline f32x4 distance(const Args &p, int n, int k0, int half, const float *k_pos,
+                                     int axis) const {
+        if (SIDE && p.q_pos) {
+            const float *at_n = k_pos + 8 * n + 4 * half;
+            f32x4 d = away(*(const f32x4 *)at_n, pos[0]);
+            if (p.axes > 1)
+                d += away(*(const f32x4 *)(at_n + axis), pos[1]);
+            if (p.axes > 2)
+                d += away(*(const f32x4 *)(at_n + 2 * axis), pos[2]);
+            return d;
+        }
+        const float from = (float)(at - k0 - 4 * half);
+        return away(f32x4{8.f * n, 8.f * n + 1.f, 8.f * n + 2.f, 8.f * n + 3.f}, from);
     }
     // x where the lane does not see the key; docs: the block's documents in LDS
     __device__ inline void hide(const Args &p, f32x16 &s, float x, int k0, int half,
@@ -444,6 +456,51 @@ template <typename T> __device__ inline void put(const Args &p, int64_t at, x4<T
         for (int j = 0; j < 4; ++j)
             z[j] = (T)(x[j] - (float)y[j]);
         *(x4<T> *)((T *)p.out_low + at) = z;
+    }
+}
+
+// For the gradients: products s become weights p, products ds = do v become
+// p (ds - delta) slant, the cap's slope included.  Four elements at a time, so that nothing but
+// s and ds is held: bias(n), lse(n) and delta(n) give those of elements 4n .. 4n + 3, in base 2
+// but for delta.
+template <typename T, bool DS, typename Bias, typename Lse, typename Delta>
+__device__ inline void weigh(const Args &p, f32x16 &s, f32x16 &ds, Bias bias, Lse lse,
+                             Delta delta) {
+    if (p.cap > 0.f) {
+        const float in = p.scale / p.cap, out = p.cap * kLog2e;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            f32x4 l = lse(n), d;
+            if constexpr (DS)
+                d = delta(n);
+            if (p.slopes)
+                l += bias(n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 4 * n + e;
+                const float t = cap_tanh<T>(s[i] * in);
+                s[i] = __builtin_amdgcn_exp2f(fmaf(out, t, -l[e]));
+                if constexpr (DS)
+                    ds[i] = s[i] * (ds[i] - d[e]) * fmaf(-t, t, 1.f);
+            }
+        }
+    } else {
+        const float m = p.scale * kLog2e;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            f32x4 l = lse(n), d;
+            if constexpr (DS)
+                d = delta(n);
+            if (p.slopes)
+                l += bias(n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 4 * n + e;
+                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], m, -l[e]));
+                if constexpr (DS)
+                    ds[i] = s[i] * (ds[i] - d[e]);
+            }
+        }
     }
 }
 

@@ -60,6 +60,7 @@ attend_tokens(const Args p) {
     const int qi = q_real ? r % p.Lq : p.Lq;
     const int head = kvh * group + (q_real ? r / p.Lq : 0);
     const Limits lim(p, b);
+    const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
     const int all_limit = lim.of(p.Lq - 1), full_limit = lim.of(0);
     const QueryLane<T, true> rows(p, lim, b, head, qi);
 
@@ -155,8 +156,8 @@ attend_tokens(const Args p) {
         f32x16 s[1] = {f32x16{}};
 #pragma unroll
         for (int c = 0; c < C; ++c)
-            s[0] = mma32(L::row8(sk, lane & 31, 2 * c + half), qf[c], s[0]);
-        rows.score(p, s[0], nullptr, k0, half, &s_pos[wave][0][0], 32);
+            s[0] = mma32(L::row8(sk, row_at, 0, c), qf[c], s[0]);
+        rows.score(p, s[0], k0, half, &s_pos[wave][0][0], 32);
         if (masked)
             rows.hide(p, s[0], -kInf, k0, half, s_docs[wave]);
         soften<T>(s, o, rows.factor(p), top, sum);
@@ -165,7 +166,7 @@ attend_tokens(const Args p) {
             const x8<T> w = pack8<T>(s[0], t);
 #pragma unroll
             for (int i = 0; i < DB; ++i)
-                o[i] = mma32(L::col8(sv, 16 * t, i, lane), w, o[i]);
+                o[i] = mma32(L::col8(sv, col_at, 16 * t, i), w, o[i]);
         }
     }
 
