@@ -20,32 +20,43 @@ namespace attn {
 
 template <typename T, int DP> struct BackwardShape {
     static constexpr int kRows = sizeof(T) == 4 && DP == 256 ? 32 : 64; // rows of a tile in LDS
-    // The kernel over keys holds k, v, dk and dv of 32 keys a wave.  Where that leaves no
-    // registers for two waves a SIMD (128 features of 16 bits; any 256), dk and dv take a pass
-    // each: one product of five is made twice, but two waves hide each other's waits.
-    static constexpr bool kTwoPasses = (sizeof(T) == 2 && DP >= 128) || DP == 256;
     static constexpr int kOccupancy = sizeof(T) * DP <= 256 ? 2 : 1;
-    static constexpr int kKvOccupancy = sizeof(T) * DP <= 192 || (sizeof(T) == 2 && DP == 128)
-                                            ? 2
-                                            : 1;
+    // The kernel over keys takes 32 keys a wave and needs two waves a SIMD that hide each
+    // other's waits.  Rows of 128 bytes and less leave the registers for that.  With rows of 256
+    // bytes k and v move to LDS, and two teams of four waves share the same 128 keys, each with
+    // every other tile of queries (packed documents of 128 features: 440 us; 595 with one
+    // team and k and v in registers, 700 with a pass for dk and one for dv; but 125 in place of
+    // 104 for pairs of 64 features).  Larger rows leave room for one team only.
+    static constexpr int kTeams = Tile<T, DP>::U == 16 ? 2 : 1;
+    static constexpr int kKvRows = kTeams == 2 ? 32 : kRows;
+    static constexpr bool kKeysInLds = kTeams == 2;
+    static constexpr int kKvOccupancy = Tile<T, DP>::U <= 8 ? 2 : 1; // blocks a compute unit
+    // rows of 256: dk and dv by a pass each, the registers hold one of them
+    static constexpr bool kTwoPasses = DP == 256;
 };
 
 // WHICH: 1 dv, 2 dk, 3 both
 template <typename T, int DP, bool SIDE, int WHICH>
-__global__ __launch_bounds__(256, (BackwardShape<T, DP>::kKvOccupancy)) void
+__global__ __launch_bounds__((256 * BackwardShape<T, DP>::kTeams),
+                             (BackwardShape<T, DP>::kKvOccupancy)) void
 attend_backward_kv(const Args p) {
+    using S = BackwardShape<T, DP>;
     using L = Tile<T, DP>;
-    constexpr int QT = BackwardShape<T, DP>::kRows, QB = QT / 32, C = DP / 16, DB = DP / 32;
+    constexpr int QT = S::kKvRows, QB = QT / 32, C = DP / 16, DB = DP / 32, TEAMS = S::kTeams;
     constexpr bool DV = WHICH & 1, DK = WHICH & 2;
     using B = Bring<T, DP, QT, 256>;
-    __shared__ u32x4 sq0[QT * L::U], sq1[QT * L::U];
-    __shared__ u32x4 so0[QT * L::U], so1[QT * L::U];
+    __shared__ u32x4 sq0[TEAMS][QT * L::U], sq1[TEAMS][QT * L::U];
+    __shared__ u32x4 so0[TEAMS][QT * L::U], so1[TEAMS][QT * L::U];
     // of the tile's queries: the log of the sum (base 2), delta, positions; documents
-    __shared__ __attribute__((aligned(16))) float s_row0[5][64], s_row1[5][64];
-    __shared__ __attribute__((aligned(16))) int s_docs0[64], s_docs1[64];
+    __shared__ __attribute__((aligned(16))) float s_row0[TEAMS][5][64], s_row1[TEAMS][5][64];
+    __shared__ __attribute__((aligned(16))) int s_docs0[TEAMS][64], s_docs1[TEAMS][64];
+    // k and v, and at the end the second team's results, 32 x DP floats a wave
+    constexpr int SUM = 4 * 32 * DP / 4, KEEP = 128 * L::U;
+    __shared__ u32x4 keep[TEAMS == 1 ? 1 : S::kKeysInLds && 2 * KEEP > SUM ? 2 * KEEP : SUM];
 
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int team = all_waves >> 2, wave = all_waves & 3;
+    const int tid = threadIdx.x & 255, lane = tid & 63, half = lane >> 5;
     const int k_blocks = (p.Lk + 127) / 128;
     const int group = p.H / p.Hkv;
     int id = xcd_order(blockIdx.x, gridDim.x);
@@ -64,12 +75,18 @@ attend_backward_kv(const Args p) {
 
     const T *k = (const T *)p.k + b * p.k_b + kvh * p.k_h + (k_real ? kj : 0) * p.k_l;
     const T *v = (const T *)p.v + b * p.v_b + kvh * p.v_h + (k_real ? kj : 0) * p.v_l;
-    x8<T> kf[C], vf[C];
+    x8<T> kf[S::kKeysInLds ? 1 : C], vf[S::kKeysInLds ? 1 : C];
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        kf[c] = global8<T>(k, 16 * c + 8 * half, p.D, k_real);
-        if constexpr (DK)
-            vf[c] = global8<T>(v, 16 * c + 8 * half, p.D, k_real);
+        const x8<T> x = global8<T>(k, 16 * c + 8 * half, p.D, k_real);
+        const x8<T> y = global8<T>(v, 16 * c + 8 * half, p.D, k_real);
+        if constexpr (S::kKeysInLds) { // the same by either team
+            L::put8(keep, row_at, 32 * wave, c, x);
+            L::put8(keep + KEEP, row_at, 32 * wave, c, y);
+        } else {
+            kf[c] = x;
+            vf[c] = y;
+        }
     }
     float my_pos[3] = {0.f, 0.f, 0.f};
     if (SIDE && p.k_pos && kj < p.Lk)
@@ -107,15 +124,35 @@ attend_backward_kv(const Args p) {
         dv[i] = f32x16{};
     }
 
-    // the tiles of one query head after the other's: at head g, tile (t64, sub)
-    int g = 0, t64, sub = 0;
+    // the tiles of one query head after the other's, dealt to the teams in turn: this team's is
+    // at (g, t64, sub), the last given out at (all_g, all_t, all_sub)
+    int all_g = 0, all_t, all_sub = 0, g, t64, sub;
+    int4 qd_next = {0, 0, 0, 0}; // documents of this team's tile
+    bool first_team_more = false;
     TileWalk walk;
     auto advance = [&]() {
-        t64 = walk.next(lane);
-        while (t64 >= t_end && g + 1 < group) {
-            ++g;
+        all_t = walk.next(lane);
+        while (all_t >= t_end && all_g + 1 < group) {
+            ++all_g;
             walk.start(q_tiles, mine, first / 64, t_end, lane);
-            t64 = walk.next(lane);
+            all_t = walk.next(lane);
+        }
+    };
+    auto deal = [&]() {
+#pragma unroll
+        for (int n = 0; n < TEAMS; ++n) {
+            if (n == 0)
+                first_team_more = all_t < t_end;
+            if (n == team) {
+                g = all_g;
+                t64 = all_t;
+                sub = all_sub;
+                qd_next = walk.docs;
+            }
+            if (all_t < t_end && (++all_sub == 64 / QT || all_t * 64 + all_sub * QT >= p.Lq)) {
+                all_sub = 0;
+                advance();
+            }
         }
     };
     auto fetch = [&](u32x4 *sq, u32x4 *so, float (*s_row)[64], int *s_docs) {
@@ -142,15 +179,15 @@ attend_backward_kv(const Args p) {
     auto step = [&](u32x4 *sq, u32x4 *so, float (*s_row)[64], int *s_docs, u32x4 *next_q,
                     u32x4 *next_o, float (*next_row)[64], int *next_docs) {
         const int q0 = t64 * 64 + sub * QT, head = kvh * group + g;
-        const int4 qd = walk.docs;
+        const int4 qd = qd_next;
+        const bool here = t64 < t_end; // the last tile may be the other team's
         arrived();
         __syncthreads(); // this tile is here, and the other buffer is done with
-        if (++sub == 64 / QT || q0 + QT >= p.Lq) {
-            sub = 0;
-            advance();
-        }
+        deal();
         if (t64 < t_end)
             fetch(next_q, next_o, next_row, next_docs);
+        if (!here)
+            return;
 
         const int last = min(q0 + QT, p.Lq) - 1;
         bool use = kw < lim.of(last), dirty = q0 + QT > p.Lq;
@@ -160,10 +197,15 @@ attend_backward_kv(const Args p) {
             masked = masked || !docs_same(qd, wave_docs);
             dirty = dirty || qd.z;
         }
-        if (dirty) { // the same for all waves
-            B::clear(sq, q0, p.Lq, q_docs, s_docs, tid);
-            B::clear(so, q0, p.Lq, q_docs, s_docs, tid);
-            __syncthreads();
+        if (dirty && use) {
+            // Each wave clears all of the rows itself (with the others, the same zeros), so that
+            // none has to wait: the teams are not at the same tile.
+            for (int n = lane; n < QT * L::U; n += 64) {
+                const int r = n / L::U;
+                if (q0 + r >= p.Lq || (q_docs && s_docs[r] < 0))
+                    sq[n] = so[n] = u32x4{0u, 0u, 0u, 0u};
+            }
+            wave_fence();
         }
         if (!use)
             return;
@@ -174,9 +216,17 @@ attend_backward_kv(const Args p) {
             f32x16 s = {}, ds = {};
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                s = mma32(L::row8(sq, row_at, 32 * qb, c), kf[c], s);
+                x8<T> kc, vc;
+                if constexpr (S::kKeysInLds) {
+                    kc = L::row8(keep, row_at, 32 * wave, c);
+                    vc = L::row8(keep + KEEP, row_at, 32 * wave, c);
+                } else {
+                    kc = kf[c];
+                    vc = vf[c];
+                }
+                s = mma32(L::row8(sq, row_at, 32 * qb, c), kc, s);
                 if constexpr (DK)
-                    ds = mma32(L::row8(so, row_at, 32 * qb, c), vf[c], ds);
+                    ds = mma32(L::row8(so, row_at, 32 * qb, c), vc, ds);
             }
             const float from = (float)(kj - q0 - 32 * qb - 4 * half - lim.offset);
             weigh<T, DK>(
@@ -233,23 +283,59 @@ attend_backward_kv(const Args p) {
         }
     };
 
-    B::pad(sq0, p.D, tid);
-    B::pad(sq1, p.D, tid);
-    B::pad(so0, p.D, tid);
-    B::pad(so1, p.D, tid);
+    B::pad(sq0[team], p.D, tid);
+    B::pad(sq1[team], p.D, tid);
+    B::pad(so0[team], p.D, tid);
+    B::pad(so1[team], p.D, tid);
     if (p.D < DP)
         __syncthreads();
     walk.start(q_tiles, mine, first / 64, t_end, lane);
     advance();
+    deal();
     if (t64 < t_end)
-        fetch(sq0, so0, s_row0, s_docs0);
-    while (t64 < t_end) {
-        step(sq0, so0, s_row0, s_docs0, sq1, so1, s_row1, s_docs1);
-        if (t64 >= t_end)
+        fetch(sq0[team], so0[team], s_row0[team], s_docs0[team]);
+    // the first team has a tile wherever the second one has
+    while (first_team_more) {
+        step(sq0[team], so0[team], s_row0[team], s_docs0[team], sq1[team], so1[team],
+             s_row1[team], s_docs1[team]);
+        if (!first_team_more)
             break;
-        step(sq1, so1, s_row1, s_docs1, sq0, so0, s_row0, s_docs0);
+        step(sq1[team], so1[team], s_row1[team], s_docs1[team], sq0[team], so0[team],
+             s_row0[team], s_docs0[team]);
     }
 
+    if constexpr (TEAMS == 2) { // the second team's results to the first, dk and then dv
+        const auto join = [&](f32x16 (&x)[DB]) {
+            f32x4 *at = (f32x4 *)keep + wave * (8 * DP) + lane;
+            __syncthreads();
+            if (team == 1) {
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        at[64 * (4 * i + e)] = (f32x4){x[i][4 * e], x[i][4 * e + 1],
+                                                       x[i][4 * e + 2], x[i][4 * e + 3]};
+            }
+            __syncthreads();
+            if (team == 0) {
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const f32x4 y = at[64 * (4 * i + e)];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            x[i][4 * e + j] += y[j];
+                    }
+            }
+        };
+        if constexpr (DK)
+            join(dk);
+        if constexpr (DV)
+            join(dv);
+        if (team == 1)
+            return;
+    }
     if (kj >= p.Lk)
         return;
     const int64_t at = (((int64_t)b * p.Lk + kj) * p.Hkv + kvh) * p.D;
@@ -500,12 +586,13 @@ int run_delta(const Args &a, const float *lse, float *base2, float *delta, hipSt
 }
 
 template <typename T, int DP, bool SIDE> void start_backward_kv(const Args &a, hipStream_t s) {
+    constexpr int N = 256 * BackwardShape<T, DP>::kTeams;
     const dim3 grid((unsigned)((int64_t)((a.Lk + 127) / 128) * a.Hkv * a.B));
     if constexpr (BackwardShape<T, DP>::kTwoPasses) {
-        attend_backward_kv<T, DP, SIDE, 1><<<grid, 256, 0, s>>>(a);
-        attend_backward_kv<T, DP, SIDE, 2><<<grid, 256, 0, s>>>(a);
+        attend_backward_kv<T, DP, SIDE, 1><<<grid, N, 0, s>>>(a);
+        attend_backward_kv<T, DP, SIDE, 2><<<grid, N, 0, s>>>(a);
     } else {
-        attend_backward_kv<T, DP, SIDE, 3><<<grid, 256, 0, s>>>(a);
+        attend_backward_kv<T, DP, SIDE, 3><<<grid, N, 0, s>>>(a);
     }
 }
 

@@ -123,6 +123,17 @@ template <typename T, int DP> struct Tile {
         }
     }
 
+    // writes what row8() reads
+    __device__ static inline void put8(u32x4 *t, uint32_t row, int r0, int c, x8<T> x) {
+        char *to = (char *)t + r0 * U * 16;
+        if constexpr (sizeof(T) == 2) {
+            *(x8<T> *)(to + (row ^ (32u * c))) = x;
+        } else {
+            *(f32x4 *)(to + (row ^ (64u * c))) = (f32x4){x[0], x[1], x[2], x[3]};
+            *(f32x4 *)(to + (row ^ (64u * c + 16u))) = (f32x4){x[4], x[5], x[6], x[7]};
+        }
+    }
+
     // column operand: column 32 db + lane % 32, rows r0 + 8(j/4) + 4(lane / 32) + j%4
     __device__ static inline x8<T> col8(const u32x4 *t, uint32_t col, int r0, int db) {
         const char *from = (const char *)t + r0 * U * 16;
@@ -248,6 +259,14 @@ __device__ inline void bring_word(void *to, const void *from) {
 }
 
 __device__ inline void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// LDS writes of a wave are seen by its later reads as they are: both go through in order.
+// This keeps the compiler from moving them.
+__device__ inline void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // 8 elements of a row in memory (a row operand that stays in registers)
 template <typename T>

@@ -24,14 +24,6 @@ template <typename T, int DP> struct TokensShape {
     static constexpr bool kAhead = sizeof(T) * DP <= 512;
 };
 
-// LDS writes of a wave are seen by its later reads as they are: both go through in order.
-// This keeps the compiler from moving them.
-__device__ inline void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 template <typename T, int DP>
 __global__ __launch_bounds__((64 * TokensShape<T, DP>::kWaves), 1) void
 attend_tokens(const Args p) {
