@@ -20,7 +20,7 @@ namespace attn {
 
 template <typename T, int DP> struct BackwardShape {
     static constexpr int kRows = sizeof(T) == 4 && DP == 256 ? 32 : 64; // rows of a tile in LDS
-    static constexpr int kOccupancy = sizeof(T) * DP <= 256 ? 2 : 1;
+    static constexpr int kOccupancy = sizeof(T) * DP <= 128 ? 3 : sizeof(T) * DP <= 256 ? 2 : 1;
     // The kernel over keys takes 32 keys a wave and needs two waves a SIMD that hide each
     // other's waits.  Rows of 128 bytes and less leave the registers for that.  With rows of 256
     // bytes k and v move to LDS, and two teams of four waves share the same 128 keys, each with
@@ -51,18 +51,17 @@ attend_backward_kv(const Args p) {
     __shared__ __attribute__((aligned(16))) float s_row0[TEAMS][5][64], s_row1[TEAMS][5][64];
     __shared__ __attribute__((aligned(16))) int s_docs0[TEAMS][64], s_docs1[TEAMS][64];
     // k and v, and at the end the second team's results, 32 x DP floats a wave
-    constexpr int SUM = 4 * 32 * DP / 4, KEEP = 128 * L::U;
-    __shared__ u32x4 keep[TEAMS == 1 ? 1 : S::kKeysInLds && 2 * KEEP > SUM ? 2 * KEEP : SUM];
+    constexpr int SUM = TEAMS == 2 ? 32 * DP : 1, KEEP = S::kKeysInLds ? 128 * L::U : 0;
+    __shared__ u32x4 keep[2 * KEEP > SUM ? 2 * KEEP : SUM];
 
     const int all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int team = all_waves >> 2, wave = all_waves & 3;
     const int tid = threadIdx.x & 255, lane = tid & 63, half = lane >> 5;
     const int k_blocks = (p.Lk + 127) / 128;
     const int group = p.H / p.Hkv;
-    int id = xcd_order(blockIdx.x, gridDim.x);
-    const int kb = id % k_blocks; // early keys, which most causal rows see, first
-    id /= k_blocks;
-    const int kvh = id % p.Hkv, b = id / p.Hkv;
+    const Share share(blockIdx.x, k_blocks, p.B * p.Hkv);
+    const int kb = share.block; // the first are seen by most
+    const int kvh = share.head % p.Hkv, b = share.head / p.Hkv;
     const int k0 = 128 * kb, kw = k0 + 32 * wave, kj = kw + (lane & 31);
     const Limits lim(p, b);
     const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
@@ -338,6 +337,7 @@ attend_backward_kv(const Args p) {
     }
     if (kj >= p.Lk)
         return;
+    const float out_scale = grad_scale(p);
     const int64_t at = (((int64_t)b * p.Lk + kj) * p.Hkv + kvh) * p.D;
 #pragma unroll
     for (int i = 0; i < DB; ++i)
@@ -348,7 +348,7 @@ attend_backward_kv(const Args p) {
                 x4<T> y, z;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    y[j] = (T)(dk[i][e + j] * p.scale);
+                    y[j] = (T)(dk[i][e + j] * out_scale);
                     z[j] = (T)dv[i][e + j];
                 }
                 if constexpr (DK)
@@ -373,10 +373,9 @@ attend_backward_q(const Args p) {
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q_blocks = (p.Lq + 127) / 128;
-    int id = xcd_order(blockIdx.x, gridDim.x);
-    const int qb = q_blocks - 1 - id % q_blocks;
-    id /= q_blocks;
-    const int head = id % p.H, b = id / p.H;
+    const Share share(blockIdx.x, q_blocks, p.B * p.H);
+    const int qb = q_blocks - 1 - share.block; // the last see most
+    const int head = share.head % p.H, b = share.head / p.H;
     const int kvh = head / (p.H / p.Hkv);
 
     const int q0 = qb * 128, qw = q0 + 32 * wave, qi = qw + (lane & 31);
@@ -518,6 +517,7 @@ attend_backward_q(const Args p) {
 
     if (qi >= p.Lq)
         return;
+    const float out_scale = grad_scale(p);
     T *dst = (T *)p.dq + (((int64_t)b * p.Lq + qi) * p.H + head) * p.D;
 #pragma unroll
     for (int i = 0; i < DB; ++i)
@@ -528,7 +528,7 @@ attend_backward_q(const Args p) {
                 x4<T> y;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    y[j] = (T)(dq[i][e + j] * p.scale);
+                    y[j] = (T)(dq[i][e + j] * out_scale);
                 *(x4<T> *)(dst + d) = y;
             }
         }

@@ -23,7 +23,7 @@ template <typename T, int DP> struct ForwardShape {
     static constexpr int kKeys = sizeof(T) == 4 && DP == 256 ? 32 : 64;
     static constexpr int kWaves = 4;
     static constexpr int kQueries = 32 * kWaves;
-    static constexpr int kOccupancy = sizeof(T) * DP <= 256 ? 2 : 1;
+    static constexpr int kOccupancy = sizeof(T) * DP <= 128 ? 3 : sizeof(T) * DP <= 256 ? 2 : 1;
 };
 
 template <typename T, int DP, bool SIDE>
@@ -41,13 +41,10 @@ attend_forward(const Args p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q_blocks = (p.Lq + QT - 1) / QT;
     const int group = p.H / p.Hkv;
-    // the queries of a key head together; long causal rows first
-    int id = xcd_order(blockIdx.x, gridDim.x);
-    const int qb = q_blocks - 1 - id % q_blocks;
-    id /= q_blocks;
-    const int split = id % p.splits;
-    id /= p.splits;
-    const int head = id % p.H, b = id / p.H;
+    const Share share(blockIdx.x, q_blocks, p.B * p.H * p.splits);
+    const int qb = q_blocks - 1 - share.block; // the last see most
+    const int split = share.head % p.splits, head = share.head / p.splits % p.H;
+    const int b = share.head / p.splits / p.H;
     const int kvh = head / group;
 
     const int q0 = qb * QT, qw = q0 + 32 * wave, qi = qw + (lane & 31);

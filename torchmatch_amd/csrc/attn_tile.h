@@ -309,14 +309,20 @@ struct Limits {
     }
 };
 
-// tanh(y) by exp and a reciprocal: the error, 2e-7, is absolute, and what it
-// multiplies is a score.  float32 products leave the time for the library's.
-template <typename T> __device__ inline float cap_tanh(float y) {
-    if constexpr (sizeof(T) == 4)
-        return tanhf(y);
-    const float e = __builtin_amdgcn_exp2f(y * (2.f * kLog2e));
-    return fmaf(-2.f, __builtin_amdgcn_rcpf(e + 1.f), 1.f);
-}
+// The cap, out tanh(in x), by exp and a reciprocal: with r = 1 / (e^(2 in x) + 1),
+// tanh = 1 - 2 r and its derivative is 4 r (1 - r).  The error, 2e-7 of the cap, is absolute,
+// and what it is added to is a score.  float32 products leave the time for the library's tanh.
+template <typename T> struct Cap {
+    float in, out; // times 2 log2 e; times log2 e
+    __device__ inline Cap(const Args &p)
+        : in(p.scale / p.cap * (2.f * kLog2e)), out(p.cap * kLog2e) {}
+    __device__ inline float rest(float x) const { // r
+        if constexpr (sizeof(T) == 4)
+            return 0.5f - 0.5f * tanhf(x * (in / (2.f * kLog2e)));
+        return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * in) + 1.f);
+    }
+    __device__ inline float score(float x) const { return fmaf(-2.f * out, rest(x), out); }
+};
 
 __device__ inline f32x4 away(f32x4 a, float b) {
     return (f32x4){fabsf(a[0] - b), fabsf(a[1] - b), fabsf(a[2] - b), fabsf(a[3] - b)};
@@ -353,10 +359,10 @@ template <typename T, bool SIDE> struct QueryLane {
     __device__ inline void score(const Args &p, f32x16 &s, int k0, int half, const float *k_pos,
                                  int axis) const {
         if (p.cap > 0.f) {
-            const float in = p.scale / p.cap, out = p.cap * kLog2e;
+            const Cap<T> cap(p);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                s[i] = out * cap_tanh<T>(s[i] * in);
+                s[i] = cap.score(s[i]);
         } else if (p.slopes || p.scale < 0.f) {
             const float m = p.scale * kLog2e;
 #pragma unroll
@@ -479,14 +485,17 @@ template <typename T> __device__ inline void put(const Args &p, int64_t at, x4<T
 }
 
 // For the gradients: products s become weights p, products ds = do v become
-// p (ds - delta) slant, the cap's slope included.  Four elements at a time, so that nothing but
+// p (ds - delta), with a cap times a quarter of its slope (grad_scale() has the rest).  Four elements at a time, so that nothing but
 // s and ds is held: bias(n), lse(n) and delta(n) give those of elements 4n .. 4n + 3, in base 2
 // but for delta.
+__device__ inline float grad_scale(const Args &p) {
+    return p.cap > 0.f ? 4.f * p.scale : p.scale;
+}
 template <typename T, bool DS, typename Bias, typename Lse, typename Delta>
 __device__ inline void weigh(const Args &p, f32x16 &s, f32x16 &ds, Bias bias, Lse lse,
                              Delta delta) {
     if (p.cap > 0.f) {
-        const float in = p.scale / p.cap, out = p.cap * kLog2e;
+        const Cap<T> cap(p);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             f32x4 l = lse(n), d;
@@ -494,13 +503,14 @@ __device__ inline void weigh(const Args &p, f32x16 &s, f32x16 &ds, Bias bias, Ls
                 d = delta(n);
             if (p.slopes)
                 l += bias(n);
+            l = cap.out - l;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = 4 * n + e;
-                const float t = cap_tanh<T>(s[i] * in);
-                s[i] = __builtin_amdgcn_exp2f(fmaf(out, t, -l[e]));
+                const float r = cap.rest(s[i]);
+                s[i] = __builtin_amdgcn_exp2f(fmaf(-2.f * cap.out, r, l[e]));
                 if constexpr (DS)
-                    ds[i] = s[i] * (ds[i] - d[e]) * fmaf(-t, t, 1.f);
+                    ds[i] = s[i] * (ds[i] - d[e]) * fmaf(-r, r, r);
             }
         }
     } else {
@@ -577,12 +587,30 @@ struct TileWalk {
     }
 };
 
-// Blocks are dealt to the 8 XCDs in turn; each has its own L2.  Gives every XCD a
+// Blocks are dealt to the 8 XCDs in turn; each has its own L2.  xcd_order() gives every XCD a
 // run of consecutive work items, so that those which read the same keys meet.
 __device__ inline int xcd_order(int id, int n) {
     const int per = n >> 3, rest = n & 7, x = id & 7;
     return x * per + min(x, rest) + (id >> 3);
 }
+
+// Blocks of rows of many heads, the first blocks of a head taking longest (causal): an XCD has
+// its own heads, up to four of them at a time, and starts the long blocks of these first.
+// Where heads do not divide by 8, all XCDs take the long blocks of all heads first.
+struct Share {
+    int block, head;
+    __device__ inline Share(int id, int blocks, int heads) {
+        if (heads & 7) {
+            block = id / heads;
+            head = id % heads;
+            return;
+        }
+        const int own = heads >> 3, at_once = own & 1 ? 1 : own & 2 ? 2 : 4;
+        const int j = id >> 3, run = at_once * blocks;
+        block = j % run / at_once;
+        head = (id & 7) * own + j / run * at_once + j % at_once;
+    }
+};
 
 } // namespace attn
 
