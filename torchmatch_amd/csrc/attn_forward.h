@@ -18,18 +18,28 @@
 
 namespace attn {
 
-template <typename T, int DP> struct ForwardShape {
-    // float32 rows of 256: 32 keys at a time, so that both tiles fit in LDS
-    static constexpr int kKeys = sizeof(T) == 4 && DP == 256 ? 32 : 64;
+template <typename T, int DP, bool SIDE> struct ForwardShape {
     static constexpr int kWaves = 4;
     static constexpr int kQueries = 32 * kWaves;
-    static constexpr int kOccupancy = sizeof(T) * DP <= 128 ? 3 : sizeof(T) * DP <= 256 ? 2 : 1;
+    // One wave issues a vector instruction every 8 cycles at most, two or three together one
+    // every 4, and the weights take as long as the products: what counts is waves a SIMD, and
+    // with it registers.  Three up to 128 bytes a row; with 256 bytes only where there are no
+    // documents and positions, and 32 keys at a time (causal, 32768 rows of 128 features, 16
+    // heads: 4.5 ms in place of 4.8; packed documents 192 us, 267 with three).
+    static constexpr int kBytes = sizeof(T) * DP;
+    static constexpr int kOccupancy = kBytes <= 128 || (kBytes <= 256 && !SIDE) ? 3
+                                      : kBytes <= 256                          ? 2
+                                                                               : 1;
+    // float32 rows of 256: 32 keys at a time, so that two tiles of k and v fit in LDS
+    static constexpr int kKeys = kBytes == 1024 || (kBytes > 128 && kBytes <= 256 && !SIDE)
+                                     ? 32
+                                     : 64;
 };
 
 template <typename T, int DP, bool SIDE>
-__global__ __launch_bounds__(256, (ForwardShape<T, DP>::kOccupancy)) void
+__global__ __launch_bounds__(256, (ForwardShape<T, DP, SIDE>::kOccupancy)) void
 attend_forward(const Args p) {
-    using S = ForwardShape<T, DP>;
+    using S = ForwardShape<T, DP, SIDE>;
     using L = Tile<T, DP>;
     constexpr int KT = S::kKeys, KB = KT / 32, QT = S::kQueries, C = DP / 16, DB = DP / 32;
     __shared__ u32x4 sk0[KT * L::U], sk1[KT * L::U];
@@ -274,9 +284,8 @@ __global__ __launch_bounds__(256) void attend_join(const Args p) {
 }
 
 template <typename T, int DP> int run_forward(const Args &a, hipStream_t s) {
-    const int64_t blocks = (int64_t)((a.Lq + ForwardShape<T, DP>::kQueries - 1) /
-                                     ForwardShape<T, DP>::kQueries) *
-                           a.splits * a.H * a.B;
+    constexpr int Q = ForwardShape<T, DP, true>::kQueries;
+    const int64_t blocks = (int64_t)((a.Lq + Q - 1) / Q) * a.splits * a.H * a.B;
     if (a.q_docs || a.q_pos)
         attend_forward<T, DP, true><<<dim3((unsigned)blocks), 256, 0, s>>>(a);
     else

@@ -422,6 +422,13 @@ template <typename T> constexpr float weight_shift() {
     return __is_same(T, _Float16) ? 7.f : 0.f;
 }
 
+// max over the wave's halves, of each column
+__device__ inline float max_halves(float x) {
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false,
+                                                    false);
+    return fmaxf(__int_as_float(y[0]), __int_as_float(y[1]));
+}
+
 // One step of the running softmax: scores s (keys by queries), which times mul >= 0 are in
 // base 2, become weights 2^(s mul - top).  `top` follows the largest score seen only when that
 // grew by more than 2^8: weights up to 2^8 cost no precision in float32 sums, and the output
@@ -435,7 +442,7 @@ __device__ inline void soften(f32x16 (&s)[KB], f32x16 (&o)[DB], float mul, float
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             m = fmaxf(m, s[kb][i]);
-    m = fmaxf(m, __shfl_xor(m, 32));
+    m = max_halves(m);
     // s mul - top in one rounding leaves the rounding of top in the weights, all of a row by
     // the same factor; past 2^11 that would show in 16 bits, so there products come first and
     // the largest weight stays a power of two

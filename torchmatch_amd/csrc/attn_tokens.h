@@ -89,6 +89,7 @@ attend_tokens(const Args p) {
     for (int i = 0; i < DB; ++i)
         o[i] = f32x16{};
     float top = -kInf, sum = 0.f;
+    const float factor = rows.factor(p);
 
     u32x4 *sk = tiles[wave][0], *sv = tiles[wave][1];
     Stage<T, DP, 32, 64> gk, gv;
@@ -152,7 +153,7 @@ attend_tokens(const Args p) {
         rows.score(p, s[0], k0, half, &s_pos[wave][0][0], 32);
         if (masked)
             rows.hide(p, s[0], -kInf, k0, half, s_docs[wave]);
-        soften<T>(s, o, rows.factor(p), top, sum);
+        soften<T>(s, o, factor, top, sum);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const x8<T> w = pack8<T>(s[0], t);
