@@ -51,9 +51,10 @@ size_t docs_bytes(const tm_attention *a) {
 bool few(const tm_attention *a) { return a->Lq <= 32; }
 
 // Keys are split over blocks when there are too few rows to fill the chip.  Few queries are
-// bound by reading the keys: about four blocks for each of the 256 compute units keep them
-// busy whatever the rows' lengths, with a tile of 64 keys or more for each of a block's
-// 8 waves.  Else a block needs at least four tiles, so that its start and the join are worth it.
+// bound by reading the keys, by one block of 8 waves a compute unit: two such blocks for each
+// of the 256 in turn where rows are equally long, four where their lengths differ, so that
+// the short ones leave no unit idle, and at least 32 keys a wave.  Else a block needs at least
+// four tiles, so that its start and the join are worth it.
 struct Splits {
     int n, tiles;
 };
@@ -62,8 +63,8 @@ Splits splits_of(const tm_attention *a) {
     int64_t blocks, want, most;
     if (few(a)) {
         blocks = (int64_t)((a->H / a->Hkv * a->Lq + 31) / 32) * a->Hkv * a->B;
-        want = (1024 + blocks - 1) / blocks;
-        most = tiles / 8;
+        want = std::max<int64_t>(1, (a->lengths ? 1024 : 512) / blocks);
+        most = tiles / 4;
     } else {
         blocks = (int64_t)((a->Lq + 127) / 128) * a->H * a->B;
         want = blocks >= 256 ? 1 : (512 + blocks - 1) / blocks;

@@ -258,7 +258,13 @@ __device__ inline void bring_word(void *to, const void *from) {
                                      (__attribute__((address_space(3))) void *)to, 4, 0, 0);
 }
 
-__device__ inline void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// Waits until at most LATER of this wave's loads are not there yet; they arrive in order.
+template <int LATER = 0> __device__ inline void arrived() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LATER) : "memory");
+}
+
+// What is read from LDS into the result x has been read past this point.
+__device__ inline void made_here(f32x16 &x) { asm volatile("" : "+v"(x)::"memory"); }
 
 // LDS writes of a wave are seen by its later reads as they are: both go through in order.
 // This keeps the compiler from moving them.
