@@ -11,7 +11,7 @@ namespace attn {
 struct Args {
     const void *q, *k, *v, *dout;
     void *out, *out_low, *dq, *dk, *dv; // contiguous (B, L, heads, D); out_low may be null
-    float *lse; // (B, H, Lq), natural logarithm, -inf for empty rows; backward: base 2, +inf
+    float *lse; // (B, H, Lq), natural logarithm, -inf for empty rows; backward: see attend_delta
     const float *delta;       // (B, H, Lq): sum over d of out * dout
     const float *slopes;      // (H) or null
     const float *q_pos, *k_pos; // (B, L, axes), or null: distance of indices

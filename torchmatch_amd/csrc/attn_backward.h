@@ -47,7 +47,7 @@ attend_backward_kv(const Args p) {
     using B = Bring<T, DP, QT, 256>;
     __shared__ u32x4 sq0[TEAMS][QT * L::U], sq1[TEAMS][QT * L::U];
     __shared__ u32x4 so0[TEAMS][QT * L::U], so1[TEAMS][QT * L::U];
-    // of the tile's queries: the log of the sum (base 2), delta, positions; documents
+    // of the tile's queries: where exponents start, delta, positions; documents
     __shared__ __attribute__((aligned(16))) float s_row0[TEAMS][5][64], s_row1[TEAMS][5][64];
     __shared__ __attribute__((aligned(16))) int s_docs0[TEAMS][64], s_docs1[TEAMS][64];
     // k and v, and at the end the second team's results, 32 x DP floats a wave
@@ -229,7 +229,7 @@ attend_backward_kv(const Args p) {
             }
             const float from = (float)(kj - q0 - 32 * qb - 4 * half - lim.offset);
             weigh<T, DK>(
-                p, s, ds,
+                p, s, ds, slope,
                 [&](int n) -> f32x4 {
                     const int j = 32 * qb + 8 * n + 4 * half;
                     f32x4 d;
@@ -243,7 +243,7 @@ attend_backward_kv(const Args p) {
                         d = away(f32x4{8.f * n, 8.f * n + 1.f, 8.f * n + 2.f, 8.f * n + 3.f},
                                  from);
                     }
-                    return d * slope;
+                    return d;
                 },
                 [&](int n) { return *(const f32x4 *)(s_row[0] + 32 * qb + 8 * n + 4 * half); },
                 [&](int n) { return *(const f32x4 *)(s_row[1] + 32 * qb + 8 * n + 4 * half); });
@@ -401,7 +401,7 @@ attend_backward_q(const Args p) {
         of[c] = global8<T>(dout, 16 * c + 8 * half, p.D, q_real);
     }
     const int64_t row = ((int64_t)b * p.H + head) * p.Lq + qi;
-    const float lse = qi < p.Lq ? p.lse[row] : kInf;
+    const float base = qi < p.Lq ? p.lse[row] : -kInf;
     const float delta = qi < p.Lq ? p.delta[row] : 0.f;
 
     constexpr int per64 = 64 / KT;
@@ -481,12 +481,11 @@ attend_backward_q(const Args p) {
                 ds = mma32(L::row8(sv, row_at, 32 * kb, c), of[c], ds);
             }
             weigh<T, true>(
-                p, s, ds,
+                p, s, ds, rows.slope,
                 [&](int n) {
-                    return rows.distance(p, n, k0 + 32 * kb, half, &s_pos[0][32 * kb], 64) *
-                           rows.slope;
+                    return rows.distance(p, n, k0 + 32 * kb, half, &s_pos[0][32 * kb], 64);
                 },
-                [&](int) { return f32x4{lse, lse, lse, lse}; },
+                [&](int) { return f32x4{base, base, base, base}; },
                 [&](int) { return f32x4{delta, delta, delta, delta}; });
             if (masked)
                 rows.hide(p, ds, 0.f, k0 + 32 * kb, half, s_docs + 32 * kb);
@@ -534,8 +533,9 @@ attend_backward_q(const Args p) {
         }
 }
 
-// delta of each query and head, and the log of its sum in base 2 (+inf for an empty row, which
-// makes all its weights zero).  16 bytes a thread, DP / E threads a row.  From the output as
+// delta of each query and head, and what the exponents of its weights start from: minus the log
+// of its sum in base 2, plus the cap's share (Cap::score); -inf for an empty row, which makes
+// all its weights zero.  16 bytes a thread, DP / E threads a row.  From the output as
 // it was before it was rounded, in two parts: the rounding alone would add as much error to dq
 // and dk as that of ds does.
 template <typename T, int N> // N threads a row: a power of two, N * E >= D
@@ -567,7 +567,7 @@ __global__ __launch_bounds__(256) void attend_delta(const Args p, const float *l
         const int64_t at = (b * p.H + head) * p.Lq + i;
         const float l = lse[at];
         delta[at] = x;
-        base2[at] = l == -kInf ? kInf : l * kLog2e;
+        base2[at] = l == -kInf ? -kInf : p.cap * kLog2e - l * kLog2e;
     }
 }
 

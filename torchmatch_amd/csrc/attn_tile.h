@@ -497,31 +497,39 @@ template <typename T> __device__ inline void put(const Args &p, int64_t at, x4<T
     }
 }
 
-// For the gradients: products s become weights p, products ds = do v become
-// p (ds - delta), with a cap times a quarter of its slope (grad_scale() has the rest).  Four elements at a time, so that nothing but
-// s and ds is held: bias(n), lse(n) and delta(n) give those of elements 4n .. 4n + 3, in base 2
-// but for delta.
+// For the gradients: products s become weights p, products ds = do v become p (ds - delta), with
+// a cap times a quarter of its slope (grad_scale() has the rest).  Four elements at a time, so
+// that nothing but s and ds is held: dist(n), base(n) and delta(n) give what belongs to elements
+// 4n .. 4n + 3: the distance, what attend_delta left of the log of the row's sum, and delta.
 __device__ inline float grad_scale(const Args &p) {
     return p.cap > 0.f ? 4.f * p.scale : p.scale;
 }
-template <typename T, bool DS, typename Bias, typename Lse, typename Delta>
-__device__ inline void weigh(const Args &p, f32x16 &s, f32x16 &ds, Bias bias, Lse lse,
-                             Delta delta) {
+template <typename T, bool DS, typename Dist, typename Base, typename Delta>
+__device__ inline void weigh(const Args &p, f32x16 &s, f32x16 &ds, float slope, Dist dist,
+                             Base base, Delta delta) {
+    const auto exponent = [&](int n) {
+        f32x4 x = base(n);
+        if (p.slopes) {
+            const f32x4 d = dist(n);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[e] = fmaf(-slope, d[e], x[e]);
+        }
+        return x;
+    };
     if (p.cap > 0.f) {
         const Cap<T> cap(p);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            f32x4 l = lse(n), d;
+            const f32x4 x = exponent(n);
+            f32x4 d;
             if constexpr (DS)
                 d = delta(n);
-            if (p.slopes)
-                l += bias(n);
-            l = cap.out - l;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = 4 * n + e;
                 const float r = cap.rest(s[i]);
-                s[i] = __builtin_amdgcn_exp2f(fmaf(-2.f * cap.out, r, l[e]));
+                s[i] = __builtin_amdgcn_exp2f(fmaf(-2.f * cap.out, r, x[e]));
                 if constexpr (DS)
                     ds[i] = s[i] * (ds[i] - d[e]) * fmaf(-r, r, r);
             }
@@ -530,15 +538,14 @@ __device__ inline void weigh(const Args &p, f32x16 &s, f32x16 &ds, Bias bias, Ls
         const float m = p.scale * kLog2e;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            f32x4 l = lse(n), d;
+            const f32x4 x = exponent(n);
+            f32x4 d;
             if constexpr (DS)
                 d = delta(n);
-            if (p.slopes)
-                l += bias(n);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = 4 * n + e;
-                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], m, -l[e]));
+                s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], m, x[e]));
                 if constexpr (DS)
                     ds[i] = s[i] * (ds[i] - d[e]);
             }
