@@ -346,8 +346,9 @@ enum { TM_POS_F32 = 0, TM_POS_I32 = 1, TM_POS_I64 = 2 };
  * dividing H: query head h reads key head h / (H / Hkv).  They may be strided
  * (strides in elements, D contiguous); addresses and strides must be multiples
  * of 16 bytes and so must D (TM_ERR_INVALID_ARGUMENT, TM_ERR_UNSUPPORTED_SHAPE),
- * D at most tm_attention_max_head_dim(), and rows must be less than
- * TM_ATTENTION_MAX_ROW_BYTES apart.
+ * D at most tm_attention_max_head_dim(), rows must be less than
+ * TM_ATTENTION_MAX_ROW_BYTES apart, and B H (Lq / 32) and B Hkv (Lk / 128), rounded
+ * up, below TM_ATTENTION_MAX_BLOCKS.
  *
  *   s_ij = scale * q_i . k_j
  *   s_ij = cap * tanh(s_ij / cap)                       where cap > 0
@@ -361,7 +362,7 @@ enum { TM_POS_F32 = 0, TM_POS_I32 = 1, TM_POS_I64 = 2 };
  *   with documents: q_docs_i == k_docs_j >= 0.
  * A query that sees nothing gets zeros, lse = -inf and no gradient.  Keys past
  * every limit and rows of negative documents may hold anything, NaN included. */
-enum { TM_ATTENTION_MAX_ROW_BYTES = 1 << 26 };
+enum { TM_ATTENTION_MAX_ROW_BYTES = 1 << 26, TM_ATTENTION_MAX_BLOCKS = 1 << 23 };
 typedef struct tm_attention {
     const void *q, *k, *v;
     int64_t q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h;

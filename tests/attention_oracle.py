@@ -92,9 +92,9 @@ def attention(q, k, v, see, *, scale, cap=0.0, slopes=None, q_positions=None, k_
     e = (u + f) * ds.abs() + z * sees + p * (e + f * (do.abs() @ vv.abs().transpose(2, 3)))
     shared = lambda t: t.unflatten(1, (hkv, group)).sum(2).permute(0, 2, 1, 3)  # noqa: E731
     dq = scale * (ds @ kk)
-    res["dq"] = (back(dq), back(scale * (e @ kk.abs()) + u * dq.abs() + z))
+    res["dq"] = (back(dq), back(abs(scale) * (e @ kk.abs()) + u * dq.abs() + z))
     dk = shared(scale * (ds.transpose(2, 3) @ qq))
-    res["dk"] = (dk, shared(scale * (e.transpose(2, 3) @ qq.abs())) + u * dk.abs() + z)
+    res["dk"] = (dk, shared(abs(scale) * (e.transpose(2, 3) @ qq.abs())) + u * dk.abs() + z)
     dv = shared(p.transpose(2, 3) @ do)
     w = (u + f) * p + z * sees
     res["dv"] = (dv, shared(w.transpose(2, 3) @ do.abs()) + u * dv.abs() + z)

@@ -394,3 +394,59 @@ def test_refusals(device):
                    k_positions=torch.zeros(2, 9, 4, device=device))
     with pytest.raises(NotImplementedError, match="slopes"):
         att.attend(q, k, k, slopes=slopes.clone().requires_grad_(True))
+
+
+def test_opcheck(device):
+    """Schemas, fake kernels and autograd registration agree with the kernels."""
+    q = torch.randn(2, 40, 4, 32, device=device, requires_grad=True)
+    k = torch.randn(2, 70, 2, 32, device=device, requires_grad=True)
+    v = torch.randn(2, 70, 2, 32, device=device, requires_grad=True)
+    tests = ("test_schema", "test_faketensor", "test_autograd_registration")
+    torch.library.opcheck(torch.ops.attention.attend.default, (q, k, v), {"scale": 0.2},
+                          test_utils=tests)
+    lengths = torch.tensor([70, 9], dtype=torch.int32, device=device)
+    torch.library.opcheck(torch.ops.attention.attend.default,
+                          (q.bfloat16(), k.bfloat16(), v.bfloat16()),
+                          {"scale": 0.2, "cap": 3.0, "causal": True, "lengths": lengths},
+                          test_utils=tests)
+    freqs = att.rotary_frequencies((8, 8))
+    pos = torch.rand(2, 40, 2, device=device)
+    torch.library.opcheck(torch.ops.attention.rotate.default, (q, pos, freqs, [8, 8]),
+                          test_utils=tests)
+
+
+def test_second_derivative_is_refused(device):
+    q, k, v = (torch.randn(1, 8, 2, 32, device=device, requires_grad=True) for _ in range(3))
+    (g,) = torch.autograd.grad(att.attend(q, k, v).square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="derivative|not implemented"):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h,hkv,b", [(2, 2, 4), (1, 1, 5), (16, 4, 2), (3, 1, 1)])
+def test_many_heads_and_batches(device, dtype, h, hkv, b):
+    """Heads that do and do not divide by the chip's eight dies."""
+    _case(device, dtype, b, 260, 260, h, hkv, 64, causal=True, seed=h + b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_documents_of_every_head_dim(device, dtype, d):
+    rows = [_ids((0, 70), (-1, 9), (2, 130), (3, 41))]
+    _case(device, dtype, 1, 250, 250, 4, 2, d, causal=True, docs=rows, axes=2, cap=10.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_negative_and_zero_scale(device, dtype):
+    g = torch.Generator().manual_seed(23)
+    q, k, v, do = (torch.randn(1, n, 2, 64, generator=g).to(dtype).to(device)
+                   for n in (50, 90, 90, 50))
+    see = visible(1, 50, 90)
+    for scale in (-0.2, 0.0):
+        for t in (q, k, v):
+            t.requires_grad_(True)
+        out = att.attend(q, k, v, scale=scale)
+        want = attention(q, k, v, see, scale=scale, dout=do)
+        assert_within(out, *want["out"], "out")
+        for name, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), do)):
+            assert_within(x, *want[name], name)

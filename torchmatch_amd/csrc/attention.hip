@@ -85,7 +85,10 @@ int check(const tm_attention *a) {
     const int unit = a->dtype == TM_F32 ? 4 : 8;
     if (a->D > tm_attention_max_head_dim() || a->D % unit)
         return TM_ERR_UNSUPPORTED_SHAPE;
-    if ((int64_t)a->B * ((a->Lq + 63) / 64 + (a->Lk + 63) / 64 + 1) * a->H >= INT32_MAX)
+    // blocks of up to 512 threads, of which a launch takes less than 2^32
+    if (a->Lq > INT32_MAX - 256 || a->Lk > INT32_MAX - 256 ||
+        a->B * std::max((int64_t)a->H * ((a->Lq + 31) / 32),
+                        (int64_t)a->Hkv * ((a->Lk + 127) / 128)) >= TM_ATTENTION_MAX_BLOCKS)
         return TM_ERR_UNSUPPORTED_SHAPE;
     if (!(a->scale == a->scale) || !(a->cap >= 0.f) || (!a->q_docs != !a->k_docs) ||
         (!a->q_positions != !a->k_positions) || (a->q_positions && !a->slopes))

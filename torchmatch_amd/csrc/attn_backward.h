@@ -14,6 +14,8 @@
 #ifndef TORCHMATCH_AMD_ATTN_BACKWARD_H
 #define TORCHMATCH_AMD_ATTN_BACKWARD_H
 
+#include <algorithm>
+
 #include "attn_tile.h"
 
 namespace attn {
@@ -542,32 +544,35 @@ template <typename T, int N> // N threads a row: a power of two, N * E >= D
 __global__ __launch_bounds__(256) void attend_delta(const Args p, const float *lse,
                                                     float *base2, float *delta) {
     constexpr int E = 16 / (int)sizeof(T);
-    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) / N;
+    typedef T unit __attribute__((ext_vector_type(E)));
     const int d = (int)threadIdx.x % N * E;
-    const bool real = row < (int64_t)p.B * p.Lq * p.H;
-    const int head = (int)(row % p.H), i = (int)(row / p.H % p.Lq);
-    const int64_t b = row / p.H / p.Lq;
-    float x = 0.f;
-    if (real && d < p.D) {
-        typedef T unit __attribute__((ext_vector_type(E)));
-        const unit u = *(const unit *)((const T *)p.out + row * p.D + d);
-        const unit w =
-            *(const unit *)((const T *)p.dout + b * p.do_b + i * p.do_l + head * p.do_h + d);
-        unit r = u;
-        if (p.out_low)
-            r = *(const unit *)((const T *)p.out_low + row * p.D + d);
+    const int64_t rows = (int64_t)p.B * p.Lq * p.H;
+    for (int64_t first = (int64_t)blockIdx.x * (256 / N); first < rows;
+         first += (int64_t)gridDim.x * (256 / N)) {
+        const int64_t row = first + threadIdx.x / N;
+        const int head = (int)(row % p.H), i = (int)(row / p.H % p.Lq);
+        const int64_t b = row / p.H / p.Lq;
+        float x = 0.f;
+        if (row < rows && d < p.D) {
+            const unit u = *(const unit *)((const T *)p.out + row * p.D + d);
+            const unit w = *(const unit *)((const T *)p.dout + b * p.do_b + i * p.do_l +
+                                           head * p.do_h + d);
+            unit r = u;
+            if (p.out_low)
+                r = *(const unit *)((const T *)p.out_low + row * p.D + d);
 #pragma unroll
-        for (int j = 0; j < E; ++j)
-            x = fmaf((float)u[j] + (p.out_low ? (float)r[j] : 0.f), (float)w[j], x);
-    }
+            for (int j = 0; j < E; ++j)
+                x = fmaf((float)u[j] + (p.out_low ? (float)r[j] : 0.f), (float)w[j], x);
+        }
 #pragma unroll
-    for (int n = N / 2; n; n >>= 1)
-        x += __shfl_xor(x, n);
-    if (real && d == 0) {
-        const int64_t at = (b * p.H + head) * p.Lq + i;
-        const float l = lse[at];
-        delta[at] = x;
-        base2[at] = l == -kInf ? -kInf : p.cap * kLog2e - l * kLog2e;
+        for (int n = N / 2; n; n >>= 1)
+            x += __shfl_xor(x, n);
+        if (row < rows && d == 0) {
+            const int64_t at = (b * p.H + head) * p.Lq + i;
+            const float l = lse[at];
+            delta[at] = x;
+            base2[at] = l == -kInf ? -kInf : p.cap * kLog2e - l * kLog2e;
+        }
     }
 }
 
@@ -575,7 +580,9 @@ template <typename T>
 int run_delta(const Args &a, const float *lse, float *base2, float *delta, hipStream_t s) {
     const int64_t rows = (int64_t)a.B * a.Lq * a.H;
     const int units = a.D * (int)sizeof(T) / 16;
-    const auto grid = [&](int n) { return dim3((unsigned)((rows * n + 255) / 256)); };
+    const auto grid = [&](int n) {
+        return dim3((unsigned)std::min<int64_t>((rows * n + 255) / 256, 1 << 20));
+    };
     if (units <= 8)
         attend_delta<T, 8><<<grid(8), 256, 0, s>>>(a, lse, base2, delta);
     else if (units <= 16)

@@ -163,41 +163,6 @@ template <typename T, int DP> struct Tile {
     }
 };
 
-// The part of a tile that each of NT threads brings from memory: loaded into
-// registers early, written to LDS when the tile before it is done with.
-template <typename T, int DP, int ROWS, int NT> struct Stage {
-    using L = Tile<T, DP>;
-    static constexpr int N = (ROWS * L::U0 + NT - 1) / NT;
-    u32x4 r[N];
-
-    // rows row0 + 0 .. ROWS - 1 of a matrix of `rows` rows (stride elements
-    // apart, d of them real); what lies outside is zero, and so are rows whose
-    // id is negative (ids may be null): they may hold anything
-    __device__ inline void load(const T *base, int64_t stride, int row0, int rows, int d,
-                                const int32_t *ids, int tid) {
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int i = tid + n * NT;
-            const int row = i / L::U0, u = i % L::U0;
-            const int at = row0 + row;
-            u32x4 x = {0u, 0u, 0u, 0u};
-            if ((ROWS * L::U0 % NT == 0 || row < ROWS) && at < rows && u * L::E < d &&
-                !(ids && ids[at] < 0))
-                x = *(const u32x4 *)(base + (int64_t)at * stride + u * L::E);
-            r[n] = x;
-        }
-    }
-    __device__ inline void store(u32x4 *t, int tid) const {
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int i = tid + n * NT;
-            const int row = i / L::U0, u = i % L::U0;
-            if (ROWS * L::U0 % NT == 0 || row < ROWS)
-                t[L::at(row, u)] = r[n];
-        }
-    }
-};
-
 // A tile brought from memory straight into LDS by NT threads, without passing through
 // registers.  A wave's 64 units land next to each other, so the permutation of a row's units
 // is made on the side of the addresses: a scalar row and 32 bits a lane.  Features past the
@@ -358,7 +323,7 @@ template <typename T, bool SIDE> struct QueryLane {
     // What scores must be multiplied with after score(): plain products wait for the
     // exponential, which takes the factor along.
     __device__ static inline float factor(const Args &p) {
-        return p.cap > 0.f || p.slopes || p.scale < 0.f ? 1.f : p.scale * kLog2e;
+        return p.cap > 0.f || p.slopes || !(p.scale > 0.f) ? 1.f : p.scale * kLog2e;
     }
     // s: products with keys k0 ..; to scores times log2 e but for factor().  k_pos: the block's
     // positions in LDS, `axis` apart.
@@ -369,7 +334,7 @@ template <typename T, bool SIDE> struct QueryLane {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 s[i] = cap.score(s[i]);
-        } else if (p.slopes || p.scale < 0.f) {
+        } else if (p.slopes || !(p.scale > 0.f)) {
             const float m = p.scale * kLog2e;
 #pragma unroll
             for (int i = 0; i < 16; ++i)

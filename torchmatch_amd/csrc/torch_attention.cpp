@@ -10,6 +10,8 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <cmath>
 #include <tuple>
 #include <vector>
 
@@ -54,7 +56,8 @@ Tensor readable(const Tensor &t) {
         return at::constant_pad_nd(t, {0, unit - d % unit}).contiguous();
     const bool ok = (d == 1 || t.stride(3) == 1) && step_of(t, 0) % unit == 0 &&
                     step_of(t, 1) % unit == 0 &&
-                    step_of(t, 1) * t.element_size() < TM_ATTENTION_MAX_ROW_BYTES && step_of(t, 2) % unit == 0 &&
+                    step_of(t, 1) * t.element_size() < TM_ATTENTION_MAX_ROW_BYTES &&
+                    step_of(t, 2) % unit == 0 &&
                     reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
     return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
@@ -115,7 +118,10 @@ Problem problem(const Tensor &q, const Tensor &k, const Tensor &v, const OptTens
     TORCH_CHECK_VALUE(D >= 1 && D <= tm_attention_max_head_dim(), "attend: heads hold 1 to ",
                       tm_attention_max_head_dim(), " features, got ", D);
     TORCH_CHECK_VALUE(B <= INT32_MAX && Lq <= INT32_MAX - 256 && Lk <= INT32_MAX - 256 &&
-                          B * ((Lq + 63) / 64 + (Lk + 63) / 64 + 1) * H < INT32_MAX,
+                          H <= INT32_MAX &&
+                          (double)B * std::max((double)H * (double)((Lq + 31) / 32),
+                                               (double)Hkv * (double)((Lk + 127) / 128)) <
+                              TM_ATTENTION_MAX_BLOCKS,
                       "attend: too many rows for one call: q ", q.sizes(), ", k ", k.sizes());
     TORCH_CHECK_VALUE(std::isfinite(scale), "attend: scale must be finite, got ", scale);
     TORCH_CHECK_VALUE(cap >= 0. && std::isfinite(cap),
