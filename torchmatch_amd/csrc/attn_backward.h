@@ -494,9 +494,19 @@ attend_backward_q(const Args p) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const x8<T> w = pack8<T>(ds, t);
+                x8<T> rest = w;
+                if constexpr (sizeof(T) == 2) {
 #pragma unroll
-                for (int i = 0; i < DB; ++i)
-                    dq[i] = mma32(L::col8(sk, col_at, 32 * kb + 16 * t, i), w, dq[i]);
+                    for (int j = 0; j < 8; ++j)
+                        rest[j] = (T)(ds[8 * t + j] - (float)w[j]);
+                }
+#pragma unroll
+                for (int i = 0; i < DB; ++i) {
+                    const x8<T> kt = L::col8(sk, col_at, 32 * kb + 16 * t, i);
+                    dq[i] = mma32(kt, w, dq[i]);
+                    if constexpr (sizeof(T) == 2)
+                        dq[i] = mma32(kt, rest, dq[i]);
+                }
             }
         }
     };
