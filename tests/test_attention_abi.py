@@ -33,6 +33,7 @@ def _forward(**changes):
     ({"D": 264}, _native.TM_ERR_UNSUPPORTED_SHAPE),
     ({"scale": float("nan")}, _native.TM_ERR_INVALID_ARGUMENT),
     ({"cap": -1.0}, _native.TM_ERR_INVALID_ARGUMENT),
+    ({"cap": 2000.0}, _native.TM_ERR_UNSUPPORTED_SHAPE),
     ({"q_docs": 4096}, _native.TM_ERR_INVALID_ARGUMENT),
     ({"slopes": 4096, "q_positions": 4096, "axes": 1}, _native.TM_ERR_INVALID_ARGUMENT),
     ({"q_positions": 4096, "k_positions": 4096, "axes": 1}, _native.TM_ERR_INVALID_ARGUMENT),

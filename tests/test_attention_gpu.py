@@ -88,6 +88,17 @@ def test_prefix_and_lengths(device, dtype):
     _case(device, dtype, 3, 70, 200, 2, 1, 64, lengths=[0, 65, 200])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cap", [0.25, 100.0, 1024.0])
+def test_small_and_large_caps(device, dtype, cap):
+    """Large caps leave scores nearly as they are: nothing may be lost to their size.  The
+    16-bit kernels' tanh is good to 2^-22 of the cap; a cap of 1024 adds 2^-12 to what
+    weights may be off, less than a float16 rounding."""
+    if dtype == torch.float16 and cap > 500:
+        cap = 500.0  # 2^-13: stays within the 2^-11 of a weight's rounding
+    _case(device, dtype, 1, 90, 150, 2, 2, 64, cap=cap, causal=False)
+
+
 def _ids(*parts):
     return [i for i, n in parts for _ in range(n)]
 
@@ -373,6 +384,8 @@ def test_refusals(device):
             1, 1, 1, 300, device=device)]))
     with pytest.raises(ValueError, match="cap"):
         att.attend(q, k, k, cap=-1.0)
+    with pytest.raises(ValueError, match="at most 1024"):
+        att.attend(q.half(), k.half(), k.half(), cap=2000.0)
     with pytest.raises(ValueError, match="scale"):
         att.attend(q, k, k, scale=float("nan"))
     with pytest.raises(ValueError, match="causal"):

@@ -11,6 +11,9 @@ import torch
 
 from torchmatch_amd.attention import ops
 
+# the overloads themselves: resolving them takes microseconds of every call
+_ATTEND, _ROTATE = ops.attend.default, ops.rotate.default
+
 
 def _on_device(t: torch.Tensor, who: str, name: str) -> None:
     if not isinstance(t, torch.Tensor):
@@ -54,7 +57,7 @@ def attend(  # noqa: PLR0913
     and query head h reads key head ``h // (H // Hkv)``.
 
     Scores are ``scale * q.k`` (``scale`` is ``D ** -0.5`` by default), then
-    ``cap * tanh(score / cap)`` where ``cap > 0``, then less
+    ``cap * tanh(score / cap)`` where ``cap > 0`` (at most 1024 for 16-bit types), then less
     ``slopes[h]`` times the distance of the pair: of ``q_positions`` (B, Lq, axes) and
     ``k_positions`` (B, Lk, axes), summed over 1 to 3 axes, or of the indices where no
     positions are given.  What a query sees:
@@ -63,7 +66,7 @@ def attend(  # noqa: PLR0913
     * ``causal``: query i stands at ``i + length - Lq`` and sees keys up to there, and the
       first ``prefix[b]`` keys wherever it stands;
     * ``q_docs`` (B, Lq), ``k_docs`` (B, Lk): keys of the same document; negative ids are
-      padding.  ``k_docs`` is ``q_docs`` where it is not given.
+      padding, and ids fit 32 bits.  ``k_docs`` is ``q_docs`` where it is not given.
 
     A query that sees nothing gets zeros, and ``-inf`` for its log-sum.  Any strides;
     features contiguous and rows 16-byte aligned are read in place, else copied.
@@ -85,8 +88,8 @@ def attend(  # noqa: PLR0913
         lengths = _rows(lengths, batch, 1, torch.int32)
         q_positions = _rows(q_positions, batch, 3, torch.float32)
         k_positions = _rows(k_positions, batch, 3, torch.float32)
-    out, lse = ops.attend(q, k, v, slopes, q_positions, k_positions, q_docs, k_docs, prefix,
-                          lengths, scale=scale, cap=cap, causal=causal)
+    out, lse = _ATTEND(q, k, v, slopes, q_positions, k_positions, q_docs, k_docs, prefix,
+                       lengths, scale=scale, cap=cap, causal=causal)
     return (out, lse) if return_lse else out
 
 
@@ -129,4 +132,4 @@ def rotate(
     _on_device(x, "rotate", "x")
     if positions.ndim == 2 and x.ndim == 4:
         positions = positions.unsqueeze(0).expand(x.shape[0], -1, -1)
-    return ops.rotate(x, positions, freqs, sections, interleaved, inverse)
+    return _ROTATE(x, positions, freqs, sections, interleaved, inverse)

@@ -90,6 +90,8 @@ int check(const tm_attention *a) {
         a->B * std::max((int64_t)a->H * ((a->Lq + 31) / 32),
                         (int64_t)a->Hkv * ((a->Lk + 127) / 128)) >= TM_ATTENTION_MAX_BLOCKS)
         return TM_ERR_UNSUPPORTED_SHAPE;
+    if (a->dtype != TM_F32 && a->cap > TM_ATTENTION_MAX_CAP_16)
+        return TM_ERR_UNSUPPORTED_SHAPE;
     if (!(a->scale == a->scale) || !(a->cap >= 0.f) || (!a->q_docs != !a->k_docs) ||
         (!a->q_positions != !a->k_positions) || (a->q_positions && !a->slopes))
         return TM_ERR_INVALID_ARGUMENT;

@@ -546,7 +546,7 @@ attend_backward_q(const Args p) {
 }
 
 // delta of each query and head, and what the exponents of its weights start from: minus the log
-// of its sum in base 2, plus the cap's share (Cap::score); -inf for an empty row, which makes
+// of its sum in base 2, plus the cap's share (Cap); -inf for an empty row, which makes
 // all its weights zero.  16 bytes a thread, DP / E threads a row.  From the output as
 // it was before it was rounded, in two parts: the rounding alone would add as much error to dq
 // and dk as that of ds does.
@@ -581,7 +581,7 @@ __global__ __launch_bounds__(256) void attend_delta(const Args p, const float *l
             const int64_t at = (b * p.H + head) * p.Lq + i;
             const float l = lse[at];
             delta[at] = x;
-            base2[at] = l == -kInf ? -kInf : p.cap * kLog2e - l * kLog2e;
+            base2[at] = l == -kInf ? -kInf : Cap<T>::share(p) - l * kLog2e;
         }
     }
 }

@@ -280,19 +280,31 @@ struct Limits {
     }
 };
 
-// The cap, out tanh(in x), by exp and a reciprocal: with r = 1 / (e^(2 in x) + 1),
-// tanh = 1 - 2 r and its derivative is 4 r (1 - r).  The error, 2e-7 of the cap, is absolute,
-// and what it is added to is a score.  float32 products leave the time for the library's tanh.
+// The cap, cap tanh(scale x / cap) in base 2.  For 16-bit inputs by exp and a reciprocal: with
+// r = 1 / (e^(2 y) + 1), tanh y = 1 - 2 r and its derivative is 4 r (1 - r).  The error, 2e-7 of
+// the cap, is absolute, and what it is added to is a score: caps up to 1024 stay below
+// the rounding of float16 weights.  float32 products leave the time for the library's tanh.
 template <typename T> struct Cap {
-    float in, out; // times 2 log2 e; times log2 e
+    static constexpr bool kByExp = sizeof(T) == 2;
+    float in, out;
     __device__ inline Cap(const Args &p)
-        : in(p.scale / p.cap * (2.f * kLog2e)), out(p.cap * kLog2e) {}
-    __device__ inline float rest(float x) const { // r
-        if constexpr (sizeof(T) == 4)
-            return 0.5f - 0.5f * tanhf(x * (in / (2.f * kLog2e)));
-        return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * in) + 1.f);
+        : in(p.scale / p.cap * (kByExp ? 2.f * kLog2e : 1.f)), out(p.cap * kLog2e) {}
+    // r, or tanh
+    __device__ inline float part(float x) const {
+        if constexpr (kByExp)
+            return __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * in) + 1.f);
+        else
+            return tanhf(x * in);
     }
-    __device__ inline float score(float x) const { return fmaf(-2.f * out, rest(x), out); }
+    // the score's distance from share()
+    __device__ inline float add(float part, float to) const {
+        return fmaf(kByExp ? -2.f * out : out, part, to);
+    }
+    __device__ static inline float share(const Args &p) { return kByExp ? p.cap * kLog2e : 0.f; }
+    // a quarter of the derivative
+    __device__ inline float slope(float part) const {
+        return kByExp ? fmaf(-part, part, part) : fmaf(-0.25f * part, part, 0.25f);
+    }
 };
 
 __device__ inline f32x4 away(f32x4 a, float b) {
@@ -331,9 +343,10 @@ template <typename T, bool SIDE> struct QueryLane {
                                  int axis) const {
         if (p.cap > 0.f) {
             const Cap<T> cap(p);
+            const float from = Cap<T>::share(p);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                s[i] = cap.score(s[i]);
+                s[i] = cap.add(cap.part(s[i]), from);
         } else if (p.slopes || !(p.scale > 0.f)) {
             const float m = p.scale * kLog2e;
 #pragma unroll
@@ -493,10 +506,10 @@ __device__ inline void weigh(const Args &p, f32x16 &s, f32x16 &ds, float slope, 
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = 4 * n + e;
-                const float r = cap.rest(s[i]);
-                s[i] = __builtin_amdgcn_exp2f(fmaf(-2.f * cap.out, r, x[e]));
+                const float r = cap.part(s[i]);
+                s[i] = __builtin_amdgcn_exp2f(cap.add(r, x[e]));
                 if constexpr (DS)
-                    ds[i] = s[i] * (ds[i] - d[e]) * fmaf(-r, r, r);
+                    ds[i] = s[i] * (ds[i] - d[e]) * cap.slope(r);
             }
         }
     } else {

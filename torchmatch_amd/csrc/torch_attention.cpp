@@ -126,6 +126,9 @@ Problem problem(const Tensor &q, const Tensor &k, const Tensor &v, const OptTens
     TORCH_CHECK_VALUE(std::isfinite(scale), "attend: scale must be finite, got ", scale);
     TORCH_CHECK_VALUE(cap >= 0. && std::isfinite(cap),
                       "attend: cap must be positive, or 0 for none, got ", cap);
+    TORCH_CHECK_VALUE(p.a.dtype == TM_F32 || cap <= TM_ATTENTION_MAX_CAP_16,
+                      "attend: cap must be at most ", (int)TM_ATTENTION_MAX_CAP_16,
+                      " for 16-bit types, got ", cap);
     TORCH_CHECK_VALUE(q_pos.has_value() == k_pos.has_value(),
                       "attend: give both q_positions and k_positions, or neither");
     TORCH_CHECK_VALUE(!q_pos.has_value() || slopes.has_value(),
