@@ -45,12 +45,25 @@ __device__ inline double position(const RotateArgs &p, int64_t i) {
     }
 }
 
+// (cos, sin) of N consecutive pairs, N even, read 16 bytes at a time
+template <int N> struct Turns {
+    f32x4 w[N / 2];
+    __device__ inline explicit Turns(const float2 *from) {
+#pragma unroll
+        for (int n = 0; n < N / 2; ++n)
+            w[n] = ((const f32x4 *)from)[n];
+    }
+    __device__ inline float2 at(int j) const {
+        return make_float2(w[j / 2][2 * (j % 2)], w[j / 2][2 * (j % 2) + 1]);
+    }
+};
+
 constexpr int kTable = 4096; // (cos, sin) of a block, 32 KB
 
 // V: elements a load (16 bytes, or 1 where strides, sizes or addresses do not allow it)
 template <typename T, int V>
 __global__ __launch_bounds__(256) void rotate_pairs(const RotateArgs p) {
-    __shared__ float2 table[kTable];
+    __shared__ __attribute__((aligned(16))) float2 table[kTable];
     const int64_t first = (int64_t)blockIdx.x * p.per_block;
     const int tokens = (int)min((int64_t)p.per_block, p.tokens - first);
     for (int i = threadIdx.x; i < tokens * p.pairs; i += 256) {
@@ -106,9 +119,10 @@ __global__ __launch_bounds__(256) void rotate_pairs(const RotateArgs p) {
             } else if (p.interleaved) {
                 const U a = *(const U *)(src + item * V);
                 U y;
+                Turns<V / 2> turns(cs);
 #pragma unroll
                 for (int j = 0; j < V / 2; ++j) {
-                    const float2 w = cs[j];
+                    const float2 w = turns.at(j);
                     const float u = (float)a[2 * j], v = (float)a[2 * j + 1];
                     y[2 * j] = (T)(u * w.x - v * w.y);
                     y[2 * j + 1] = (T)(v * w.x + u * w.y);
@@ -118,9 +132,10 @@ __global__ __launch_bounds__(256) void rotate_pairs(const RotateArgs p) {
                 const U a = *(const U *)(src + item * V);
                 const U b = *(const U *)(src + p.pairs + item * V);
                 U y, z;
+                Turns<V> turns(cs);
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float2 w = cs[j];
+                    const float2 w = turns.at(j);
                     const float u = (float)a[j], v = (float)b[j];
                     y[j] = (T)(u * w.x - v * w.y);
                     z[j] = (T)(v * w.x + u * w.y);
