@@ -463,3 +463,13 @@ def test_negative_and_zero_scale(device, dtype):
         assert_within(out, *want["out"], "out")
         for name, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, (q, k, v), do)):
             assert_within(x, *want[name], name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_blocks_of_documents(device, dtype, causal):
+    """More blocks than run at once: those that see most tiles are started first."""
+    rows = [_ids((3, 5), (0, 300), (1, 700), (2, 100)),
+            _ids((0, 900), (-1, 50), (4, 155))]
+    _case(device, dtype, 2, 1105, 1105, 32, 32, 32, causal=causal, docs=rows,
+          lengths=[1105, 1000], qk=0.7)

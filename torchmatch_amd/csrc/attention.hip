@@ -2,7 +2,7 @@
 #include <algorithm>
 
 #include "../../include/torchmatch_amd.h"
-#include "attn.h"
+#include "attn_tile.h"
 
 namespace {
 
@@ -35,6 +35,54 @@ __global__ __launch_bounds__(256) void attend_docs(const int32_t *q_docs, const 
         (keys ? k_tiles : q_tiles)[t] = make_int4(lo, hi, hidden, 0);
 }
 
+// With documents, how long a block of 128 queries or keys takes has nothing to do with where it
+// stands.  Puts those that visit most tiles first, for each batch row: a workgroup counts the
+// tiles of its row's blocks and then ranks them (blockIdx.y 0: queries, 1: keys).
+constexpr int kMaxOrdered = 8192;
+__global__ __launch_bounds__(1024) void attend_order(const Args p, int32_t *q_order,
+                                                     int32_t *k_order) {
+    __shared__ int cost[kMaxOrdered];
+    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool keys = blockIdx.y;
+    const int nq = (p.Lq + 63) / 64, nk = (p.Lk + 63) / 64;
+    const int own = keys ? nk : nq, blocks = (own + 1) / 2; // of two summaries each
+    const int4 *mine_of = (keys ? p.k_tiles : p.q_tiles) + (int64_t)b * own;
+    const int4 *others = (keys ? p.q_tiles + (int64_t)b * nq : p.k_tiles + (int64_t)b * nk);
+    const attn::Limits lim(p, b);
+    for (int i = wave; i < blocks; i += 16) {
+        int4 mine = mine_of[2 * i];
+        if (2 * i + 1 < own) {
+            const int4 o = mine_of[2 * i + 1];
+            mine.x = min(mine.x, o.x);
+            mine.y = max(mine.y, o.y);
+        }
+        int first = 0, end;
+        if (keys) {
+            end = 128 * i < lim.length ? nq : 0;
+            if (lim.causal && 128 * i >= lim.prefix)
+                first = min(nq, max(0, 128 * i - lim.offset) / 64);
+        } else {
+            end = (lim.of(min(128 * i + 128, p.Lq) - 1) + 63) / 64;
+        }
+        int n = 0;
+        for (int t = first; t < end; t += 64) {
+            const bool in = t + lane < end;
+            n += __popcll(__ballot(in && attn::docs_meet(others[min(t + lane, end - 1)], mine)));
+        }
+        if (!lane)
+            cost[i] = n;
+    }
+    __syncthreads();
+    int32_t *order = (keys ? k_order : q_order) + (int64_t)b * blocks;
+    for (int i = threadIdx.x; i < blocks; i += 1024) {
+        const int c = cost[i];
+        int rank = 0;
+        for (int j = 0; j < blocks; ++j)
+            rank += cost[j] > c || (cost[j] == c && (keys ? j < i : j > i));
+        order[rank] = i;
+    }
+}
+
 int padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : d <= 128 ? 128 : 256; }
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -43,7 +91,14 @@ size_t docs_bytes(const tm_attention *a) {
     if (!a->q_docs)
         return 0;
     const size_t tiles = (size_t)a->B * ((a->Lq + 63) / 64 + (a->Lk + 63) / 64);
-    return align256(tiles * sizeof(int4));
+    const size_t blocks = (size_t)a->B * ((a->Lq + 127) / 128 + (a->Lk + 127) / 128);
+    return align256(tiles * sizeof(int4)) + align256(blocks * sizeof(int32_t));
+}
+
+// Worth a launch where the blocks of `rows` rows and `heads` heads are more than run at once.
+bool ordered(const tm_attention *a, int64_t rows, int64_t heads, int at_once) {
+    const int64_t blocks = (rows + 127) / 128;
+    return blocks <= kMaxOrdered && blocks * heads * a->B > at_once;
 }
 
 // Few queries: the kernel that packs the queries of a key head's group into 32 rows.
@@ -139,7 +194,8 @@ Args args_of(const tm_attention *a) {
      : a->dtype == TM_F16 ? attn::call##_f16(__VA_ARGS__)                                         \
                           : attn::call##_f32(__VA_ARGS__))
 
-int summarise_docs(const tm_attention *a, Args &p, char *ws, hipStream_t stream) {
+int summarise_docs(const tm_attention *a, Args &p, char *ws, bool q_order, bool k_order,
+                   hipStream_t stream) {
     if (!a->q_docs)
         return 0;
     const int64_t nq = (a->Lq + 63) / 64, nk = (a->Lk + 63) / 64;
@@ -148,6 +204,14 @@ int summarise_docs(const tm_attention *a, Args &p, char *ws, hipStream_t stream)
     p.k_tiles = k_tiles;
     attend_docs<<<dim3((unsigned)((a->B * (nq + nk) + 3) / 4)), 256, 0, stream>>>(
         a->q_docs, a->k_docs, a->B, a->Lq, a->Lk, q_tiles, k_tiles);
+    if (q_order || k_order) {
+        int32_t *order = (int32_t *)(ws + align256(a->B * (nq + nk) * sizeof(int4)));
+        int32_t *of_keys = order + (int64_t)a->B * ((a->Lq + 127) / 128);
+        attend_order<<<dim3(a->B, k_order ? 2 : 1), 1024, 0, stream>>>(p, order, of_keys);
+        p.q_order = order;
+        if (k_order)
+            p.k_order = of_keys;
+    }
     return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 
@@ -185,7 +249,7 @@ extern "C" int tm_attention_forward(const tm_attention *a, void *out, void *out_
     p.out_low = a->dtype == TM_F32 ? nullptr : out_low;
     p.lse = lse;
     char *ws = (char *)workspace;
-    if (summarise_docs(a, p, ws, stream))
+    if (summarise_docs(a, p, ws, !few(a) && ordered(a, a->Lq, a->H, 512), false, stream))
         return TM_ERR_LAUNCH;
     ws += docs_bytes(a);
     const Splits s = splits_of(a);
@@ -236,7 +300,9 @@ extern "C" int tm_attention_backward(const tm_attention *a, const void *out,
     p.do_b = do_b, p.do_l = do_l, p.do_h = do_h;
     p.dq = dq, p.dk = dk, p.dv = dv;
     char *ws = (char *)workspace;
-    if (summarise_docs(a, p, ws, stream))
+    const bool q_order = a->Lq && ordered(a, a->Lq, a->H, 512);
+    const bool k_order = q_order && a->Lk && ordered(a, a->Lk, a->Hkv, 256);
+    if (summarise_docs(a, p, ws, q_order, k_order, stream))
         return TM_ERR_LAUNCH;
     float *delta = (float *)(ws + docs_bytes(a));
     float *base2 = (float *)((char *)delta +

@@ -17,7 +17,8 @@ struct Args {
     const float *q_pos, *k_pos; // (B, L, axes), or null: distance of indices
     const int32_t *q_docs, *k_docs; // (B, L) or null
     const int4 *q_tiles, *k_tiles;  // (B, L / 64) summaries of the documents, or null
-    const int32_t *prefix, *lengths; // (B) or null
+    const int32_t *q_order, *k_order; // (B, blocks of 128), which to start with first, or null
+    const int32_t *prefix, *lengths;  // (B) or null
     // partial results of a split over keys
     float *part_o;  // (splits, B, H, Lq, DP)
     float2 *part_ml; // (splits, B, H, Lq): what weights are relative to (base 2), their sum

@@ -62,8 +62,9 @@ attend_backward_kv(const Args p) {
     const int k_blocks = (p.Lk + 127) / 128;
     const int group = p.H / p.Hkv;
     const Share share(blockIdx.x, k_blocks, p.B * p.Hkv);
-    const int kb = share.block; // the first are seen by most
     const int kvh = share.head % p.Hkv, b = share.head / p.Hkv;
+    const int kb = SIDE && p.k_order ? scalar(p.k_order[(int64_t)b * k_blocks + share.block])
+                                     : share.block; // the first are seen by most
     const int k0 = 128 * kb, kw = k0 + 32 * wave, kj = kw + (lane & 31);
     const Limits lim(p, b);
     const uint32_t row_at = L::row_lane(lane), col_at = L::col_lane(lane);
@@ -376,8 +377,9 @@ attend_backward_q(const Args p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int q_blocks = (p.Lq + 127) / 128;
     const Share share(blockIdx.x, q_blocks, p.B * p.H);
-    const int qb = q_blocks - 1 - share.block; // the last see most
     const int head = share.head % p.H, b = share.head / p.H;
+    const int qb = SIDE && p.q_order ? scalar(p.q_order[(int64_t)b * q_blocks + share.block])
+                                     : q_blocks - 1 - share.block; // the last see most
     const int kvh = head / (p.H / p.Hkv);
 
     const int q0 = qb * 128, qw = q0 + 32 * wave, qi = qw + (lane & 31);

@@ -52,9 +52,10 @@ attend_forward(const Args p) {
     const int q_blocks = (p.Lq + QT - 1) / QT;
     const int group = p.H / p.Hkv;
     const Share share(blockIdx.x, q_blocks, p.B * p.H * p.splits);
-    const int qb = q_blocks - 1 - share.block; // the last see most
     const int split = share.head % p.splits, head = share.head / p.splits % p.H;
     const int b = share.head / p.splits / p.H;
+    const int qb = SIDE && p.q_order ? scalar(p.q_order[(int64_t)b * q_blocks + share.block])
+                                     : q_blocks - 1 - share.block; // the last see most
     const int kvh = head / group;
 
     const int q0 = qb * QT, qw = q0 + 32 * wave, qi = qw + (lane & 31);

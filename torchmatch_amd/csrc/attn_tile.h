@@ -592,6 +592,9 @@ __device__ inline int xcd_order(int id, int n) {
     return x * per + min(x, rest) + (id >> 3);
 }
 
+// a value that is the same in all lanes
+__device__ inline int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // Blocks of rows of many heads, the first blocks of a head taking longest (causal): an XCD has
 // its own heads, up to four of them at a time, and starts the long blocks of these first.
 // Where heads do not divide by 8, all XCDs take the long blocks of all heads first.
