@@ -36,26 +36,29 @@ __global__ __launch_bounds__(256) void attend_docs(const int32_t *q_docs, const 
 }
 
 // With documents, how long a block of 128 queries or keys takes has nothing to do with where it
-// stands.  Puts those that visit most tiles first, for each batch row: a workgroup counts the
-// tiles of its row's blocks and then ranks them (blockIdx.y 0: queries, 1: keys).
-constexpr int kMaxOrdered = 8192;
+// stands.  Puts those that visit most tiles first, for each batch row: a workgroup brings the
+// summaries of both sides into LDS, counts for each of its row's blocks the tiles that meet it
+// and ranks the blocks, a wave a block (blockIdx.y 0: queries, 1: keys).
+constexpr int kMaxOrdered = 2048;
 __global__ __launch_bounds__(1024) void attend_order(const Args p, int32_t *q_order,
                                                      int32_t *k_order) {
+    __shared__ int2 own[2 * kMaxOrdered], others[2 * kMaxOrdered];
     __shared__ int cost[kMaxOrdered];
     const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const bool keys = blockIdx.y;
     const int nq = (p.Lq + 63) / 64, nk = (p.Lk + 63) / 64;
-    const int own = keys ? nk : nq, blocks = (own + 1) / 2; // of two summaries each
-    const int4 *mine_of = (keys ? p.k_tiles : p.q_tiles) + (int64_t)b * own;
-    const int4 *others = (keys ? p.q_tiles + (int64_t)b * nq : p.k_tiles + (int64_t)b * nk);
+    const int n_own = keys ? nk : nq, n_others = keys ? nq : nk, blocks = (n_own + 1) / 2;
+    const int4 *from_own = (keys ? p.k_tiles : p.q_tiles) + (int64_t)b * n_own;
+    const int4 *from_others = (keys ? p.q_tiles : p.k_tiles) + (int64_t)b * n_others;
     const attn::Limits lim(p, b);
+    for (int t = threadIdx.x; t < n_own; t += 1024)
+        own[t] = make_int2(from_own[t].x, from_own[t].y);
+    for (int t = threadIdx.x; t < n_others; t += 1024)
+        others[t] = make_int2(from_others[t].x, from_others[t].y);
+    __syncthreads();
     for (int i = wave; i < blocks; i += 16) {
-        int4 mine = mine_of[2 * i];
-        if (2 * i + 1 < own) {
-            const int4 o = mine_of[2 * i + 1];
-            mine.x = min(mine.x, o.x);
-            mine.y = max(mine.y, o.y);
-        }
+        const int2 m = own[2 * i], o = own[min(2 * i + 1, n_own - 1)];
+        const int lo = min(m.x, o.x), hi = max(m.y, o.y);
         int first = 0, end;
         if (keys) {
             end = 128 * i < lim.length ? nq : 0;
@@ -66,20 +69,24 @@ __global__ __launch_bounds__(1024) void attend_order(const Args p, int32_t *q_or
         }
         int n = 0;
         for (int t = first; t < end; t += 64) {
-            const bool in = t + lane < end;
-            n += __popcll(__ballot(in && attn::docs_meet(others[min(t + lane, end - 1)], mine)));
+            const int2 x = others[min(t + lane, end - 1)];
+            n += __popcll(__ballot(t + lane < end && x.x <= hi && lo <= x.y));
         }
         if (!lane)
             cost[i] = n;
     }
     __syncthreads();
     int32_t *order = (keys ? k_order : q_order) + (int64_t)b * blocks;
-    for (int i = threadIdx.x; i < blocks; i += 1024) {
+    for (int i = wave; i < blocks; i += 16) {
         const int c = cost[i];
         int rank = 0;
-        for (int j = 0; j < blocks; ++j)
-            rank += cost[j] > c || (cost[j] == c && (keys ? j < i : j > i));
-        order[rank] = i;
+        for (int t = 0; t < blocks; t += 64) {
+            const int j = t + lane, x = cost[min(j, blocks - 1)];
+            const bool before = x > c || (x == c && (keys ? j < i : j > i));
+            rank += __popcll(__ballot(j < blocks && before));
+        }
+        if (!lane)
+            order[rank] = i;
     }
 }
 
@@ -97,8 +104,8 @@ size_t docs_bytes(const tm_attention *a) {
 
 // Worth a launch where the blocks of `rows` rows and `heads` heads are more than run at once.
 bool ordered(const tm_attention *a, int64_t rows, int64_t heads, int at_once) {
-    const int64_t blocks = (rows + 127) / 128;
-    return blocks <= kMaxOrdered && blocks * heads * a->B > at_once;
+    return std::max(a->Lq, a->Lk) <= 128 * kMaxOrdered &&
+           (rows + 127) / 128 * heads * a->B > at_once;
 }
 
 // Few queries: the kernel that packs the queries of a key head's group into 32 rows.
