@@ -280,6 +280,23 @@ def test_gradient_against_differences(device, cap, axes, causal):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("h,hkv,lq,lk,d", [(12, 1, 70, 130, 64), (7, 1, 513, 129, 32),
+                                           (1, 1, 900, 40, 128), (10, 2, 257, 300, 256),
+                                           (5, 1, 1, 33, 96), (1, 1, 641, 641, 80)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_gradients_of_few_key_blocks(device, dtype, h, hkv, lq, lk, d, causal):
+    """Gradients of k and v that many query heads or queries share over few keys."""
+    _case(device, dtype, 2, lq, lk, h, hkv, d, causal=causal, cap=5.0, axes=1,
+          lengths=[lk, lk // 3])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_of_few_key_blocks_of_documents(device, dtype):
+    rows = [_ids((0, 3), (1, 200), (2, 1), (-1, 130), (3, 90))]
+    _case(device, dtype, 1, 424, 424, 6, 1, 64, causal=True, docs=rows)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_same_bits(device, dtype):
     """The same call gives the same bits, forward and backward, on any stream."""
     g = torch.Generator().manual_seed(13)

@@ -137,6 +137,38 @@ Splits splits_of(const tm_attention *a) {
     return {(tiles + per - 1) / per, per};
 }
 
+// The kernel over keys has a block for 128 keys of a key head that takes the group's query heads
+// in turn: few blocks, and long ones, where one key head serves many.  Up to a block a compute
+// unit, the group's heads and then the queries are split over up to 512 blocks of at least two
+// tiles of 64 queries each, whose float32 sums a second kernel adds in their order.  The whole
+// backward pass, whole against split, us: 16384 causal, H 8, Hkv 1, D 128, bf16 (128 blocks)
+// 5486, 2212; 4096 causal, H 4, Hkv 1, D 64 (32) 585, 174; 3 x 515 causal, H 32, Hkv 8, D 128,
+// f32 (120) 826, 487; 333, H 4, D 64, f32 (12) 111, 84; 2 x 2048, H 8, D 64, f16 (256) 134, 129;
+// 4096, H 6, D 128, bf16 (192) 335, 353.  256 blocks and 1024 were as fast or slower.
+struct KvSplits {
+    int n, heads, tiles;
+};
+KvSplits kv_splits_of(const tm_attention *a) {
+    const int group = a->H / a->Hkv, tiles = std::max((a->Lq + 63) / 64, 1);
+    const int64_t blocks = (int64_t)((a->Lk + 127) / 128) * a->Hkv * a->B;
+    const int64_t want =
+        blocks > 256 || !blocks ? 1
+                                : std::min<int64_t>(512 / blocks, (int64_t)group * tiles / 2);
+    if (want <= 1)
+        return {1, group, tiles};
+    const int heads = (int)((group + std::min<int64_t>(group, want) - 1) /
+                            std::min<int64_t>(group, want));
+    const int over_heads = (group + heads - 1) / heads;
+    const int over_tiles = (int)std::max<int64_t>(
+        1, std::min<int64_t>(want / over_heads, tiles / 2));
+    const int per = (tiles + over_tiles - 1) / over_tiles;
+    return {over_heads * ((tiles + per - 1) / per), heads, per};
+}
+size_t kv_part_bytes(const tm_attention *a) { // of dk, or dv
+    const KvSplits s = kv_splits_of(a);
+    return s.n > 1 ? align256((size_t)s.n * a->B * a->Lk * a->Hkv * a->D * sizeof(float)) : 0;
+}
+
 // What every call must hold; sizes of zero are the callers' to answer.
 int check(const tm_attention *a) {
     if (!a || a->B < 0 || a->Lq < 0 || a->Lk < 0 || a->H < 1 || a->Hkv < 1 || a->H % a->Hkv ||
@@ -278,7 +310,8 @@ extern "C" int tm_attention_forward(const tm_attention *a, void *out, void *out_
 extern "C" size_t tm_attention_backward_workspace_bytes(const tm_attention *a) {
     if (check(a) != TM_OK)
         return 0;
-    return docs_bytes(a) + 2 * align256((size_t)a->B * a->H * a->Lq * sizeof(float));
+    return docs_bytes(a) + 2 * align256((size_t)a->B * a->H * a->Lq * sizeof(float)) +
+           2 * kv_part_bytes(a);
 }
 
 extern "C" int tm_attention_backward(const tm_attention *a, const void *out,
@@ -316,10 +349,17 @@ extern "C" int tm_attention_backward(const tm_attention *a, const void *out,
                              align256((size_t)a->B * a->H * a->Lq * sizeof(float)));
     p.delta = delta;
     p.lse = base2;
+    const KvSplits kv = kv_splits_of(a);
+    p.kv_splits = kv.n, p.kv_heads = kv.heads, p.kv_tiles = kv.tiles;
+    p.part_dk = (float *)((char *)base2 +
+                          align256((size_t)a->B * a->H * a->Lq * sizeof(float)));
+    p.part_dv = (float *)((char *)p.part_dk + kv_part_bytes(a));
     const int dp = padded(a->D);
     if (a->Lq && ATTN_BY_TYPE(delta, p, lse, base2, delta, stream))
         return TM_ERR_LAUNCH;
     if (a->Lk && ATTN_BY_TYPE(backward_kv, p, dp, stream))
+        return TM_ERR_LAUNCH;
+    if (a->Lk && kv.n > 1 && ATTN_BY_TYPE(backward_join, p, stream))
         return TM_ERR_LAUNCH;
     if (a->Lq && ATTN_BY_TYPE(backward_q, p, dp, stream))
         return TM_ERR_LAUNCH;

@@ -22,6 +22,10 @@ struct Args {
     // partial results of a split over keys
     float *part_o;  // (splits, B, H, Lq, DP)
     float2 *part_ml; // (splits, B, H, Lq): what weights are relative to (base 2), their sum
+    // gradients of k and v split over the heads of a group (kv_heads each) and the queries
+    // (kv_tiles tiles of 64 each): their partial sums (kv_splits, B, Lk, Hkv, D), or null
+    float *part_dk, *part_dv;
+    int32_t kv_splits, kv_heads, kv_tiles;
     // strides in elements
     int64_t q_b, q_l, q_h, k_b, k_l, k_h, v_b, v_l, v_h, do_b, do_l, do_h;
     int32_t B, Lq, Lk, H, Hkv, D;
@@ -35,6 +39,7 @@ struct Args {
     int tokens_##type(const Args &, int dp, hipStream_t);                                         \
     int join_##type(const Args &, int dp, hipStream_t);                                           \
     int backward_kv_##type(const Args &, int dp, hipStream_t);                                    \
+    int backward_join_##type(const Args &, hipStream_t);                                          \
     int backward_q_##type(const Args &, int dp, hipStream_t);                                     \
     int delta_##type(const Args &, const float *lse, float *base2, float *delta, hipStream_t);
 ATTN_DECLARE(bf16)

@@ -61,8 +61,9 @@ attend_backward_kv(const Args p) {
     const int tid = threadIdx.x & 255, lane = tid & 63, half = lane >> 5;
     const int k_blocks = (p.Lk + 127) / 128;
     const int group = p.H / p.Hkv;
-    const Share share(blockIdx.x, k_blocks, p.B * p.Hkv);
-    const int kvh = share.head % p.Hkv, b = share.head / p.Hkv;
+    const Share share(blockIdx.x, k_blocks, p.B * p.Hkv * p.kv_splits);
+    const int split = share.head % p.kv_splits;
+    const int kvh = share.head / p.kv_splits % p.Hkv, b = share.head / p.kv_splits / p.Hkv;
     const int kb = SIDE && p.k_order ? scalar(p.k_order[(int64_t)b * k_blocks + share.block])
                                      : share.block; // the first are seen by most
     const int k0 = 128 * kb, kw = k0 + 32 * wave, kj = kw + (lane & 31);
@@ -104,7 +105,12 @@ attend_backward_kv(const Args p) {
     else if (lim.causal && k0 >= lim.prefix)
         first = min(p.Lq, max(0, k0 - lim.offset));
     const int nq = (p.Lq + 63) / 64, nk = (p.Lk + 63) / 64;
-    const int t_end = first < p.Lq ? nq : 0;
+    // this split's heads of the group, and tiles of queries
+    const int head_splits = (group + p.kv_heads - 1) / p.kv_heads;
+    const int g_begin = split % head_splits * p.kv_heads;
+    const int g_end = min(group, g_begin + p.kv_heads);
+    const int t_begin = max(first / 64, split / head_splits * p.kv_tiles);
+    const int t_end = first < p.Lq ? min(nq, (split / head_splits + 1) * p.kv_tiles) : 0;
     const int4 *q_tiles = SIDE && p.q_tiles ? p.q_tiles + (int64_t)b * nq : nullptr;
     const int32_t *q_docs = SIDE && p.q_docs ? p.q_docs + (int64_t)b * p.Lq : nullptr;
     const float *q_pos = SIDE && p.q_pos ? p.q_pos + (int64_t)b * p.Lq * p.axes : nullptr;
@@ -128,15 +134,15 @@ attend_backward_kv(const Args p) {
 
     // the tiles of one query head after the other's, dealt to the teams in turn: this team's is
     // at (g, t64, sub), the last given out at (all_g, all_t, all_sub)
-    int all_g = 0, all_t, all_sub = 0, g, t64, sub;
+    int all_g = g_begin, all_t, all_sub = 0, g, t64, sub;
     int4 qd_next = {0, 0, 0, 0}; // documents of this team's tile
     bool first_team_more = false;
     TileWalk walk;
     auto advance = [&]() {
         all_t = walk.next(lane);
-        while (all_t >= t_end && all_g + 1 < group) {
+        while (all_t >= t_end && all_g + 1 < g_end) {
             ++all_g;
-            walk.start(q_tiles, mine, first / 64, t_end, lane);
+            walk.start(q_tiles, mine, t_begin, t_end, lane);
             all_t = walk.next(lane);
         }
     };
@@ -291,7 +297,7 @@ attend_backward_kv(const Args p) {
     B::pad(so1[team], p.D, tid);
     if (p.D < DP)
         __syncthreads();
-    walk.start(q_tiles, mine, first / 64, t_end, lane);
+    walk.start(q_tiles, mine, t_begin, t_end, lane);
     advance();
     deal();
     if (t64 < t_end)
@@ -342,6 +348,24 @@ attend_backward_kv(const Args p) {
         return;
     const float out_scale = grad_scale(p);
     const int64_t at = (((int64_t)b * p.Lk + kj) * p.Hkv + kvh) * p.D;
+    if (p.kv_splits > 1) {
+        const int64_t part = (int64_t)split * p.B * p.Lk * p.Hkv * p.D + at;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int d = 32 * i + 2 * e + 4 * half;
+                if (d < p.D) {
+                    if constexpr (DK)
+                        *(f32x4 *)(p.part_dk + part + d) =
+                            f32x4{dk[i][e], dk[i][e + 1], dk[i][e + 2], dk[i][e + 3]} * out_scale;
+                    if constexpr (DV)
+                        *(f32x4 *)(p.part_dv + part + d) =
+                            f32x4{dv[i][e], dv[i][e + 1], dv[i][e + 2], dv[i][e + 3]};
+                }
+            }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < DB; ++i)
 #pragma unroll
@@ -604,9 +628,31 @@ int run_delta(const Args &a, const float *lse, float *base2, float *delta, hipSt
     return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 
+// Sums the splits' partial gradients, in their order: 4 elements of dk and dv a thread.
+template <typename T> __global__ __launch_bounds__(256) void attend_join_kv(const Args p) {
+    const int64_t n = (int64_t)p.B * p.Lk * p.Hkv * p.D;
+    for (int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < n;
+         i += (int64_t)gridDim.x * 1024) {
+        f32x4 dk = *(const f32x4 *)(p.part_dk + i), dv = *(const f32x4 *)(p.part_dv + i);
+        for (int s = 1; s < p.kv_splits; ++s) {
+            dk += *(const f32x4 *)(p.part_dk + s * n + i);
+            dv += *(const f32x4 *)(p.part_dv + s * n + i);
+        }
+        *(x4<T> *)((T *)p.dk + i) = __builtin_convertvector(dk, x4<T>);
+        *(x4<T> *)((T *)p.dv + i) = __builtin_convertvector(dv, x4<T>);
+    }
+}
+
+template <typename T> int run_backward_join(const Args &a, hipStream_t s) {
+    const int64_t blocks = ((int64_t)a.B * a.Lk * a.Hkv * a.D + 1023) / 1024;
+    attend_join_kv<T><<<dim3((unsigned)std::min<int64_t>(blocks, 4096)), 256, 0, s>>>(a);
+    return hipGetLastError() == hipSuccess ? 0 : 1;
+}
+
 template <typename T, int DP, bool SIDE> void start_backward_kv(const Args &a, hipStream_t s) {
     constexpr int N = 256 * BackwardShape<T, DP>::kTeams;
-    const dim3 grid((unsigned)((int64_t)((a.Lk + 127) / 128) * a.Hkv * a.B));
+    const dim3 grid((unsigned)((int64_t)((a.Lk + 127) / 128) * a.Hkv * a.B *
+                               a.kv_splits));
     if constexpr (BackwardShape<T, DP>::kTwoPasses) {
         attend_backward_kv<T, DP, SIDE, 1><<<grid, N, 0, s>>>(a);
         attend_backward_kv<T, DP, SIDE, 2><<<grid, N, 0, s>>>(a);

@@ -25,6 +25,8 @@ int backward_q_bf16(const Args &a, int dp, hipStream_t s) {
     }
 }
 
+int backward_join_bf16(const Args &a, hipStream_t s) { return run_backward_join<__bf16>(a, s); }
+
 int delta_bf16(const Args &a, const float *lse, float *base2, float *delta, hipStream_t s) {
     return run_delta<__bf16>(a, lse, base2, delta, s);
 }

@@ -25,6 +25,8 @@ int backward_q_f16(const Args &a, int dp, hipStream_t s) {
     }
 }
 
+int backward_join_f16(const Args &a, hipStream_t s) { return run_backward_join<_Float16>(a, s); }
+
 int delta_f16(const Args &a, const float *lse, float *base2, float *delta, hipStream_t s) {
     return run_delta<_Float16>(a, lse, base2, delta, s);
 }
