@@ -4,7 +4,8 @@
 // Both form the weights again from the forward pass's log of the sum:
 //     p = exp(s - lse),  dp = do v^T,  ds = p (dp - delta) (1 - tanh^2)
 // with delta = sum over d of out do.  attend_backward_kv owns keys (32 a wave) and runs over the
-// queries, of every head that shares them:
+// queries, of every head that shares them, or of a part of these where blocks are few
+// (attend_join_kv adds the parts):
 //     dv^T += do^T p,  dk^T += q^T ds      (weights as queries by keys)
 // attend_backward_q owns queries and runs over the keys:
 //     dq^T += k^T ds^T                      (weights as keys by queries)
@@ -26,9 +27,11 @@ template <typename T, int DP> struct BackwardShape {
     // The kernel over keys takes 32 keys a wave and needs two waves a SIMD that hide each
     // other's waits.  Rows of 128 bytes and less leave the registers for that.  With rows of 256
     // bytes k and v move to LDS, and two teams of four waves share the same 128 keys, each with
-    // every other tile of queries (packed documents of 128 features: 440 us; 595 with one
-    // team and k and v in registers, 700 with a pass for dk and one for dv; but 125 in place of
-    // 104 for pairs of 64 features).  Larger rows leave room for one team only.
+    // every other tile of queries (2 x 8192 packed in documents, 128 features, with blocks as
+    // they stand: 440 us; 595 with one team and k and v in registers, 700 with a pass for dk and
+    // one for dv; but 125 in place of 104 for pairs of sets of 64 features).  With the longest
+    // blocks first these two take 345 and 87 us: waits for tiles and barriers bound them, with
+    // matrix products under way in a sixth of the cycles.  Larger rows leave room for one team.
     static constexpr int kTeams = Tile<T, DP>::U == 16 ? 2 : 1;
     static constexpr int kKvRows = kTeams == 2 ? 32 : kRows;
     static constexpr bool kKeysInLds = kTeams == 2;
@@ -629,6 +632,7 @@ int run_delta(const Args &a, const float *lse, float *base2, float *delta, hipSt
 }
 
 // Sums the splits' partial gradients, in their order: 4 elements of dk and dv a thread.
+// Bound by memory: 11 us for 4 parts of 3 x 515 keys of 8 heads of 128 float32 features.
 template <typename T> __global__ __launch_bounds__(256) void attend_join_kv(const Args p) {
     const int64_t n = (int64_t)p.B * p.Lk * p.Hkv * p.D;
     for (int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < n;
