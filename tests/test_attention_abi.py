@@ -53,6 +53,26 @@ def test_refusals(changes, code):
     assert _forward(**changes) == code
 
 
+@pytest.mark.parametrize("changes", [{"B": 0}, {"Lq": 0}, {"Lk": 0}, {"B": 0, "Lq": 1},
+                                     {"Lq": 0, "Lk": 0}, {"B": 0, "q_docs": 4096, "k_docs": 4096}])
+def test_workspaces_of_nothing(changes):
+    """Sizes of zero have a workspace of their own size, not a division by zero blocks."""
+    lib, a = _native.lib(), _problem(**changes)
+    assert lib.tm_attention_workspace_bytes(ctypes.byref(a)) == 0
+    assert lib.tm_attention_backward_workspace_bytes(ctypes.byref(a)) <= 2 * 256 * 75
+
+
+def test_workspaces_of_split_key_gradients():
+    """Few key blocks: float32 parts of dk and dv; many: none."""
+    size = lambda **c: _native.lib().tm_attention_backward_workspace_bytes(  # noqa: E731
+        ctypes.byref(_problem(**c)))
+    sums = lambda b, lq: 2 * ((b * 8 * lq * 4 + 255) // 256 * 256)  # noqa: E731
+    part = 2 * 500 * 2 * 64 * 4  # of one split
+    assert (size() - sums(2, 300)) % (2 * part) == 0 and size() - sums(2, 300) >= 2 * 2 * part
+    assert size(B=64) == sums(64, 300)
+    assert size(Lk=0) == sums(2, 300)
+
+
 def test_workspaces():
     lib = _native.lib()
     size = lambda **c: lib.tm_attention_workspace_bytes(ctypes.byref(_problem(**c)))  # noqa: E731

@@ -123,6 +123,8 @@ struct Splits {
 Splits splits_of(const tm_attention *a) {
     const int tiles = std::max((a->Lk + 63) / 64, 1);
     int64_t blocks, want, most;
+    if (a->B == 0 || a->Lq == 0)
+        return {1, tiles};
     if (few(a)) {
         blocks = (int64_t)((a->H / a->Hkv * a->Lq + 31) / 32) * a->Hkv * a->B;
         want = std::max<int64_t>(1, (a->lengths ? 1024 : 512) / blocks);
@@ -149,7 +151,7 @@ struct KvSplits {
     int n, heads, tiles;
 };
 KvSplits kv_splits_of(const tm_attention *a) {
-    const int group = a->H / a->Hkv, tiles = std::max((a->Lq + 63) / 64, 1);
+    const int group = a->H / a->Hkv, tiles = (a->Lq + 63) / 64;
     const int64_t blocks = (int64_t)((a->Lk + 127) / 128) * a->Hkv * a->B;
     const int64_t want =
         blocks > 256 || !blocks ? 1
@@ -316,7 +318,8 @@ extern "C" size_t tm_attention_backward_workspace_bytes(const tm_attention *a) {
 
 extern "C" int tm_attention_backward(const tm_attention *a, const void *out,
                                      const void *out_low, const float *lse, const void *dout,
-                                     int64_t do_b, int64_t do_l, int64_t do_h, void *dq, void *dk, void *dv, void *workspace,
+                                     int64_t do_b, int64_t do_l, int64_t do_h, void *dq,
+                                     void *dk, void *dv, void *workspace,
                                      size_t workspace_bytes, hipStream_t stream) {
     const int rc = check(a);
     if (rc != TM_OK)
