@@ -11,7 +11,8 @@
 //     dq^T += k^T ds^T                      (weights as keys by queries)
 // Seven products in place of the five of one kernel that would have to add dq from many
 // blocks.  p and ds are rounded to the inputs' type for the second products, as the forward
-// pass rounds its weights; sums stay in float32.
+// pass rounds its weights, and held in half precision's range (grad_shift, Column); sums stay in
+// float32.
 #ifndef TORCHMATCH_AMD_ATTN_BACKWARD_H
 #define TORCHMATCH_AMD_ATTN_BACKWARD_H
 
@@ -134,6 +135,7 @@ attend_backward_kv(const Args p) {
         dk[i] = f32x16{};
         dv[i] = f32x16{};
     }
+    Column<T> column;
 
     // the tiles of one query head after the other's, dealt to the teams in turn: this team's is
     // at (g, t64, sub), the last given out at (all_g, all_t, all_sub)
@@ -276,6 +278,8 @@ attend_backward_kv(const Args p) {
                     }
                 }
             }
+            if constexpr (DK)
+                column.fit(ds, dk);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 if constexpr (DV) {
@@ -285,7 +289,7 @@ attend_backward_kv(const Args p) {
                         dv[i] = mma32(L::col8(so, col_at, 32 * qb + 16 * t, i), w, dv[i]);
                 }
                 if constexpr (DK) {
-                    const x8<T> w = pack8<T>(ds, t);
+                    const x8<T> w = column.pack(ds, t);
 #pragma unroll
                     for (int i = 0; i < DB; ++i)
                         dk[i] = mma32(L::col8(sq, col_at, 32 * qb + 16 * t, i), w, dk[i]);
@@ -315,6 +319,13 @@ attend_backward_kv(const Args p) {
              s_row0[team], s_docs0[team]);
     }
 
+    if constexpr (DK)
+        column.undo(dk);
+    if constexpr (DV && grad_shift<T>() != 0) {
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+            dv[i] *= 1.f / (1 << grad_shift<T>());
+    }
     if constexpr (TEAMS == 2) { // the second team's results to the first, dk and then dv
         const auto join = [&](f32x16 (&x)[DB]) {
             f32x4 *at = (f32x4 *)keep + wave * (8 * DP) + lane;
@@ -459,6 +470,7 @@ attend_backward_q(const Args p) {
 #pragma unroll
     for (int i = 0; i < DB; ++i)
         dq[i] = f32x16{};
+    Column<T> column;
 
     const int seen = min(block_limit, p.Lk); // keys past it may hold anything
     int t64 = walk.next(lane), sub = 0;
@@ -520,15 +532,13 @@ attend_backward_q(const Args p) {
                 [&](int) { return f32x4{delta, delta, delta, delta}; });
             if (masked)
                 rows.hide(p, ds, 0.f, k0 + 32 * kb, half, s_docs + 32 * kb);
+            column.fit(ds, dq);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const x8<T> w = pack8<T>(ds, t);
+                const x8<T> w = column.pack(ds, t);
                 x8<T> rest = w;
-                if constexpr (sizeof(T) == 2) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        rest[j] = (T)(ds[8 * t + j] - (float)w[j]);
-                }
+                if constexpr (sizeof(T) == 2)
+                    rest = column.rest(ds, t, w);
 #pragma unroll
                 for (int i = 0; i < DB; ++i) {
                     const x8<T> kt = L::col8(sk, col_at, 32 * kb + 16 * t, i);
@@ -555,6 +565,7 @@ attend_backward_q(const Args p) {
         step(sk1, sv1, s_docs1, s_pos1, sk0, sv0, s_docs0, s_pos0);
     }
 
+    column.undo(dq);
     if (qi >= p.Lq)
         return;
     const float out_scale = grad_scale(p);
@@ -575,8 +586,8 @@ attend_backward_q(const Args p) {
 }
 
 // delta of each query and head, and what the exponents of its weights start from: minus the log
-// of its sum in base 2, plus the cap's share (Cap); -inf for an empty row, which makes
-// all its weights zero.  16 bytes a thread, DP / E threads a row.  From the output as
+// of its sum in base 2, plus the cap's share (Cap) and grad_shift(); -inf for an empty row,
+// which makes all its weights zero.  16 bytes a thread, DP / E threads a row.  From the output as
 // it was before it was rounded, in two parts: the rounding alone would add as much error to dq
 // and dk as that of ds does.
 template <typename T, int N> // N threads a row: a power of two, N * E >= D
@@ -610,7 +621,7 @@ __global__ __launch_bounds__(256) void attend_delta(const Args p, const float *l
             const int64_t at = (b * p.H + head) * p.Lq + i;
             const float l = lse[at];
             delta[at] = x;
-            base2[at] = l == -kInf ? -kInf : Cap<T>::share(p) - l * kLog2e;
+            base2[at] = l == -kInf ? -kInf : Cap<T>::share(p) - l * kLog2e + grad_shift<T>();
         }
     }
 }

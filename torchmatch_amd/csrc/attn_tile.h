@@ -413,6 +413,78 @@ __device__ inline float max_halves(float x) {
     return fmaxf(__int_as_float(y[0]), __int_as_float(y[1]));
 }
 
+// The gradients' kernels hold weights, which are 1 at most, as many powers of two up: 2^-14 may be
+// shared by many keys (2^-28 keeps all of its bits this way).
+template <typename T> constexpr int grad_shift() { return __is_same(T, _Float16) ? 14 : 0; }
+
+// Gradients of scores, ds, are as large or small as the output's gradient makes them, and half
+// precision holds 2^-14 to 2^15 with all bits.  A lane's results are of one column (a query or a
+// key), whose sums any factor leaves as they are but for itself: its ds go by a power of two
+// that brings the largest to 2^8 and follows when one passes 2^15, the sums with it (exactly).
+// What then lies below the normal numbers is 2^-22 of the column's largest or less.  Other
+// types have float32's range and no factor.  Without it ds of 2^-14 lost bits and ds past 65504
+// made gradients NaN that are finite; it costs a gradient in half precision 4 to 6 % (2 x 2048,
+// 8 heads, us: 64 features 128, 133; 128 features 215, 226), and 17 % at 256 features (521, 607),
+// where the sums no longer stay in the accumulation registers.
+template <typename T> struct Column {
+    static constexpr bool kScaled = __is_same(T, _Float16);
+    int up = 60; // 2^60 times the largest that a finite call can have is finite in float32
+
+    // Before a block x of the column's ds is packed: `up` for it, and `sums` along.
+    template <int DB> __device__ inline void fit(const f32x16 &x, f32x16 (&sums)[DB]) {
+        if constexpr (kScaled) {
+            float most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                most = fmaxf(most, fabsf(x[i]));
+            if (__any(__builtin_ldexpf(most, up) >= 32768.f)) {
+                most = max_halves(most);
+                const bool past = __builtin_ldexpf(most, up) >= 32768.f;
+                const int by = past ? 9 - __builtin_amdgcn_frexp_expf(most) - up : 0;
+                const float r = __builtin_ldexpf(1.f, by);
+                up += by;
+#pragma unroll
+                for (int i = 0; i < DB; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        sums[i][e] *= r;
+            }
+        }
+    }
+    // elements 8t .. of x by that factor, and what rounding took off them: a multiplication and
+    // a conversion are one instruction
+    __device__ inline x8<T> pack(const f32x16 &x, int t) const {
+        if constexpr (!kScaled)
+            return pack8<T>(x, t);
+        const float by = __builtin_ldexpf(1.f, up);
+        x8<T> r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            r[j] = (T)fmaf(x[8 * t + j], by, 0.f);
+        return r;
+    }
+    __device__ inline x8<T> rest(const f32x16 &x, int t, x8<T> w) const {
+        const float by = __builtin_ldexpf(1.f, up);
+        x8<T> r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            r[j] = kScaled ? (T)fmaf(x[8 * t + j], by, -(float)w[j])
+                           : (T)(x[8 * t + j] - (float)w[j]);
+        return r;
+    }
+    // the sums as they would be without scale and grad_shift()
+    template <int DB> __device__ inline void undo(f32x16 (&sums)[DB]) const {
+        if constexpr (kScaled) {
+            const float r = __builtin_ldexpf(1.f, -up - grad_shift<T>());
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    sums[i][e] *= r;
+        }
+    }
+};
+
 // One step of the running softmax: scores s (keys by queries), which times mul >= 0 are in
 // base 2, become weights 2^(s mul - top).  `top` follows the largest score seen only when that
 // grew by more than 2^8: weights up to 2^8 cost no precision in float32 sums, and the output
@@ -475,8 +547,9 @@ template <typename T> __device__ inline void put(const Args &p, int64_t at, x4<T
     }
 }
 
-// For the gradients: products s become weights p, products ds = do v become p (ds - delta), with
-// a cap times a quarter of its slope (grad_scale() has the rest).  Four elements at a time, so
+// For the gradients: products s become weights p (times 2^grad_shift, which base() holds), products
+// ds = do v become p (ds - delta), with a cap times a quarter of its slope (grad_scale() has
+// the rest).  Four elements at a time, so
 // that nothing but s and ds is held: dist(n), base(n) and delta(n) give what belongs to elements
 // 4n .. 4n + 3: the distance, what attend_delta left of the log of the row's sum, and delta.
 __device__ inline float grad_scale(const Args &p) {
