@@ -388,12 +388,18 @@ int tm_attention_forward(const tm_attention *a, void *out, void *out_low, float 
 
 /* Gradients of q, k and v (contiguous, the inputs' type) from out, out_low
  * (or NULL) and lse of the forward call and the output's gradient, (B, Lq, H, D) with its own strides.
- * The same call gives the same bits: nothing is added by atomics. */
+ * The same call gives the same bits: nothing is added by atomics.
+ * tm_attention_backward_lse also takes the gradient of lse, dlse: (B, H, Lq) float32, contiguous,
+ * or NULL for none; what it holds for a row that sees nothing is not used. */
 size_t tm_attention_backward_workspace_bytes(const tm_attention *a);
 int tm_attention_backward(const tm_attention *a, const void *out, const void *out_low,
                           const float *lse, const void *dout, int64_t do_b, int64_t do_l,
                           int64_t do_h, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
                           hipStream_t stream);
+int tm_attention_backward_lse(const tm_attention *a, const void *out, const void *out_low,
+                              const float *lse, const float *dlse, const void *dout, int64_t do_b,
+                              int64_t do_l, int64_t do_h, void *dq, void *dk, void *dv,
+                              void *workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* Rotation of feature pairs.  x is (B, L, H, D) of `dtype` with strides in
  * elements (D contiguous); out is (B, L, H, D), contiguous.  positions are

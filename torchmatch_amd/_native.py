@@ -185,6 +185,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             ctypes.c_int64, _VP, _VP, _VP, _VP, ctypes.c_size_t, _VP,
         ],
     ),
+    "tm_attention_backward_lse": (
+        ctypes.c_int,
+        [
+            ctypes.POINTER(Attention), _VP, _VP, _VP, _VP, _VP, ctypes.c_int64, ctypes.c_int64,
+            ctypes.c_int64, _VP, _VP, _VP, _VP, ctypes.c_size_t, _VP,
+        ],
+    ),
     "tm_rotate": (ctypes.c_int, [ctypes.POINTER(Rotation), _VP, _VP]),
 }
 

@@ -72,7 +72,8 @@ def attend(  # noqa: PLR0913
     features contiguous and rows 16-byte aligned are read in place, else copied.
     bfloat16, float16 or float32; sums and softmax are float32.  Differentiable in q, k
     and v, with the same bits each time.  Returns ``out`` (B, Lq, H, D), with
-    ``return_lse`` also the logarithm of each row's sum, (B, H, Lq) float32.
+    ``return_lse`` also the logarithm of each row's sum, (B, H, Lq) float32, which is
+    differentiable too (a row that sees nothing passes no gradient on).
     """
     _on_device(q, "attend", "q")
     _on_device(k, "attend", "k")

@@ -321,6 +321,16 @@ extern "C" int tm_attention_backward(const tm_attention *a, const void *out,
                                      int64_t do_b, int64_t do_l, int64_t do_h, void *dq,
                                      void *dk, void *dv, void *workspace,
                                      size_t workspace_bytes, hipStream_t stream) {
+    return tm_attention_backward_lse(a, out, out_low, lse, nullptr, dout, do_b, do_l, do_h, dq,
+                                     dk, dv, workspace, workspace_bytes, stream);
+}
+
+extern "C" int tm_attention_backward_lse(const tm_attention *a, const void *out,
+                                         const void *out_low, const float *lse,
+                                         const float *dlse, const void *dout, int64_t do_b,
+                                         int64_t do_l, int64_t do_h, void *dq, void *dk,
+                                         void *dv, void *workspace, size_t workspace_bytes,
+                                         hipStream_t stream) {
     const int rc = check(a);
     if (rc != TM_OK)
         return rc;
@@ -340,6 +350,7 @@ extern "C" int tm_attention_backward(const tm_attention *a, const void *out,
     p.out = const_cast<void *>(out);
     p.out_low = a->dtype == TM_F32 ? nullptr : const_cast<void *>(out_low);
     p.dout = dout;
+    p.dlse = dlse;
     p.do_b = do_b, p.do_l = do_l, p.do_h = do_h;
     p.dq = dq, p.dk = dk, p.dv = dv;
     char *ws = (char *)workspace;

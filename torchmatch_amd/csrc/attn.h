@@ -12,7 +12,8 @@ struct Args {
     const void *q, *k, *v, *dout;
     void *out, *out_low, *dq, *dk, *dv; // contiguous (B, L, heads, D); out_low may be null
     float *lse; // (B, H, Lq), natural logarithm, -inf for empty rows; backward: see attend_delta
-    const float *delta;       // (B, H, Lq): sum over d of out * dout
+    const float *delta;       // (B, H, Lq): sum over d of out * dout, less dlse
+    const float *dlse;        // (B, H, Lq): the gradient of lse, or null
     const float *slopes;      // (H) or null
     const float *q_pos, *k_pos; // (B, L, axes), or null: distance of indices
     const int32_t *q_docs, *k_docs; // (B, L) or null

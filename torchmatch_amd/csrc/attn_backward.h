@@ -3,7 +3,7 @@
 //
 // Both form the weights again from the forward pass's log of the sum:
 //     p = exp(s - lse),  dp = do v^T,  ds = p (dp - delta) (1 - tanh^2)
-// with delta = sum over d of out do.  attend_backward_kv owns keys (32 a wave) and runs over the
+// with delta = sum over d of out do, less the gradient of lse (whose own is p).  attend_backward_kv owns keys (32 a wave) and runs over the
 // queries, of every head that shares them, or of a part of these where blocks are few
 // (attend_join_kv adds the parts):
 //     dv^T += do^T p,  dk^T += q^T ds      (weights as queries by keys)
@@ -620,7 +620,8 @@ __global__ __launch_bounds__(256) void attend_delta(const Args p, const float *l
         if (row < rows && d == 0) {
             const int64_t at = (b * p.H + head) * p.Lq + i;
             const float l = lse[at];
-            delta[at] = x;
+            // an empty row has no gradient, whatever a loss makes of its -inf
+            delta[at] = l == -kInf ? 0.f : p.dlse ? x - p.dlse[at] : x;
             base2[at] = l == -kInf ? -kInf : Cap<T>::share(p) - l * kLog2e + grad_shift<T>();
         }
     }

@@ -224,7 +224,8 @@ attend_backward_hip(const Tensor &dout, const Tensor &q, const Tensor &k, const 
                     const Tensor &out, const Tensor &out_low, const Tensor &lse,
                     const OptTensor &slopes, const OptTensor &q_pos, const OptTensor &k_pos,
                     const OptTensor &q_docs, const OptTensor &k_docs, const OptTensor &prefix,
-                    const OptTensor &lengths, double scale, double cap, bool causal) {
+                    const OptTensor &lengths, const OptTensor &dlse, double scale, double cap,
+                    bool causal) {
     const c10::DeviceGuard guard(q.device());
     const Problem p = problem(q, k, v, slopes, q_pos, k_pos, q_docs, k_docs, prefix, lengths,
                               scale, cap, causal);
@@ -239,6 +240,14 @@ attend_backward_hip(const Tensor &dout, const Tensor &q, const Tensor &k, const 
     TORCH_CHECK_VALUE(lse.dim() == 3 && lse.size(0) == q.size(0) && lse.size(1) == q.size(2) &&
                           lse.size(2) == q.size(1) && lse.is_contiguous(),
                       "attend_backward: lse must be a contiguous (B, H, Lq)");
+    Tensor dl;
+    if (dlse.has_value()) {
+        TORCH_CHECK_TYPE(dlse->scalar_type() == at::kFloat,
+                         "attend_backward: dlse must be float32, got ", dlse->scalar_type());
+        TORCH_CHECK_VALUE(dlse->sizes() == lse.sizes() && dlse->device() == q.device(),
+                          "attend_backward: dlse must be as lse, got ", dlse->sizes());
+        dl = dlse->contiguous();
+    }
     const bool has_low = out_low.numel() && p.a.dtype != TM_F32;
     TORCH_CHECK_VALUE(!has_low || (out_low.sizes() == q.sizes() &&
                                    out_low.device() == q.device() &&
@@ -251,11 +260,12 @@ attend_backward_hip(const Tensor &dout, const Tensor &q, const Tensor &k, const 
     if (dq.numel() || dk.numel()) {
         const size_t bytes = tm_attention_backward_workspace_bytes(&p.a);
         Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
-        check_rc(tm_attention_backward(&p.a, o.const_data_ptr(),
-                                       has_low ? low.const_data_ptr() : nullptr,
-                                       lse.const_data_ptr<float>(), g.const_data_ptr(), step_of(g, 0), step_of(g, 1),
-                                       step_of(g, 2), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                       ws.data_ptr(), bytes, current_stream(q)),
+        check_rc(tm_attention_backward_lse(
+                     &p.a, o.const_data_ptr(), has_low ? low.const_data_ptr() : nullptr,
+                     lse.const_data_ptr<float>(),
+                     dl.defined() ? dl.const_data_ptr<float>() : nullptr, g.const_data_ptr(),
+                     step_of(g, 0), step_of(g, 1), step_of(g, 2), dq.data_ptr(), dk.data_ptr(),
+                     dv.data_ptr(), ws.data_ptr(), bytes, current_stream(q)),
                  "attend_backward");
     }
     return {narrowed(dq, p.d), narrowed(dk, p.d), narrowed(dv, p.d)};
@@ -352,14 +362,16 @@ struct AttendFunction : torch::autograd::Function<AttendFunction> {
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["cap"] = cap;
         ctx->saved_data["causal"] = causal;
-        ctx->mark_non_differentiable({lse});
+        // either output may go unused: no zeros are made up for its gradient
+        ctx->set_materialize_grads(false);
         return {out, lse};
     }
     static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
         const auto s = ctx->get_saved_variables();
         variable_list result(7);
-        if (!grads[0].defined())
+        if (!grads[0].defined() && !grads[1].defined())
             return result;
+        const Tensor dout = grads[0].defined() ? grads[0] : at::zeros_like(s[3]);
         const auto opt = [&](int i) { return s[i].defined() ? OptTensor(s[i]) : OptTensor(); };
         static auto op =
             c10::Dispatcher::singleton()
@@ -368,10 +380,12 @@ struct AttendFunction : torch::autograd::Function<AttendFunction> {
                     const Tensor &, const Tensor &, const Tensor &, const Tensor &,
                     const Tensor &, const Tensor &, const Tensor &, const OptTensor &,
                     const OptTensor &, const OptTensor &, const OptTensor &, const OptTensor &,
-                    const OptTensor &, const OptTensor &, double, double, bool)>();
+                    const OptTensor &, const OptTensor &, const OptTensor &, double, double,
+                    bool)>();
         auto [dq, dk, dv] =
-            op.call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], opt(6), opt(7), opt(8),
-                    opt(9), opt(10), opt(11), opt(12), ctx->saved_data["scale"].toDouble(),
+            op.call(dout, s[0], s[1], s[2], s[3], s[4], s[5], opt(6), opt(7), opt(8), opt(9),
+                    opt(10), opt(11), opt(12),
+                    grads[1].defined() ? OptTensor(grads[1]) : OptTensor(), ctx->saved_data["scale"].toDouble(),
                     ctx->saved_data["cap"].toDouble(), ctx->saved_data["causal"].toBool());
         result[0] = dq;
         result[1] = dk;
@@ -465,8 +479,8 @@ TORCH_LIBRARY(attention, m) {
           "Tensor out_low, Tensor lse, "
           "Tensor? slopes=None, Tensor? q_positions=None, Tensor? k_positions=None, "
           "Tensor? q_docs=None, Tensor? k_docs=None, Tensor? prefix=None, "
-          "Tensor? lengths=None, *, float scale, float cap=0., bool causal=False) "
-          "-> (Tensor, Tensor, Tensor)");
+          "Tensor? lengths=None, Tensor? dlse=None, *, float scale, float cap=0., "
+          "bool causal=False) -> (Tensor, Tensor, Tensor)");
     m.def("rotate(Tensor x, Tensor positions, Tensor freqs, int[] sections, "
           "bool interleaved=False, bool inverse=False) -> Tensor");
 }
