@@ -74,6 +74,7 @@ def attend(  # noqa: PLR0913
     and v, with the same bits each time.  Returns ``out`` (B, Lq, H, D), with
     ``return_lse`` also the logarithm of each row's sum, (B, H, Lq) float32, which is
     differentiable too (a row that sees nothing passes no gradient on).
+    Reverse mode, once: second derivatives and forward mode are refused.
     """
     _on_device(q, "attend", "q")
     _on_device(k, "attend", "k")
@@ -128,7 +129,7 @@ def rotate(
 
     bfloat16, float16 or float32, any strides; positions are float32, int32 or int64,
     (L, axes) where the batch shares them.  Angles are exact to float32 at any position.
-    Differentiable in x.
+    Differentiable in x, in both modes and any number of times.
     """
     _on_device(x, "rotate", "x")
     if positions.ndim == 2 and x.ndim == 4:

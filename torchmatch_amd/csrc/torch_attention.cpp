@@ -332,11 +332,15 @@ Tensor rotate_hip(const Tensor &x, const Tensor &positions, const Tensor &freqs,
 
 // ---- autograd ---------------------------------------------------------------------
 
-bool wants_grad(const Tensor &t) { return t.requires_grad(); }
+bool wants_grad(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+// Whether forward-mode differentiation is under way (it goes by no grad mode): below autograd
+// the tangent would be lost without a word.
+bool has_tangent(const Tensor &t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
 
 void constant(const OptTensor &t, const char *op, const char *name) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!t.has_value() || !t->requires_grad(), op, ": no gradient for ",
-                                name);
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.has_value() || !(wants_grad(*t) || has_tangent(*t)), op,
+                                ": no gradient for ", name);
 }
 
 template <typename... R>
@@ -401,14 +405,14 @@ std::tuple<Tensor, Tensor> attend_autograd(const Tensor &q, const Tensor &k, con
                                            const OptTensor &lengths, double scale, double cap,
                                            bool causal) {
     const std::vector<OptTensor> masks = {slopes, q_pos, k_pos, q_docs, k_docs, prefix, lengths};
-    if (at::GradMode::is_enabled()) {
-        constant(slopes, "attend", "slopes");
-        constant(q_pos, "attend", "q_positions");
-        constant(k_pos, "attend", "k_positions");
-        if (wants_grad(q) || wants_grad(k) || wants_grad(v)) {
-            auto r = AttendFunction::apply(q, k, v, masks, scale, cap, causal);
-            return {r[0], r[1]};
-        }
+    constant(slopes, "attend", "slopes");
+    constant(q_pos, "attend", "q_positions");
+    constant(k_pos, "attend", "k_positions");
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(q) && !has_tangent(k) && !has_tangent(v),
+                                "attend: no forward-mode derivative");
+    if (wants_grad(q) || wants_grad(k) || wants_grad(v)) {
+        auto r = AttendFunction::apply(q, k, v, masks, scale, cap, causal);
+        return {r[0], r[1]};
     }
     at::AutoDispatchBelowADInplaceOrView below;
     static auto op = c10::Dispatcher::singleton()
@@ -453,12 +457,17 @@ struct RotateFunction : torch::autograd::Function<RotateFunction> {
 
 Tensor rotate_autograd(const Tensor &x, const Tensor &positions, const Tensor &freqs,
                        at::IntArrayRef sections, bool interleaved, bool inverse) {
-    if (at::GradMode::is_enabled()) {
-        constant(positions, "rotate", "positions");
-        constant(freqs, "rotate", "freqs");
-        if (wants_grad(x))
-            return RotateFunction::apply(x, positions, freqs, sections, interleaved, inverse);
+    constant(positions, "rotate", "positions");
+    constant(freqs, "rotate", "freqs");
+    if (has_tangent(x)) { // linear in x: the tangent turns as x does
+        const auto [primal, tangent] = at::_unpack_dual(x, /*level=*/0);
+        return at::_make_dual(
+            rotate_autograd(primal, positions, freqs, sections, interleaved, inverse),
+            rotate_autograd(tangent, positions, freqs, sections, interleaved, inverse),
+            /*level=*/0);
     }
+    if (wants_grad(x))
+        return RotateFunction::apply(x, positions, freqs, sections, interleaved, inverse);
     at::AutoDispatchBelowADInplaceOrView below;
     return call_rotate(x, positions, freqs, sections, interleaved, inverse);
 }
