@@ -76,7 +76,9 @@ const float *floats(const OptTensor &t, const Tensor &q, const char *name, at::I
     TORCH_CHECK_VALUE(t->device() == q.device(), "attend: ", name, " must be on q's device");
     TORCH_CHECK_VALUE(t->sizes() == sizes && t->is_contiguous(), "attend: ", name,
                       " must be contiguous of shape ", sizes, ", got ", t->sizes());
-    return t->numel() ? t->const_data_ptr<float>() : nullptr;
+    // never null where given: an empty one stands for rows that are not there
+    static const float none = 0.f;
+    return t->numel() ? t->const_data_ptr<float>() : &none;
 }
 
 const int32_t *ints(const OptTensor &t, const Tensor &q, const char *name, at::IntArrayRef sizes) {
@@ -87,7 +89,6 @@ const int32_t *ints(const OptTensor &t, const Tensor &q, const char *name, at::I
     TORCH_CHECK_VALUE(t->device() == q.device(), "attend: ", name, " must be on q's device");
     TORCH_CHECK_VALUE(t->sizes() == sizes && t->is_contiguous(), "attend: ", name,
                       " must be contiguous of shape ", sizes, ", got ", t->sizes());
-    // never null where given: an empty one stands for rows that are not there
     static const int32_t none = 0;
     return t->numel() ? t->const_data_ptr<int32_t>() : &none;
 }
