@@ -1,4 +1,5 @@
-"""Calls at the edge of attention.attend's arguments: sets without points."""
+"""Calls at the edge of attention.attend's arguments: sets without points, batches of
+millions of short rows."""
 
 from __future__ import annotations
 
@@ -28,3 +29,27 @@ def test_empty_sets_with_positions(device, b, lq, lk, axes, docs):
     out.sum().backward()
     for t in (q, k, v):
         assert t.grad.shape == t.shape and (t.grad == 0).all()
+
+
+@pytest.mark.parametrize("b,lq,lk", [(1 << 22, 2, 3), ((1 << 22) - 1, 1, 130),
+                                     ((1 << 23) // 5, 130, 1)])
+def test_millions_of_short_rows_of_documents(device, b, lq, lk):
+    """As many batch rows as the limit on blocks admits, or half of it: each as in a call of a
+    few rows, forward and backward."""
+    d = 8
+    g = torch.Generator(device=device).manual_seed(1)
+    q, k, v, do = (torch.randn(b, n, 1, d, device=device, generator=g).half()
+                   for n in (lq, lk, lk, lq))
+    q_docs, k_docs = (torch.randint(-1, 2, (b, n), device=device, generator=g, dtype=torch.int32)
+                      for n in (lq, lk))
+
+    def run(rows):
+        t = [x[rows].clone().requires_grad_(True) for x in (q, k, v)]
+        out = att.attend(*t, q_docs=q_docs[rows], k_docs=k_docs[rows])
+        return (out.detach(), *torch.autograd.grad(out, t, do[rows]))
+
+    every = run(slice(0, b))
+    for first in (0, b // 2 - 500, b - 1000):
+        rows = slice(first, first + 1000)
+        for x, y in zip(every, run(rows)):
+            assert torch.equal(x[rows], y)

@@ -38,14 +38,14 @@ __global__ __launch_bounds__(256) void attend_docs(const int32_t *q_docs, const 
 // With documents, how long a block of 128 queries or keys takes has nothing to do with where it
 // stands.  Puts those that visit most tiles first, for each batch row: a workgroup brings the
 // summaries of both sides into LDS, counts for each of its row's blocks the tiles that meet it
-// and ranks the blocks, a wave a block (blockIdx.y 0: queries, 1: keys).
+// and ranks the blocks, a wave a block (blockIdx.y + first_side 0: queries, 1: keys).
 constexpr int kMaxOrdered = 2048;
-__global__ __launch_bounds__(1024) void attend_order(const Args p, int32_t *q_order,
-                                                     int32_t *k_order) {
+__global__ __launch_bounds__(1024) void attend_order(const Args p, int first_side,
+                                                     int32_t *q_order, int32_t *k_order) {
     __shared__ int2 own[2 * kMaxOrdered], others[2 * kMaxOrdered];
     __shared__ int cost[kMaxOrdered];
     const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const bool keys = blockIdx.y;
+    const bool keys = blockIdx.y + first_side;
     const int nq = (p.Lq + 63) / 64, nk = (p.Lk + 63) / 64;
     const int n_own = keys ? nk : nq, n_others = keys ? nq : nk, blocks = (n_own + 1) / 2;
     const int4 *from_own = (keys ? p.k_tiles : p.q_tiles) + (int64_t)b * n_own;
@@ -107,6 +107,10 @@ bool ordered(const tm_attention *a, int64_t rows, int64_t heads, int at_once) {
     return std::max(a->Lq, a->Lk) <= 128 * kMaxOrdered &&
            (rows + 127) / 128 * heads * a->B > at_once;
 }
+
+// One block has no order.  Two or more in a batch row also keep the launch, B workgroups of
+// 1024 threads, below 2^32 of them: B is then below TM_ATTENTION_MAX_BLOCKS / 2.
+bool several(int64_t rows) { return rows > 128; }
 
 // Few queries: the kernel that packs the queries of a key head's group into 32 rows.
 // Above 32 queries the other kernel's 128 rows a block are no longer mostly empty.
@@ -181,7 +185,8 @@ int check(const tm_attention *a) {
     const int unit = a->dtype == TM_F32 ? 4 : 8;
     if (a->D > tm_attention_max_head_dim() || a->D % unit)
         return TM_ERR_UNSUPPORTED_SHAPE;
-    // blocks of up to 512 threads, of which a launch takes less than 2^32
+    // blocks of up to 512 threads, of which a launch takes less than 2^32 (attend_order, of 1024,
+    // is launched where this admits half as many batch rows: see several())
     if (a->Lq > INT32_MAX - 256 || a->Lk > INT32_MAX - 256 ||
         a->B * std::max((int64_t)a->H * ((a->Lq + 31) / 32),
                         (int64_t)a->Hkv * ((a->Lk + 127) / 128)) >= TM_ATTENTION_MAX_BLOCKS)
@@ -248,8 +253,10 @@ int summarise_docs(const tm_attention *a, Args &p, char *ws, bool q_order, bool 
     if (q_order || k_order) {
         int32_t *order = (int32_t *)(ws + align256(a->B * (nq + nk) * sizeof(int4)));
         int32_t *of_keys = order + (int64_t)a->B * ((a->Lq + 127) / 128);
-        attend_order<<<dim3(a->B, k_order ? 2 : 1), 1024, 0, stream>>>(p, order, of_keys);
-        p.q_order = order;
+        attend_order<<<dim3(a->B, q_order + k_order), 1024, 0, stream>>>(p, !q_order, order,
+                                                                         of_keys);
+        if (q_order)
+            p.q_order = order;
         if (k_order)
             p.k_order = of_keys;
     }
@@ -290,7 +297,7 @@ extern "C" int tm_attention_forward(const tm_attention *a, void *out, void *out_
     p.out_low = a->dtype == TM_F32 ? nullptr : out_low;
     p.lse = lse;
     char *ws = (char *)workspace;
-    if (summarise_docs(a, p, ws, !few(a) && ordered(a, a->Lq, a->H, 512), false, stream))
+    if (summarise_docs(a, p, ws, several(a->Lq) && ordered(a, a->Lq, a->H, 512), false, stream))
         return TM_ERR_LAUNCH;
     ws += docs_bytes(a);
     const Splits s = splits_of(a);
@@ -354,8 +361,8 @@ extern "C" int tm_attention_backward_lse(const tm_attention *a, const void *out,
     p.do_b = do_b, p.do_l = do_l, p.do_h = do_h;
     p.dq = dq, p.dk = dk, p.dv = dv;
     char *ws = (char *)workspace;
-    const bool q_order = a->Lq && ordered(a, a->Lq, a->H, 512);
-    const bool k_order = q_order && a->Lk && ordered(a, a->Lk, a->Hkv, 256);
+    const bool many = a->Lq && ordered(a, a->Lq, a->H, 512), q_order = many && several(a->Lq);
+    const bool k_order = many && several(a->Lk) && ordered(a, a->Lk, a->Hkv, 256);
     if (summarise_docs(a, p, ws, q_order, k_order, stream))
         return TM_ERR_LAUNCH;
     float *delta = (float *)(ws + docs_bytes(a));
