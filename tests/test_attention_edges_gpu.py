@@ -1,11 +1,12 @@
 """Calls at the edge of attention.attend's arguments: sets without points, batches of
-millions of short rows."""
+millions of short rows, limits past 32 bits."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
+from attention_oracle import assert_within, attention, visible
 from torchmatch_amd import attention as att
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +54,21 @@ def test_millions_of_short_rows_of_documents(device, b, lq, lk):
         rows = slice(first, first + 1000)
         for x, y in zip(every, run(rows)):
             assert torch.equal(x[rows], y)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_limits_past_32_bits(device, dtype):
+    """Lengths and prefixes of int64: those past the keys see all of them, negative ones none."""
+    b, lq, lk = 5, 40, 70
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(b, n, 2, 64, generator=g).to(dtype).to(device) for n in (lq, lk, lk))
+    far = [2**31, 2**32 + 5, 2**63 - 1, -2**31 - 1, -2**63]
+    near = [lk, lk, lk, 0, 0]
+    see = visible(b, lq, lk, lengths=near)
+    want = attention(q, k, v, see, scale=64 ** -0.5)
+    out = att.attend(q, k, v, lengths=torch.tensor(far, device=device))
+    assert_within(out, *want["out"], "out by lengths")
+    see = visible(b, lq, lk, causal=True, prefix=near)
+    want = attention(q, k, v, see, scale=64 ** -0.5)
+    out = att.attend(q, k, v, causal=True, prefix=torch.tensor(far, device=device))
+    assert_within(out, *want["out"], "out by prefixes")

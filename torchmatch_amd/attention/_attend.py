@@ -36,6 +36,13 @@ def _rows(t: torch.Tensor | None, batch: int, ndim: int, dtype: torch.dtype):
     return t.contiguous()
 
 
+def _limits(t: torch.Tensor | None, batch: int):
+    """Numbers of keys: past 32 bits they mean all of them, as any number past the keys does."""
+    if t is not None and t.dtype == torch.int64:
+        t = t.clamp(0, 2**31 - 1)
+    return _rows(t, batch, 1, torch.int32)
+
+
 def attend(  # noqa: PLR0913
     q: torch.Tensor,
     k: torch.Tensor,
@@ -62,7 +69,7 @@ def attend(  # noqa: PLR0913
     ``k_positions`` (B, Lk, axes), summed over 1 to 3 axes, or of the indices where no
     positions are given.  What a query sees:
 
-    * ``lengths`` (B,): the first ``lengths[b]`` keys (all by default);
+    * ``lengths`` (B,): the first ``lengths[b]`` keys (all by default, and where it is larger);
     * ``causal``: query i stands at ``i + length - Lq`` and sees keys up to there, and the
       first ``prefix[b]`` keys wherever it stands;
     * ``q_docs`` (B, Lq), ``k_docs`` (B, Lk): keys of the same document; negative ids are
@@ -86,8 +93,7 @@ def attend(  # noqa: PLR0913
         batch = q.shape[0] if q.ndim else 0
         q_docs = _rows(q_docs, batch, 2, torch.int32)
         k_docs = q_docs if k_docs is None else _rows(k_docs, batch, 2, torch.int32)
-        prefix = _rows(prefix, batch, 1, torch.int32)
-        lengths = _rows(lengths, batch, 1, torch.int32)
+        prefix, lengths = _limits(prefix, batch), _limits(lengths, batch)
         q_positions = _rows(q_positions, batch, 3, torch.float32)
         k_positions = _rows(k_positions, batch, 3, torch.float32)
     out, lse = _ATTEND(q, k, v, slopes, q_positions, k_positions, q_docs, k_docs, prefix,
