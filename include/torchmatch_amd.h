@@ -363,6 +363,7 @@ enum { TM_POS_F32 = 0, TM_POS_I32 = 1, TM_POS_I64 = 2 };
  * A query that sees nothing gets zeros, lse = -inf and no gradient.  Keys past
  * every limit and rows of negative documents may hold anything, NaN included. */
 enum { TM_ATTENTION_MAX_ROW_BYTES = 1 << 26, TM_ATTENTION_MAX_BLOCKS = 1 << 23 };
+/* |scale|, cap and, with a cap, |scale| / cap are 2^126 at most (TM_ERR_INVALID_ARGUMENT). */
 enum { TM_ATTENTION_MAX_CAP_16 = 1024 }; /* 16-bit types: tanh is good to 2e-7 of the cap */
 typedef struct tm_attention {
     const void *q, *k, *v;

@@ -1,5 +1,6 @@
 """Calls at the edge of attention.attend's arguments: sets without points, batches of
-millions of short rows, limits past 32 bits."""
+millions of short rows, limits past 32 bits,
+numbers that float32 does not hold."""
 
 from __future__ import annotations
 
@@ -10,6 +11,8 @@ from attention_oracle import assert_within, attention, visible
 from torchmatch_amd import attention as att
 
 pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 
 
 @pytest.mark.parametrize("b,lq,lk", [(0, 3, 4), (2, 0, 4), (2, 3, 0), (2, 0, 0), (2, 40, 0),
@@ -72,3 +75,22 @@ def test_limits_past_32_bits(device, dtype):
     want = attention(q, k, v, see, scale=64 ** -0.5)
     out = att.attend(q, k, v, causal=True, prefix=torch.tensor(far, device=device))
     assert_within(out, *want["out"], "out by prefixes")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_numbers_that_float32_does_not_hold(device, dtype):
+    q, k, v = (torch.randn(1, 9, 1, 64, device=device).to(dtype) for _ in range(3))
+    for scale in (1e39, -1e300):
+        with pytest.raises(ValueError, match="scale"):
+            att.attend(q, k, v, scale=scale)
+    with pytest.raises(ValueError, match="cap"):
+        att.attend(q, k, v, cap=1e-46)  # not "no cap"
+    with pytest.raises(ValueError, match="cap"):
+        att.attend(q, k, v, cap=1e-39)  # scale / cap is infinite: 0 * inf where q.k is 0
+    if dtype == torch.float32:
+        with pytest.raises(ValueError, match="cap"):
+            att.attend(q, k, v, cap=1e38)
+    zero = torch.zeros_like(q)
+    out = att.attend(zero, k, v, cap=1e-30)
+    assert_within(out, *attention(zero, k, v, visible(1, 9, 9), scale=0.125, cap=1e-30)["out"],
+                  "out")

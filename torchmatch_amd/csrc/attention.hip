@@ -1,5 +1,6 @@
 // attention.hip -- the C entries of the attention operators: checks, workspace, launches.
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/torchmatch_amd.h"
 #include "attn_tile.h"
@@ -193,7 +194,12 @@ int check(const tm_attention *a) {
         return TM_ERR_UNSUPPORTED_SHAPE;
     if (a->dtype != TM_F32 && a->cap > TM_ATTENTION_MAX_CAP_16)
         return TM_ERR_UNSUPPORTED_SHAPE;
-    if (!(a->scale == a->scale) || !(a->cap >= 0.f) || (!a->q_docs != !a->k_docs) ||
+    // what the kernels make of these, up to 4 times as much, stays finite
+    const float most = 0x1p126f;
+    if (!(std::fabs(a->scale) <= most) || !(a->cap >= 0.f) || !(a->cap <= most) ||
+        (a->cap > 0.f && !(std::fabs(a->scale / a->cap) <= most)))
+        return TM_ERR_INVALID_ARGUMENT;
+    if ((!a->q_docs != !a->k_docs) ||
         (!a->q_positions != !a->k_positions) || (a->q_positions && !a->slopes))
         return TM_ERR_INVALID_ARGUMENT;
     if (a->q_positions && (a->axes < 1 || a->axes > 3))

@@ -124,9 +124,14 @@ Problem problem(const Tensor &q, const Tensor &k, const Tensor &v, const OptTens
                                                (double)Hkv * (double)((Lk + 127) / 128)) <
                               TM_ATTENTION_MAX_BLOCKS,
                       "attend: too many rows for one call: q ", q.sizes(), ", k ", k.sizes());
-    TORCH_CHECK_VALUE(std::isfinite(scale), "attend: scale must be finite, got ", scale);
-    TORCH_CHECK_VALUE(cap >= 0. && std::isfinite(cap),
-                      "attend: cap must be positive, or 0 for none, got ", cap);
+    // as float32 numbers, with room for the factors that the kernels put to them
+    const double most = 0x1p126;
+    TORCH_CHECK_VALUE(std::abs(scale) <= most, "attend: scale must be finite in float32, got ",
+                      scale);
+    TORCH_CHECK_VALUE(cap >= 0. && cap <= most && (cap == 0.) == ((float)cap == 0.f),
+                      "attend: cap must be positive in float32, or 0 for none, got ", cap);
+    TORCH_CHECK_VALUE(cap == 0. || std::abs((float)scale / (float)cap) <= (float)most,
+                      "attend: cap is too small for a scale of ", scale, ", got ", cap);
     TORCH_CHECK_VALUE(p.a.dtype == TM_F32 || cap <= TM_ATTENTION_MAX_CAP_16,
                       "attend: cap must be at most ", (int)TM_ATTENTION_MAX_CAP_16,
                       " for 16-bit types, got ", cap);
