@@ -408,7 +408,8 @@ int tm_attention_backward_lse(const tm_attention *a, const void *out, const void
  * sections[a] pairs turn by axis a: pair p of a token by the angle
  * positions[axis(p)] * freqs[p] (the opposite angle with `inverse`, which is the
  * gradient).  Pair p is features p and P + p, or 2p and 2p + 1 where
- * interleaved, P the number of pairs; the features past 2 P are copied. */
+ * interleaved, P the number of pairs; the features past 2 P are copied.  P is at most 4096, H D
+ * at most 2^24 and B L less than 2^24 (4096 / P), rounded down (TM_ERR_UNSUPPORTED_SHAPE). */
 enum { TM_ROTATE_MAX_AXES = 4 };
 typedef struct tm_rotation {
     const void *x, *positions;

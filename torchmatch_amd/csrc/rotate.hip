@@ -191,11 +191,14 @@ extern "C" int tm_rotate(const tm_rotation *r, void *out, hipStream_t stream) {
     // for each compute unit; the table's size bounds it too
     int64_t per = std::max<int64_t>(1, 1024 / per_token);
     per = std::min(per, std::max<int64_t>(1, p.tokens / 1024));
+    // and a launch takes less than 2^32 threads, 2^24 blocks
+    const int64_t most = (1 << 24) - 1;
+    per = std::max(per, (p.tokens + most - 1) / most);
     if (p.pairs)
         per = std::min<int64_t>(per, kTable / p.pairs);
     p.per_block = (int32_t)per;
     const int64_t blocks = (p.tokens + per - 1) / per;
-    if (blocks > INT32_MAX)
+    if (blocks > most)
         return TM_ERR_UNSUPPORTED_SHAPE;
     const unsigned n = (unsigned)blocks;
     if (r->dtype == TM_BF16)
