@@ -29,8 +29,7 @@ hipStream_t current_stream(const Tensor &t) {
 }
 
 void check_rc(int rc, const char *op) {
-    TORCH_CHECK(rc != TM_ERR_LAUNCH, op, ": kernel launch failed: ",
-                hipGetErrorString(hipGetLastError()));
+    TORCH_CHECK(rc != TM_ERR_LAUNCH, op, ": kernel launch failed"); // the entry took the error
     TORCH_CHECK(rc == TM_OK, op, ": the library refused the call (code ", rc, ")");
 }
 
@@ -395,8 +394,9 @@ struct AttendFunction : torch::autograd::Function<AttendFunction> {
         auto [dq, dk, dv] =
             op.call(dout, s[0], s[1], s[2], s[3], s[4], s[5], opt(6), opt(7), opt(8), opt(9),
                     opt(10), opt(11), opt(12),
-                    grads[1].defined() ? OptTensor(grads[1]) : OptTensor(), ctx->saved_data["scale"].toDouble(),
-                    ctx->saved_data["cap"].toDouble(), ctx->saved_data["causal"].toBool());
+                    grads[1].defined() ? OptTensor(grads[1]) : OptTensor(),
+                    ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble(),
+                    ctx->saved_data["causal"].toBool());
         result[0] = dq;
         result[1] = dk;
         result[2] = dv;
