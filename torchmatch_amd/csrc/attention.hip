@@ -149,9 +149,10 @@ Splits splits_of(const tm_attention *a) {
 // unit, the group's heads and then the queries are split over up to 512 blocks of at least two
 // tiles of 64 queries each, whose float32 sums a second kernel adds in their order.  The whole
 // backward pass, whole against split, us: 16384 causal, H 8, Hkv 1, D 128, bf16 (128 blocks)
-// 5486, 2212; 4096 causal, H 4, Hkv 1, D 64 (32) 585, 174; 3 x 515 causal, H 32, Hkv 8, D 128,
-// f32 (120) 826, 487; 333, H 4, D 64, f32 (12) 111, 84; 2 x 2048, H 8, D 64, f16 (256) 134, 129;
-// 4096, H 6, D 128, bf16 (192) 335, 353.  256 blocks and 1024 were as fast or slower.
+// 5562, 2272; 4096 causal, H 4, Hkv 1, D 64 (32) 590, 169; 3 x 515 causal, H 32, Hkv 8, D 128,
+// f32 (120) 836, 479; 333, H 4, D 64, f32 (12) 109, 80; 4 x 2048 causal, H 16, Hkv 4, D 128, bf16
+// (256) 453, 358; 4096, H 6, D 128, bf16 (192) 329, 351.  256 blocks and 1024 were as fast or
+// slower.
 struct KvSplits {
     int n, heads, tiles;
 };

@@ -3,16 +3,16 @@
 //
 // Both form the weights again from the forward pass's log of the sum:
 //     p = exp(s - lse),  dp = do v^T,  ds = p (dp - delta) (1 - tanh^2)
-// with delta = sum over d of out do, less the gradient of lse (whose own is p).  attend_backward_kv owns keys (32 a wave) and runs over the
-// queries, of every head that shares them, or of a part of these where blocks are few
-// (attend_join_kv adds the parts):
+// with delta = sum over d of out do, less the gradient of lse (whose own is p).
+// attend_backward_kv owns keys (32 a wave) and runs over the queries, of every head that shares
+// them, or of a part of these where blocks are few (attend_join_kv adds the parts):
 //     dv^T += do^T p,  dk^T += q^T ds      (weights as queries by keys)
 // attend_backward_q owns queries and runs over the keys:
 //     dq^T += k^T ds^T                      (weights as keys by queries)
-// Seven products in place of the five of one kernel that would have to add dq from many
-// blocks.  p and ds are rounded to the inputs' type for the second products, as the forward
-// pass rounds its weights, and held in half precision's range (grad_shift, Column); sums stay in
-// float32.
+// Eight products (dq takes two; seven for float32, whose ds is not rounded) in place of the five
+// of one kernel that would have to add dq from many blocks.  p and ds are rounded to the inputs'
+// type for the second products, as the forward pass rounds its weights, and held in half
+// precision's range (grad_shift, Column); sums stay in float32.
 #ifndef TORCHMATCH_AMD_ATTN_BACKWARD_H
 #define TORCHMATCH_AMD_ATTN_BACKWARD_H
 
@@ -31,8 +31,9 @@ template <typename T, int DP> struct BackwardShape {
     // every other tile of queries (2 x 8192 packed in documents, 128 features, with blocks as
     // they stand: 440 us; 595 with one team and k and v in registers, 700 with a pass for dk and
     // one for dv; but 125 in place of 104 for pairs of sets of 64 features).  With the longest
-    // blocks first these two take 345 and 87 us: waits for tiles and barriers bound them, with
-    // matrix products under way in a sixth of the cycles.  Larger rows leave room for one team.
+    // blocks first these two take 336 and 87 us: waits (for tiles, barriers and, at 128 features,
+    // nine registers in scratch) bound them, with matrix products under way in a fifth and a
+    // sixth of the cycles.  Larger rows leave room for one team.
     static constexpr int kTeams = Tile<T, DP>::U == 16 ? 2 : 1;
     static constexpr int kKvRows = kTeams == 2 ? 32 : kRows;
     static constexpr bool kKeysInLds = kTeams == 2;

@@ -25,8 +25,9 @@ template <typename T, int DP, bool SIDE> struct ForwardShape {
     // every 4, and the weights take as long as the products: what counts is waves a SIMD, and
     // with it registers.  Three up to 128 bytes a row; with 256 bytes only where there are no
     // documents and positions, and 32 keys at a time (causal, 32768 rows of 128 features, 16
-    // heads: 4.5 ms in place of 4.8, 0.97 PFLOP/s; 2 x 8192 packed in documents, with blocks
-    // as they stand, 192 us, 267 with three, and 170 with the longest blocks first).
+    // heads: 4.5 to 4.6 ms in place of 4.8, 0.96 PFLOP/s, though five registers are in scratch;
+    // 2 x 8192 packed in documents, with blocks as they stand, 192 us, 267 with three, and 160
+    // with the longest blocks first).
     static constexpr int kBytes = sizeof(T) * DP;
     static constexpr int kOccupancy = kBytes <= 128 || (kBytes <= 256 && !SIDE) ? 3
                                       : kBytes <= 256                          ? 2
