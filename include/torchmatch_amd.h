@@ -420,6 +420,40 @@ typedef struct tm_rotation {
 } tm_rotation;
 int tm_rotate(const tm_rotation *r, void *out, hipStream_t stream);
 
+/* The same with each head normed first:
+ *   y = R(x (mean_d x_d^2 + eps)^-1/2 w)
+ * weight: (groups, D) contiguous, of weight_type (rotation.dtype or TM_F32), or NULL for ones; row g
+ * is for heads[g] heads, which follow each other and make up all H.  D is at most
+ * TM_NORM_MAX_HEAD_DIM (TM_ERR_UNSUPPORTED_SHAPE), rotation.inverse 0.  Sums are float32.
+ * out: (B, L, H, D), contiguous. */
+enum { TM_NORM_MAX_GROUPS = 8, TM_NORM_MAX_HEAD_DIM = 512 };
+typedef struct tm_norm_rotation {
+    tm_rotation rotation;
+    const void *weight;
+    int32_t weight_type, groups;
+    int32_t heads[8];
+    float eps;
+} tm_norm_rotation;
+int tm_norm_rotate(const tm_norm_rotation *n, void *out, hipStream_t stream);
+
+/* Gradients from that of the output, (B, L, H, D) with its own strides: dx (B, L, H, D), contiguous,
+ * and dweight, as weight; either may be NULL.  workspace (needed for dweight): device, at least
+ * tm_norm_rotate_backward_workspace_bytes(n), 16-byte aligned, any contents.  The same call gives the
+ * same bits. */
+size_t tm_norm_rotate_backward_workspace_bytes(const tm_norm_rotation *n);
+int tm_norm_rotate_backward(const tm_norm_rotation *n, const void *dout, int64_t do_b, int64_t do_l,
+                            int64_t do_h, void *dx, void *dweight, void *workspace,
+                            size_t workspace_bytes, hipStream_t stream);
+
+/* Dropout of `count` elements that lie one after the other.  Element i stays where word i % 4 of the
+ * ten-round Philox 4x32 generator is at least round(p 2^32); the counter's words are i / 4 (low, high) and
+ * offset (low, high), the key's seed (low, high).
+ *   out_i = residual_i + x_i / (1 - p) where it stays, residual_i elsewhere
+ * residual may be NULL; out may be x or residual.  seed_at: where the seed lies on the device when
+ * the kernel runs, or NULL for `seed`.  The gradient is the same call on the output's. */
+int tm_dropout(const void *x, const void *residual, void *out, int64_t count, int32_t dtype, double p,
+               uint64_t seed, const int64_t *seed_at, uint64_t offset, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -38,8 +38,9 @@ HIP_SOURCES = ["jv_batch.hip", "jv_large.hip", "jv_unpack.hip", "sinkhorn.hip", 
                "sinkhorn_resident.hip", "sk_tiles_narrow.hip", "sk_tiles_wide.hip",
                "sk_tiles_f64.hip", "attention.hip", "attn_forward_bf16.hip",
                "attn_forward_f16.hip", "attn_forward_f32.hip", "attn_backward_bf16.hip",
-               "attn_backward_f16.hip", "attn_backward_f32.hip", "rotate.hip"]
-OPS_SOURCES = ["torch_ops.cpp", "torch_attention.cpp"]
+               "attn_backward_f16.hip", "attn_backward_f32.hip", "rotate.hip", "norm_rotate.hip",
+               "dropout.hip"]
+OPS_SOURCES = ["torch_ops.cpp", "torch_attention.cpp", "torch_layers.cpp"]
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = "gfx950"
 

@@ -60,6 +60,15 @@ class Rotation(ctypes.Structure):
     ]
 
 
+class NormRotation(ctypes.Structure):
+    """``tm_norm_rotation``: heads to norm and turn."""
+
+    _fields_ = [
+        ("rotation", Rotation), ("weight", ctypes.c_void_p), ("weight_type", ctypes.c_int32),
+        ("groups", ctypes.c_int32), ("heads", ctypes.c_int32 * 8), ("eps", ctypes.c_float),
+    ]
+
+
 # symbol -> (restype, argtypes); the declarations of include/torchmatch_amd.h
 _VP = ctypes.c_void_p
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -193,6 +202,24 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ],
     ),
     "tm_rotate": (ctypes.c_int, [ctypes.POINTER(Rotation), _VP, _VP]),
+    "tm_norm_rotate": (ctypes.c_int, [ctypes.POINTER(NormRotation), _VP, _VP]),
+    "tm_norm_rotate_backward_workspace_bytes": (
+        ctypes.c_size_t, [ctypes.POINTER(NormRotation)]
+    ),
+    "tm_norm_rotate_backward": (
+        ctypes.c_int,
+        [
+            ctypes.POINTER(NormRotation), _VP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+            _VP, _VP, _VP, ctypes.c_size_t, _VP,
+        ],
+    ),
+    "tm_dropout": (
+        ctypes.c_int,
+        [
+            _VP, _VP, _VP, ctypes.c_int64, ctypes.c_int32, ctypes.c_double, ctypes.c_uint64, _VP,
+            ctypes.c_uint64, _VP,
+        ],
+    ),
 }
 
 

@@ -1,12 +1,14 @@
 """Attention for matching networks on MI355X: the layers that produce the scores which
 :mod:`torchmatch_amd.assignment` and :mod:`torchmatch_amd.transport` solve on.
 
-Registers ``torch.ops.attention.attend`` and ``torch.ops.attention.rotate``.
+Attention itself, and what a layer has around it.  Registers ``torch.ops.attention.attend``,
+``rotate``, ``norm_rotate`` and ``dropout``.
 """
 
 from __future__ import annotations
 
 from torchmatch_amd.attention import ops
 from torchmatch_amd.attention._attend import attend, rotary_frequencies, rotate
+from torchmatch_amd.attention._layers import dropout, norm_rotate
 
-__all__ = ["attend", "ops", "rotary_frequencies", "rotate"]
+__all__ = ["attend", "dropout", "norm_rotate", "ops", "rotary_frequencies", "rotate"]

@@ -11,6 +11,9 @@ _load()
 attend = torch.ops.attention.attend
 attend_backward = torch.ops.attention.attend_backward
 rotate = torch.ops.attention.rotate
+norm_rotate = torch.ops.attention.norm_rotate
+norm_rotate_backward = torch.ops.attention.norm_rotate_backward
+dropout = torch.ops.attention.dropout
 
 
 @torch.library.register_fake("attention::attend")
@@ -43,4 +46,27 @@ def _rotate_fake(x, positions, freqs, sections, interleaved=False, inverse=False
     return x.new_empty(x.shape)
 
 
-__all__ = ["attend", "attend_backward", "rotate"]
+@torch.library.register_fake("attention::norm_rotate")
+def _norm_rotate_fake(x, weight, positions, freqs, sections, heads, eps, interleaved=False):
+    del weight, positions, freqs, sections, heads, eps, interleaved
+    torch._check(x.dim() == 4, lambda: "x must be 4D (B, L, heads, D)")
+    return x.new_empty(x.shape)
+
+
+@torch.library.register_fake("attention::norm_rotate_backward")
+def _norm_rotate_backward_fake(dout, x, weight, positions, freqs, sections, heads, eps,
+                               interleaved=False, need_x=True, need_weight=True):
+    del dout, positions, freqs, sections, heads, eps, interleaved
+    return (x.new_empty(x.shape if need_x else (0,)),
+            weight.new_empty(weight.shape) if need_weight and weight is not None
+            else x.new_empty(0))
+
+
+@torch.library.register_fake("attention::dropout")
+def _dropout_fake(x, p, seed=0, offset=0, seed_at=None, residual=None):
+    del p, seed, offset, seed_at, residual
+    return x.new_empty(x.shape)
+
+
+__all__ = ["attend", "attend_backward", "dropout", "norm_rotate", "norm_rotate_backward",
+           "rotate"]

@@ -6,59 +6,25 @@
 // and written once.  A block takes a few tokens; it computes their cosines and sines once
 // into LDS, whatever the number of heads, and then streams the heads through.
 //
-// The angle is reduced to a fraction of a turn in double precision (positions may be in the
-// hundred thousands; a float32 product would be off by 1e-2 there), a few operations per
-// token and pair that the heads share.
-#include "../../include/torchmatch_amd.h"
-
-#include <hip/hip_runtime.h>
-#include <stdint.h>
+// The angle's reduction in double precision is a few operations per token and pair that the
+// heads share.
+#include "rotate.h"
 
 #include <algorithm>
 
 namespace {
 
-typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-template <typename T, int V> struct Unit;
-template <> struct Unit<__bf16, 8> { using type = b16x8; };
-template <> struct Unit<_Float16, 8> { using type = h16x8; };
-template <> struct Unit<float, 4> { using type = f32x4; };
+using rot::kTable;
+using rot::Turns;
+using rot::Unit;
 
 struct RotateArgs {
-    const void *x, *pos;
-    const float *freqs;
+    rot::Places at;
+    const void *x;
     void *out;
-    int64_t x_b, x_l, x_h, pos_b, tokens;
-    int32_t L, H, D, pairs, axes, pos_type, interleaved, per_block;
-    int32_t ends[TM_ROTATE_MAX_AXES]; // the first pair past each axis
-    float sign;
+    int64_t x_b, x_l, x_h, tokens;
+    int32_t L, H, D, pairs, interleaved, per_block;
 };
-
-__device__ inline double position(const RotateArgs &p, int64_t i) {
-    switch (p.pos_type) {
-    case TM_POS_F32: return (double)((const float *)p.pos)[i];
-    case TM_POS_I32: return (double)((const int32_t *)p.pos)[i];
-    default: return (double)((const int64_t *)p.pos)[i];
-    }
-}
-
-// (cos, sin) of N consecutive pairs, N even, read 16 bytes at a time
-template <int N> struct Turns {
-    f32x4 w[N / 2];
-    __device__ inline explicit Turns(const float2 *from) {
-#pragma unroll
-        for (int n = 0; n < N / 2; ++n)
-            w[n] = ((const f32x4 *)from)[n];
-    }
-    __device__ inline float2 at(int j) const {
-        return make_float2(w[j / 2][2 * (j % 2)], w[j / 2][2 * (j % 2) + 1]);
-    }
-};
-
-constexpr int kTable = 4096; // (cos, sin) of a block, 32 KB
 
 // V: elements a load (16 bytes, or 1 where strides, sizes or addresses do not allow it)
 template <typename T, int V>
@@ -69,21 +35,7 @@ __global__ __launch_bounds__(256) void rotate_pairs(const RotateArgs p) {
     for (int i = threadIdx.x; i < tokens * p.pairs; i += 256) {
         const int pair = i % p.pairs;
         const int64_t t = first + i / p.pairs;
-        int axis = 0;
-#pragma unroll
-        for (int a = 0; a + 1 < TM_ROTATE_MAX_AXES; ++a)
-            axis += a + 1 < p.axes && pair >= p.ends[a];
-        const double turns = position(p, t / p.L * p.pos_b + t % p.L * p.axes + axis) *
-                             (double)p.freqs[pair] * 0.15915494309189533577;
-        const float r = (float)(turns - rint(turns));
-        float c, s;
-        if constexpr (sizeof(T) == 4) {
-            sincospif(2.f * r, &s, &c);
-        } else { // to 2^-20, which 16 bits do not show
-            s = __builtin_amdgcn_sinf(r);
-            c = __builtin_amdgcn_cosf(r);
-        }
-        table[i] = make_float2(c, p.sign * s);
+        table[i] = rot::turn_of<T>(p.at, t / p.L * p.at.pos_b + t % p.L * p.at.axes, pair);
     }
     __syncthreads();
 
@@ -154,19 +106,13 @@ template <typename T, int V> void launch(const RotateArgs &p, unsigned blocks, h
 } // namespace
 
 extern "C" int tm_rotate(const tm_rotation *r, void *out, hipStream_t stream) {
-    if (!r || r->B < 0 || r->L < 0 || r->H < 0 || r->D < 1 || r->axes < 1 ||
-        r->axes > TM_ROTATE_MAX_AXES || r->dtype < TM_BF16 || r->dtype > TM_F32 ||
-        r->pos_type < TM_POS_F32 || r->pos_type > TM_POS_I64)
+    if (!r || r->B < 0 || r->L < 0 || r->H < 0 || r->D < 1 || r->dtype < TM_BF16 ||
+        r->dtype > TM_F32)
         return TM_ERR_INVALID_ARGUMENT;
     RotateArgs p = {};
-    for (int a = 0; a < r->axes; ++a) {
-        if (r->sections[a] < 0 || r->sections[a] > r->D)
-            return TM_ERR_INVALID_ARGUMENT;
-        p.pairs += r->sections[a];
-        p.ends[a] = p.pairs;
-    }
-    if (2 * (int64_t)p.pairs > r->D)
-        return TM_ERR_INVALID_ARGUMENT;
+    if (const int rc = rot::places(*r, p.at))
+        return rc;
+    p.pairs = p.at.pairs;
     if (p.pairs > kTable || r->D > 2 * kTable || (int64_t)r->H * r->D > (1 << 24))
         return TM_ERR_UNSUPPORTED_SHAPE;
     p.tokens = (int64_t)r->B * r->L;
@@ -174,11 +120,10 @@ extern "C" int tm_rotate(const tm_rotation *r, void *out, hipStream_t stream) {
         return TM_OK;
     if (!r->x || !out || !r->positions || (p.pairs && !r->freqs))
         return TM_ERR_INVALID_ARGUMENT;
-    p.x = r->x, p.pos = r->positions, p.freqs = r->freqs, p.out = out;
-    p.x_b = r->x_b, p.x_l = r->x_l, p.x_h = r->x_h, p.pos_b = r->pos_b;
-    p.L = r->L, p.H = r->H, p.D = r->D, p.axes = r->axes, p.pos_type = r->pos_type;
+    p.x = r->x, p.out = out;
+    p.x_b = r->x_b, p.x_l = r->x_l, p.x_h = r->x_h;
+    p.L = r->L, p.H = r->H, p.D = r->D;
     p.interleaved = r->interleaved ? 1 : 0;
-    p.sign = r->inverse ? -1.f : 1.f;
 
     const int size = r->dtype == TM_F32 ? 4 : 2, unit = 16 / size;
     const bool wide = !(((uintptr_t)r->x | (uintptr_t)out) % 16) && !(r->x_b % unit) &&
