@@ -454,6 +454,36 @@ int tm_norm_rotate_backward(const tm_norm_rotation *n, const void *dout, int64_t
 int tm_dropout(const void *x, const void *residual, void *out, int64_t count, int32_t dtype, double p,
                uint64_t seed, const int64_t *seed_at, uint64_t offset, hipStream_t stream);
 
+/* The gated feed-forward block on T rows:
+ *   y = (act(x gate^T) * (x up^T)) down^T
+ * x is (T, C), gate and up are (F, C), down is (O, F), of `dtype`, rows `_l` elements apart; addresses
+ * and rows at multiples of 16 bytes, fewer than TM_FF_MAX_ROW_BYTES from row to row; where C (F for
+ * down) elements do not fill whole units of 16 bytes, the last unit's rest is zeros.  Sums are float32; the
+ * hidden features are rounded to `dtype` once, as are their gradients (float16 holds these
+ * times a power of two that brings the largest |dout| to 1 .. 2). */
+enum { TM_SILU = 0, TM_GELU = 1, TM_GELU_TANH = 2, TM_RELU = 3 };
+enum { TM_FF_MAX_ROW_BYTES = 1 << 23, TM_FF_MAX_BLOCKS = 1 << 22 };
+typedef struct tm_feed_forward {
+    const void *x, *gate, *up, *down;
+    int64_t x_l, w_l, down_l; /* w_l: of gate and of up */
+    int32_t dtype, activation, T, C, F, O;
+} tm_feed_forward;
+
+/* out: (T, O), contiguous.  saved: for the gradients, tm_feed_forward_saved_bytes(f) bytes, or NULL.
+ * workspace, saved: device, 16-byte aligned, any contents. */
+size_t tm_feed_forward_workspace_bytes(const tm_feed_forward *f);
+size_t tm_feed_forward_saved_bytes(const tm_feed_forward *f);
+int tm_feed_forward_forward(const tm_feed_forward *f, void *out, void *saved, void *workspace,
+                            size_t workspace_bytes, hipStream_t stream);
+
+/* Gradients from that of the output, (T, O) with rows do_l elements apart as x's are: dx (T, C), dgate
+ * and dup (F, C), ddown (O, F), contiguous; those not asked for are NULL, dgate and dup go together.
+ * The same call gives the same bits: nothing is added by atomics. */
+size_t tm_feed_forward_backward_workspace_bytes(const tm_feed_forward *f);
+int tm_feed_forward_backward(const tm_feed_forward *f, const void *saved, const void *dout,
+                             int64_t do_l, void *dx, void *dgate, void *dup, void *ddown,
+                             void *workspace, size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

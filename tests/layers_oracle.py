@@ -91,3 +91,87 @@ def dropout(x, p, seed, offset=0, residual=None):
     r = residual.detach().double().cpu() if residual is not None else torch.zeros_like(kept)
     y = r + kept
     return y, u * y.abs() + z + 4 * ULP * (kept.abs() + r.abs())
+
+
+# ---- feed_forward --------------------------------------------------------------------
+
+
+def _activation(a, name):
+    """Value, slope, and how much the slope changes with a, at most."""
+    if name == "silu":
+        s = torch.sigmoid(a)
+        return a * s, s * (1 + a * (1 - s)), 0.5
+    if name == "relu":
+        return a.clamp(min=0), (a > 0).double(), 0.0
+    if name == "gelu":
+        cdf = 0.5 * torch.erfc(-a / 2**0.5)
+        return a * cdf, cdf + a * torch.exp(-a * a / 2) / (2 * torch.pi) ** 0.5, 0.8
+    k = (2 / torch.pi) ** 0.5
+    t = torch.tanh(k * (a + 0.044715 * a**3))
+    return 0.5 * a * (1 + t), \
+        0.5 * (1 + t) + 0.5 * a * (1 - t * t) * k * (1 + 3 * 0.044715 * a * a), 0.8
+
+
+def feed_forward(x, gate, up, down, activation, dy=None):
+    """name -> (value, bound, spread) of y (and dx, dgate, dup, ddown) in float64, on x's device.
+
+    bound: every product's sum is off by its length times 2^-23 of its terms' sizes (float32), an
+    activation by 2^-19 |a| (16 bits: hardware exponentials; float32 2^-21), a slope by as much of
+    1 + |a|; h, da and db are rounded (u); a and b are saved with 2^-15 (16-bit types).
+    spread: what independent roundings of h, da and db by one part put a result off by, in squares.
+    """
+    dtype, c = x.dtype, x.shape[-1]
+    u, z = UNIT[dtype] or ULP, FLOOR[dtype]
+    half = dtype != torch.float32
+    cut, act_off = (2.0**-15, 2.0**-19) if half else (0.0, 2.0**-21)
+    xd, g, w, d = (t.detach().double() for t in (x, gate, up, down))
+    xd = xd.reshape(-1, c)
+    length = lambda n: n * 2.0**-23  # noqa: E731
+    a, b = xd @ g.t(), xd @ w.t()
+    ea, eb = (length(c) * (xd.abs() @ m.abs().t()) for m in (g, w))
+    act, slope, bend = _activation(a, activation)
+
+    def slope_off(ea):
+        if activation == "relu":
+            return (a.abs() <= ea).double()
+        return bend * ea + act_off * (1 + a.abs())
+
+    h = act * b
+    eh = (slope.abs() * ea + bend * ea * ea + act_off * a.abs()) * (b.abs() + eb) + act.abs() * eb
+    eh = eh + u * h.abs() + z
+    y = h @ d.t()
+    ey = eh @ d.abs().t() + length(len(gate)) * (h.abs() @ d.abs().t()) + u * y.abs() + z
+    found = {"y": (y.view(*x.shape[:-1], -1), ey.view(*x.shape[:-1], -1),
+                   (h.square() @ d.square().t()).sqrt().view(*x.shape[:-1], -1))}
+    if dy is None:
+        return found
+    dyd = dy.detach().double().reshape(len(xd), -1)
+    dh = dyd @ d
+    edh = length(len(down)) * (dyd.abs() @ d.abs())
+    ea, eb = ea + cut * a.abs(), eb + cut * b.abs()
+    es = slope_off(ea)
+    da, db = dh * b * slope, dh * act
+    top = dyd.abs().max().item() if dyd.numel() else 1.0
+    zg = z * 2 * top  # float16: held times a power of two that brings dy to 1 .. 2
+    eda = edh * (b * slope).abs() + dh.abs() * (eb * slope.abs() + (b.abs() + eb) * es) \
+        + (u + 4 * ULP) * da.abs() + zg
+    edb = edh * act.abs() + dh.abs() * (slope.abs() * ea + bend * ea * ea + act_off * a.abs()) \
+        + (u + 4 * ULP) * db.abs() + zg
+    # h again, from what was saved
+    eh = (slope.abs() * ea + bend * ea * ea + act_off * a.abs()) * (b.abs() + eb) \
+        + act.abs() * eb + u * h.abs() + z
+
+    def product(terms, n):
+        value = sum(p @ q for p, q, _ in terms)
+        size = sum(p.abs() @ q.abs() for p, q, _ in terms)
+        off = sum(e @ q.abs() for _, q, e in terms)
+        spread = sum(p.square() @ q.square() for p, q, _ in terms).sqrt()
+        return value, off + length(n) * size + u * value.abs() + z, spread
+
+    v = product([(da, g, eda), (db, w, edb)], 2 * len(gate))
+    found["dx"] = tuple(t.view(x.shape) for t in v)
+    n = len(xd)
+    found["dgate"] = product([(da.t(), xd, eda.t())], n)
+    found["dup"] = product([(db.t(), xd, edb.t())], n)
+    found["ddown"] = tuple(t.t() for t in product([(h.t(), dyd, eh.t())], n))
+    return found

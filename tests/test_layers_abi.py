@@ -84,6 +84,73 @@ def test_norm_rotate_backward_refusals():
     assert back(dw=None, B=0) == _native.TM_OK
 
 
+def _block(**changes):
+    fields = {"x": 4096, "gate": 4096, "up": 4096, "down": 4096, "x_l": 64, "w_l": 64,
+              "down_l": 96, "dtype": _native.TM_BF16, "activation": _native.TM_SILU, "T": 10,
+              "C": 64, "F": 96, "O": 32}
+    fields.update(changes)
+    return _native.FeedForward(**fields)
+
+
+@pytest.mark.parametrize("changes,code", [
+    ({"T": 0}, _native.TM_OK),
+    ({"T": -1}, _native.TM_ERR_INVALID_ARGUMENT),
+    ({"C": 0}, _native.TM_ERR_INVALID_ARGUMENT),
+    ({"F": 0}, _native.TM_ERR_INVALID_ARGUMENT),
+    ({"O": -5}, _native.TM_ERR_INVALID_ARGUMENT),
+    ({"dtype": 3}, _native.TM_ERR_INVALID_ARGUMENT),
+    ({"activation": 4}, _native.TM_ERR_INVALID_ARGUMENT),
+    ({"x": 4098}, _native.TM_ERR_INVALID_ARGUMENT),
+    ({"gate": None}, _native.TM_ERR_INVALID_ARGUMENT),
+    ({"x_l": 68}, _native.TM_ERR_INVALID_ARGUMENT),
+    ({"w_l": 56}, _native.TM_ERR_INVALID_ARGUMENT),
+    ({"down_l": -96}, _native.TM_ERR_INVALID_ARGUMENT),
+    ({"x_l": 1 << 22}, _native.TM_ERR_UNSUPPORTED_SHAPE),
+    ({"T": 2**31 - 1}, _native.TM_ERR_UNSUPPORTED_SHAPE),
+    ({"T": 1 << 30, "O": 1 << 20}, _native.TM_ERR_UNSUPPORTED_SHAPE),
+    ({}, _native.TM_ERR_WORKSPACE),
+])
+def test_feed_forward_refusals(changes, code):
+    f = _block(**changes)
+    assert _native.lib().tm_feed_forward_forward(ctypes.byref(f), 4096, None, None, 0,
+                                                 None) == code
+
+
+def test_feed_forward_backward_refusals():
+    lib = _native.lib()
+    size = lib.tm_feed_forward_backward_workspace_bytes(ctypes.byref(_block()))
+    assert size >= 3 * 10 * 96 * 2
+
+    def back(saved=4096, dout=4096, do_l=32, dx=4096, dgate=4096, dup=4096, ddown=4096, ws=4096,
+             bytes_=size, **changes):
+        f = _block(**changes)
+        return lib.tm_feed_forward_backward(ctypes.byref(f), saved, dout, do_l, dx, dgate, dup,
+                                            ddown, ws, bytes_, None)
+
+    assert back(bytes_=size - 1) == _native.TM_ERR_WORKSPACE
+    assert back(ws=None) == _native.TM_ERR_WORKSPACE
+    assert back(ws=4098) == _native.TM_ERR_WORKSPACE
+    assert back(dgate=None) == _native.TM_ERR_INVALID_ARGUMENT
+    assert back(do_l=31) == _native.TM_ERR_INVALID_ARGUMENT
+    assert back(do_l=24) == _native.TM_ERR_INVALID_ARGUMENT
+    assert back(saved=None) == _native.TM_ERR_INVALID_ARGUMENT
+    assert back(dout=None) == _native.TM_ERR_INVALID_ARGUMENT
+    assert back(do_l=1 << 22) == _native.TM_ERR_UNSUPPORTED_SHAPE
+    assert back(dx=None, dgate=None, dup=None, ddown=None) == _native.TM_OK
+    assert back(dgate=None, dup=None, ddown=None, T=0) == _native.TM_OK
+
+
+def test_feed_forward_sizes():
+    lib = _native.lib()
+    saved = lambda **c: lib.tm_feed_forward_saved_bytes(ctypes.byref(_block(**c)))  # noqa: E731
+    assert saved() == 10 * 96 * 6 and saved(dtype=_native.TM_F32) == 10 * 96 * 8
+    assert saved(F=90, down_l=96) == 10 * 96 * 6
+    assert saved(T=0) == 0
+    size = lib.tm_feed_forward_workspace_bytes(ctypes.byref(_block()))
+    assert size >= 10 * 96 * 2
+    assert lib.tm_feed_forward_workspace_bytes(ctypes.byref(_block(T=0))) == 0
+
+
 def test_dropout_refusals():
     drop = lambda x=4096, out=4096, n=8, dtype=0, p=0.5: _native.lib().tm_dropout(  # noqa: E731
         x, None, out, n, dtype, p, 0, None, 0, None)
@@ -120,6 +187,15 @@ def test_fake_kernels():
         dx, dw = torch.ops.attention.norm_rotate_backward(y, x, w, pos, f, [8], [3, 1], 1e-6)
         assert dx.shape == x.shape and dw.shape == w.shape and dw.dtype == torch.float32
         assert torch.ops.attention.dropout(x, 0.1, residual=x).shape == x.shape
+        w, d = (torch.empty(n, m, dtype=torch.bfloat16, device="cuda")
+                for n, m in ((20, 16), (5, 20)))
+        y = torch.ops.attention.feed_forward(x, w, w, d, "silu")
+        assert y.shape == (2, 7, 4, 5) and y.dtype == x.dtype
+        _, saved = torch.ops.attention.feed_forward_save(x, w, w, d, "silu")
+        assert saved.shape == (56 * 24 * 6,) and saved.dtype == torch.uint8
+        grads = torch.ops.attention.feed_forward_backward(y, x, w, w, d, saved, "silu",
+                                                          need_up=False)
+        assert [g.shape for g in grads] == [x.shape, w.shape, (0,), d.shape]
 
 
 def test_tangents_without_a_device():

@@ -39,7 +39,7 @@ HIP_SOURCES = ["jv_batch.hip", "jv_large.hip", "jv_unpack.hip", "sinkhorn.hip", 
                "sk_tiles_f64.hip", "attention.hip", "attn_forward_bf16.hip",
                "attn_forward_f16.hip", "attn_forward_f32.hip", "attn_backward_bf16.hip",
                "attn_backward_f16.hip", "attn_backward_f32.hip", "rotate.hip", "norm_rotate.hip",
-               "dropout.hip"]
+               "dropout.hip", "feed_forward.hip", "ff_bf16.hip", "ff_f16.hip", "ff_f32.hip"]
 OPS_SOURCES = ["torch_ops.cpp", "torch_attention.cpp", "torch_layers.cpp"]
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 ARCH = "gfx950"

@@ -31,6 +31,7 @@ TM_JV_FLAG_DONE = 0x80000000
 
 TM_BF16, TM_F16, TM_F32 = 0, 1, 2
 TM_POS_F32, TM_POS_I32, TM_POS_I64 = 0, 1, 2
+TM_SILU, TM_GELU, TM_GELU_TANH, TM_RELU = 0, 1, 2, 3
 
 
 class Attention(ctypes.Structure):
@@ -66,6 +67,16 @@ class NormRotation(ctypes.Structure):
     _fields_ = [
         ("rotation", Rotation), ("weight", ctypes.c_void_p), ("weight_type", ctypes.c_int32),
         ("groups", ctypes.c_int32), ("heads", ctypes.c_int32 * 8), ("eps", ctypes.c_float),
+    ]
+
+
+class FeedForward(ctypes.Structure):
+    """``tm_feed_forward``: a gated feed-forward block."""
+
+    _fields_ = [
+        *((n, ctypes.c_void_p) for n in ("x", "gate", "up", "down")),
+        *((n, ctypes.c_int64) for n in ("x_l", "w_l", "down_l")),
+        *((n, ctypes.c_int32) for n in ("dtype", "activation", "T", "C", "F", "O")),
     ]
 
 
@@ -211,6 +222,21 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [
             ctypes.POINTER(NormRotation), _VP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
             _VP, _VP, _VP, ctypes.c_size_t, _VP,
+        ],
+    ),
+    "tm_feed_forward_saved_bytes": (ctypes.c_size_t, [ctypes.POINTER(FeedForward)]),
+    "tm_feed_forward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FeedForward)]),
+    "tm_feed_forward_forward": (
+        ctypes.c_int, [ctypes.POINTER(FeedForward), _VP, _VP, _VP, ctypes.c_size_t, _VP]
+    ),
+    "tm_feed_forward_backward_workspace_bytes": (
+        ctypes.c_size_t, [ctypes.POINTER(FeedForward)]
+    ),
+    "tm_feed_forward_backward": (
+        ctypes.c_int,
+        [
+            ctypes.POINTER(FeedForward), _VP, _VP, ctypes.c_int64, _VP, _VP, _VP, _VP, _VP,
+            ctypes.c_size_t, _VP,
         ],
     ),
     "tm_dropout": (

@@ -1,5 +1,5 @@
 """What stands around attention in a layer of a matching network (no reference counterpart):
-queries and keys normed and turned in one pass, dropout.
+queries and keys normed and turned in one pass, the gated feed-forward block, dropout.
 
 Arguments are checked by the ops (``csrc/torch_layers.cpp``).  Device tensors only:
 there is no host fallback.
@@ -13,6 +13,7 @@ from torchmatch_amd.attention import ops
 from torchmatch_amd.attention._attend import _on_device
 
 _NORM_ROTATE, _DROPOUT = ops.norm_rotate.default, ops.dropout.default
+_FEED_FORWARD = ops.feed_forward.default
 
 
 def norm_rotate(  # noqa: PLR0913
@@ -47,6 +48,31 @@ def norm_rotate(  # noqa: PLR0913
         if weight is not None and weight.ndim == 1:
             weight = weight.unsqueeze(0)
     return _NORM_ROTATE(x, weight, positions, freqs, sections, heads, eps, interleaved)
+
+
+def feed_forward(
+    x: torch.Tensor,
+    gate: torch.Tensor,
+    up: torch.Tensor,
+    down: torch.Tensor,
+    *,
+    activation: str = "silu",
+) -> torch.Tensor:
+    """``(act(x @ gate.T) * (x @ up.T)) @ down.T``: the gated feed-forward block.
+
+    ``x`` is (..., C), ``gate`` and ``up`` are (F, C) and ``down`` is (O, F), as linear layers hold
+    them; gate and up may be the halves of one matrix.  ``activation`` is "silu", "gelu",
+    "gelu_tanh" (its approximation) or "relu".  Features contiguous and rows at multiples of 16
+    bytes are read in place, else copied; sizes that do not fill 16 bytes are padded.
+
+    bfloat16, float16 or float32, all of one type.  Products are summed in float32; the hidden
+    features are rounded to the type once, as are their gradients.  Half precision's hidden
+    features have its range (65504); their gradients are scaled by the output's, so that no loss
+    scaling is needed but for the results' own range.  Differentiable in all four, with the same
+    bits each time; only the gradients that are asked for are computed.  Reverse mode, once.
+    """
+    _on_device(x, "feed_forward", "x")
+    return _FEED_FORWARD(x, gate, up, down, activation)
 
 
 def dropout(

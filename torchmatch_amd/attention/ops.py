@@ -14,6 +14,8 @@ rotate = torch.ops.attention.rotate
 norm_rotate = torch.ops.attention.norm_rotate
 norm_rotate_backward = torch.ops.attention.norm_rotate_backward
 dropout = torch.ops.attention.dropout
+feed_forward = torch.ops.attention.feed_forward
+feed_forward_backward = torch.ops.attention.feed_forward_backward
 
 
 @torch.library.register_fake("attention::attend")
@@ -68,5 +70,27 @@ def _dropout_fake(x, p, seed=0, offset=0, seed_at=None, residual=None):
     return x.new_empty(x.shape)
 
 
-__all__ = ["attend", "attend_backward", "dropout", "norm_rotate", "norm_rotate_backward",
-           "rotate"]
+@torch.library.register_fake("attention::feed_forward")
+def _feed_forward_fake(x, gate, up, down, activation):
+    del gate, up, activation
+    return x.new_empty((*x.shape[:-1], down.shape[0]))
+
+
+@torch.library.register_fake("attention::feed_forward_save")
+def _feed_forward_save_fake(x, gate, up, down, activation):
+    rows, hidden = x.numel() // x.shape[-1], (gate.shape[0] + 7) // 8 * 8
+    size = 8 if x.dtype == torch.float32 else 6  # bytes for each hidden feature
+    return (_feed_forward_fake(x, gate, up, down, activation),
+            x.new_empty(rows * hidden * size, dtype=torch.uint8))
+
+
+@torch.library.register_fake("attention::feed_forward_backward")
+def _feed_forward_backward_fake(dout, x, gate, up, down, saved, activation,  # noqa: PLR0913
+                                need_x=True, need_gate=True, need_up=True, need_down=True):
+    del dout, saved, activation
+    return tuple(x.new_empty(t.shape if need else (0,)) for t, need in
+                 ((x, need_x), (gate, need_gate), (up, need_up), (down, need_down)))
+
+
+__all__ = ["attend", "attend_backward", "dropout", "feed_forward", "feed_forward_backward",
+           "norm_rotate", "norm_rotate_backward", "rotate"]

@@ -1,0 +1,272 @@
+// feed_forward.hip -- the gated feed-forward block: checks, sizes of tiles, launches.  The products
+// are in ff_tile.h.
+//
+//     a = x G^T, b = x U^T, h = act(a) b, y = h D^T
+//     dh = dy D; da = dh b act'(a), db = dh act(a); dx = da G + db U; dG = da^T x, dU = db^T x, dD = dy^T h
+//
+// Forward two launches: both projections with the activation and the product in the first's
+// epilogue, then D.  Backward: dh, in whose epilogue da, db and h again; dx; dG and dU together;
+// dD.  h, da and db are rounded to the inputs' type once, as operands of the next product have to be.  a and b
+// are not rounded to it: they are saved with 16 bits after the leading one (ff_tile.h), since each
+// enters two gradients that are rounded again (with a and b in bfloat16 those are off by 1.75
+// roundings, so by 1.42).
+#include "ff.h"
+
+#include "../../include/torchmatch_amd.h"
+
+#include <algorithm>
+
+namespace {
+
+using ff::Args;
+using ff::Kind;
+
+constexpr int64_t kMaxRows = INT32_MAX - 256;
+
+int size_of(const tm_feed_forward &f) { return f.dtype == TM_F32 ? 4 : 2; }
+int64_t hidden_row(const tm_feed_forward &f) { return ((int64_t)f.F + 7) / 8 * 8; }
+int64_t hidden_bytes(const tm_feed_forward &f) { // (T, hidden) of the inputs' type
+    return ((int64_t)f.T * hidden_row(f) * size_of(f) + 255) / 256 * 256;
+}
+
+// Tiles of a product and how often its k is split.
+struct Plan {
+    bool big;
+    int splits, split_steps;
+    size_t part; // bytes of partial sums
+};
+Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, int segments,
+          int batches) {
+    const int64_t step = 128 / size_of(f);
+    const auto tiles = [&](int64_t t) {
+        return (M + t - 1) / t * ((N + t - 1) / t) * batches * (kind == ff::kUp ? 2 : 1);
+    };
+    // rounds of blocks times a block's work, in tiles of 128 x 128: 256 blocks of the large tiles
+    // run at once, 512 of the small ones, which take a sixth longer for their share
+    const int64_t large = tiles(256), small = tiles(128);
+    const double t_large = (double)((large + 255) / 256) * 4.;
+    const double t_small = (double)((small + 511) / 512) * 2. * 7. / 6.;
+    Plan r = {t_large <= t_small, 1, 0, 0};
+    const int64_t steps = (K + step - 1) / step * segments;
+    const bool may = kind == ff::kDown || kind == ff::kInput || kind == ff::kWeights;
+    if (may && !r.big && small < 384)
+        r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(1, small),
+                                                               steps / 8));
+    r.split_steps = (int)((steps + r.splits - 1) / r.splits);
+    if (r.split_steps)
+        r.splits = (int)((steps + r.split_steps - 1) / r.split_steps);
+    r.splits = std::max(r.splits, 1);
+    if (r.splits > 1)
+        r.part = (size_t)r.splits * batches * M * N * sizeof(float);
+    return r;
+}
+
+Plan plan_up(const tm_feed_forward &f) { return plan(f, ff::kUp, f.T, f.F, f.C, 1, 1); }
+Plan plan_down(const tm_feed_forward &f) { return plan(f, ff::kDown, f.T, f.O, f.F, 1, 1); }
+Plan plan_hidden(const tm_feed_forward &f) { return plan(f, ff::kHidden, f.T, f.F, f.O, 1, 1); }
+Plan plan_input(const tm_feed_forward &f) { return plan(f, ff::kInput, f.T, f.C, f.F, 2, 1); }
+Plan plan_weights(const tm_feed_forward &f) {
+    return plan(f, ff::kWeights, f.F, f.C, f.T, 1, 2);
+}
+Plan plan_output(const tm_feed_forward &f) { return plan(f, ff::kWeights, f.O, f.F, f.T, 1, 1); }
+
+int check(const tm_feed_forward *f) {
+    if (!f || f->T < 0 || f->C < 1 || f->F < 1 || f->O < 1 || f->dtype < TM_BF16 ||
+        f->dtype > TM_F32 || f->activation < TM_SILU || f->activation > TM_RELU)
+        return TM_ERR_INVALID_ARGUMENT;
+    const int64_t unit = 16 / size_of(*f);
+    const auto odd = [&](const void *p, int64_t l, int64_t n) {
+        return (uintptr_t)p % 16 || l % unit || l < 0 || (l && l < n);
+    };
+    if (odd(f->x, f->x_l, f->C) || odd(f->gate, f->w_l, f->C) || odd(f->up, f->w_l, f->C) ||
+        odd(f->down, f->down_l, f->F))
+        return TM_ERR_INVALID_ARGUMENT;
+    const int64_t most = TM_FF_MAX_ROW_BYTES / size_of(*f);
+    if (f->x_l >= most || f->w_l >= most || f->down_l >= most ||
+        f->C >= most || f->O >= most || hidden_row(*f) >= most || f->T > kMaxRows)
+        return TM_ERR_UNSUPPORTED_SHAPE;
+    const auto blocks = [](int64_t m, int64_t n) { return ((m + 127) / 128) * ((n + 63) / 64); };
+    if (std::max({blocks(f->T, f->F), blocks(f->T, f->O), blocks(f->T, f->C),
+                  2 * blocks(f->F, f->C), blocks(f->O, f->F)}) > TM_FF_MAX_BLOCKS)
+        return TM_ERR_UNSUPPORTED_SHAPE;
+    return TM_OK;
+}
+
+int product(const tm_feed_forward &f, Args p, Kind kind, const Plan &how, void *part,
+            hipStream_t stream) {
+    p.splits = how.splits;
+    p.split_steps = how.split_steps;
+    p.part = how.part ? (float *)part : nullptr;
+    p.activation = f.activation;
+    const auto run = f.dtype == TM_BF16  ? ff::product_bf16
+                     : f.dtype == TM_F16 ? ff::product_f16
+                                         : ff::product_f32;
+    const auto join = f.dtype == TM_BF16  ? ff::join_bf16
+                      : f.dtype == TM_F16 ? ff::join_f16
+                                          : ff::join_f32;
+    if (run(p, kind, how.big, stream) || (p.part && join(p, stream)))
+        return TM_ERR_LAUNCH;
+    return TM_OK;
+}
+
+Args args(int64_t M, int64_t N, int64_t K) {
+    Args p = {};
+    p.M = (int32_t)M, p.N = (int32_t)N, p.K = (int32_t)K;
+    p.segments = p.batches = 1;
+    return p;
+}
+
+// rows of `out` at multiples of 16 bytes
+int wide(const tm_feed_forward &f, const void *out, int64_t l) {
+    return !((uintptr_t)out % 16) && l % (16 / size_of(f)) == 0;
+}
+
+void set_saved(const tm_feed_forward &f, Args &p, const void *saved) {
+    const int64_t plane = (int64_t)f.T * hidden_row(f) * size_of(f);
+    for (int n = 0; n < (f.dtype == TM_F32 ? 2 : 3); ++n)
+        p.saved[n] = (char *)const_cast<void *>(saved) + n * plane;
+}
+
+// The largest |x| of what each block takes of (rows, n), half precision.
+__global__ __launch_bounds__(256) void ff_most(const _Float16 *x, int64_t l, int rows, int n,
+                                               float *most) {
+    typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+    __shared__ float waves[4];
+    const int units = (n + 7) / 8; // a row's last unit ends in zeros
+    float m = 0.f;
+    for (int row = blockIdx.x; row < rows; row += ff::kMostParts)
+        for (int u = threadIdx.x; u < units; u += 256) {
+            const h16x8 v = *(const h16x8 *)(x + row * l + 8 * u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                m = fmaxf(m, fabsf((float)v[j]));
+        }
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2)
+        m = fmaxf(m, __shfl_xor(m, k));
+    if (threadIdx.x % 64 == 0)
+        waves[threadIdx.x / 64] = m;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        most[blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+}
+
+} // namespace
+
+extern "C" size_t tm_feed_forward_saved_bytes(const tm_feed_forward *f) {
+    if (check(f))
+        return 0;
+    return (size_t)(f->dtype == TM_F32 ? 2 : 3) * f->T * hidden_row(*f) * size_of(*f);
+}
+
+extern "C" size_t tm_feed_forward_workspace_bytes(const tm_feed_forward *f) {
+    if (check(f) || !f->T)
+        return 0;
+    return hidden_bytes(*f) + plan_down(*f).part;
+}
+
+extern "C" int tm_feed_forward_forward(const tm_feed_forward *f, void *out, void *saved,
+                                       void *workspace, size_t workspace_bytes,
+                                       hipStream_t stream) {
+    if (const int rc = check(f))
+        return rc;
+    if (!f->T)
+        return TM_OK;
+    if (!f->x || !f->gate || !f->up || !f->down || !out || (uintptr_t)saved % 16)
+        return TM_ERR_INVALID_ARGUMENT;
+    if (!workspace || (uintptr_t)workspace % 16 ||
+        workspace_bytes < tm_feed_forward_workspace_bytes(f))
+        return TM_ERR_WORKSPACE;
+    Args p = args(f->T, f->F, f->C);
+    p.a[0] = f->x, p.a_l = f->x_l;
+    p.b[0] = f->gate, p.b[1] = f->up, p.b_l = f->w_l;
+    p.out[0] = workspace, p.out_l = hidden_row(*f);
+    if (saved)
+        set_saved(*f, p, saved);
+    if (const int rc = product(*f, p, ff::kUp, plan_up(*f), nullptr, stream))
+        return rc;
+    p = args(f->T, f->O, f->F);
+    p.a[0] = workspace, p.a_l = hidden_row(*f);
+    p.b[0] = f->down, p.b_l = f->down_l;
+    p.out[0] = out, p.out_l = f->O, p.wide = wide(*f, out, f->O);
+    return product(*f, p, ff::kDown, plan_down(*f), (char *)workspace + hidden_bytes(*f), stream);
+}
+
+extern "C" size_t tm_feed_forward_backward_workspace_bytes(const tm_feed_forward *f) {
+    if (check(f))
+        return 0;
+    return ff::kMostParts * sizeof(float) + 3 * hidden_bytes(*f) +
+           std::max({plan_input(*f).part, plan_weights(*f).part, plan_output(*f).part});
+}
+
+extern "C" int tm_feed_forward_backward(const tm_feed_forward *f, const void *saved,
+                                        const void *dout, int64_t do_l, void *dx, void *dgate,
+                                        void *dup, void *ddown, void *workspace,
+                                        size_t workspace_bytes, hipStream_t stream) {
+    if (const int rc = check(f))
+        return rc;
+    const int64_t unit = 16 / size_of(*f);
+    if (!dgate != !dup || (uintptr_t)dout % 16 || do_l % unit || do_l < 0 ||
+        (do_l && do_l < f->O))
+        return TM_ERR_INVALID_ARGUMENT;
+    if (do_l >= TM_FF_MAX_ROW_BYTES / size_of(*f))
+        return TM_ERR_UNSUPPORTED_SHAPE;
+    if (!dgate && !ddown && (!dx || !f->T))
+        return TM_OK;
+    if (!workspace || (uintptr_t)workspace % 16 ||
+        workspace_bytes < tm_feed_forward_backward_workspace_bytes(f))
+        return TM_ERR_WORKSPACE;
+    float *most = (float *)workspace;
+    char *h = (char *)workspace + ff::kMostParts * sizeof(float);
+    char *da = h + hidden_bytes(*f), *db = da + hidden_bytes(*f), *part = db + hidden_bytes(*f);
+    Args p;
+    const bool scaled = f->dtype == TM_F16 && f->T;
+    if (f->T) {
+        if (!f->x || !f->gate || !f->up || !f->down || !saved || (uintptr_t)saved % 16 || !dout)
+            return TM_ERR_INVALID_ARGUMENT;
+        if (scaled) {
+            ff_most<<<dim3(ff::kMostParts), 256, 0, stream>>>((const _Float16 *)dout, do_l, f->T,
+                                                             f->O, most);
+            if (hipGetLastError() != hipSuccess)
+                return TM_ERR_LAUNCH;
+        }
+        p = args(f->T, f->F, f->O);
+        p.a[0] = dout, p.a_l = do_l;
+        p.b[0] = f->down, p.b_l = f->down_l;
+        p.out[0] = h, p.da = da, p.db = db, p.out_l = hidden_row(*f);
+        p.most = scaled ? most : nullptr;
+        set_saved(*f, p, saved);
+        if (const int rc = product(*f, p, ff::kHidden, plan_hidden(*f), nullptr, stream))
+            return rc;
+        if (dx) {
+            p = args(f->T, f->C, f->F);
+            p.segments = 2;
+            p.a[0] = da, p.a[1] = db, p.a_l = hidden_row(*f);
+            p.b[0] = f->gate, p.b[1] = f->up, p.b_l = f->w_l;
+            p.out[0] = dx, p.out_l = f->C, p.wide = wide(*f, dx, f->C);
+            p.most = scaled ? most : nullptr;
+            if (const int rc = product(*f, p, ff::kInput, plan_input(*f), part, stream))
+                return rc;
+        }
+    }
+    if (dgate) { // without rows: zeros, here and below
+        p = args(f->F, f->C, f->T);
+        p.batches = 2;
+        p.a[0] = da, p.a[1] = db, p.a_l = hidden_row(*f);
+        p.b[0] = p.b[1] = f->x, p.b_l = f->x_l;
+        p.out[0] = dgate, p.out[1] = dup, p.out_l = f->C;
+        p.wide = wide(*f, dgate, f->C) && wide(*f, dup, f->C);
+        p.most = scaled ? most : nullptr;
+        if (const int rc = product(*f, p, ff::kWeights, plan_weights(*f), part, stream))
+            return rc;
+    }
+    if (ddown) {
+        p = args(f->O, f->F, f->T);
+        p.a[0] = dout, p.a_l = do_l;
+        p.b[0] = h, p.b_l = hidden_row(*f);
+        p.out[0] = ddown, p.out_l = f->F, p.wide = wide(*f, ddown, f->F);
+        if (const int rc = product(*f, p, ff::kWeights, plan_output(*f), part, stream))
+            return rc;
+    }
+    return TM_OK;
+}

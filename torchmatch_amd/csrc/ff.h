@@ -1,0 +1,43 @@
+// ff.h -- the arguments of the feed-forward kernels and what their files call of each other.
+#ifndef TORCHMATCH_AMD_FF_H
+#define TORCHMATCH_AMD_FF_H
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace ff {
+
+// One product, or two of one shape:  out[m][n] = sum over k of a[m][k] b[n][k].
+// An operand's rows hold consecutive k, or (strided) consecutive m or n, a row for each k.
+struct Args {
+    const void *a[2], *b[2]; // a second one: of the next `k`s (segments), of the next product
+                             // (batches), or b of the up projection (gated)
+    void *out[2];            // rows of out_l, T; gated: h; hidden: h
+    int64_t a_l, b_l, out_l; // elements from row to row
+    // what the gated product saves and the hidden one reads, each (m, hidden) with rows of
+    // out_l: a and b, or the upper halves of their float32 bits and a third of the next
+    // eight bits of each
+    void *saved[3];
+    void *da, *db;      // hidden: gradients of a and b, rows of out_l
+    const float *most;  // kMostParts maxima of |dy|, or null: no scale
+    float *part;        // (splits, batches, M, N) sums, or null
+    int32_t M, N, K;    // K: of one segment
+    int32_t segments, batches, splits, split_steps;
+    int32_t activation, wide; // wide: out rows are at multiples of 16 bytes
+};
+
+constexpr int kMostParts = 256;
+enum Kind { kUp, kDown, kHidden, kInput, kWeights, kKinds };
+
+// Non-zero: a launch failed.  big: tiles of 256 x 256, else of 128 x 128.
+#define FF_DECLARE(type)                                                                         \
+    int product_##type(const Args &, Kind, bool big, hipStream_t);                               \
+    int join_##type(const Args &, hipStream_t);
+FF_DECLARE(bf16)
+FF_DECLARE(f16)
+FF_DECLARE(f32)
+#undef FF_DECLARE
+
+} // namespace ff
+
+#endif

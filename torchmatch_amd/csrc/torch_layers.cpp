@@ -1,5 +1,5 @@
 // torch_layers.cpp -- the `attention` ops of the layer around attention over the C ABI: normed
-// rotation, dropout.  Argument checks, layout, workspace, autograd.
+// rotation, the gated feed-forward block, dropout.  Argument checks, layout, workspace, autograd.
 #include "torch_support.h"
 
 namespace {
@@ -174,6 +174,200 @@ Tensor norm_rotate_autograd(const Tensor &x, const OptTensor &weight, const Tens
     return op.call(x, weight, positions, freqs, sections, heads, eps, interleaved);
 }
 
+// ---- feed_forward -----------------------------------------------------------------
+
+int activation_code(c10::string_view name) {
+    static const char *const names[] = {"silu", "gelu", "gelu_tanh", "relu"}; // TM_SILU ..
+    for (int i = 0; i < 4; ++i)
+        if (name == names[i])
+            return i;
+    TORCH_CHECK_VALUE(false, "feed_forward: activation must be silu, gelu, gelu_tanh or relu, got ",
+                      name);
+}
+
+// (rows, n) as the kernels read it: features contiguous and padded with zeros to 16 bytes, rows at
+// multiples of 16 bytes.  Views that are, are read in place; others are copied.
+Tensor rows_of(const Tensor &t) {
+    const int64_t n = t.size(-1), unit = 16 / t.element_size();
+    const Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / n, n});
+    if (n % unit)
+        return at::constant_pad_nd(r, {0, unit - n % unit}).contiguous();
+    const int64_t l = step_of(r, 0);
+    const bool ok = (n == 1 || r.stride(1) == 1) && l % unit == 0 && (l == 0 || l >= n) &&
+                    l * r.element_size() < TM_FF_MAX_ROW_BYTES &&
+                    reinterpret_cast<uintptr_t>(r.const_data_ptr()) % 16 == 0;
+    return ok ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+
+// The arguments, checked, as the library takes them.
+struct Block {
+    tm_feed_forward f = {};
+    Tensor x, gate, up, down; // as read
+    std::vector<int64_t> out; // the output's shape
+    Block(const Tensor &x_, const Tensor &gate_, const Tensor &up_, const Tensor &down_,
+          c10::string_view activation) {
+        TORCH_CHECK_VALUE(x_.dim() >= 1 && gate_.dim() == 2 && up_.dim() == 2 && down_.dim() == 2,
+                          "feed_forward: x must be (..., C), gate and up (F, C) and down (O, F), got ",
+                          x_.sizes(), ", ", gate_.sizes(), ", ", up_.sizes(), " and ",
+                          down_.sizes());
+        f.dtype = dtype_code(x_, "feed_forward", "x");
+        for (const Tensor *w : {&gate_, &up_, &down_}) {
+            TORCH_CHECK_VALUE(w->device() == x_.device(),
+                              "feed_forward: x and the weights must be on one device");
+            TORCH_CHECK_TYPE(w->scalar_type() == x_.scalar_type(),
+                             "feed_forward: x and the weights must have one dtype, got ",
+                             x_.scalar_type(), " and ", w->scalar_type());
+        }
+        f.activation = activation_code(activation);
+        const int64_t C = x_.size(-1), F = gate_.size(0), O = down_.size(0);
+        TORCH_CHECK_VALUE(C >= 1 && F >= 1 && O >= 1, "feed_forward: sizes must be positive, got x ",
+                          x_.sizes(), ", gate ", gate_.sizes(), ", down ", down_.sizes());
+        TORCH_CHECK_VALUE(gate_.size(1) == C && up_.sizes() == gate_.sizes(),
+                          "feed_forward: gate and up must be (F, ", C, ") as x is, got ",
+                          gate_.sizes(), " and ", up_.sizes());
+        TORCH_CHECK_VALUE(down_.size(1) == F, "feed_forward: down must be (O, ", F,
+                          ") as gate is, got ", down_.sizes());
+        const int64_t T = x_.numel() / C;
+        const int64_t most = TM_FF_MAX_ROW_BYTES / x_.element_size() - 16;
+        const auto blocks = [](int64_t m, int64_t n) {
+            return ((double)m + 127.) / 128. * (((double)n + 63.) / 64.);
+        };
+        TORCH_CHECK_VALUE(T <= INT32_MAX - 256 && C < most && F < most && O < most &&
+                              std::max({blocks(T, F), blocks(T, O), blocks(T, C),
+                                        2. * blocks(F, C), blocks(O, F)}) <=
+                                  TM_FF_MAX_BLOCKS,
+                          "feed_forward: too many rows for one call: x ", x_.sizes(), ", gate ",
+                          gate_.sizes(), ", down ", down_.sizes());
+        out = x_.sizes().vec();
+        out.back() = O;
+        f.T = (int32_t)T, f.C = (int32_t)C, f.F = (int32_t)F, f.O = (int32_t)O;
+        x = rows_of(x_), gate = rows_of(gate_), up = rows_of(up_), down = rows_of(down_);
+        if (step_of(gate, 0) != step_of(up, 0)) // the kernels take one stride for both
+            gate = gate.contiguous(), up = up.contiguous();
+        f.x = x.const_data_ptr(), f.gate = gate.const_data_ptr();
+        f.up = up.const_data_ptr(), f.down = down.const_data_ptr();
+        f.x_l = step_of(x, 0), f.w_l = step_of(gate, 0), f.down_l = step_of(down, 0);
+    }
+};
+
+std::tuple<Tensor, Tensor> feed(const Tensor &x, const Tensor &gate, const Tensor &up,
+                                const Tensor &down, c10::string_view activation, bool save) {
+    const c10::DeviceGuard guard(x.device());
+    const Block p(x, gate, up, down, activation);
+    const auto bytes = x.options().dtype(at::kByte);
+    Tensor out = at::empty(p.out, x.options());
+    Tensor saved = at::empty({save ? (int64_t)tm_feed_forward_saved_bytes(&p.f) : 0}, bytes);
+    if (p.f.T) {
+        const Tensor ws = at::empty({(int64_t)tm_feed_forward_workspace_bytes(&p.f)}, bytes);
+        check_rc(tm_feed_forward_forward(&p.f, out.data_ptr(), save ? saved.data_ptr() : nullptr,
+                                         ws.data_ptr(), (size_t)ws.numel(), current_stream(x)),
+                 "feed_forward");
+    }
+    return {out, saved};
+}
+
+Tensor feed_forward_hip(const Tensor &x, const Tensor &gate, const Tensor &up, const Tensor &down,
+                        c10::string_view activation) {
+    return std::get<0>(feed(x, gate, up, down, activation, false));
+}
+
+std::tuple<Tensor, Tensor> feed_forward_save_hip(const Tensor &x, const Tensor &gate,
+                                                 const Tensor &up, const Tensor &down,
+                                                 c10::string_view activation) {
+    return feed(x, gate, up, down, activation, true);
+}
+
+// what is not asked for is empty
+std::tuple<Tensor, Tensor, Tensor, Tensor>
+feed_forward_backward_hip(const Tensor &dout, const Tensor &x, const Tensor &gate,
+                          const Tensor &up, const Tensor &down, const Tensor &saved,
+                          c10::string_view activation, bool need_x, bool need_gate, bool need_up,
+                          bool need_down) {
+    const c10::DeviceGuard guard(x.device());
+    const Block p(x, gate, up, down, activation);
+    TORCH_CHECK_VALUE(dout.sizes() == at::IntArrayRef(p.out) && dout.device() == x.device(),
+                      "feed_forward_backward: dout must be as the output ",
+                      at::IntArrayRef(p.out), ", got ", dout.sizes());
+    TORCH_CHECK_TYPE(dout.scalar_type() == x.scalar_type(),
+                     "feed_forward_backward: dout must have x's dtype");
+    TORCH_CHECK_VALUE(saved.device() == x.device() && saved.scalar_type() == at::kByte &&
+                          saved.is_contiguous() &&
+                          saved.numel() == (int64_t)tm_feed_forward_saved_bytes(&p.f),
+                      "feed_forward_backward: saved must be what the forward pass saved");
+    const bool pair = need_gate || need_up;
+    const auto made = [&](bool need, const Tensor &t) {
+        return at::empty(need ? t.sizes() : at::IntArrayRef{0}, x.options());
+    };
+    Tensor dx = made(need_x, x), dgate = made(pair, gate), dup = made(pair, up),
+           ddown = made(need_down, down);
+    const auto place = [](bool need, Tensor &t) { return need ? t.data_ptr() : nullptr; };
+    const Tensor g = rows_of(dout);
+    const Tensor ws = at::empty({(int64_t)tm_feed_forward_backward_workspace_bytes(&p.f)},
+                                x.options().dtype(at::kByte));
+    check_rc(tm_feed_forward_backward(&p.f, saved.const_data_ptr(), g.const_data_ptr(),
+                                      step_of(g, 0), place(need_x && p.f.T, dx),
+                                      place(pair, dgate), place(pair, dup),
+                                      place(need_down, ddown), ws.data_ptr(), (size_t)ws.numel(),
+                                      current_stream(x)),
+             "feed_forward_backward");
+    return {dx, need_gate ? dgate : made(false, gate), need_up ? dup : made(false, up), ddown};
+}
+
+struct FeedForwardFunction : torch::autograd::Function<FeedForwardFunction> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &gate,
+                          const Tensor &up, const Tensor &down, std::string activation) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        static auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("attention::feed_forward_save", "")
+                             .typed<std::tuple<Tensor, Tensor>(
+                                 const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                                 c10::string_view)>();
+        auto [out, saved] = op.call(x, gate, up, down, activation);
+        ctx->save_for_backward({x, gate, up, down, saved});
+        ctx->saved_data["activation"] = activation;
+        return out;
+    }
+    static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
+        variable_list result(5);
+        if (!grads[0].defined())
+            return result;
+        const auto s = ctx->get_saved_variables();
+        bool need[4];
+        for (int i = 0; i < 4; ++i)
+            need[i] = ctx->needs_input_grad(i);
+        static auto op =
+            c10::Dispatcher::singleton()
+                .findSchemaOrThrow("attention::feed_forward_backward", "")
+                .typed<std::tuple<Tensor, Tensor, Tensor, Tensor>(
+                    const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                    const Tensor &, const Tensor &, c10::string_view, bool, bool, bool, bool)>();
+        auto [dx, dgate, dup, ddown] =
+            op.call(grads[0], s[0], s[1], s[2], s[3], s[4],
+                    ctx->saved_data["activation"].toStringRef(), need[0], need[1], need[2],
+                    need[3]);
+        const Tensor all[] = {dx, dgate, dup, ddown};
+        for (int i = 0; i < 4; ++i)
+            if (need[i])
+                result[i] = all[i];
+        return result;
+    }
+};
+
+Tensor feed_forward_autograd(const Tensor &x, const Tensor &gate, const Tensor &up,
+                             const Tensor &down, c10::string_view activation) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(x) && !has_tangent(gate) && !has_tangent(up) &&
+                                    !has_tangent(down),
+                                "feed_forward: no forward-mode derivative");
+    if (wants_grad(x) || wants_grad(gate) || wants_grad(up) || wants_grad(down))
+        return FeedForwardFunction::apply(x, gate, up, down, std::string(activation));
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("attention::feed_forward", "")
+                         .typed<Tensor(const Tensor &, const Tensor &, const Tensor &,
+                                       const Tensor &, c10::string_view)>();
+    return op.call(x, gate, up, down, activation);
+}
+
 // ---- dropout ----------------------------------------------------------------------
 
 Tensor dropout_hip(const Tensor &x, double p, int64_t seed, int64_t offset,
@@ -276,6 +470,13 @@ TORCH_LIBRARY_FRAGMENT(attention, m) {
     m.def("norm_rotate_backward(Tensor dout, Tensor x, Tensor? weight, Tensor positions, "
           "Tensor freqs, int[] sections, int[] heads, float eps, bool interleaved=False, "
           "bool need_x=True, bool need_weight=True) -> (Tensor, Tensor)");
+    m.def("feed_forward(Tensor x, Tensor gate, Tensor up, Tensor down, str activation) -> Tensor");
+    // the same with what feed_forward_backward needs of the hidden features
+    m.def("feed_forward_save(Tensor x, Tensor gate, Tensor up, Tensor down, str activation) -> "
+          "(Tensor, Tensor)");
+    m.def("feed_forward_backward(Tensor dout, Tensor x, Tensor gate, Tensor up, Tensor down, "
+          "Tensor saved, str activation, bool need_x=True, bool need_gate=True, "
+          "bool need_up=True, bool need_down=True) -> (Tensor, Tensor, Tensor, Tensor)");
     // the seed lies in seed_at where it is given
     m.def("dropout(Tensor x, float p, int seed=0, int offset=0, Tensor? seed_at=None, "
           "Tensor? residual=None) -> Tensor");
@@ -284,11 +485,17 @@ TORCH_LIBRARY_FRAGMENT(attention, m) {
 TORCH_LIBRARY_IMPL(attention, CUDA, m) {
     m.impl("norm_rotate", &norm_rotate_hip);
     m.impl("norm_rotate_backward", &norm_rotate_backward_hip);
+    m.impl("feed_forward", &feed_forward_hip);
+    m.impl("feed_forward_save", &feed_forward_save_hip);
+    m.impl("feed_forward_backward", &feed_forward_backward_hip);
     m.impl("dropout", &dropout_hip);
 }
 
 TORCH_LIBRARY_IMPL(attention, Autograd, m) {
     m.impl("norm_rotate", &norm_rotate_autograd);
     m.impl("norm_rotate_backward", torch::autograd::autogradNotImplementedFallback());
+    m.impl("feed_forward", &feed_forward_autograd);
+    m.impl("feed_forward_save", torch::autograd::autogradNotImplementedFallback());
+    m.impl("feed_forward_backward", torch::autograd::autogradNotImplementedFallback());
     m.impl("dropout", &dropout_autograd);
 }
