@@ -119,7 +119,7 @@ def test_feed_forward_refusals(changes, code):
 def test_feed_forward_backward_refusals():
     lib = _native.lib()
     size = lib.tm_feed_forward_backward_workspace_bytes(ctypes.byref(_block()))
-    assert size >= 3 * 10 * 96 * 2
+    assert size >= 2 * 10 * 96 * 2
 
     def back(saved=4096, dout=4096, do_l=32, dx=4096, dgate=4096, dup=4096, ddown=4096, ws=4096,
              bytes_=size, **changes):
@@ -143,8 +143,8 @@ def test_feed_forward_backward_refusals():
 def test_feed_forward_sizes():
     lib = _native.lib()
     saved = lambda **c: lib.tm_feed_forward_saved_bytes(ctypes.byref(_block(**c)))  # noqa: E731
-    assert saved() == 10 * 96 * 6 and saved(dtype=_native.TM_F32) == 10 * 96 * 8
-    assert saved(F=90, down_l=96) == 10 * 96 * 6
+    assert saved() == 10 * 96 * 8 and saved(dtype=_native.TM_F32) == 10 * 96 * 12
+    assert saved(F=90, down_l=96) == 10 * 96 * 8
     assert saved(T=0) == 0
     size = lib.tm_feed_forward_workspace_bytes(ctypes.byref(_block()))
     assert size >= 10 * 96 * 2
@@ -192,7 +192,7 @@ def test_fake_kernels():
         y = torch.ops.attention.feed_forward(x, w, w, d, "silu")
         assert y.shape == (2, 7, 4, 5) and y.dtype == x.dtype
         _, saved = torch.ops.attention.feed_forward_save(x, w, w, d, "silu")
-        assert saved.shape == (56 * 24 * 6,) and saved.dtype == torch.uint8
+        assert saved.shape == (56 * 24 * 8,) and saved.dtype == torch.uint8
         grads = torch.ops.attention.feed_forward_backward(y, x, w, w, d, saved, "silu",
                                                           need_up=False)
         assert [g.shape for g in grads] == [x.shape, w.shape, (0,), d.shape]

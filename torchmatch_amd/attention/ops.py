@@ -79,7 +79,7 @@ def _feed_forward_fake(x, gate, up, down, activation):
 @torch.library.register_fake("attention::feed_forward_save")
 def _feed_forward_save_fake(x, gate, up, down, activation):
     rows, hidden = x.numel() // x.shape[-1], (gate.shape[0] + 7) // 8 * 8
-    size = 8 if x.dtype == torch.float32 else 6  # bytes for each hidden feature
+    size = 12 if x.dtype == torch.float32 else 8  # bytes for each hidden feature
     return (_feed_forward_fake(x, gate, up, down, activation),
             x.new_empty(rows * hidden * size, dtype=torch.uint8))
 

@@ -2,10 +2,11 @@
 // are in ff_tile.h.
 //
 //     a = x G^T, b = x U^T, h = act(a) b, y = h D^T
-//     dh = dy D; da = dh b act'(a), db = dh act(a); dx = da G + db U; dG = da^T x, dU = db^T x, dD = dy^T h
+//     dh = dy D; da = dh b act'(a), db = dh act(a);
+//     dx = da G + db U; dG = da^T x, dU = db^T x, dD = dy^T h
 //
 // Forward two launches: both projections with the activation and the product in the first's
-// epilogue, then D.  Backward: dh, in whose epilogue da, db and h again; dx; dG and dU together;
+// epilogue, then D.  Backward: dh, in whose epilogue da and db; dx; dG and dU together;
 // dD.  h, da and db are rounded to the inputs' type once, as operands of the next product have to be.  a and b
 // are not rounded to it: they are saved with 16 bits after the leading one (ff_tile.h), since each
 // enters two gradients that are rounded again (with a and b in bfloat16 those are off by 1.75
@@ -31,12 +32,15 @@ int64_t hidden_bytes(const tm_feed_forward &f) { // (T, hidden) of the inputs' t
 
 // Tiles of a product and how often its k is split.
 struct Plan {
-    bool big;
+    int size;
+    bool tokens;
     int splits, split_steps;
     size_t part; // bytes of partial sums
 };
 Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, int segments,
           int batches) {
+    if (M <= ff::kTokens && (kind == ff::kUp || kind == ff::kDown))
+        return {ff::kSmall, true, 1, 0, 0};
     const int64_t step = 128 / size_of(f);
     const auto tiles = [&](int64_t t) {
         return (M + t - 1) / t * ((N + t - 1) / t) * batches * (kind == ff::kUp ? 2 : 1);
@@ -46,10 +50,10 @@ Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, 
     const int64_t large = tiles(256), small = tiles(128);
     const double t_large = (double)((large + 255) / 256) * 4.;
     const double t_small = (double)((small + 511) / 512) * 2. * 7. / 6.;
-    Plan r = {t_large <= t_small, 1, 0, 0};
+    Plan r = {f.dtype != TM_F32 && t_large <= t_small ? ff::kLarge : ff::kSmall, false, 1, 0, 0};
     const int64_t steps = (K + step - 1) / step * segments;
     const bool may = kind == ff::kDown || kind == ff::kInput || kind == ff::kWeights;
-    if (may && !r.big && small < 384)
+    if (may && r.size == ff::kSmall && small < 384)
         r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(1, small),
                                                                steps / 8));
     r.split_steps = (int)((steps + r.splits - 1) / r.splits);
@@ -98,13 +102,19 @@ int product(const tm_feed_forward &f, Args p, Kind kind, const Plan &how, void *
     p.split_steps = how.split_steps;
     p.part = how.part ? (float *)part : nullptr;
     p.activation = f.activation;
+    if (how.tokens) {
+        const auto tokens = f.dtype == TM_BF16  ? ff::tokens_bf16
+                            : f.dtype == TM_F16 ? ff::tokens_f16
+                                                : ff::tokens_f32;
+        return tokens(p, kind, stream) ? TM_ERR_LAUNCH : TM_OK;
+    }
     const auto run = f.dtype == TM_BF16  ? ff::product_bf16
                      : f.dtype == TM_F16 ? ff::product_f16
                                          : ff::product_f32;
     const auto join = f.dtype == TM_BF16  ? ff::join_bf16
                       : f.dtype == TM_F16 ? ff::join_f16
                                           : ff::join_f32;
-    if (run(p, kind, how.big, stream) || (p.part && join(p, stream)))
+    if (run(p, kind, how.size, stream) || (p.part && join(p, stream)))
         return TM_ERR_LAUNCH;
     return TM_OK;
 }
@@ -121,10 +131,14 @@ int wide(const tm_feed_forward &f, const void *out, int64_t l) {
     return !((uintptr_t)out % 16) && l % (16 / size_of(f)) == 0;
 }
 
+// What is saved: (T, hidden) planes of the type's size, for a and b and then h.
+int planes(const tm_feed_forward &f) { return f.dtype == TM_F32 ? 2 : 3; }
+void *plane(const tm_feed_forward &f, const void *saved, int n) {
+    return (char *)const_cast<void *>(saved) + n * ((int64_t)f.T * hidden_row(f) * size_of(f));
+}
 void set_saved(const tm_feed_forward &f, Args &p, const void *saved) {
-    const int64_t plane = (int64_t)f.T * hidden_row(f) * size_of(f);
-    for (int n = 0; n < (f.dtype == TM_F32 ? 2 : 3); ++n)
-        p.saved[n] = (char *)const_cast<void *>(saved) + n * plane;
+    for (int n = 0; n < planes(f); ++n)
+        p.saved[n] = plane(f, saved, n);
 }
 
 // The largest |x| of what each block takes of (rows, n), half precision.
@@ -156,7 +170,7 @@ __global__ __launch_bounds__(256) void ff_most(const _Float16 *x, int64_t l, int
 extern "C" size_t tm_feed_forward_saved_bytes(const tm_feed_forward *f) {
     if (check(f))
         return 0;
-    return (size_t)(f->dtype == TM_F32 ? 2 : 3) * f->T * hidden_row(*f) * size_of(*f);
+    return (size_t)(planes(*f) + 1) * f->T * hidden_row(*f) * size_of(*f);
 }
 
 extern "C" size_t tm_feed_forward_workspace_bytes(const tm_feed_forward *f) {
@@ -180,13 +194,14 @@ extern "C" int tm_feed_forward_forward(const tm_feed_forward *f, void *out, void
     Args p = args(f->T, f->F, f->C);
     p.a[0] = f->x, p.a_l = f->x_l;
     p.b[0] = f->gate, p.b[1] = f->up, p.b_l = f->w_l;
-    p.out[0] = workspace, p.out_l = hidden_row(*f);
+    void *h = saved ? plane(*f, saved, planes(*f)) : workspace;
+    p.out[0] = h, p.out_l = hidden_row(*f);
     if (saved)
         set_saved(*f, p, saved);
     if (const int rc = product(*f, p, ff::kUp, plan_up(*f), nullptr, stream))
         return rc;
     p = args(f->T, f->O, f->F);
-    p.a[0] = workspace, p.a_l = hidden_row(*f);
+    p.a[0] = h, p.a_l = hidden_row(*f);
     p.b[0] = f->down, p.b_l = f->down_l;
     p.out[0] = out, p.out_l = f->O, p.wide = wide(*f, out, f->O);
     return product(*f, p, ff::kDown, plan_down(*f), (char *)workspace + hidden_bytes(*f), stream);
@@ -195,7 +210,7 @@ extern "C" int tm_feed_forward_forward(const tm_feed_forward *f, void *out, void
 extern "C" size_t tm_feed_forward_backward_workspace_bytes(const tm_feed_forward *f) {
     if (check(f))
         return 0;
-    return ff::kMostParts * sizeof(float) + 3 * hidden_bytes(*f) +
+    return ff::kMostParts * sizeof(float) + 2 * hidden_bytes(*f) +
            std::max({plan_input(*f).part, plan_weights(*f).part, plan_output(*f).part});
 }
 
@@ -217,8 +232,8 @@ extern "C" int tm_feed_forward_backward(const tm_feed_forward *f, const void *sa
         workspace_bytes < tm_feed_forward_backward_workspace_bytes(f))
         return TM_ERR_WORKSPACE;
     float *most = (float *)workspace;
-    char *h = (char *)workspace + ff::kMostParts * sizeof(float);
-    char *da = h + hidden_bytes(*f), *db = da + hidden_bytes(*f), *part = db + hidden_bytes(*f);
+    char *da = (char *)workspace + ff::kMostParts * sizeof(float);
+    char *db = da + hidden_bytes(*f), *part = db + hidden_bytes(*f);
     Args p;
     const bool scaled = f->dtype == TM_F16 && f->T;
     if (f->T) {
@@ -233,7 +248,7 @@ extern "C" int tm_feed_forward_backward(const tm_feed_forward *f, const void *sa
         p = args(f->T, f->F, f->O);
         p.a[0] = dout, p.a_l = do_l;
         p.b[0] = f->down, p.b_l = f->down_l;
-        p.out[0] = h, p.da = da, p.db = db, p.out_l = hidden_row(*f);
+        p.da = da, p.db = db, p.out_l = hidden_row(*f);
         p.most = scaled ? most : nullptr;
         set_saved(*f, p, saved);
         if (const int rc = product(*f, p, ff::kHidden, plan_hidden(*f), nullptr, stream))
@@ -263,7 +278,7 @@ extern "C" int tm_feed_forward_backward(const tm_feed_forward *f, const void *sa
     if (ddown) {
         p = args(f->O, f->F, f->T);
         p.a[0] = dout, p.a_l = do_l;
-        p.b[0] = h, p.b_l = hidden_row(*f);
+        p.b[0] = f->T ? plane(*f, saved, planes(*f)) : nullptr, p.b_l = hidden_row(*f);
         p.out[0] = ddown, p.out_l = f->F, p.wide = wide(*f, ddown, f->F);
         if (const int rc = product(*f, p, ff::kWeights, plan_output(*f), part, stream))
             return rc;

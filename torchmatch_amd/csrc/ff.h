@@ -12,7 +12,7 @@ namespace ff {
 struct Args {
     const void *a[2], *b[2]; // a second one: of the next `k`s (segments), of the next product
                              // (batches), or b of the up projection (gated)
-    void *out[2];            // rows of out_l, T; gated: h; hidden: h
+    void *out[2];            // rows of out_l, T; gated: h; hidden: not used
     int64_t a_l, b_l, out_l; // elements from row to row
     // what the gated product saves and the hidden one reads, each (m, hidden) with rows of
     // out_l: a and b, or the upper halves of their float32 bits and a third of the next
@@ -27,11 +27,16 @@ struct Args {
 };
 
 constexpr int kMostParts = 256;
-enum Kind { kUp, kDown, kHidden, kInput, kWeights, kKinds };
+enum Kind { kUp, kDown, kHidden, kInput, kWeights };
+enum { kSmall, kLarge }; // tiles: 128 x 128, 256 x 256
 
-// Non-zero: a launch failed.  big: tiles of 256 x 256, else of 128 x 128.
+// Products of up to this many rows take product_tokens.
+constexpr int kTokens = 32;
+
+// Non-zero: a launch failed.
 #define FF_DECLARE(type)                                                                         \
-    int product_##type(const Args &, Kind, bool big, hipStream_t);                               \
+    int product_##type(const Args &, Kind, int size, hipStream_t);                               \
+    int tokens_##type(const Args &, Kind, hipStream_t);                                          \
     int join_##type(const Args &, hipStream_t);
 FF_DECLARE(bf16)
 FF_DECLARE(f16)

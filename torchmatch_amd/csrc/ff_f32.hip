@@ -1,10 +1,13 @@
 // ff_f32.hip -- the feed-forward products of one type.
-#include "ff_tile.h"
+#include "ff_tokens.h"
 
 namespace ff {
 
-int product_f32(const Args &p, Kind kind, bool big, hipStream_t stream) {
-    return run<float>(p, kind, big, stream);
+int product_f32(const Args &p, Kind kind, int size, hipStream_t stream) {
+    return run<float>(p, kind, size, stream);
+}
+int tokens_f32(const Args &p, Kind kind, hipStream_t stream) {
+    return run_tokens<float>(p, kind, stream);
 }
 int join_f32(const Args &p, hipStream_t stream) { return run_join<float>(p, stream); }
 

@@ -2,10 +2,10 @@
 // their results before they are written.
 //
 //     h = act(x G^T) * (x U^T),  y = h D^T                               (rows by rows)
-//     dh = dy D -> da, db, h;  dx = da G + db U                            (rows by columns)
+//     dh = dy D -> da, db;  dx = da G + db U                               (rows by columns)
 //     dG = da^T x, dU = db^T x, dD = dy^T h                                (columns by columns)
 //
-// A block has BM x BN of the result, a wave 64 columns of it.  Tiles of 128 bytes of k go from memory
+// A block has BM x BN of the result.  Tiles of 128 bytes of k go from memory
 // straight into LDS, two buffers, one barrier a tile.  Operands whose rows hold k are read by rows, others
 // by transposed reads (attn_tile.h has the tiles' layout), so nothing is transposed in memory.  The
 // result's columns lie along a lane's registers; a wave turns them through LDS, 32 rows at a
@@ -27,8 +27,6 @@ using attn::mma32;
 using attn::u32x4;
 using attn::x8;
 
-typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-
 // ---- activations ------------------------------------------------------------------
 
 // The activation's value and slope.  16-bit types take the hardware's exponential and reciprocal
@@ -39,45 +37,60 @@ template <typename T> __device__ inline float exp_of(float x) {
 template <typename T> __device__ inline float over(float x) { // 1 / x
     return sizeof(T) == 2 ? __builtin_amdgcn_rcpf(x) : 1.f / x;
 }
-template <typename T> __device__ inline float2 activate(float a, int kind) {
-    switch (kind) {
-    case TM_SILU: {
-        const float s = over<T>(1.f + exp_of<T>(-a));
-        return make_float2(a * s, s * (1.f + a * (1.f - s)));
-    }
-    case TM_RELU: return make_float2(fmaxf(a, 0.f), a > 0.f ? 1.f : 0.f);
-    case TM_GELU: {
+template <typename T, int KIND> __device__ inline float2 activate(float a) {
+    if constexpr (KIND == TM_SILU) {
+        const float s = over<T>(1.f + exp_of<T>(-a)), v = a * s;
+        return make_float2(v, fmaf(v, 1.f - s, s));
+    } else if constexpr (KIND == TM_RELU) {
+        return make_float2(fmaxf(a, 0.f), a > 0.f ? 1.f : 0.f);
+    } else if constexpr (KIND == TM_GELU) {
         const float cdf = 0.5f * erfcf(-0.70710678118654752440f * a);
         return make_float2(a * cdf, cdf + a * 0.39894228040143267794f * exp_of<T>(-0.5f * a * a));
-    }
-    default: { // the approximation by tanh
+    } else { // the approximation by tanh
         const float k = 0.79788456080286535588f;
         const float t = tanhf(k * (a + 0.044715f * a * a * a));
         const float half = 0.5f * (1.f + t);
         return make_float2(a * half, half + 0.5f * a * (1.f - t * t) * k *
                                                 (1.f + 3.f * 0.044715f * a * a));
     }
-    }
+}
+// f(j, the activation) for j < V, the choice outside the loop
+template <typename T, int V, typename F>
+__device__ inline void activate_all(int kind, F f) {
+    const auto all = [&](auto act) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            f(j, act);
+    };
+    if (kind == TM_SILU)
+        all([](float a) { return activate<T, TM_SILU>(a); });
+    else if (kind == TM_RELU)
+        all([](float a) { return activate<T, TM_RELU>(a); });
+    else if (kind == TM_GELU)
+        all([](float a) { return activate<T, TM_GELU>(a); });
+    else
+        all([](float a) { return activate<T, TM_GELU_TANH>(a); });
 }
 
 // ---- tiles ------------------------------------------------------------------------
 
-template <typename T> constexpr int kStep = 128 / (int)sizeof(T); // k a tile
+template <typename T> constexpr int kStep = 128 / (int)sizeof(T); // k a tile: whole lines of memory
 
-// One operand's tile, ROWS x kStep, brought by NT threads.  STRIDED: a row for each k.
-template <typename T, int ROWS, bool STRIDED, int NT> struct Feed {
+// One operand's tile, ROWS x kStep, brought by NT threads.  STRIDED: a row for each k.  HALF: HALF rows of one
+// matrix, HALF of another, in turn (0: one matrix).
+template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
     static constexpr int BK = kStep<T>, E = 16 / (int)sizeof(T);
     using L = attn::Tile<T, STRIDED ? ROWS : BK>;
     static constexpr int SIZE = (STRIDED ? BK : ROWS) * L::U; // units
     static constexpr int N = SIZE / NT, STEP = NT / L::U;
     static_assert(SIZE % NT == 0 && NT % L::U == 0 && L::U == L::U0);
 
+    static constexpr int READS = sizeof(T) == 4 ? (STRIDED ? 8 : 2) : STRIDED ? 2 : 1; // an operand's
+
     uint32_t off[N]; // bytes from the tile's first element, its k aside
     int unit[N];     // not strided: the unit of k
 
-    // left: rows (columns) from the tile's first on; GATED: 32 rows of the one matrix, 32 of the
-    // other, in turn
-    template <bool GATED>
+    // left: rows (columns) from the tile's first on
     __device__ inline void start(int tid, int64_t stride, int left) {
         const int row = tid / L::U, pos = tid % L::U;
         const uint32_t bytes = (uint32_t)stride * (uint32_t)sizeof(T);
@@ -88,34 +101,34 @@ template <typename T, int ROWS, bool STRIDED, int NT> struct Feed {
             if constexpr (STRIDED) {
                 off[n] = (uint32_t)r * bytes + 16u * min(u, (left - 1) / E);
             } else {
-                const int real = GATED ? (r >> 6) * 32 + (r & 31) : r;
+                const int real = HALF ? r / (2 * HALF + !HALF) * HALF + r % (HALF + !HALF) : r;
                 off[n] = (uint32_t)min(real, left - 1) * bytes + 16u * u;
             }
         }
     }
-    // which matrix of a gated pair load n is of: the same for a whole wave
-    __device__ static inline int of_pair(int tid, int n) {
-        return attn::scalar((tid / L::U + n * STEP) >> 5) & 1;
+    // whether load n is of the second matrix: the same for a whole wave
+    __device__ static inline bool of_second(int tid, int n) {
+        return HALF && attn::scalar((tid / L::U + n * STEP) / (HALF + !HALF)) & 1;
     }
-    // from: the tile's first element; second: of the other matrix (gated)
-    template <bool GATED>
-    __device__ inline void load(u32x4 *t, const char *from, const char *second, int tid) const {
+    // from: the tile's first element; second: of the other matrix; mask: 0 for its first 16 bytes
+    // over and over
+    __device__ inline void load(u32x4 *t, const char *from, const char *second, int tid,
+                                uint32_t mask) const {
         u32x4 *to = t + attn::scalar(tid & ~63);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const char *s = GATED && of_pair(tid, n) ? second : from;
+            const char *s = of_second(tid, n) ? second : from;
             __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void *)(s + off[n]),
+                (const __attribute__((address_space(1))) void *)(s + (off[n] & mask)),
                 (__attribute__((address_space(3))) void *)(to + n * NT), 16, 0, 0);
         }
     }
     // the last tile, of which `left` k are there: zeros past them
-    template <bool GATED>
     __device__ inline void load_last(u32x4 *t, const char *from, const char *second, int tid,
                                      int left) const {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const char *s = GATED && of_pair(tid, n) ? second : from;
+            const char *s = of_second(tid, n) ? second : from;
             const bool real = STRIDED ? tid / L::U + n * STEP < left : unit[n] * E < left;
             u32x4 x = {0u, 0u, 0u, 0u};
             if (real)
@@ -168,58 +181,71 @@ template <typename T, int ROWS, bool STRIDED, int NT> struct Feed {
 
 // ---- results ----------------------------------------------------------------------
 
-template <typename T> __device__ inline void put8(T *to, f32x8 x) {
-    typedef T U __attribute__((ext_vector_type(8)));
-    if constexpr (sizeof(T) == 2) {
+template <int V> using fv = float __attribute__((ext_vector_type(V)));
+
+// V floats as T, in units of up to 16 bytes
+template <typename T, int V> __device__ inline void put(T *to, fv<V> x) {
+    constexpr int N = sizeof(T) == 4 ? 4 : V;
+    typedef T U __attribute__((ext_vector_type(N)));
+#pragma unroll
+    for (int k = 0; k < V; k += N) {
         U y;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            y[j] = (T)x[j];
-        *(U *)to = y;
-    } else {
-        *(f32x4 *)to = (f32x4){x[0], x[1], x[2], x[3]};
-        *(f32x4 *)(to + 4) = (f32x4){x[4], x[5], x[6], x[7]};
+        for (int j = 0; j < N; ++j)
+            y[j] = (T)x[k + j];
+        *(U *)(to + k) = y;
     }
 }
 
 // a and b as they are saved: float32, or its first 24 bits (truncated: what a gradient then is off
-// by, 2^-15, is far below the rounding of the gradients to 16 bits)
-template <typename T> __device__ inline void save(const Args &p, int64_t at, f32x8 a, f32x8 b) {
+// by, 2^-15, is far below the rounding of the gradients to 16 bits), the upper 16 in a plane
+// each and the next eight of both in a third.
+__device__ inline uint32_t bytes(uint32_t hi, uint32_t lo, uint32_t which) {
+    return __builtin_amdgcn_perm(hi, lo, which); // bytes 0 - 3 of lo, 4 - 7 of hi, 12: zero
+}
+template <typename T, int V>
+__device__ inline void save(const Args &p, int64_t at, fv<V> a, fv<V> b) {
     if constexpr (sizeof(T) == 4) {
-        put8((float *)p.saved[0] + at, a);
-        put8((float *)p.saved[1] + at, b);
+        put<float, V>((float *)p.saved[0] + at, a);
+        put<float, V>((float *)p.saved[1] + at, b);
     } else {
-        u16x8 x, y, z;
+        typedef uint32_t U __attribute__((ext_vector_type(V / 2)));
+        U x, y, z;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t u = __float_as_uint(a[j]), v = __float_as_uint(b[j]);
-            x[j] = (uint16_t)(u >> 16);
-            y[j] = (uint16_t)(v >> 16);
-            z[j] = (uint16_t)((u & 0xff00u) | (v >> 8 & 0xffu));
+        for (int j = 0; j < V / 2; ++j) {
+            const uint32_t a0 = __float_as_uint(a[2 * j]), a1 = __float_as_uint(a[2 * j + 1]);
+            const uint32_t b0 = __float_as_uint(b[2 * j]), b1 = __float_as_uint(b[2 * j + 1]);
+            x[j] = bytes(a1, a0, 0x07060302);
+            y[j] = bytes(b1, b0, 0x07060302);
+            z[j] = bytes(bytes(a1, b1, 0x0c0c0501), bytes(a0, b0, 0x0c0c0501), 0x05040100);
         }
-        *(u16x8 *)((uint16_t *)p.saved[0] + at) = x;
-        *(u16x8 *)((uint16_t *)p.saved[1] + at) = y;
-        *(u16x8 *)((uint16_t *)p.saved[2] + at) = z;
+        *(U *)((uint16_t *)p.saved[0] + at) = x;
+        *(U *)((uint16_t *)p.saved[1] + at) = y;
+        *(U *)((uint16_t *)p.saved[2] + at) = z;
     }
 }
-template <typename T> __device__ inline void saved(const Args &p, int64_t at, f32x8 &a, f32x8 &b) {
-    if constexpr (sizeof(T) == 4) {
-        const f32x4 *u = (const f32x4 *)((const float *)p.saved[0] + at);
-        const f32x4 *v = (const f32x4 *)((const float *)p.saved[1] + at);
-        const f32x4 u0 = u[0], u1 = u[1], v0 = v[0], v1 = v[1];
-        a = (f32x8){u0[0], u0[1], u0[2], u0[3], u1[0], u1[1], u1[2], u1[3]};
-        b = (f32x8){v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-    } else {
-        const u16x8 x = *(const u16x8 *)((const uint16_t *)p.saved[0] + at);
-        const u16x8 y = *(const u16x8 *)((const uint16_t *)p.saved[1] + at);
-        const u16x8 z = *(const u16x8 *)((const uint16_t *)p.saved[2] + at);
+template <typename T> struct Saved { // 8 of them, as they lie in memory
+    u32x4 u[sizeof(T) == 4 ? 4 : 3];
+    __device__ inline void load(const Args &p, int64_t at) {
+#pragma unroll
+        for (int n = 0; n < (sizeof(T) == 4 ? 4 : 3); ++n)
+            u[n] = sizeof(T) == 4 ? ((const u32x4 *)((const float *)p.saved[n / 2] + at))[n % 2]
+                                  : *(const u32x4 *)((const uint16_t *)p.saved[n] + at);
+    }
+    __device__ inline void give(f32x8 &a, f32x8 &b) const {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            a[j] = __uint_as_float((uint32_t)x[j] << 16 | (z[j] & 0xff00u));
-            b[j] = __uint_as_float((uint32_t)y[j] << 16 | (uint32_t)(z[j] & 0xffu) << 8);
+            if constexpr (sizeof(T) == 4) {
+                a[j] = __uint_as_float(u[j / 4][j % 4]);
+                b[j] = __uint_as_float(u[2 + j / 4][j % 4]);
+            } else {
+                const uint32_t x = u[0][j / 2], y = u[1][j / 2], z = u[2][j / 2];
+                a[j] = __uint_as_float(bytes(x, z, j % 2 ? 0x0706030c : 0x0504010c));
+                b[j] = __uint_as_float(bytes(y, z, j % 2 ? 0x0706020c : 0x0504000c));
+            }
         }
     }
-}
+};
 
 // The power of two that brings the largest |dy| to 1 .. 2: half precision holds gradients of the
 // hidden features times this (they are as small as the loss makes them, and lose bits below 2^-14).
@@ -244,7 +270,7 @@ __device__ inline void put_row(const Args &p, int batch, int split, int64_t m, i
     if (p.part) {
         float *to = p.part + (((int64_t)split * p.batches + batch) * p.M + m) * p.N + n;
         if (p.N % 4 == 0 && n + 8 <= p.N) {
-            put8(to, x);
+            put<float, 8>(to, x);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -255,7 +281,7 @@ __device__ inline void put_row(const Args &p, int batch, int split, int64_t m, i
     }
     T *to = (T *)p.out[batch] + m * p.out_l + n;
     if (p.wide && n + 8 <= p.N) {
-        put8(to, x);
+        put<T, 8>(to, x);
     } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -265,63 +291,111 @@ __device__ inline void put_row(const Args &p, int batch, int split, int64_t m, i
 }
 
 // h, and a and b where they are saved; zeros past the hidden features
-template <typename T>
-__device__ inline void put_hidden(const Args &p, int64_t m, int n, f32x8 a, f32x8 b) {
-    f32x8 h;
+template <typename T, int V>
+__device__ inline void put_hidden(const Args &p, int64_t m, int n, fv<V> a, fv<V> b) {
+    fv<V> h;
+    activate_all<T, V>(p.activation, [&](int j, auto act) { h[j] = act(a[j]).x * b[j]; });
+    if (n + V > p.N) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        h[j] = activate<T>(a[j], p.activation).x * b[j];
-        if (n + j >= p.N)
-            h[j] = a[j] = b[j] = 0.f;
+        for (int j = 0; j < V; ++j)
+            if (n + j >= p.N)
+                h[j] = a[j] = b[j] = 0.f;
     }
     const int64_t at = m * p.out_l + n;
     if (p.saved[0])
-        save<T>(p, at, a, b);
-    put8((T *)p.out[0] + at, h);
+        save<T, V>(p, at, a, b);
+    put<T, V>((T *)p.out[0] + at, h);
 }
 
+// The gradients of a and b from that of h (half precision: times 2^up); what was saved past the
+// hidden features is zero, dh there anything.
 template <typename T>
-__device__ inline void put_grads(const Args &p, int64_t m, int n, f32x8 dh, int up) {
+__device__ inline void put_grads(const Args &p, int64_t m, int n, f32x8 dh, const Saved<T> &kept,
+                                 int up) {
     const int64_t at = m * p.out_l + n;
-    const float by = __builtin_ldexpf(1.f, up);
-    f32x8 a, b, h, da, db;
-    saved<T>(p, at, a, b);
+    f32x8 a, b, da, db;
+    kept.give(a, b);
+    if constexpr (__is_same(T, _Float16))
+        dh *= __builtin_ldexpf(1.f, up);
+    activate_all<T, 8>(p.activation, [&](int j, auto act) {
+        const float2 v = act(a[j]);
+        da[j] = dh[j] * b[j] * v.y;
+        db[j] = dh[j] * v.x;
+    });
+    if (n + 8 > p.N) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float2 act = activate<T>(a[j], p.activation);
-        const bool real = n + j < p.N;
-        h[j] = real ? act.x * b[j] : 0.f;
-        da[j] = real ? dh[j] * by * b[j] * act.y : 0.f;
-        db[j] = real ? dh[j] * by * act.x : 0.f;
+        for (int j = 0; j < 8; ++j)
+            if (n + j >= p.N)
+                da[j] = db[j] = 0.f;
     }
-    put8((T *)p.out[0] + at, h);
-    put8((T *)p.da + at, da);
-    put8((T *)p.db + at, db);
+    put<T, 8>((T *)p.da + at, da);
+    put<T, 8>((T *)p.db + at, db);
 }
 
 // ---- the product ------------------------------------------------------------------
+
+// The order of a tile's instructions: PRODUCTS a run of 16 k, in its first quarter the READS of the next
+// run, so that they are there in time, and in the second half of the first two runs the LOADS of
+// the next tile.  Sent for at once, the loads hold up every wave, later they are late (8192 x 2048
+// of 5632 k: 154 us; loads at once 170, over four runs 166, reads over the whole run 158).
+template <int RUNS, int PRODUCTS, int READS, int LOADS, int PARTS> struct Order {
+    template <int R, int I> __device__ static inline void one() {
+        __builtin_amdgcn_sched_group_barrier(0x008, PARTS, 0); // matrix products
+        constexpr int FIRST = PRODUCTS / 4, LAST = PRODUCTS / 2, HALF = (LOADS + 1) / 2;
+        if constexpr (I < FIRST)
+            __builtin_amdgcn_sched_group_barrier(
+                0x100, READS * (I + 1) / FIRST - READS * I / FIRST, 0); // reads of LDS
+        if constexpr (R < 2 && I >= PRODUCTS - LAST) {
+            constexpr int J = I - (PRODUCTS - LAST);
+            __builtin_amdgcn_sched_group_barrier(
+                0x020, HALF * (J + 1) / LAST - HALF * J / LAST, 0); // loads from memory
+        }
+        if constexpr (I + 1 < PRODUCTS)
+            one<R, I + 1>();
+        else if constexpr (R + 1 < RUNS)
+            one<R + 1, 0>();
+    }
+    __device__ static inline void runs() { one<0, 0>(); }
+};
 
 template <Kind K> struct Shape { // which operands are strided
     static constexpr bool kA = K == kWeights, kB = K != kUp && K != kDown;
 };
 
-template <bool BIG> struct Size {
-    static constexpr int BM = BIG ? 256 : 128, BN = BM, MB = BIG ? 4 : 2; // MB: 32 rows each
-    static constexpr int NT = BIG ? 512 : 256;
+// Meets the block's other waves when this one's loads have arrived and its reads and writes of LDS are
+// done.
+__device__ inline void meet() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A block's waves by rows and columns and what each has of the result, in 32 x 32.  Large tiles: one block of
+// eight waves a compute unit, small ones: two of four.  The large gated one's waves have 64
+// columns of either projection, so that rows of 128 bytes are written.
+template <Kind K, int SIZE> struct Size {
+    static constexpr int WM = 2, WN = SIZE == kLarge ? 4 : 2, MB = SIZE == kLarge ? 4 : 2, NB = 2;
+};
+template <> struct Size<kUp, kLarge> {
+    static constexpr int WM = 4, WN = 2, MB = 2, NB = 4;
 };
 
-template <typename T, Kind KIND, bool BIG>
-__global__ __launch_bounds__((Size<BIG>::NT), 2) void product(const Args p) {
-    using Z = Size<BIG>;
-    constexpr int BM = Z::BM, BN = Z::BN, NT = Z::NT, MB = Z::MB, NB = 2, BK = kStep<T>;
+template <typename T, Kind KIND, int SIZE>
+__global__ __launch_bounds__((64 * Size<KIND, SIZE>::WM * Size<KIND, SIZE>::WN), 2) void
+product(const Args p) {
+    using Z = Size<KIND, SIZE>;
+    constexpr int MB = Z::MB, NB = Z::NB, BM = 32 * MB * Z::WM, BN = 32 * NB * Z::WN;
+    constexpr int NT = 64 * Z::WM * Z::WN, BK = kStep<T>;
     constexpr bool GATED = KIND == kUp;
     constexpr int TN = GATED ? BN / 2 : BN; // columns of the result a block
-    using FA = Feed<T, BM, Shape<KIND>::kA, NT>;
-    using FB = Feed<T, BN, Shape<KIND>::kB, NT>;
+    constexpr int HALF = 16 * NB; // gated: columns of either projection a wave
+    using FA = Feed<T, BM, Shape<KIND>::kA, NT, 0>;
+    using FB = Feed<T, BN, Shape<KIND>::kB, NT, GATED ? HALF : 0>;
+    // Apart, so that the compiler sees that a tile on its way is not the one that is read.
     __shared__ u32x4 a0[FA::SIZE], a1[FA::SIZE], b0[FB::SIZE], b1[FB::SIZE];
 
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
-    const int wave = attn::scalar(tid >> 6), wm = wave / (BN / 64), wn = wave % (BN / 64);
+    const int wave = attn::scalar(tid >> 6), wm = wave / Z::WN, wn = wave % Z::WN;
     const int mt = (p.M + BM - 1) / BM, nt = (p.N + TN - 1) / TN;
     // tiles in bands of 8 rows of tiles, a run of them an XCD: those which share operands meet
     // in its L2
@@ -336,26 +410,42 @@ __global__ __launch_bounds__((Size<BIG>::NT), 2) void product(const Args p) {
 
     FA fa;
     FB fb;
-    fa.template start<false>(tid, p.a_l, p.M - m0);
-    fb.template start<GATED>(tid, p.b_l, p.N - n0);
+    fa.start(tid, p.a_l, p.M - m0);
+    fb.start(tid, p.b_l, p.N - n0);
     const int spk = (p.K + BK - 1) / BK; // steps a segment
     const int s0 = split * p.split_steps, s1 = min(s0 + p.split_steps, spk * p.segments);
     const uint32_t at_a = FA::lane_at(lane), at_b = FB::lane_at(lane);
 
+    // the tiles' first elements at k = 0, of either segment; gated: of gate and up
+    const int64_t off_a = Shape<KIND>::kA ? m0 : m0 * p.a_l, step_a = Shape<KIND>::kA ? p.a_l : 1;
+    const int64_t off_b = Shape<KIND>::kB ? n0 : n0 * p.b_l, step_b = Shape<KIND>::kB ? p.b_l : 1;
+    const T *from_a0 = (const T *)p.a[batch] + off_a, *from_a1 = (const T *)p.a[1] + off_a;
+    const T *from_b0 = (const T *)p.b[batch] + off_b, *from_b1 = (const T *)p.b[1] + off_b;
+
+    const auto is_whole = [&](int s) { return (s < spk ? s + 1 : s + 1 - spk) * BK <= p.K; };
+    // sends for tile s where there is one and it is whole; else for what nobody reads (the first 16
+    // bytes over and over), so that there is no branch among the products
     const auto fetch = [&](int s, u32x4 *ta, u32x4 *tb) {
+        const bool here = s < s1 && is_whole(s);
+        const int seg = here && s >= spk ? 1 : 0, k = here ? (s - seg * spk) * BK : 0;
+        const T *pa = (KIND == kInput && seg ? from_a1 : from_a0) + k * step_a;
+        const T *pb = (KIND == kInput && seg ? from_b1 : from_b0) + k * step_b;
+        const T *pu = GATED ? from_b1 + k : nullptr;
+        const uint32_t mask = here ? ~0u : 0u;
+        fa.load(ta, (const char *)pa, nullptr, tid, mask);
+        fb.load(tb, (const char *)pb, (const char *)pu, tid, mask);
+    };
+    // the last tile of a segment, if it is not whole
+    const auto fetch_rest = [&](int s, u32x4 *ta, u32x4 *tb) {
+        if (s >= s1 || is_whole(s))
+            return;
         const int seg = s >= spk ? 1 : 0, k = (s - seg * spk) * BK;
-        const int which = KIND == kInput ? seg : batch;
-        const T *pa = (const T *)p.a[which], *pb = (const T *)p.b[which];
-        pa += Shape<KIND>::kA ? k * p.a_l + m0 : m0 * p.a_l + k;
-        pb += Shape<KIND>::kB ? k * p.b_l + n0 : n0 * p.b_l + k;
-        const T *pu = GATED ? (const T *)p.b[1] + n0 * p.b_l + k : nullptr;
-        if (k + BK <= p.K) {
-            fa.template load<false>(ta, (const char *)pa, nullptr, tid);
-            fb.template load<GATED>(tb, (const char *)pb, (const char *)pu, tid);
-        } else {
-            fa.template load_last<false>(ta, (const char *)pa, nullptr, tid, p.K - k);
-            fb.template load_last<GATED>(tb, (const char *)pb, (const char *)pu, tid, p.K - k);
-        }
+        const T *pa = (KIND == kInput && seg ? from_a1 : from_a0) + k * step_a;
+        const T *pb = (KIND == kInput && seg ? from_b1 : from_b0) + k * step_b;
+        const T *pu = GATED ? from_b1 + k : nullptr;
+        attn::arrived(); // what fetch() sent for is not to land on it
+        fa.load_last(ta, (const char *)pa, nullptr, tid, p.K - k);
+        fb.load_last(tb, (const char *)pb, (const char *)pu, tid, p.K - k);
     };
 
     f32x16 acc[NB][MB];
@@ -364,80 +454,124 @@ __global__ __launch_bounds__((Size<BIG>::NT), 2) void product(const Args p) {
 #pragma unroll
         for (int j = 0; j < MB; ++j)
             acc[i][j] = f32x16{};
-    const auto step = [&](int s, const u32x4 *ta, const u32x4 *tb, u32x4 *next_a, u32x4 *next_b) {
-        attn::arrived();
-        __syncthreads(); // this tile is here, and the other buffer is done with
-        if (s + 1 < s1)
-            fetch(s + 1, next_a, next_b);
+    // operands of two runs of 16 k
+    x8<T> x0[MB], y0[NB], x1[MB], y1[NB];
+    const auto read = [&](const u32x4 *ta, const u32x4 *tb, int c, x8<T>(&x)[MB], x8<T>(&y)[NB]) {
 #pragma unroll
-        for (int c = 0; c < BK / 16; ++c) {
-            x8<T> x[MB], y[NB];
+        for (int i = 0; i < NB; ++i)
+            y[i] = FB::operand(tb, at_b, NB * wn + i, c);
+#pragma unroll
+        for (int j = 0; j < MB; ++j)
+            x[j] = FA::operand(ta, at_a, MB * wm + j, c);
+    };
+    const auto multiply = [&](const x8<T>(&x)[MB], const x8<T>(&y)[NB]) {
+#pragma unroll
+        for (int j = 0; j < MB; ++j)
 #pragma unroll
             for (int i = 0; i < NB; ++i)
-                y[i] = FB::operand(tb, at_b, NB * wn + i, c);
-#pragma unroll
-            for (int j = 0; j < MB; ++j)
-                x[j] = FA::operand(ta, at_a, MB * wm + j, c);
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-#pragma unroll
-                for (int j = 0; j < MB; ++j)
-                    acc[i][j] = mma32(y[i], x[j], acc[i][j]);
+                acc[i][j] = mma32(y[i], x[j], acc[i][j]);
+    };
+    // One tile: while a run of 16 k is multiplied the next one is read, in the first the last of the
+    // tile before, so that the matrix cores wait neither for LDS nor for the barrier between
+    // tiles.  The next tile is sent for between the products of the first two runs: sent for at
+    // once, its loads would hold up every wave (16 cycles each, of all waves).
+    constexpr int RUNS = BK / 16;
+    const auto tile = [&](const u32x4 *ta, const u32x4 *tb) {
+        read(ta, tb, 0, x0, y0);
+        multiply(x1, y1);
+        read(ta, tb, 1, x1, y1);
+        multiply(x0, y0);
+        if constexpr (RUNS == 4) {
+            read(ta, tb, 2, x0, y0);
+            multiply(x1, y1);
+            read(ta, tb, 3, x1, y1);
+            multiply(x0, y0);
         }
     };
-    if (s0 < s1)
+    const auto step = [&](int s, u32x4 *ta, u32x4 *tb, u32x4 *next_a, u32x4 *next_b) {
+        fetch(s + 1, next_a, next_b);
+        tile(ta, tb);
+        Order<RUNS, NB * MB, NB * FB::READS + MB * FA::READS, FA::N + FB::N,
+              sizeof(T) == 4 ? 8 : 1>::runs();
+        fetch_rest(s + 1, next_a, next_b);
+        meet();
+    };
+#pragma unroll
+    for (int j = 0; j < MB; ++j)
+        x1[j] = x8<T>{};
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+        y1[i] = x8<T>{};
+    if (s0 < s1) {
         fetch(s0, a0, b0);
+        fetch_rest(s0, a0, b0);
+        meet();
+    }
     for (int s = s0; s < s1; s += 2) {
         step(s, a0, b0, a1, b1);
         if (s + 1 < s1)
             step(s + 1, a1, b1, a0, b0);
     }
+    multiply(x1, y1);
 
     const int up = KIND == kHidden || KIND == kInput || KIND == kWeights ? grad_up<T>(p, lane) : 0;
     const float down = __builtin_ldexpf(1.f, -up);
-    // 32 rows at a time through LDS: what was a lane's column becomes rows
+    // A wave's rows, 32 at a time, through LDS: what was a lane's column becomes rows.  Units of 16
+    // bytes are permuted by the row, so that rows meet other banks.
     __syncthreads();
-    constexpr int ROW = 68; // floats: 16 bytes more than 64, so that rows meet other banks
-    constexpr int PER = NT / 64 / 4; // waves that share a buffer
-    static_assert(PER * 32 * ROW * 4 <= FA::SIZE * 16 && PER * 32 * ROW * 4 <= FB::SIZE * 16);
-    u32x4 *buffer = wave / PER == 0 ? a0 : wave / PER == 1 ? a1 : wave / PER == 2 ? b0 : b1;
-    float *turn = (float *)buffer + wave % PER * 32 * ROW;
+    constexpr int ROW = 8 * NB, PER = FA::SIZE / (32 * ROW); // units a row; waves a buffer
+    static_assert(FA::SIZE == FB::SIZE && 4 * PER >= Z::WM * Z::WN);
+    f32x4 *turn = (f32x4 *)(wave / PER == 0 ? a0 : wave / PER == 1 ? a1 : wave / PER == 2 ? b0 : b1) +
+                  wave % PER * 32 * ROW;
+    // a lane has 8 columns of PARTS rows of 32
+    constexpr int LANES = (GATED ? HALF : 32 * NB) / 8, PARTS = LANES / 2;
+    const int row = lane / LANES, col = lane % LANES * 8;
+    const int n = n0 + (GATED ? HALF : 32 * NB) * wn + col;
+    const bool here = n < (GATED || KIND == kHidden ? p.out_l : (int64_t)p.N);
+    const int mw = m0 + 32 * MB * wm + row;
+    Saved<T> kept[KIND == kHidden ? PARTS : 1]; // sent for 32 rows ahead
+    if constexpr (KIND == kHidden) {
 #pragma unroll
+        for (int k = 0; k < PARTS; ++k) {
+            const int m = mw + 64 / LANES * k;
+            if (m < p.M && here)
+                kept[k].load(p, m * p.out_l + n);
+        }
+    }
+    // one copy of what follows: the sums move up in the registers
+#pragma unroll 1
     for (int j = 0; j < MB; ++j) {
         attn::wave_fence();
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                *(f32x4 *)(turn + (lane & 31) * ROW + 32 * i + 8 * q + 4 * half) =
-                    (f32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
-                            acc[i][j][4 * q + 3]};
+                turn[(lane & 31) * ROW + ((8 * i + 2 * q + half) ^ (lane & 15))] =
+                    (f32x4){acc[i][0][4 * q], acc[i][0][4 * q + 1], acc[i][0][4 * q + 2],
+                            acc[i][0][4 * q + 3]};
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int k = 0; k + 1 < MB; ++k)
+                acc[i][k] = acc[i][k + 1];
         attn::wave_fence();
-        const int mw = m0 + 32 * (MB * wm + j);
-        const auto read8 = [&](int r, int col) {
-            const f32x4 *from = (const f32x4 *)(turn + r * ROW + col);
-            const f32x4 lo = from[0], hi = from[1];
+        const auto read8 = [&](int r, int c) {
+            const f32x4 lo = turn[r * ROW + ((c >> 2) ^ (r & 15))];
+            const f32x4 hi = turn[r * ROW + (((c >> 2) + 1) ^ (r & 15))];
             return (f32x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         };
-        if constexpr (GATED) {
 #pragma unroll
-            for (int n16 = 0; n16 < 2; ++n16) {
-                const int r = (lane >> 2) + 16 * n16;
-                const int col = 8 * (lane & 3), n = n0 + 32 * wn + col;
-                if (mw + r < p.M && n < p.out_l)
-                    put_hidden<T>(p, mw + r, n, read8(r, col), read8(r, col + 32));
-            }
-        } else {
-#pragma unroll KIND == kHidden ? 1 : 4
-            for (int n8 = 0; n8 < 4; ++n8) {
-                const int r = (lane >> 3) + 8 * n8;
-                const int col = 8 * (lane & 7), n = n0 + 64 * wn + col;
-                if constexpr (KIND == kHidden) {
-                    if (mw + r < p.M && n < p.out_l)
-                        put_grads<T>(p, mw + r, n, read8(r, col), up);
+        for (int k = 0; k < PARTS; ++k) {
+            const int r = row + 64 / LANES * k, m = mw + 32 * j + 64 / LANES * k;
+            if (m < p.M && here) {
+                if constexpr (GATED) {
+                    put_hidden<T, 8>(p, m, n, read8(r, col), read8(r, col + HALF));
+                } else if constexpr (KIND == kHidden) {
+                    put_grads<T>(p, m, n, read8(r, col), kept[k], up);
+                    if (j + 1 < MB && m + 32 < p.M)
+                        kept[k].load(p, (m + 32) * p.out_l + n);
                 } else {
-                    if (mw + r < p.M && n < p.N)
-                        put_row<T>(p, batch, split, mw + r, n, read8(r, col) * down);
+                    put_row<T>(p, batch, split, m, n, read8(r, col) * down);
                 }
             }
         }
@@ -466,27 +600,29 @@ template <typename T> __global__ __launch_bounds__(256) void join(const Args p) 
             to[j] = (T)sum[j];
 }
 
-template <typename T, Kind KIND, bool BIG> int launch(const Args &p, hipStream_t stream) {
-    using Z = Size<BIG>;
-    const int tn = KIND == kUp ? Z::BN / 2 : Z::BN;
-    const int64_t blocks = (int64_t)((p.M + Z::BM - 1) / Z::BM) * ((p.N + tn - 1) / tn) *
-                           p.batches * p.splits;
+template <typename T, Kind KIND, int SIZE> int launch(const Args &p, hipStream_t stream) {
+    using Z = Size<KIND, SIZE>;
+    constexpr int BM = 32 * Z::MB * Z::WM, TN = (KIND == kUp ? 16 : 32) * Z::NB * Z::WN;
+    const int64_t blocks = (int64_t)((p.M + BM - 1) / BM) * ((p.N + TN - 1) / TN) * p.batches *
+                           p.splits;
     if (!blocks)
         return 0;
-    product<T, KIND, BIG><<<dim3((unsigned)blocks), Z::NT, 0, stream>>>(p);
+    product<T, KIND, SIZE><<<dim3((unsigned)blocks), 64 * Z::WM * Z::WN, 0, stream>>>(p);
     return hipGetLastError() != hipSuccess;
 }
 
-template <typename T> int run(const Args &p, Kind kind, bool big, hipStream_t stream) {
+template <typename T, Kind KIND> int launch_size(const Args &p, int size, hipStream_t stream) {
+    return size == kLarge ? launch<T, KIND, kLarge>(p, stream)
+                          : launch<T, KIND, kSmall>(p, stream);
+}
+
+template <typename T> int run(const Args &p, Kind kind, int size, hipStream_t stream) {
     switch (kind) {
-    case kUp: return big ? launch<T, kUp, true>(p, stream) : launch<T, kUp, false>(p, stream);
-    case kDown: return big ? launch<T, kDown, true>(p, stream) : launch<T, kDown, false>(p, stream);
-    case kHidden:
-        return big ? launch<T, kHidden, true>(p, stream) : launch<T, kHidden, false>(p, stream);
-    case kInput:
-        return big ? launch<T, kInput, true>(p, stream) : launch<T, kInput, false>(p, stream);
-    default:
-        return big ? launch<T, kWeights, true>(p, stream) : launch<T, kWeights, false>(p, stream);
+    case kUp: return launch_size<T, kUp>(p, size, stream);
+    case kDown: return launch_size<T, kDown>(p, size, stream);
+    case kHidden: return launch_size<T, kHidden>(p, size, stream);
+    case kInput: return launch_size<T, kInput>(p, size, stream);
+    default: return launch_size<T, kWeights>(p, size, stream);
     }
 }
 
