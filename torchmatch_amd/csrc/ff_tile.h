@@ -85,7 +85,7 @@ template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
     static constexpr int N = SIZE / NT, STEP = NT / L::U;
     static_assert(SIZE % NT == 0 && NT % L::U == 0 && L::U == L::U0);
 
-    static constexpr int READS = sizeof(T) == 4 ? (STRIDED ? 8 : 2) : STRIDED ? 2 : 1; // an operand's
+    static constexpr int READS = STRIDED ? 2 : 1; // an operand's (16-bit types)
 
     uint32_t off[N]; // bytes from the tile's first element, its k aside
     int unit[N];     // not strided: the unit of k
@@ -178,6 +178,71 @@ template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
         }
     }
 };
+
+// ---- products ---------------------------------------------------------------------
+
+// float32 numbers as sums of three bfloat16 ones of 8 bits each, exactly: six products of these,
+// at sixteen times the rate of float32 ones, leave out 2^-24 of |y x| at most, with
+// either sign.  Infinite numbers become NaN.
+struct Parts {
+    u32x4 hi, mid, lo; // eight bfloat16 each
+    __device__ inline void set(f32x8 x) {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+        const auto pair = [](f32x2 v) {
+            return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b16x2));
+        };
+        const auto left = [](f32x2 v, uint32_t of) {
+            return f32x2{v[0] - __uint_as_float(of << 16), v[1] - __uint_as_float(of & 0xffff0000u)};
+        };
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            f32x2 v = {x[2 * j], x[2 * j + 1]};
+            hi[j] = pair(v);
+            v = left(v, hi[j]);
+            mid[j] = pair(v);
+            lo[j] = pair(left(v, mid[j]));
+        }
+    }
+};
+// An operand as the products take it.
+template <typename T> struct Operand {
+    x8<T> x;
+    __device__ inline void set(x8<T> v) { x = v; }
+    __device__ inline void made_here() {}
+};
+template <> struct Operand<float> : Parts {
+    // not after the next branch, away from the products that it is to run beside
+    __device__ inline void made_here() { asm volatile("" : "+v"(hi), "+v"(mid), "+v"(lo)); }
+};
+
+// c[i][j] += y[i] x[j] over 16 k
+template <typename T, int NB, int MB>
+__device__ inline void multiply(const Operand<T> (&y)[NB], const Operand<T> (&x)[MB],
+                                f32x16 (&c)[NB][MB]) {
+    if constexpr (sizeof(T) == 4) {
+        const auto all = [&](u32x4 Parts::*u, u32x4 Parts::*v) {
+#pragma unroll
+            for (int j = 0; j < MB; ++j)
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+                    c[i][j] = mma32(__builtin_bit_cast(attn::b16x8, y[i].*u),
+                                    __builtin_bit_cast(attn::b16x8, x[j].*v), c[i][j]);
+        };
+        all(&Parts::hi, &Parts::lo); // the smallest first
+        all(&Parts::lo, &Parts::hi);
+        all(&Parts::mid, &Parts::mid);
+        all(&Parts::hi, &Parts::mid);
+        all(&Parts::mid, &Parts::hi);
+        all(&Parts::hi, &Parts::hi);
+    } else {
+#pragma unroll
+        for (int j = 0; j < MB; ++j)
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+                c[i][j] = mma32(y[i].x, x[j].x, c[i][j]);
+    }
+}
 
 // ---- results ----------------------------------------------------------------------
 
@@ -338,9 +403,9 @@ __device__ inline void put_grads(const Args &p, int64_t m, int n, f32x8 dh, cons
 // run, so that they are there in time, and in the second half of the first two runs the LOADS of
 // the next tile.  Sent for at once, the loads hold up every wave, later they are late (8192 x 2048
 // of 5632 k: 154 us; loads at once 170, over four runs 166, reads over the whole run 158).
-template <int RUNS, int PRODUCTS, int READS, int LOADS, int PARTS> struct Order {
+template <int RUNS, int PRODUCTS, int READS, int LOADS> struct Order {
     template <int R, int I> __device__ static inline void one() {
-        __builtin_amdgcn_sched_group_barrier(0x008, PARTS, 0); // matrix products
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // matrix products
         constexpr int FIRST = PRODUCTS / 4, LAST = PRODUCTS / 2, HALF = (LOADS + 1) / 2;
         if constexpr (I < FIRST)
             __builtin_amdgcn_sched_group_barrier(
@@ -350,6 +415,24 @@ template <int RUNS, int PRODUCTS, int READS, int LOADS, int PARTS> struct Order 
             __builtin_amdgcn_sched_group_barrier(
                 0x020, HALF * (J + 1) / LAST - HALF * J / LAST, 0); // loads from memory
         }
+        if constexpr (I + 1 < PRODUCTS)
+            one<R, I + 1>();
+        else if constexpr (R + 1 < RUNS)
+            one<R + 1, 0>();
+    }
+    __device__ static inline void runs() { one<0, 0>(); }
+};
+
+// float32: a run's numbers are read and taken apart while the run before is multiplied.
+template <int RUNS, int PRODUCTS, int READS, int LOADS> struct OrderParts {
+    template <int R, int I> __device__ static inline void one() {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // matrix products
+        if constexpr (I < 4)
+            __builtin_amdgcn_sched_group_barrier(0x100, READS / 4, 0); // reads of LDS
+        else
+            __builtin_amdgcn_sched_group_barrier(0x002, 8, 0); // taking apart
+        if constexpr (R == 0 && I >= 4 && I < 4 + LOADS)
+            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0); // loads from memory
         if constexpr (I + 1 < PRODUCTS)
             one<R, I + 1>();
         else if constexpr (R + 1 < RUNS)
@@ -455,21 +538,15 @@ product(const Args p) {
         for (int j = 0; j < MB; ++j)
             acc[i][j] = f32x16{};
     // operands of two runs of 16 k
-    x8<T> x0[MB], y0[NB], x1[MB], y1[NB];
-    const auto read = [&](const u32x4 *ta, const u32x4 *tb, int c, x8<T>(&x)[MB], x8<T>(&y)[NB]) {
+    Operand<T> x0[MB], y0[NB], x1[MB], y1[NB];
+    const auto read = [&](const u32x4 *ta, const u32x4 *tb, int c, Operand<T>(&x)[MB],
+                          Operand<T>(&y)[NB]) {
 #pragma unroll
         for (int i = 0; i < NB; ++i)
-            y[i] = FB::operand(tb, at_b, NB * wn + i, c);
+            y[i].set(FB::operand(tb, at_b, NB * wn + i, c));
 #pragma unroll
         for (int j = 0; j < MB; ++j)
-            x[j] = FA::operand(ta, at_a, MB * wm + j, c);
-    };
-    const auto multiply = [&](const x8<T>(&x)[MB], const x8<T>(&y)[NB]) {
-#pragma unroll
-        for (int j = 0; j < MB; ++j)
-#pragma unroll
-            for (int i = 0; i < NB; ++i)
-                acc[i][j] = mma32(y[i], x[j], acc[i][j]);
+            x[j].set(FA::operand(ta, at_a, MB * wm + j, c));
     };
     // One tile: while a run of 16 k is multiplied the next one is read, in the first the last of the
     // tile before, so that the matrix cores wait neither for LDS nor for the barrier between
@@ -478,30 +555,38 @@ product(const Args p) {
     constexpr int RUNS = BK / 16;
     const auto tile = [&](const u32x4 *ta, const u32x4 *tb) {
         read(ta, tb, 0, x0, y0);
-        multiply(x1, y1);
+        multiply<T>(y1, x1, acc);
         read(ta, tb, 1, x1, y1);
-        multiply(x0, y0);
+        multiply<T>(y0, x0, acc);
         if constexpr (RUNS == 4) {
             read(ta, tb, 2, x0, y0);
-            multiply(x1, y1);
+            multiply<T>(y1, x1, acc);
             read(ta, tb, 3, x1, y1);
-            multiply(x0, y0);
+            multiply<T>(y0, x0, acc);
         }
+#pragma unroll
+        for (int j = 0; j < MB; ++j)
+            x1[j].made_here();
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+            y1[i].made_here();
     };
     const auto step = [&](int s, u32x4 *ta, u32x4 *tb, u32x4 *next_a, u32x4 *next_b) {
         fetch(s + 1, next_a, next_b);
         tile(ta, tb);
-        Order<RUNS, NB * MB, NB * FB::READS + MB * FA::READS, FA::N + FB::N,
-              sizeof(T) == 4 ? 8 : 1>::runs();
+        if constexpr (sizeof(T) == 2)
+            Order<RUNS, NB * MB, NB * FB::READS + MB * FA::READS, FA::N + FB::N>::runs();
+        else
+            OrderParts<RUNS, NB * MB * 6, 2 * (NB + MB), FA::N + FB::N>::runs();
         fetch_rest(s + 1, next_a, next_b);
         meet();
     };
 #pragma unroll
     for (int j = 0; j < MB; ++j)
-        x1[j] = x8<T>{};
+        x1[j] = {};
 #pragma unroll
     for (int i = 0; i < NB; ++i)
-        y1[i] = x8<T>{};
+        y1[i] = {};
     if (s0 < s1) {
         fetch(s0, a0, b0);
         fetch_rest(s0, a0, b0);
@@ -512,7 +597,7 @@ product(const Args p) {
         if (s + 1 < s1)
             step(s + 1, a1, b1, a0, b0);
     }
-    multiply(x1, y1);
+    multiply<T>(y1, x1, acc);
 
     const int up = KIND == kHidden || KIND == kInput || KIND == kWeights ? grad_up<T>(p, lane) : 0;
     const float down = __builtin_ldexpf(1.f, -up);
@@ -612,8 +697,10 @@ template <typename T, Kind KIND, int SIZE> int launch(const Args &p, hipStream_t
 }
 
 template <typename T, Kind KIND> int launch_size(const Args &p, int size, hipStream_t stream) {
-    return size == kLarge ? launch<T, KIND, kLarge>(p, stream)
-                          : launch<T, KIND, kSmall>(p, stream);
+    if constexpr (sizeof(T) == 2) // float32's operands do not fit in registers with large tiles
+        if (size == kLarge)
+            return launch<T, KIND, kLarge>(p, stream);
+    return launch<T, KIND, kSmall>(p, stream);
 }
 
 template <typename T> int run(const Args &p, Kind kind, int size, hipStream_t stream) {
