@@ -31,7 +31,7 @@ enum Kind { kUp, kDown, kHidden, kInput, kWeights };
 enum { kSmall, kLarge }; // tiles: 128 x 128, 256 x 256
 
 // Products of up to this many rows take product_tokens.
-constexpr int kTokens = 32;
+constexpr int kTokens = 64;
 
 // Non-zero: a launch failed.
 #define FF_DECLARE(type)                                                                         \

@@ -2,10 +2,11 @@
 // once bounds them.
 //
 // A block has 16 rows of the weights (of gate and of up), its waves a part of k each, so that a product
-// of few rows of weights still fills the card; their sums meet in LDS, in order.  A wave loads 64
-// bytes of 16 rows at once, straight into the operands of 16 x 16 products with up to 16 GROUPS
-// rows of x, which all blocks share in L2.  The contraction takes its indices in the order in
-// which lanes hold them, for both operands alike.
+// of few rows of weights still fills the card; their sums meet in LDS, in order.  A wave brings whole
+// lines of 16 rows and of x into its own part of LDS, two or three pieces ahead of its 16 x 16
+// products, and meets the others at the end only.  (Operands straight from memory, 64 bytes of
+// each row a load: 26 and 77 us for the two timed calls of few tokens.)  The contraction
+// takes its indices in the order in which lanes hold them, for both operands alike.
 #ifndef TORCHMATCH_AMD_FF_TOKENS_H
 #define TORCHMATCH_AMD_FF_TOKENS_H
 
@@ -39,79 +40,133 @@ template <> struct Unit16<float> {
     }
 };
 
-constexpr int kTokenWaves = 16;
-
-// split_steps: pieces of 64 bytes of k a wave
-template <typename T, bool GATED, int GROUPS>
-__global__ __launch_bounds__(64 * kTokenWaves) void product_tokens(const Args p) {
-    constexpr int E = 16 / (int)sizeof(T), MATRICES = GATED ? 2 : 1;
-    constexpr int AT_ONCE = GROUPS == 1 ? 8 : 4; // pieces under way
-    __shared__ f32x4 sums[kTokenWaves][MATRICES * GROUPS][64];
-    const int lane = threadIdx.x & 63, quarter = lane >> 4, col = lane & 15;
-    const int wave = attn::scalar(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int n0 = blockIdx.x * 16;
-    const char *w[MATRICES], *x[GROUPS];
-    bool real[GROUPS];
+// 16 rows of 128 bytes, brought straight into LDS by one wave, whole lines of memory; units of 16
+// bytes are permuted by the row, so that a unit of each row is read without bank conflicts.
+struct Rows16 {
+    uint32_t off[2]; // bytes from the first row
+    int unit[2];
+    __device__ static inline int swz(int row) { return (row >> 1 & 1) << 2 | (row >> 2 & 3); }
+    __device__ inline void start(int lane, int64_t row_bytes, int rows) {
 #pragma unroll
-    for (int i = 0; i < MATRICES; ++i)
-        w[i] = (const char *)((const T *)p.b[i] + (int64_t)min(n0 + col, p.N - 1) * p.b_l) +
-               16 * quarter;
-#pragma unroll
-    for (int g = 0; g < GROUPS; ++g) {
-        real[g] = 16 * g + col < p.M;
-        x[g] = (const char *)((const T *)p.a[0] +
-                              (int64_t)min(16 * g + col, p.M - 1) * p.a_l) + 16 * quarter;
+        for (int n = 0; n < 2; ++n) {
+            const int row = (lane >> 3) + 8 * n;
+            unit[n] = (lane & 7) ^ swz(row);
+            off[n] = (uint32_t)min(row, rows - 1) * (uint32_t)row_bytes;
+        }
     }
+    // piece: which 8 units of the rows; past the last of `units` that one again
+    __device__ inline void load(u32x4 *t, const char *from, int piece, int units) const {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void *)(
+                    from + off[n] + 16u * (uint32_t)min(8 * piece + unit[n], units - 1)),
+                (__attribute__((address_space(3))) void *)(t + 64 * n), 16, 0, 0);
+    }
+    // row lane % 16, unit 4 half + lane / 16
+    __device__ static inline u32x4 operand(const u32x4 *t, int lane, int half) {
+        const int row = lane & 15;
+        return t[8 * row + ((4 * half + (lane >> 4)) ^ swz(row))];
+    }
+};
+
+// WAVES share k; split_steps: pieces of 128 bytes of k a wave
+template <typename T, bool GATED, int GROUPS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void product_tokens(const Args p) {
+    constexpr int E = 16 / (int)sizeof(T), MATRICES = GATED ? 2 : 1, PER = MATRICES + GROUPS;
+    constexpr int SLOTS = GATED ? 2 : 3, LOADS = 2 * PER; // pieces on their way, their loads
+    // Apart, so that the compiler sees that what is on its way is not what is read.
+    __shared__ u32x4 s0[WAVES][PER * 128], s1[WAVES][PER * 128],
+        s2[SLOTS > 2 ? WAVES : 1][SLOTS > 2 ? PER * 128 : 1];
+    const int lane = threadIdx.x & 63, quarter = lane >> 4, col = lane & 15;
+    const int wave = attn::scalar(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * 16;
+    Rows16 w, x[GROUPS];
+    w.start(lane, p.b_l * (int)sizeof(T), p.N - n0);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+        x[g].start(lane, p.a_l * (int)sizeof(T), max(p.M - 16 * g, 1));
+    const int units = (p.K + E - 1) / E, pieces = (units + 7) / 8;
+    const int c0 = wave * p.split_steps, c1 = min(pieces, c0 + p.split_steps);
+
+    const auto fetch = [&](int c, u32x4 *t) {
+        // past the end: the last piece again, which nobody reads
+        c = min(c, pieces - 1);
+#pragma unroll
+        for (int i = 0; i < MATRICES; ++i)
+            w.load(t + 128 * i, (const char *)((const T *)p.b[i] + n0 * p.b_l), c, units);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+            x[g].load(t + 128 * (MATRICES + g), (const char *)((const T *)p.a[0] +
+                      (int64_t)min(16 * g, p.M - 1) * p.a_l), c, units);
+    };
     f32x4 acc[MATRICES][GROUPS];
 #pragma unroll
     for (int i = 0; i < MATRICES; ++i)
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g)
             acc[i][g] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int pieces = (p.K + 4 * E - 1) / (4 * E);
-    const int end = min(pieces, (wave + 1) * p.split_steps);
-    const int units = (p.K + E - 1) / E; // of a row; the last one ends in zeros
-    for (int c0 = wave * p.split_steps; c0 < end; c0 += AT_ONCE) {
-        u32x4 a[AT_ONCE][MATRICES], b[AT_ONCE][GROUPS];
+    const auto step = [&](int c, u32x4 *t) {
+        attn::arrived<(SLOTS - 1) * LOADS>();
+        u32x4 v[2][PER];
 #pragma unroll
-        for (int c = 0; c < AT_ONCE; ++c) {
-            const bool here = c0 + c < end && 4 * (c0 + c) + quarter < units;
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < MATRICES; ++i) {
-                a[c][i] = u32x4{0u, 0u, 0u, 0u};
-                if (here) // read once: not kept in the caches
-                    a[c][i] = __builtin_nontemporal_load((const u32x4 *)(w[i] + 64 * (c0 + c)));
-            }
+            for (int i = 0; i < PER; ++i)
+                v[h][i] = Rows16::operand(t + 128 * i, lane, h);
+        if (8 * c + 8 > units) { // zeros past the end
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                b[c][g] = u32x4{0u, 0u, 0u, 0u};
-                if (here && real[g])
-                    b[c][g] = *(const u32x4 *)(x[g] + 64 * (c0 + c));
-            }
+            for (int h = 0; h < 2; ++h)
+                if (8 * c + 4 * h + quarter >= units)
+#pragma unroll
+                    for (int i = 0; i < PER; ++i)
+                        v[h][i] = u32x4{0u, 0u, 0u, 0u};
         }
 #pragma unroll
-        for (int c = 0; c < AT_ONCE; ++c)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
                 for (int i = 0; i < MATRICES; ++i)
-                    acc[i][g] = Unit16<T>::mma(a[c][i], b[c][g], acc[i][g]);
+                    acc[i][g] = Unit16<T>::mma(v[h][i], v[h][MATRICES + g], acc[i][g]);
+        // what was read has arrived in registers: its place is free
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        fetch(c + SLOTS, t);
+    };
+    if (c0 < c1) {
+        fetch(c0, s0[wave]);
+        fetch(c0 + 1, s1[wave]);
+        if constexpr (SLOTS > 2)
+            fetch(c0 + 2, s2[wave]);
+        for (int c = c0; c < c1; c += SLOTS) {
+            step(c, s0[wave]);
+            if (c + 1 < c1)
+                step(c + 1, s1[wave]);
+            if constexpr (SLOTS > 2)
+                if (c + 2 < c1)
+                    step(c + 2, s2[wave]);
+        }
+        attn::arrived();
     }
+    __syncthreads();
+    f32x4(*sums)[64] = (f32x4(*)[64])s0; // [wave][MATRICES * GROUPS][64]
+    static_assert(MATRICES * GROUPS * 64 <= PER * 128);
 #pragma unroll
     for (int i = 0; i < MATRICES; ++i)
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g)
-            sums[wave][i * GROUPS + g][lane] = acc[i][g];
+            sums[(wave * MATRICES + i) * GROUPS + g][lane] = acc[i][g];
     __syncthreads();
     // a wave each group: token 16 g + col, weights' rows n .. n + 3
-    for (int g = wave; g < GROUPS; g += waves) {
+    for (int g = wave; g < GROUPS; g += WAVES) {
         const int m = 16 * g + col, n = n0 + 4 * quarter;
         f32x4 s[MATRICES];
 #pragma unroll
         for (int i = 0; i < MATRICES; ++i) {
-            s[i] = sums[0][i * GROUPS + g][lane];
-            for (int v = 1; v < waves; ++v)
-                s[i] += sums[v][i * GROUPS + g][lane];
+            s[i] = sums[i * GROUPS + g][lane];
+#pragma unroll
+            for (int v = 1; v < WAVES; ++v)
+                s[i] += sums[(v * MATRICES + i) * GROUPS + g][lane];
         }
         if (m >= p.M)
             continue;
@@ -128,18 +183,27 @@ __global__ __launch_bounds__(64 * kTokenWaves) void product_tokens(const Args p)
     }
 }
 
-template <typename T, bool GATED> int launch_tokens(Args p, hipStream_t stream) {
-    const int64_t blocks = (p.out_l > p.N && GATED ? p.out_l + 15 : (int64_t)p.N + 15) / 16;
-    const int pieces = (p.K + 64 / (int)sizeof(T) - 1) / (64 / (int)sizeof(T));
-    // eight waves or more for each compute unit, of two pieces or more each
-    int waves = 1;
-    while (waves < kTokenWaves && blocks * waves < 2048 && pieces >= 4 * waves)
-        waves *= 2;
-    p.split_steps = (pieces + waves - 1) / waves;
+template <typename T, bool GATED, int GROUPS> void launch_waves(Args p, hipStream_t stream) {
+    const unsigned blocks = (unsigned)(((GATED ? p.out_l : (int64_t)p.N) + 15) / 16);
+    const int pieces = (int)(((int64_t)p.K * (int)sizeof(T) + 127) / 128);
+    // few blocks: more waves each, so that enough is on its way (LDS has room for that up to 32 rows)
+    if constexpr (GROUPS <= 2)
+        if (blocks <= 256 && pieces > 4) {
+            p.split_steps = (pieces + 7) / 8;
+            product_tokens<T, GATED, GROUPS, 8><<<dim3(blocks), 512, 0, stream>>>(p);
+            return;
+        }
+    p.split_steps = (pieces + 3) / 4;
+    product_tokens<T, GATED, GROUPS, 4><<<dim3(blocks), 256, 0, stream>>>(p);
+}
+
+template <typename T, bool GATED> int launch_tokens(const Args &p, hipStream_t stream) {
     if (p.M <= 16)
-        product_tokens<T, GATED, 1><<<dim3((unsigned)blocks), 64 * waves, 0, stream>>>(p);
+        launch_waves<T, GATED, 1>(p, stream);
+    else if (p.M <= 32)
+        launch_waves<T, GATED, 2>(p, stream);
     else
-        product_tokens<T, GATED, 2><<<dim3((unsigned)blocks), 64 * waves, 0, stream>>>(p);
+        launch_waves<T, GATED, 4>(p, stream);
     return hipGetLastError() != hipSuccess;
 }
 
