@@ -60,6 +60,8 @@ Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, 
     if (r.split_steps)
         r.splits = (int)((steps + r.split_steps - 1) / r.split_steps);
     r.splits = std::max(r.splits, 1);
+    if (r.size == ff::kSmall && small * r.splits <= 256) // one block a compute unit at most
+        r.size = ff::kDeep;
     if (r.splits > 1)
         r.part = (size_t)r.splits * batches * M * N * sizeof(float);
     return r;

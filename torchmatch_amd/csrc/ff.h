@@ -28,7 +28,7 @@ struct Args {
 
 constexpr int kMostParts = 256;
 enum Kind { kUp, kDown, kHidden, kInput, kWeights };
-enum { kSmall, kLarge }; // tiles: 128 x 128, 256 x 256
+enum { kSmall, kDeep, kLarge }; // tiles: 128 x 128, with four in LDS in place of two, 256 x 256
 
 // Products of up to this many rows take product_tokens.
 constexpr int kTokens = 64;

@@ -445,26 +445,29 @@ template <Kind K> struct Shape { // which operands are strided
     static constexpr bool kA = K == kWeights, kB = K != kUp && K != kDown;
 };
 
-// Meets the block's other waves when this one's loads have arrived and its reads and writes of LDS are
-// done.
-__device__ inline void meet() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+// Meets the block's other waves when all but LATER of this one's loads have arrived and its reads and
+// writes of LDS are done.  (__syncthreads() would wait for every load, those of later tiles too.)
+template <int LATER> __device__ inline void meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LATER) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
 
-// A block's waves by rows and columns and what each has of the result, in 32 x 32.  Large tiles: one block of
-// eight waves a compute unit, small ones: two of four.  The large gated one's waves have 64
-// columns of either projection, so that rows of 128 bytes are written.
+// A block's waves by rows and columns, what each has of the result, in 32 x 32, and the tiles in LDS.
+// Large tiles: one block of eight waves a compute unit, small ones: two of four.  Where there is no
+// second block to hide the waits, four tiles do (128 x 2048 through 5632: ? -> ? us).  The
+// large gated one's waves have 64 columns of either projection, so that rows of 128 bytes are written.
 template <Kind K, int SIZE> struct Size {
     static constexpr int WM = 2, WN = SIZE == kLarge ? 4 : 2, MB = SIZE == kLarge ? 4 : 2, NB = 2;
+    static constexpr int TILES = SIZE == kDeep ? 4 : 2;
 };
 template <> struct Size<kUp, kLarge> {
-    static constexpr int WM = 4, WN = 2, MB = 2, NB = 4;
+    static constexpr int WM = 4, WN = 2, MB = 2, NB = 4, TILES = 2;
 };
 
 template <typename T, Kind KIND, int SIZE>
-__global__ __launch_bounds__((64 * Size<KIND, SIZE>::WM * Size<KIND, SIZE>::WN), 2) void
+__global__ __launch_bounds__((64 * Size<KIND, SIZE>::WM * Size<KIND, SIZE>::WN),
+                             (SIZE == kDeep ? 1 : 2)) void
 product(const Args p) {
     using Z = Size<KIND, SIZE>;
     constexpr int MB = Z::MB, NB = Z::NB, BM = 32 * MB * Z::WM, BN = 32 * NB * Z::WN;
@@ -475,7 +478,10 @@ product(const Args p) {
     using FA = Feed<T, BM, Shape<KIND>::kA, NT, 0>;
     using FB = Feed<T, BN, Shape<KIND>::kB, NT, GATED ? HALF : 0>;
     // Apart, so that the compiler sees that a tile on its way is not the one that is read.
+    constexpr int TILES = Z::TILES, LOADS = FA::N + FB::N; // a thread's, of a tile
     __shared__ u32x4 a0[FA::SIZE], a1[FA::SIZE], b0[FB::SIZE], b1[FB::SIZE];
+    __shared__ u32x4 a2[TILES > 2 ? FA::SIZE : 1], a3[TILES > 2 ? FA::SIZE : 1],
+        b2[TILES > 2 ? FB::SIZE : 1], b3[TILES > 2 ? FB::SIZE : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
     const int wave = attn::scalar(tid >> 6), wm = wave / Z::WN, wn = wave % Z::WN;
@@ -571,15 +577,17 @@ product(const Args p) {
         for (int i = 0; i < NB; ++i)
             y1[i].made_here();
     };
+    // tile s; its place's neighbour, which is free, takes the last one that is on its way.  Each
+    // fetch() is LOADS loads, so that counts tell which have arrived.
     const auto step = [&](int s, u32x4 *ta, u32x4 *tb, u32x4 *next_a, u32x4 *next_b) {
-        fetch(s + 1, next_a, next_b);
+        fetch(s + TILES - 1, next_a, next_b);
         tile(ta, tb);
         if constexpr (sizeof(T) == 2)
             Order<RUNS, NB * MB, NB * FB::READS + MB * FA::READS, FA::N + FB::N>::runs();
         else
             OrderParts<RUNS, NB * MB * 6, 2 * (NB + MB), FA::N + FB::N>::runs();
-        fetch_rest(s + 1, next_a, next_b);
-        meet();
+        fetch_rest(s + TILES - 1, next_a, next_b);
+        meet<(TILES - 2) * LOADS>();
     };
 #pragma unroll
     for (int j = 0; j < MB; ++j)
@@ -588,19 +596,37 @@ product(const Args p) {
     for (int i = 0; i < NB; ++i)
         y1[i] = {};
     if (s0 < s1) {
-        fetch(s0, a0, b0);
-        fetch_rest(s0, a0, b0);
-        meet();
+        const auto first = [&](int s, u32x4 *ta, u32x4 *tb) {
+            fetch(s, ta, tb);
+            fetch_rest(s, ta, tb);
+        };
+        first(s0, a0, b0);
+        if constexpr (TILES > 2) {
+            first(s0 + 1, a1, b1);
+            first(s0 + 2, a2, b2);
+        }
+        meet<(TILES - 2) * LOADS>();
     }
-    for (int s = s0; s < s1; s += 2) {
-        step(s, a0, b0, a1, b1);
-        if (s + 1 < s1)
-            step(s + 1, a1, b1, a0, b0);
+    for (int s = s0; s < s1; s += TILES) {
+        if constexpr (TILES == 2) {
+            step(s, a0, b0, a1, b1);
+            if (s + 1 < s1)
+                step(s + 1, a1, b1, a0, b0);
+        } else {
+            step(s, a0, b0, a3, b3);
+            if (s + 1 < s1)
+                step(s + 1, a1, b1, a0, b0);
+            if (s + 2 < s1)
+                step(s + 2, a2, b2, a1, b1);
+            if (s + 3 < s1)
+                step(s + 3, a3, b3, a2, b2);
+        }
     }
     multiply<T>(y1, x1, acc);
 
     const int up = KIND == kHidden || KIND == kInput || KIND == kWeights ? grad_up<T>(p, lane) : 0;
     const float down = __builtin_ldexpf(1.f, -up);
+    attn::arrived(); // the last fetches, of nothing, are not to land on what follows
     // A wave's rows, 32 at a time, through LDS: what was a lane's column becomes rows.  Units of 16
     // bytes are permuted by the row, so that rows meet other banks.
     __syncthreads();
@@ -700,7 +726,8 @@ template <typename T, Kind KIND> int launch_size(const Args &p, int size, hipStr
     if constexpr (sizeof(T) == 2) // float32's operands do not fit in registers with large tiles
         if (size == kLarge)
             return launch<T, KIND, kLarge>(p, stream);
-    return launch<T, KIND, kSmall>(p, stream);
+    return size == kDeep ? launch<T, KIND, kDeep>(p, stream)
+                         : launch<T, KIND, kSmall>(p, stream);
 }
 
 template <typename T> int run(const Args &p, Kind kind, int size, hipStream_t stream) {
