@@ -424,9 +424,9 @@ int tm_rotate(const tm_rotation *r, void *out, hipStream_t stream);
  *   y = R(x (mean_d x_d^2 + eps)^-1/2 w)
  * weight: (groups, D) contiguous, of weight_type (rotation.dtype or TM_F32), or NULL for ones; row g
  * is for heads[g] heads, which follow each other and make up all H.  D is at most
- * TM_NORM_MAX_HEAD_DIM (TM_ERR_UNSUPPORTED_SHAPE), rotation.inverse 0.  Sums are float32.
+ * TM_NORM_MAX_HEAD_DIM and H TM_NORM_MAX_HEADS (TM_ERR_UNSUPPORTED_SHAPE), rotation.inverse 0.  Sums are float32.
  * out: (B, L, H, D), contiguous. */
-enum { TM_NORM_MAX_GROUPS = 8, TM_NORM_MAX_HEAD_DIM = 512 };
+enum { TM_NORM_MAX_GROUPS = 8, TM_NORM_MAX_HEAD_DIM = 512, TM_NORM_MAX_HEADS = 1 << 16 };
 typedef struct tm_norm_rotation {
     tm_rotation rotation;
     const void *weight;
@@ -468,6 +468,11 @@ typedef struct tm_feed_forward {
     int64_t x_l, w_l, down_l; /* w_l: of gate and of up */
     int32_t dtype, activation, T, C, F, O;
 } tm_feed_forward;
+
+/* (rows, n) as the block takes it: rows of n elements, x_l apart, each followed by zeros up to 16
+ * bytes, one after the other in out (16-byte aligned). */
+int tm_pad_rows(const void *x, int64_t x_l, int64_t rows, int32_t n, int32_t dtype, void *out,
+                hipStream_t stream);
 
 /* out: (T, O), contiguous.  saved: for the gradients, tm_feed_forward_saved_bytes(f) bytes, or NULL.
  * workspace, saved: device, 16-byte aligned, any contents. */

@@ -59,6 +59,7 @@ def _normed(**changes):
     ({"pos_type": 3}, _native.TM_ERR_INVALID_ARGUMENT),
     ({"x": None}, _native.TM_ERR_INVALID_ARGUMENT),
     ({"D": 513}, _native.TM_ERR_UNSUPPORTED_SHAPE),
+    ({"H": 65537, "D": 1, "sections": (0,), "heads": (65537,)}, _native.TM_ERR_UNSUPPORTED_SHAPE),
 ])
 def test_norm_rotate_refusals(changes, code):
     a = _normed(**changes)
@@ -138,6 +139,15 @@ def test_feed_forward_backward_refusals():
     assert back(do_l=1 << 22) == _native.TM_ERR_UNSUPPORTED_SHAPE
     assert back(dx=None, dgate=None, dup=None, ddown=None) == _native.TM_OK
     assert back(dgate=None, dup=None, ddown=None, T=0) == _native.TM_OK
+
+
+def test_pad_rows_refusals():
+    pad = lambda x=4096, l=5, rows=3, n=5, dtype=0, out=4096: _native.lib().tm_pad_rows(  # noqa: E731
+        x, l, rows, n, dtype, out, None)
+    assert pad(rows=0) == _native.TM_OK
+    for bad in ({"rows": -1}, {"n": 0}, {"dtype": 3}, {"out": 4098}, {"x": None}, {"out": None}):
+        assert pad(**bad) == _native.TM_ERR_INVALID_ARGUMENT
+    assert pad(rows=1 << 40) == _native.TM_ERR_UNSUPPORTED_SHAPE
 
 
 def test_feed_forward_sizes():

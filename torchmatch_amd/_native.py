@@ -224,6 +224,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _VP, _VP, _VP, ctypes.c_size_t, _VP,
         ],
     ),
+    "tm_pad_rows": (
+        ctypes.c_int,
+        [_VP, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, _VP, _VP],
+    ),
     "tm_feed_forward_saved_bytes": (ctypes.c_size_t, [ctypes.POINTER(FeedForward)]),
     "tm_feed_forward_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(FeedForward)]),
     "tm_feed_forward_forward": (

@@ -167,7 +167,46 @@ __global__ __launch_bounds__(256) void ff_most(const _Float16 *x, int64_t l, int
         most[blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
 }
 
+// 16 bytes a thread of rows of n elements, zeros past them
+template <typename U, int E>
+__global__ __launch_bounds__(256) void ff_pad(const U *x, int64_t l, int64_t rows, int n, int units,
+                                              U *out) {
+    typedef U V __attribute__((ext_vector_type(E)));
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = i / units;
+    if (row >= rows)
+        return;
+    const int e = (int)(i - row * units) * E;
+    V v;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        v[j] = e + j < n ? x[row * l + e + j] : (U)0;
+    ((V *)out)[i] = v;
+}
+
 } // namespace
+
+extern "C" int tm_pad_rows(const void *x, int64_t x_l, int64_t rows, int32_t n, int32_t dtype,
+                           void *out, hipStream_t stream) {
+    if (rows < 0 || n < 1 || dtype < TM_BF16 || dtype > TM_F32 || (uintptr_t)out % 16)
+        return TM_ERR_INVALID_ARGUMENT;
+    if (!rows)
+        return TM_OK;
+    if (!x || !out)
+        return TM_ERR_INVALID_ARGUMENT;
+    const int e = dtype == TM_F32 ? 4 : 8, units = (int)(((int64_t)n + e - 1) / e);
+    const int64_t most = (int64_t)((1 << 24) - 1) * 256;
+    if (rows > most / units)
+        return TM_ERR_UNSUPPORTED_SHAPE;
+    const unsigned blocks = (unsigned)((rows * units + 255) / 256);
+    if (e == 8)
+        ff_pad<uint16_t, 8><<<dim3(blocks), 256, 0, stream>>>((const uint16_t *)x, x_l, rows, n,
+                                                             units, (uint16_t *)out);
+    else
+        ff_pad<uint32_t, 4><<<dim3(blocks), 256, 0, stream>>>((const uint32_t *)x, x_l, rows, n,
+                                                             units, (uint32_t *)out);
+    return hipGetLastError() == hipSuccess ? TM_OK : TM_ERR_LAUNCH;
+}
 
 extern "C" size_t tm_feed_forward_saved_bytes(const tm_feed_forward *f) {
     if (check(f))

@@ -29,7 +29,9 @@ template <int V> struct Floats {
 };
 template <int V> using fv = typename Floats<V>::type;
 
+constexpr int kMaxPiece = 1 << 21; // heads of a block's tokens at a time: see quotient()
 constexpr int kMaxItems = 8;  // a lane's, of one head
+constexpr int kBlocks = 1024; // of a backward pass, about
 constexpr int kJoinCols = 32; // columns of dw a block of norm_join
 
 struct NormArgs {
@@ -161,12 +163,51 @@ __device__ inline void weights_of(fv<V> &a, fv<V> &b, const float *w, const Item
     }
 }
 
-// the sum over the lanes of a head
+// The sum over the lanes of a head, 2^lane_bits neighbours.  Up to 16 lanes by moves within a row:
+// once the lanes of four (eight) hold the same sum, a mirrored lane holds that of the others.
+template <int CTRL> __device__ inline float moved(float x) {
+    return __int_as_float(
+        __builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
 __device__ inline float over_head(float x, int lane_bits) {
-    for (int n = 0; n < lane_bits; ++n)
-        x += __shfl_xor(x, 1 << n);
+    if (lane_bits > 0)
+        x += moved<0xB1>(x); // quad_perm [1, 0, 3, 2]
+    if (lane_bits > 1)
+        x += moved<0x4E>(x); // quad_perm [2, 3, 0, 1]
+    if (lane_bits > 2)
+        x += moved<0x141>(x); // row_half_mirror
+    if (lane_bits > 3)
+        x += moved<0x140>(x); // row_mirror
+    if (lane_bits > 4)
+        x += __shfl_xor(x, 16);
+    if (lane_bits > 5)
+        x += __shfl_xor(x, 32);
     return x;
 }
+
+// i / n for 0 <= i < 2^21 by its reciprocal: the product is off by 2^-23 of itself at most, and (i + 1/2) / n
+// is 1 / (2 n), 2^-22 of it, or more away from a whole number
+__device__ inline int quotient(int i, float reciprocal) {
+    return (int)(((float)i + 0.5f) * reciprocal);
+}
+
+// Where token `n` after (b0, l0) stands; a block's tokens cross few rows of the batch
+struct At {
+    int64_t b;
+    uint32_t l;
+    __device__ inline At(const NormArgs &p, int64_t b0, uint32_t l0, int n) : b(b0), l(l0 + n) {
+        if (p.L >= p.per_block) {
+            if (l >= (uint32_t)p.L) {
+                l -= p.L;
+                b += 1;
+            }
+        } else {
+            const uint32_t rows = l / (uint32_t)p.L;
+            l -= rows * p.L;
+            b += rows;
+        }
+    }
+};
 
 __device__ inline float weight_at(const NormArgs &p, int i, bool f32, bool bf16) {
     if (!p.weight)
@@ -180,12 +221,12 @@ __device__ inline float weight_at(const NormArgs &p, int i, bool f32, bool bf16)
 template <typename T>
 __device__ inline void fill_table(float2 *table, const NormArgs &p, int64_t b0, uint32_t l0,
                                   int tokens) {
+    const float per_pair = 1.f / p.at.pairs;
     for (int i = threadIdx.x; i < tokens * p.at.pairs; i += 256) {
-        const int token = i / p.at.pairs;
-        const uint32_t l = l0 + token, rows = l / (uint32_t)p.L;
-        table[i] = rot::turn_of<T>(
-            p.at, (b0 + rows) * p.at.pos_b + (int64_t)(l - rows * p.L) * p.at.axes,
-            i - token * p.at.pairs);
+        const int token = quotient(i, per_pair);
+        const At at(p, b0, l0, token);
+        table[i] = rot::turn_of<T>(p.at, at.b * p.at.pos_b + (int64_t)at.l * p.at.axes,
+                                   i - token * p.at.pairs);
     }
 }
 
@@ -207,7 +248,7 @@ __global__ __launch_bounds__(256) void norm_rotate(const NormArgs p) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
         item[k].template set<V>(p, lane + (k << p.lane_bits));
-    const float share = 1.f / p.D;
+    const float share = 1.f / p.D, per_head = 1.f / p.H;
     __syncthreads();
 
     constexpr int AT_ONCE = 2; // heads whose loads are under way together
@@ -218,11 +259,11 @@ __global__ __launch_bounds__(256) void norm_rotate(const NormArgs p) {
 #pragma unroll
         for (int n = 0; n < AT_ONCE; ++n) {
             const int i = min(i0 + n * subs, heads - 1);
-            token[n] = i / p.H;
+            token[n] = quotient(i, per_head);
             head[n] = i - token[n] * p.H;
-            const uint32_t l = l0 + token[n], rows = l / (uint32_t)p.L;
-            const T *src = (const T *)p.x + (b0 + rows) * p.x_b +
-                           (int64_t)(l - rows * p.L) * p.x_l + head[n] * p.x_h;
+            const At at(p, b0, l0, token[n]);
+            const T *src =
+                (const T *)p.x + at.b * p.x_b + (int64_t)at.l * p.x_l + head[n] * p.x_h;
 #pragma unroll
             for (int k = 0; k < K; ++k)
                 read<T, V>(a[n][k], b[n][k], src, item[k]);
@@ -286,6 +327,7 @@ __global__ __launch_bounds__(256) void norm_rotate_backward(const NormArgs p) {
     }
     const float share = 1.f / p.D;
     const int head0 = p.first_head[row], n_heads = p.first_head[row + 1] - head0;
+    const float per_head = 1.f / n_heads;
     const int blocks = p.first_block[row + 1] - p.first_block[row];
     for (int64_t first = (int64_t)(blockIdx.x - p.first_block[row]) * p.per_block;
          first < p.tokens; first += (int64_t)blocks * p.per_block) {
@@ -297,11 +339,12 @@ __global__ __launch_bounds__(256) void norm_rotate_backward(const NormArgs p) {
         __syncthreads();
         const int heads = tokens * n_heads;
         for (int i = sub; i < heads; i += subs) {
-            const int token = i / n_heads, head = head0 + i - token * n_heads;
-            const uint32_t l = l0 + token, rows = l / (uint32_t)p.L;
-            const int64_t b = b0 + rows, at = l - rows * p.L;
-            const T *src = (const T *)p.x + b * p.x_b + at * p.x_l + head * p.x_h;
-            const T *grad = (const T *)p.dout + b * p.do_b + at * p.do_l + head * p.do_h;
+            const int token = quotient(i, per_head), head = head0 + i - token * n_heads;
+            const At at(p, b0, l0, token);
+            const T *src =
+                (const T *)p.x + at.b * p.x_b + (int64_t)at.l * p.x_l + head * p.x_h;
+            const T *grad =
+                (const T *)p.dout + at.b * p.do_b + (int64_t)at.l * p.do_l + head * p.do_h;
             fv<V> xa[K], xb[K], ga[K], gb[K];
 #pragma unroll
             for (int k = 0; k < K; ++k) {
@@ -371,9 +414,22 @@ __global__ __launch_bounds__(32 * kJoinCols) void norm_join(const NormArgs p, W 
     const int row = blockIdx.x / per_row, col = threadIdx.x % kJoinCols;
     const int d = blockIdx.x % per_row * kJoinCols + col, lane = threadIdx.x / kJoinCols;
     float sum = 0.f;
-    if (d < p.D)
-        for (int b = p.first_block[row] + lane; b < p.first_block[row + 1]; b += 32)
-            sum += p.part[(int64_t)b * p.D + d];
+    if (d < p.D) {
+        const float *from = p.part + d;
+        int b = p.first_block[row] + lane;
+        const int end = p.first_block[row + 1];
+        for (; b + 7 * 32 < end; b += 8 * 32) { // eight on their way
+            float x[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                x[n] = from[(int64_t)(b + 32 * n) * p.D];
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                sum += x[n];
+        }
+        for (; b < end; b += 32)
+            sum += from[(int64_t)b * p.D];
+    }
     sums[lane][col] = sum;
     __syncthreads();
     if (lane == 0 && d < p.D) {
@@ -407,7 +463,7 @@ int prepare(const tm_norm_rotation *n, NormArgs &p) {
     if (heads != r.H)
         return TM_ERR_INVALID_ARGUMENT;
     p.first_head[n->groups] = (int32_t)heads;
-    if (r.D > TM_NORM_MAX_HEAD_DIM || (int64_t)r.H * r.D > (1 << 24))
+    if (r.D > TM_NORM_MAX_HEAD_DIM || r.H > TM_NORM_MAX_HEADS)
         return TM_ERR_UNSUPPORTED_SHAPE;
     p.x = r.x, p.weight = n->weight, p.weight_f32 = n->weight_type == TM_F32;
     p.x_b = r.x_b, p.x_l = r.x_l, p.x_h = r.x_h;
@@ -476,7 +532,7 @@ void deal_blocks(NormArgs &p) {
     for (int g = 0; g < p.groups; ++g) {
         const int64_t heads = p.first_head[g + 1] - p.first_head[g];
         p.first_block[g] = (int32_t)at;
-        at += std::max<int64_t>(1, std::min(most, (2048 * heads + p.H - 1) / p.H));
+        at += std::max<int64_t>(1, std::min(most, (kBlocks * heads + p.H - 1) / p.H));
     }
     p.first_block[p.groups] = (int32_t)at;
 }
@@ -491,7 +547,7 @@ int per_block(const NormArgs &p, int64_t heads, int64_t at_once) {
     per = std::max(per, (p.tokens + most - 1) / most);
     if (p.at.pairs)
         per = std::min<int64_t>(per, kTable / p.at.pairs);
-    return (int)std::min<int64_t>(per, 4096);
+    return (int)std::min<int64_t>(per, kMaxPiece / p.H);
 }
 
 int backward_sizes(NormArgs &p) {
@@ -529,7 +585,7 @@ extern "C" size_t tm_norm_rotate_backward_workspace_bytes(const tm_norm_rotation
     if (prepare(n, p) || !p.tokens)
         return 0;
     // an upper bound for either width of loads
-    return ((size_t)2048 + 2 * p.groups) * p.D * sizeof(float);
+    return ((size_t)kBlocks + 2 * p.groups) * p.D * sizeof(float);
 }
 
 extern "C" int tm_norm_rotate_backward(const tm_norm_rotation *n, const void *dout, int64_t do_b,

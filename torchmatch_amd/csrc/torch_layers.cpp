@@ -29,7 +29,8 @@ struct Normed {
            at::IntArrayRef sections, at::IntArrayRef heads, double eps, bool interleaved)
         : t("norm_rotate", x, positions, freqs, sections, interleaved, false) {
         const int64_t H = x.size(2), D = x.size(3);
-        TORCH_CHECK_VALUE(H >= 1, "norm_rotate: x must have a head, got ", x.sizes());
+        TORCH_CHECK_VALUE(H >= 1 && H <= TM_NORM_MAX_HEADS, "norm_rotate: x must have 1 to ",
+                          (int)TM_NORM_MAX_HEADS, " heads, got ", x.sizes());
         TORCH_CHECK_VALUE(D <= TM_NORM_MAX_HEAD_DIM, "norm_rotate: heads hold 1 to ",
                           (int)TM_NORM_MAX_HEAD_DIM, " features, got ", D);
         TORCH_CHECK_VALUE(eps >= 0. && (float)eps <= 3e38f,
@@ -190,9 +191,16 @@ int activation_code(c10::string_view name) {
 Tensor rows_of(const Tensor &t) {
     const int64_t n = t.size(-1), unit = 16 / t.element_size();
     const Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / n, n});
-    if (n % unit)
-        return at::constant_pad_nd(r, {0, unit - n % unit}).contiguous();
     const int64_t l = step_of(r, 0);
+    if (n % unit) {
+        const Tensor t1 = n == 1 || r.stride(1) == 1 ? r : r.contiguous();
+        Tensor padded = at::empty({r.size(0), (n + unit - 1) / unit * unit}, r.options());
+        check_rc(tm_pad_rows(t1.const_data_ptr(), step_of(t1, 0), r.size(0), (int32_t)n,
+                             dtype_code(r, "feed_forward", "x"), padded.data_ptr(),
+                             current_stream(r)),
+                 "feed_forward");
+        return padded;
+    }
     const bool ok = (n == 1 || r.stride(1) == 1) && l % unit == 0 && (l == 0 || l >= n) &&
                     l * r.element_size() < TM_FF_MAX_ROW_BYTES &&
                     reinterpret_cast<uintptr_t>(r.const_data_ptr()) % 16 == 0;
