@@ -30,41 +30,53 @@ int64_t hidden_bytes(const tm_feed_forward &f) { // (T, hidden) of the inputs' t
     return ((int64_t)f.T * hidden_row(f) * size_of(f) + 255) / 256 * 256;
 }
 
-// Tiles of a product and how often its k is split.
+// Tiles of a product; the last ones, where they would leave much of the card idle, split over k.
 struct Plan {
     int size;
     bool tokens;
-    int splits, split_steps;
+    int whole, splits, split_steps;
     size_t part; // bytes of partial sums
 };
+// Chosen by the time it takes, in us, as measured on long rows: a step of 128 bytes of k of all the
+// blocks that run at once (16-bit types: 256 large tiles 1.76, 512 small ones 1.02, 256 small ones with four
+// tiles in LDS 0.75; float32 512 small ones 2.85, 256 1.8); 3 for each round's beginning and end;
+// the split tiles' sums are written and read at 3 TB/s, by one launch more, 6.
 Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, int segments,
           int batches) {
     if (M <= ff::kTokens && (kind == ff::kUp || kind == ff::kDown))
-        return {ff::kSmall, true, 1, 0, 0};
-    const int64_t step = 128 / size_of(f);
-    const auto tiles = [&](int64_t t) {
-        return (M + t - 1) / t * ((N + t - 1) / t) * batches * (kind == ff::kUp ? 2 : 1);
-    };
-    // rounds of blocks times a block's work, in tiles of 128 x 128: 256 blocks of the large tiles
-    // run at once, 512 of the small ones, which take a sixth longer for their share
-    const int64_t large = tiles(256), small = tiles(128);
-    const double t_large = (double)((large + 255) / 256) * 4.;
-    const double t_small = (double)((small + 511) / 512) * 2. * 7. / 6.;
-    Plan r = {f.dtype != TM_F32 && t_large <= t_small ? ff::kLarge : ff::kSmall, false, 1, 0, 0};
-    const int64_t steps = (K + step - 1) / step * segments;
-    const bool may = kind == ff::kDown || kind == ff::kInput || kind == ff::kWeights;
-    if (may && r.size == ff::kSmall && small < 384)
-        r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(1, small),
-                                                               steps / 8));
-    r.split_steps = (int)((steps + r.splits - 1) / r.splits);
-    if (r.split_steps)
-        r.splits = (int)((steps + r.split_steps - 1) / r.split_steps);
-    r.splits = std::max(r.splits, 1);
-    if (r.size == ff::kSmall && small * r.splits <= 256) // one block a compute unit at most
-        r.size = ff::kDeep;
-    if (r.splits > 1)
-        r.part = (size_t)r.splits * batches * M * N * sizeof(float);
-    return r;
+        return {ff::kSmall, true, 0, 1, 0, 0};
+    const int64_t k = 128 / size_of(f), steps = (K + k - 1) / k * segments;
+    Plan best = {};
+    double least = 0.;
+    for (int size : {ff::kSmall, ff::kDeep, ff::kLarge}) {
+        if (size == ff::kLarge && f.dtype == TM_F32)
+            continue;
+        const int64_t t = size == ff::kLarge ? 256 : 128, tn = kind == ff::kUp ? t / 2 : t;
+        const int64_t tiles = (M + t - 1) / t * ((N + tn - 1) / tn) * batches;
+        const int64_t at_once = size == ff::kSmall ? 512 : 256;
+        const double step = f.dtype == TM_F32 ? (size == ff::kDeep ? 1.8 : 2.85)
+                            : size == ff::kLarge ? 1.76
+                            : size == ff::kDeep  ? 0.75
+                                                 : 1.02;
+        const int64_t rounds = tiles / at_once, rest = tiles - rounds * at_once;
+        if (size == ff::kDeep && tiles > at_once) // without a second block ends are not hidden either
+            continue;
+        for (int64_t splits = 1; splits <= 64; ++splits) {
+            if (splits > 1 && (!rest || rest * splits > at_once || steps < 8 * splits))
+                break;
+            const int64_t split_steps = (steps + splits - 1) / splits;
+            const double bytes = splits > 1 ? (double)rest * splits * t * t * 4 : 0.;
+            const double time = step * (rounds * steps + (rest ? split_steps : 0)) +
+                                3. * (rounds + (rest > 0)) +
+                                (splits > 1 ? 6. + 2. * bytes / 3e6 : 0.);
+            if (best.splits == 0 || time < least) {
+                least = time;
+                best = {size, false, (int)(splits > 1 ? rounds * at_once : tiles), (int)splits,
+                        (int)split_steps, (size_t)bytes};
+            }
+        }
+    }
+    return best;
 }
 
 Plan plan_up(const tm_feed_forward &f) { return plan(f, ff::kUp, f.T, f.F, f.C, 1, 1); }
@@ -100,9 +112,8 @@ int check(const tm_feed_forward *f) {
 
 int product(const tm_feed_forward &f, Args p, Kind kind, const Plan &how, void *part,
             hipStream_t stream) {
-    p.splits = how.splits;
-    p.split_steps = how.split_steps;
-    p.part = how.part ? (float *)part : nullptr;
+    p.whole = how.whole, p.splits = how.splits, p.split_steps = how.split_steps;
+    p.part = (float *)part;
     p.activation = f.activation;
     if (how.tokens) {
         const auto tokens = f.dtype == TM_BF16  ? ff::tokens_bf16
@@ -113,12 +124,7 @@ int product(const tm_feed_forward &f, Args p, Kind kind, const Plan &how, void *
     const auto run = f.dtype == TM_BF16  ? ff::product_bf16
                      : f.dtype == TM_F16 ? ff::product_f16
                                          : ff::product_f32;
-    const auto join = f.dtype == TM_BF16  ? ff::join_bf16
-                      : f.dtype == TM_F16 ? ff::join_f16
-                                          : ff::join_f32;
-    if (run(p, kind, how.size, stream) || (p.part && join(p, stream)))
-        return TM_ERR_LAUNCH;
-    return TM_OK;
+    return run(p, kind, how.size, stream) ? TM_ERR_LAUNCH : TM_OK;
 }
 
 Args args(int64_t M, int64_t N, int64_t K) {
@@ -217,7 +223,7 @@ extern "C" size_t tm_feed_forward_saved_bytes(const tm_feed_forward *f) {
 extern "C" size_t tm_feed_forward_workspace_bytes(const tm_feed_forward *f) {
     if (check(f) || !f->T)
         return 0;
-    return hidden_bytes(*f) + plan_down(*f).part;
+    return hidden_bytes(*f) + std::max(plan_up(*f).part, plan_down(*f).part);
 }
 
 extern "C" int tm_feed_forward_forward(const tm_feed_forward *f, void *out, void *saved,
@@ -239,20 +245,22 @@ extern "C" int tm_feed_forward_forward(const tm_feed_forward *f, void *out, void
     p.out[0] = h, p.out_l = hidden_row(*f);
     if (saved)
         set_saved(*f, p, saved);
-    if (const int rc = product(*f, p, ff::kUp, plan_up(*f), nullptr, stream))
+    char *part = (char *)workspace + hidden_bytes(*f);
+    if (const int rc = product(*f, p, ff::kUp, plan_up(*f), part, stream))
         return rc;
     p = args(f->T, f->O, f->F);
     p.a[0] = h, p.a_l = hidden_row(*f);
     p.b[0] = f->down, p.b_l = f->down_l;
     p.out[0] = out, p.out_l = f->O, p.wide = wide(*f, out, f->O);
-    return product(*f, p, ff::kDown, plan_down(*f), (char *)workspace + hidden_bytes(*f), stream);
+    return product(*f, p, ff::kDown, plan_down(*f), part, stream);
 }
 
 extern "C" size_t tm_feed_forward_backward_workspace_bytes(const tm_feed_forward *f) {
     if (check(f))
         return 0;
     return ff::kMostParts * sizeof(float) + 2 * hidden_bytes(*f) +
-           std::max({plan_input(*f).part, plan_weights(*f).part, plan_output(*f).part});
+           std::max({plan_hidden(*f).part, plan_input(*f).part, plan_weights(*f).part,
+                     plan_output(*f).part});
 }
 
 extern "C" int tm_feed_forward_backward(const tm_feed_forward *f, const void *saved,
@@ -292,7 +300,7 @@ extern "C" int tm_feed_forward_backward(const tm_feed_forward *f, const void *sa
         p.da = da, p.db = db, p.out_l = hidden_row(*f);
         p.most = scaled ? most : nullptr;
         set_saved(*f, p, saved);
-        if (const int rc = product(*f, p, ff::kHidden, plan_hidden(*f), nullptr, stream))
+        if (const int rc = product(*f, p, ff::kHidden, plan_hidden(*f), part, stream))
             return rc;
         if (dx) {
             p = args(f->T, f->C, f->F);

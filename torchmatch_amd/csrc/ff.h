@@ -20,9 +20,10 @@ struct Args {
     void *saved[3];
     void *da, *db;      // hidden: gradients of a and b, rows of out_l
     const float *most;  // kMostParts maxima of |dy|, or null: no scale
-    float *part;        // (splits, batches, M, N) sums, or null
+    float *part;        // sums of the tiles that are split
     int32_t M, N, K;    // K: of one segment
-    int32_t segments, batches, splits, split_steps;
+    int32_t segments, batches;
+    int32_t whole, splits, split_steps; // tiles that are not split; the other ones' blocks
     int32_t activation, wide; // wide: out rows are at multiples of 16 bytes
 };
 
@@ -36,8 +37,7 @@ constexpr int kTokens = 64;
 // Non-zero: a launch failed.
 #define FF_DECLARE(type)                                                                         \
     int product_##type(const Args &, Kind, int size, hipStream_t);                               \
-    int tokens_##type(const Args &, Kind, hipStream_t);                                          \
-    int join_##type(const Args &, hipStream_t);
+    int tokens_##type(const Args &, Kind, hipStream_t);
 FF_DECLARE(bf16)
 FF_DECLARE(f16)
 FF_DECLARE(f32)

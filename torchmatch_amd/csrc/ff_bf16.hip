@@ -9,6 +9,5 @@ int product_bf16(const Args &p, Kind kind, int size, hipStream_t stream) {
 int tokens_bf16(const Args &p, Kind kind, hipStream_t stream) {
     return run_tokens<__bf16>(p, kind, stream);
 }
-int join_bf16(const Args &p, hipStream_t stream) { return run_join<__bf16>(p, stream); }
 
 } // namespace ff

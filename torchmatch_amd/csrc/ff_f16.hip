@@ -9,6 +9,5 @@ int product_f16(const Args &p, Kind kind, int size, hipStream_t stream) {
 int tokens_f16(const Args &p, Kind kind, hipStream_t stream) {
     return run_tokens<_Float16>(p, kind, stream);
 }
-int join_f16(const Args &p, hipStream_t stream) { return run_join<_Float16>(p, stream); }
 
 } // namespace ff

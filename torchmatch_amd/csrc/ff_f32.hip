@@ -9,6 +9,5 @@ int product_f32(const Args &p, Kind kind, int size, hipStream_t stream) {
 int tokens_f32(const Args &p, Kind kind, hipStream_t stream) {
     return run_tokens<float>(p, kind, stream);
 }
-int join_f32(const Args &p, hipStream_t stream) { return run_join<float>(p, stream); }
 
 } // namespace ff

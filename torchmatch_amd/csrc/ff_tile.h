@@ -331,19 +331,7 @@ template <typename T> __device__ inline int grad_up(const Args &p, int lane) {
 
 // One row's 8 results from column n on.
 template <typename T>
-__device__ inline void put_row(const Args &p, int batch, int split, int64_t m, int n, f32x8 x) {
-    if (p.part) {
-        float *to = p.part + (((int64_t)split * p.batches + batch) * p.M + m) * p.N + n;
-        if (p.N % 4 == 0 && n + 8 <= p.N) {
-            put<float, 8>(to, x);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (n + j < p.N)
-                    to[j] = x[j];
-        }
-        return;
-    }
+__device__ inline void put_row(const Args &p, int batch, int64_t m, int n, f32x8 x) {
     T *to = (T *)p.out[batch] + m * p.out_l + n;
     if (p.wide && n + 8 <= p.N) {
         put<T, 8>(to, x);
@@ -465,9 +453,13 @@ template <> struct Size<kUp, kLarge> {
     static constexpr int WM = 4, WN = 2, MB = 2, NB = 4, TILES = 2;
 };
 
-template <typename T, Kind KIND, int SIZE>
-__global__ __launch_bounds__((64 * Size<KIND, SIZE>::WM * Size<KIND, SIZE>::WN),
-                             (SIZE == kDeep ? 1 : 2)) void
+// The first p.whole tiles are a block's each; the k of every other one is split over p.splits blocks, which
+// leave their sums in p.part as they lie in their registers.  JOIN: adds these, in order, and
+// does with them what is done with a whole tile's; a block of one wave for 32 rows of one
+// wave's (as many splits' sums come by fast only where many ask for them).
+template <typename T, Kind KIND, int SIZE, bool JOIN>
+__global__ __launch_bounds__((JOIN ? 64 : 64 * Size<KIND, SIZE>::WM * Size<KIND, SIZE>::WN),
+                             (SIZE == kDeep || JOIN ? 1 : 2)) void
 product(const Args p) {
     using Z = Size<KIND, SIZE>;
     constexpr int MB = Z::MB, NB = Z::NB, BM = 32 * MB * Z::WM, BN = 32 * NB * Z::WN;
@@ -479,18 +471,32 @@ product(const Args p) {
     using FB = Feed<T, BN, Shape<KIND>::kB, NT, GATED ? HALF : 0>;
     // Apart, so that the compiler sees that a tile on its way is not the one that is read.
     constexpr int TILES = Z::TILES, LOADS = FA::N + FB::N; // a thread's, of a tile
-    __shared__ u32x4 a0[FA::SIZE], a1[FA::SIZE], b0[FB::SIZE], b1[FB::SIZE];
-    __shared__ u32x4 a2[TILES > 2 ? FA::SIZE : 1], a3[TILES > 2 ? FA::SIZE : 1],
-        b2[TILES > 2 ? FB::SIZE : 1], b3[TILES > 2 ? FB::SIZE : 1];
+    constexpr int ROW = 8 * NB, PER = FA::SIZE / (32 * ROW); // see the end
+    __shared__ u32x4 a0[JOIN ? 32 * ROW : FA::SIZE], a1[JOIN ? 1 : FA::SIZE],
+        b0[JOIN ? 1 : FB::SIZE], b1[JOIN ? 1 : FB::SIZE];
+    constexpr bool MORE = TILES > 2 && !JOIN;
+    __shared__ u32x4 a2[MORE ? FA::SIZE : 1], a3[MORE ? FA::SIZE : 1], b2[MORE ? FB::SIZE : 1],
+        b3[MORE ? FB::SIZE : 1];
 
-    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5;
-    const int wave = attn::scalar(tid >> 6), wm = wave / Z::WN, wn = wave % Z::WN;
+    constexpr int WAVES = Z::WM * Z::WN;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const int wave = JOIN ? (int)blockIdx.x / MB % WAVES : attn::scalar(threadIdx.x >> 6);
+    const int tid = 64 * wave + lane, wm = wave / Z::WN, wn = wave % Z::WN;
     const int mt = (p.M + BM - 1) / BM, nt = (p.N + TN - 1) / TN;
     // tiles in bands of 8 rows of tiles, a run of them an XCD: those which share operands meet
     // in its L2
-    int id = attn::xcd_order(blockIdx.x, gridDim.x);
-    const int split = id % p.splits;
-    id /= p.splits;
+    int id, split = 0, tail = -1;
+    if (JOIN) {
+        tail = blockIdx.x / (MB * WAVES);
+        id = p.whole + tail;
+    } else if ((int)blockIdx.x < p.whole) {
+        id = attn::xcd_order(blockIdx.x, p.whole);
+    } else {
+        id = attn::xcd_order(blockIdx.x - p.whole, gridDim.x - p.whole);
+        split = id % p.splits;
+        tail = id / p.splits;
+        id = p.whole + tail;
+    }
     const int batch = id / (mt * nt);
     id -= batch * mt * nt;
     const int band = id / (8 * nt), in_band = id - band * 8 * nt;
@@ -502,7 +508,8 @@ product(const Args p) {
     fa.start(tid, p.a_l, p.M - m0);
     fb.start(tid, p.b_l, p.N - n0);
     const int spk = (p.K + BK - 1) / BK; // steps a segment
-    const int s0 = split * p.split_steps, s1 = min(s0 + p.split_steps, spk * p.segments);
+    const int steps = spk * p.segments, s0 = split * p.split_steps;
+    const int s1 = tail < 0 ? steps : min(s0 + p.split_steps, steps);
     const uint32_t at_a = FA::lane_at(lane), at_b = FB::lane_at(lane);
 
     // the tiles' first elements at k = 0, of either segment; gated: of gate and up
@@ -595,7 +602,7 @@ product(const Args p) {
 #pragma unroll
     for (int i = 0; i < NB; ++i)
         y1[i] = {};
-    if (s0 < s1) {
+    if (!JOIN && s0 < s1) {
         const auto first = [&](int s, u32x4 *ta, u32x4 *tb) {
             fetch(s, ta, tb);
             fetch_rest(s, ta, tb);
@@ -607,7 +614,7 @@ product(const Args p) {
         }
         meet<(TILES - 2) * LOADS>();
     }
-    for (int s = s0; s < s1; s += TILES) {
+    for (int s = JOIN ? s1 : s0; s < s1; s += TILES) {
         if constexpr (TILES == 2) {
             step(s, a0, b0, a1, b1);
             if (s + 1 < s1)
@@ -622,7 +629,33 @@ product(const Args p) {
                 step(s + 3, a3, b3, a2, b2);
         }
     }
-    multiply<T>(y1, x1, acc);
+    if constexpr (!JOIN)
+        multiply<T>(y1, x1, acc);
+    // where a split tile's sums lie, 16 bytes of each thread in turn
+    constexpr int SUMS = 16 * NB * MB * NT * 4; // bytes of a tile's
+    const int tails =
+        JOIN ? (int)gridDim.x / (MB * WAVES) : (int)(gridDim.x - p.whole) / p.splits;
+    const uint32_t mine = 16u * tid;
+    char *sums = (char *)p.part + ((int64_t)split * tails + tail) * SUMS;
+    const int first = JOIN ? (int)blockIdx.x % MB : 0, last = JOIN ? first + 1 : MB;
+    if constexpr (JOIN) {
+        sums += first * (4 * NB * 16 * NT);
+#pragma unroll 4
+        for (int n = 0; n < p.splits; ++n) {
+            const char *from = sums + (int64_t)n * tails * SUMS;
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const f32x4 x = *(const f32x4 *)(from + mine);
+                    from += 16 * NT;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[i][0][4 * q + e] += x[e];
+                }
+        }
+    }
+    const bool leave = !JOIN && tail >= 0;
 
     const int up = KIND == kHidden || KIND == kInput || KIND == kWeights ? grad_up<T>(p, lane) : 0;
     const float down = __builtin_ldexpf(1.f, -up);
@@ -630,41 +663,50 @@ product(const Args p) {
     // A wave's rows, 32 at a time, through LDS: what was a lane's column becomes rows.  Units of 16
     // bytes are permuted by the row, so that rows meet other banks.
     __syncthreads();
-    constexpr int ROW = 8 * NB, PER = FA::SIZE / (32 * ROW); // units a row; waves a buffer
-    static_assert(FA::SIZE == FB::SIZE && 4 * PER >= Z::WM * Z::WN);
-    f32x4 *turn = (f32x4 *)(wave / PER == 0 ? a0 : wave / PER == 1 ? a1 : wave / PER == 2 ? b0 : b1) +
-                  wave % PER * 32 * ROW;
+    // ROW units a row, PER waves a buffer
+    static_assert(FA::SIZE == FB::SIZE && 4 * PER >= WAVES);
+    const int place = JOIN ? 0 : wave / PER;
+    f32x4 *turn = (f32x4 *)(place == 0 ? a0 : place == 1 ? a1 : place == 2 ? b0 : b1) +
+                  (JOIN ? 0 : wave % PER * 32 * ROW);
     // a lane has 8 columns of PARTS rows of 32
     constexpr int LANES = (GATED ? HALF : 32 * NB) / 8, PARTS = LANES / 2;
     const int row = lane / LANES, col = lane % LANES * 8;
     const int n = n0 + (GATED ? HALF : 32 * NB) * wn + col;
     const bool here = n < (GATED || KIND == kHidden ? p.out_l : (int64_t)p.N);
-    const int mw = m0 + 32 * MB * wm + row;
+    const int mw = m0 + 32 * (MB * wm + first) + row;
     Saved<T> kept[KIND == kHidden ? PARTS : 1]; // sent for 32 rows ahead
     if constexpr (KIND == kHidden) {
 #pragma unroll
         for (int k = 0; k < PARTS; ++k) {
             const int m = mw + 64 / LANES * k;
-            if (m < p.M && here)
+            if (m < p.M && here && !leave)
                 kept[k].load(p, m * p.out_l + n);
         }
     }
     // one copy of what follows: the sums move up in the registers
 #pragma unroll 1
-    for (int j = 0; j < MB; ++j) {
+    for (int j = first; j < last; ++j) {
         attn::wave_fence();
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                turn[(lane & 31) * ROW + ((8 * i + 2 * q + half) ^ (lane & 15))] =
-                    (f32x4){acc[i][0][4 * q], acc[i][0][4 * q + 1], acc[i][0][4 * q + 2],
-                            acc[i][0][4 * q + 3]};
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 x = {acc[i][0][4 * q], acc[i][0][4 * q + 1], acc[i][0][4 * q + 2],
+                                 acc[i][0][4 * q + 3]};
+                if (leave) {
+                    *(f32x4 *)(sums + mine) = x;
+                    sums += 16 * NT;
+                    continue;
+                }
+                turn[(lane & 31) * ROW + ((8 * i + 2 * q + half) ^ (lane & 15))] = x;
+            }
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
             for (int k = 0; k + 1 < MB; ++k)
                 acc[i][k] = acc[i][k + 1];
+        if (leave)
+            continue;
         attn::wave_fence();
         const auto read8 = [&](int r, int c) {
             const f32x4 lo = turn[r * ROW + ((c >> 2) ^ (r & 15))];
@@ -673,52 +715,33 @@ product(const Args p) {
         };
 #pragma unroll
         for (int k = 0; k < PARTS; ++k) {
-            const int r = row + 64 / LANES * k, m = mw + 32 * j + 64 / LANES * k;
+            const int r = row + 64 / LANES * k, m = mw + 32 * (j - first) + 64 / LANES * k;
             if (m < p.M && here) {
                 if constexpr (GATED) {
                     put_hidden<T, 8>(p, m, n, read8(r, col), read8(r, col + HALF));
                 } else if constexpr (KIND == kHidden) {
                     put_grads<T>(p, m, n, read8(r, col), kept[k], up);
-                    if (j + 1 < MB && m + 32 < p.M)
+                    if (j + 1 < last && m + 32 < p.M)
                         kept[k].load(p, (m + 32) * p.out_l + n);
                 } else {
-                    put_row<T>(p, batch, split, m, n, read8(r, col) * down);
+                    put_row<T>(p, batch, m, n, read8(r, col) * down);
                 }
             }
         }
     }
 }
 
-// The sums of a split product, in order, 4 columns a thread where rows allow it.
-template <typename T> __global__ __launch_bounds__(256) void join(const Args p) {
-    const int64_t count = (int64_t)p.batches * p.M * p.N;
-    const int v = p.N % 4 ? 1 : 4;
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * v;
-    if (i >= count)
-        return;
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s) {
-        if (v == 4)
-            sum += *(const f32x4 *)(p.part + s * count + i);
-        else
-            sum[0] += p.part[s * count + i];
-    }
-    const int64_t row = i / p.N, batch = row / p.M;
-    T *to = (T *)p.out[batch] + (row - batch * p.M) * p.out_l + (i - row * p.N);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (j < v)
-            to[j] = (T)sum[j];
-}
-
 template <typename T, Kind KIND, int SIZE> int launch(const Args &p, hipStream_t stream) {
     using Z = Size<KIND, SIZE>;
     constexpr int BM = 32 * Z::MB * Z::WM, TN = (KIND == kUp ? 16 : 32) * Z::NB * Z::WN;
-    const int64_t blocks = (int64_t)((p.M + BM - 1) / BM) * ((p.N + TN - 1) / TN) * p.batches *
-                           p.splits;
+    const int64_t tiles = (int64_t)((p.M + BM - 1) / BM) * ((p.N + TN - 1) / TN) * p.batches;
+    const int64_t blocks = p.whole + (tiles - p.whole) * p.splits;
     if (!blocks)
         return 0;
-    product<T, KIND, SIZE><<<dim3((unsigned)blocks), 64 * Z::WM * Z::WN, 0, stream>>>(p);
+    product<T, KIND, SIZE, false><<<dim3((unsigned)blocks), 64 * Z::WM * Z::WN, 0, stream>>>(p);
+    if (tiles > p.whole)
+        product<T, KIND, SIZE == kDeep ? kSmall : SIZE, true> // their sums lie alike
+            <<<dim3((unsigned)(tiles - p.whole) * Z::MB * Z::WM * Z::WN), 64, 0, stream>>>(p);
     return hipGetLastError() != hipSuccess;
 }
 
@@ -738,14 +761,6 @@ template <typename T> int run(const Args &p, Kind kind, int size, hipStream_t st
     case kInput: return launch_size<T, kInput>(p, size, stream);
     default: return launch_size<T, kWeights>(p, size, stream);
     }
-}
-
-template <typename T> int run_join(const Args &p, hipStream_t stream) {
-    const int64_t count = (int64_t)p.batches * p.M * p.N / (p.N % 4 ? 1 : 4);
-    if (!count)
-        return 0;
-    join<T><<<dim3((unsigned)((count + 255) / 256)), 256, 0, stream>>>(p);
-    return hipGetLastError() != hipSuccess;
 }
 
 } // namespace ff

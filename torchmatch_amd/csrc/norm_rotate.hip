@@ -31,7 +31,7 @@ template <int V> using fv = typename Floats<V>::type;
 
 constexpr int kMaxPiece = 1 << 21; // heads of a block's tokens at a time: see quotient()
 constexpr int kMaxItems = 8;  // a lane's, of one head
-constexpr int kBlocks = 1024; // of a backward pass, about
+constexpr int kBlocks = 2048; // of a backward pass, about
 constexpr int kJoinCols = 32; // columns of dw a block of norm_join
 
 struct NormArgs {
