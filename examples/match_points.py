@@ -1,10 +1,11 @@
 """A small matching network end to end: attention, then transport, then assignment.
 
 Two sets of points with noisy descriptors are matched.  Both sets of every pair lie in one
-row of a packed batch: the points' features are turned by their image coordinates
-(``attention.rotate``), each set attends to itself with a bias by distance and then to the
-other one (``attention.attend``, documents keep pairs apart), and the products of the features
-are the scores.  Training follows the negative log of a softmax over rows and columns;
+row of a packed batch: the points' queries and keys are normed and turned by their image
+coordinates (``attention.norm_rotate``), each set attends to itself with a bias by distance and
+then to the other one (``attention.attend``, documents keep pairs apart), a gated feed-forward block
+follows (``attention.feed_forward``), each added with dropout (``attention.dropout``), and the
+products of the features are the scores.  Training follows the negative log of a softmax over rows and columns;
 matching solves the transport problem on the scores (``transport.matrix.solve``) and rounds
 its plan to a one-to-one mapping (``assignment.solve``).
 
@@ -25,7 +26,8 @@ sys.path.insert(0, str(Path(__file__).resolve().parents[1]))
 from torchmatch_amd import assignment, attention, transport  # noqa: E402
 
 HEADS, HEAD_DIM, SECTIONS = 4, 32, (8, 8)
-WIDTH = HEADS * HEAD_DIM
+WIDTH, HIDDEN = HEADS * HEAD_DIM, 192
+DROPOUT = 0.02
 
 
 class Block(nn.Module):
@@ -37,24 +39,33 @@ class Block(nn.Module):
         self.qkv = nn.Linear(WIDTH, 3 * WIDTH)
         self.q, self.kv = nn.Linear(WIDTH, WIDTH), nn.Linear(WIDTH, 2 * WIDTH)
         self.out_self, self.out_cross = nn.Linear(WIDTH, WIDTH), nn.Linear(WIDTH, WIDTH)
-        self.mlp = nn.Sequential(nn.Linear(WIDTH, 2 * WIDTH), nn.GELU(),
-                                 nn.Linear(2 * WIDTH, WIDTH))
+        # of queries and of keys; their products may be large where the network is sure
+        self.qk_weight = nn.Parameter(torch.ones(2, HEAD_DIM))
+        self.gate, self.up = (nn.Linear(WIDTH, HIDDEN, bias=False) for _ in range(2))
+        self.down = nn.Linear(HIDDEN, WIDTH, bias=False)
 
-    def forward(self, x, other, pos, docs, other_docs, slopes, freqs):
+    def add(self, x, y, seed, place):
+        """x and what y leaves after dropout; ``place`` tells masks of one step apart."""
+        return attention.dropout(y, DROPOUT if self.training else 0.0, seed, place, residual=x)
+
+    def forward(self, x, other, pos, docs, other_docs, slopes, freqs, seed, place):
         """``x``: (1, rows, WIDTH) of one side; ``other``: the other side's features."""
         rows = x.shape[1]
         qkv = self.qkv(self.norm_self(x)).view(1, rows, 3 * HEADS, HEAD_DIM)
-        # queries and keys lie side by side: one call turns both
-        qk = attention.rotate(qkv[:, :, :2 * HEADS], pos, freqs, SECTIONS)
+        # queries and keys lie side by side: one call norms and turns both
+        qk = attention.norm_rotate(qkv[:, :, :2 * HEADS], self.qk_weight, pos, freqs, SECTIONS,
+                                   heads=(HEADS, HEADS))
         a = attention.attend(qk[:, :, :HEADS], qk[:, :, HEADS:], qkv[:, :, 2 * HEADS:],
                              q_docs=docs, slopes=slopes, q_positions=pos, k_positions=pos)
-        x = x + self.out_self(a.flatten(2))
+        x = self.add(x, self.out_self(a.flatten(2)), seed, place)
         q = self.q(self.norm_cross(x)).view(1, rows, HEADS, HEAD_DIM)
         kv = self.kv(self.norm_cross(other)).view(1, other.shape[1], 2 * HEADS, HEAD_DIM)
         a = attention.attend(q, kv[:, :, :HEADS], kv[:, :, HEADS:], cap=30.0, q_docs=docs,
                              k_docs=other_docs)
-        x = x + self.out_cross(a.flatten(2))
-        return x + self.mlp(self.norm_mlp(x))
+        x = self.add(x, self.out_cross(a.flatten(2)), seed, place + 1)
+        y = attention.feed_forward(self.norm_mlp(x), self.gate.weight, self.up.weight,
+                                   self.down.weight)
+        return self.add(x, y, seed, place + 2)
 
 
 class Matcher(nn.Module):
@@ -68,15 +79,15 @@ class Matcher(nn.Module):
         self.register_buffer("freqs", attention.rotary_frequencies(SECTIONS, device="cpu"))
         self.register_buffer("slopes", 0.5 ** torch.arange(1.0, HEADS + 1))
 
-    def forward(self, left, right, left_pos, right_pos):
+    def forward(self, left, right, left_pos, right_pos, seed=0):
         pairs, n, m = left.shape[0], left.shape[1], right.shape[1]
         ids = torch.arange(pairs, dtype=torch.int32, device=left.device)
         docs_l, docs_r = (ids.repeat_interleave(k)[None] for k in (n, m))
         x, y = (self.embed(t).flatten(0, 1)[None] for t in (left, right))
         pos_l, pos_r = (t.flatten(0, 1)[None] for t in (left_pos, right_pos))
-        for block in self.blocks:
-            x, y = (block(x, y, pos_l, docs_l, docs_r, self.slopes, self.freqs),
-                    block(y, x, pos_r, docs_r, docs_l, self.slopes, self.freqs))
+        for i, block in enumerate(self.blocks):
+            x, y = (block(x, y, pos_l, docs_l, docs_r, self.slopes, self.freqs, seed, 6 * i),
+                    block(y, x, pos_r, docs_r, docs_l, self.slopes, self.freqs, seed, 6 * i + 3))
         x = self.head(x).view(pairs, n, WIDTH)
         y = self.head(y).view(pairs, m, WIDTH)
         return x @ y.transpose(1, 2).contiguous() / WIDTH ** 0.5
@@ -117,7 +128,7 @@ def train(steps: int = 60, pairs: int = 8, points: int = 96, features: int = 16,
     losses = []
     for step in range(steps):
         *batch, truth = sample(pairs, points, features, generator, device)
-        scores = model(*batch)
+        scores = model(*batch, seed=(seed << 32) + step)
         log_p = scores.log_softmax(2) + scores.log_softmax(1)
         loss = -log_p.gather(2, truth[..., None]).mean()
         adam.zero_grad()
@@ -127,6 +138,7 @@ def train(steps: int = 60, pairs: int = 8, points: int = 96, features: int = 16,
         if step % 10 == 0:
             log(f"step {step:3d}  loss {losses[-1]:.3f}")
     *batch, truth = sample(pairs, points, features, generator, device)
+    model.eval()
     with torch.no_grad():
         found = match(model(*batch))
     right = (found == truth).float().mean().item()

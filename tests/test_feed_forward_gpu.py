@@ -73,6 +73,14 @@ def test_large_tiles(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,c,f,o", [(300, 1032, 1000, 2056), (2050, 520, 1030, 1544),
+                                        (4400, 136, 1100, 264), (700, 2049, 264, 2500)])
+def test_split_tiles(device, dtype, rows, c, f, o):
+    """Tiles past a whole number of rounds are split over k and joined, edges among them."""
+    _check(*_inputs(dtype, rows, c, f, o, 18, device))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_few_weights_of_many_rows(device, dtype):
     """The weights' gradients are split over the rows."""
     _check(*_inputs(dtype, (3, 3001), 64, 100, 40, 5, device))

@@ -285,9 +285,10 @@ extern "C" int tm_feed_forward_backward(const tm_feed_forward *f, const void *sa
     char *db = da + hidden_bytes(*f), *part = db + hidden_bytes(*f);
     Args p;
     const bool scaled = f->dtype == TM_F16 && f->T;
-    if (f->T) {
-        if (!f->x || !f->gate || !f->up || !f->down || !saved || (uintptr_t)saved % 16 || !dout)
-            return TM_ERR_INVALID_ARGUMENT;
+    if (f->T && (!f->x || !f->gate || !f->up || !f->down || !saved || (uintptr_t)saved % 16 ||
+                 !dout))
+        return TM_ERR_INVALID_ARGUMENT;
+    if (f->T && (dx || dgate)) { // down's gradient needs h alone, which is saved
         if (scaled) {
             ff_most<<<dim3(ff::kMostParts), 256, 0, stream>>>((const _Float16 *)dout, do_l, f->T,
                                                              f->O, most);
