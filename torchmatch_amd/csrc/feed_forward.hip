@@ -38,7 +38,7 @@ struct Plan {
     size_t part; // bytes of partial sums
 };
 // Chosen by the time it takes, in us, as measured on long rows: a step of 128 bytes of k of all the
-// blocks that run at once (16-bit types: 256 large tiles 1.76, 512 small ones 1.02, 256 small ones with four
+// blocks that run at once (16-bit types: 256 large tiles 1.64, 512 small ones 0.91, 256 small ones with four
 // tiles in LDS 0.75; float32 512 small ones 2.85, 256 1.8); 3 for each round's beginning and end;
 // the split tiles' sums are written and read at 3 TB/s, by one launch more, 6.
 Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, int segments,
@@ -55,9 +55,9 @@ Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, 
         const int64_t tiles = (M + t - 1) / t * ((N + tn - 1) / tn) * batches;
         const int64_t at_once = size == ff::kSmall ? 512 : 256;
         const double step = f.dtype == TM_F32 ? (size == ff::kDeep ? 1.8 : 2.85)
-                            : size == ff::kLarge ? 1.76
+                            : size == ff::kLarge ? 1.64
                             : size == ff::kDeep  ? 0.75
-                                                 : 1.02;
+                                                 : 0.91;
         const int64_t rounds = tiles / at_once, rest = tiles - rounds * at_once;
         if (size == ff::kDeep && tiles > at_once) // without a second block ends are not hidden either
             continue;

@@ -88,7 +88,6 @@ template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
     static constexpr int READS = STRIDED ? 2 : 1; // an operand's (16-bit types)
 
     uint32_t off[N]; // bytes from the tile's first element, its k aside
-    int unit[N];     // not strided: the unit of k
 
     // left: rows (columns) from the tile's first on
     __device__ inline void start(int tid, int64_t stride, int left) {
@@ -97,7 +96,6 @@ template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int r = row + n * STEP, u = pos ^ L::swz(r);
-            unit[n] = u;
             if constexpr (STRIDED) {
                 off[n] = (uint32_t)r * bytes + 16u * min(u, (left - 1) / E);
             } else {
@@ -118,8 +116,10 @@ template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const char *s = of_second(tid, n) ? second : from;
+            uint32_t at = off[n] & mask;
+            asm("" : "+v"(at)); // so that it stays 32 bits beside a scalar address
             __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void *)(s + (off[n] & mask)),
+                (const __attribute__((address_space(1))) void *)(s + at),
                 (__attribute__((address_space(3))) void *)(to + n * NT), 16, 0, 0);
         }
     }
@@ -129,7 +129,8 @@ template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const char *s = of_second(tid, n) ? second : from;
-            const bool real = STRIDED ? tid / L::U + n * STEP < left : unit[n] * E < left;
+            const int r = tid / L::U + n * STEP;
+            const bool real = STRIDED ? r < left : (tid % L::U ^ L::swz(r)) * E < left;
             u32x4 x = {0u, 0u, 0u, 0u};
             if (real)
                 x = *(const u32x4 *)(s + off[n]);
@@ -137,49 +138,69 @@ template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
         }
     }
 
-    // Where a lane reads.
+    // Where a lane reads: a byte offset from which all reads differ by an exclusive or with a constant
+    // and a constant number of rows.
     __device__ static inline uint32_t lane_at(int lane) {
-        if constexpr (!STRIDED) {
-            return L::row_lane(lane);
+        if constexpr (sizeof(T) == 2 && !STRIDED) {
+            return 16u * L::at(lane & 15, lane >> 4);
         } else if constexpr (sizeof(T) == 2) {
-            const int d = (lane & 16) + 4 * (lane & 3);
-            return 16u * L::at(8 * (lane >> 5) + ((lane & 15) >> 2), d >> 3) + 2u * (d & 7);
+            const int d = 4 * (lane & 3);
+            return 16u * L::at(8 * (lane >> 4) + ((lane & 15) >> 2), d >> 3) + 2u * (d & 7);
+        } else if constexpr (!STRIDED) {
+            return L::row_lane(lane);
         } else {
             return 16u * L::at(8 * (lane >> 5), (lane & 31) / E) + 4u * (lane & 3);
         }
     }
-    // An operand: row (column) 32 rb + lane % 32, k 16 c + 8 (lane / 32) + 0 .. 7
+    // An operand of run c: 16-bit types row (column) 16 rb + lane % 16, k 32 c + 8 (lane / 16) + 0 .. 7;
+    // float32 row (column) 32 rb + lane % 32, k 16 c + 8 (lane / 32) + 0 .. 7
     __device__ static inline x8<T> operand(const u32x4 *t, uint32_t at, int rb, int c) {
-        if constexpr (!STRIDED) {
+        if constexpr (sizeof(T) == 2 && !STRIDED) {
+            return *(const x8<T> *)((const char *)t + rb * 16 * L::U * 16 + (at ^ (64u * c)));
+        } else if constexpr (sizeof(T) == 2) {
+            // the transposed read: each 16 lanes load 4 rows of 16 elements (4 a lane) and
+            // each lane gets one column of them
+            const char *from = (const char *)t + 32 * c * L::U * 16;
+            x8<T> r;
+#pragma unroll
+            for (int jj = 0; jj < 2; ++jj) {
+                const char *p = from + 4 * jj * L::U * 16 + (at ^ (32u * rb + 16u * jj));
+                const attn::s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) attn::s16x4 *)p);
+                const attn::x4<T> y = __builtin_bit_cast(attn::x4<T>, x);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    r[4 * jj + j] = y[j];
+            }
+            return r;
+        } else if constexpr (!STRIDED) {
             return L::row8(t, at, 32 * rb, c);
         } else {
             const char *from = (const char *)t + 16 * c * L::U * 16;
             x8<T> r;
-            if constexpr (sizeof(T) == 2) {
-                // the transposed read: each 16 lanes load 4 rows of 16 elements (4 a lane) and
-                // each lane gets one column of them
 #pragma unroll
-                for (int jj = 0; jj < 2; ++jj) {
-                    const char *p = from + 4 * jj * L::U * 16 + (at ^ (64u * rb + 16u * jj));
-                    const attn::s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) attn::s16x4 *)p);
-                    const attn::x4<T> y = __builtin_bit_cast(attn::x4<T>, x);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        r[4 * jj + j] = y[j];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    r[j] = *(const float *)(from + j * L::U * 16 +
-                                            (at ^ (16u * (8 * rb ^ L::swz(j)))));
-            }
+            for (int j = 0; j < 8; ++j)
+                r[j] = *(const float *)(from + j * L::U * 16 +
+                                        (at ^ (16u * (8 * rb ^ L::swz(j)))));
             return r;
         }
     }
 };
 
 // ---- products ---------------------------------------------------------------------
+
+// The matrix cores' products: SIDE x SIDE of the result over K indices.  Sides of 16 take less power
+// than of 32, which bounds long products: 2000 and 1880 TFLOP/s of products alone.
+template <typename T> struct Core {
+    static constexpr int SIDE = sizeof(T) == 2 ? 16 : 32, K = sizeof(T) == 2 ? 32 : 16;
+    using Sum = float __attribute__((ext_vector_type(SIDE * SIDE / 64)));
+};
+__device__ inline f32x4 mma(attn::b16x8 a, attn::b16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ inline f32x4 mma(attn::h16x8 a, attn::h16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
 
 // float32 numbers as sums of three bfloat16 ones of 8 bits each, exactly: six products of these,
 // at sixteen times the rate of float32 ones, leave out 2^-24 of |y x| at most, with
@@ -216,10 +237,10 @@ template <> struct Operand<float> : Parts {
     __device__ inline void made_here() { asm volatile("" : "+v"(hi), "+v"(mid), "+v"(lo)); }
 };
 
-// c[i][j] += y[i] x[j] over 16 k
+// c[i][j] += y[i] x[j] over a run of k
 template <typename T, int NB, int MB>
 __device__ inline void multiply(const Operand<T> (&y)[NB], const Operand<T> (&x)[MB],
-                                f32x16 (&c)[NB][MB]) {
+                                typename Core<T>::Sum (&c)[NB][MB]) {
     if constexpr (sizeof(T) == 4) {
         const auto all = [&](u32x4 Parts::*u, u32x4 Parts::*v) {
 #pragma unroll
@@ -240,7 +261,7 @@ __device__ inline void multiply(const Operand<T> (&y)[NB], const Operand<T> (&x)
         for (int j = 0; j < MB; ++j)
 #pragma unroll
             for (int i = 0; i < NB; ++i)
-                c[i][j] = mma32(y[i].x, x[j].x, c[i][j]);
+                c[i][j] = mma(y[i].x, x[j].x, c[i][j]);
     }
 }
 
@@ -387,22 +408,20 @@ __device__ inline void put_grads(const Args &p, int64_t m, int n, f32x8 dh, cons
 
 // ---- the product ------------------------------------------------------------------
 
-// The order of a tile's instructions: PRODUCTS a run of 16 k, in its first quarter the READS of the next
-// run, so that they are there in time, and in the second half of the first two runs the LOADS of
-// the next tile.  Sent for at once, the loads hold up every wave, later they are late (8192 x 2048
-// of 5632 k: 154 us; loads at once 170, over four runs 166, reads over the whole run 158).
+// The order of a tile's instructions: PRODUCTS a run of k, spread over them the READS of the
+// next run (an operand takes the place of one that was multiplied) and, in the first run from its
+// first quarter on, the LOADS of the next tile.  Sent for at once, the loads hold up every wave, later
+// they are late; reads that end earlier need more registers than there are.
 template <int RUNS, int PRODUCTS, int READS, int LOADS> struct Order {
     template <int R, int I> __device__ static inline void one() {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // matrix products
-        constexpr int FIRST = PRODUCTS / 4, LAST = PRODUCTS / 2, HALF = (LOADS + 1) / 2;
-        if constexpr (I < FIRST)
-            __builtin_amdgcn_sched_group_barrier(
-                0x100, READS * (I + 1) / FIRST - READS * I / FIRST, 0); // reads of LDS
-        if constexpr (R < 2 && I >= PRODUCTS - LAST) {
-            constexpr int J = I - (PRODUCTS - LAST);
-            __builtin_amdgcn_sched_group_barrier(
-                0x020, HALF * (J + 1) / LAST - HALF * J / LAST, 0); // loads from memory
-        }
+        constexpr int reads = READS * (I + 1) / PRODUCTS - READS * I / PRODUCTS;
+        if constexpr (reads > 0)
+            __builtin_amdgcn_sched_group_barrier(0x100, reads, 0); // reads of LDS
+        constexpr int F = PRODUCTS / 4, P = PRODUCTS - F, J = R * PRODUCTS + I - F;
+        constexpr int loads = J >= 0 && J < P ? LOADS * (J + 1) / P - LOADS * J / P : 0;
+        if constexpr (loads > 0)
+            __builtin_amdgcn_sched_group_barrier(0x020, loads, 0); // loads from memory
         if constexpr (I + 1 < PRODUCTS)
             one<R, I + 1>();
         else if constexpr (R + 1 < RUNS)
@@ -443,7 +462,7 @@ template <int LATER> __device__ inline void meet() {
 
 // A block's waves by rows and columns, what each has of the result, in 32 x 32, and the tiles in LDS.
 // Large tiles: one block of eight waves a compute unit, small ones: two of four.  Where there is no
-// second block to hide the waits, four tiles do (128 x 2048 through 5632: ? -> ? us).  The
+// second block to hide the waits, four tiles do (128 x 2048 through 5632: 56 -> 49 us).  The
 // large gated one's waves have 64 columns of either projection, so that rows of 128 bytes are written.
 template <Kind K, int SIZE> struct Size {
     static constexpr int WM = 2, WN = SIZE == kLarge ? 4 : 2, MB = SIZE == kLarge ? 4 : 2, NB = 2;
@@ -463,6 +482,9 @@ __global__ __launch_bounds__((JOIN ? 64 : 64 * Size<KIND, SIZE>::WM * Size<KIND,
 product(const Args p) {
     using Z = Size<KIND, SIZE>;
     constexpr int MB = Z::MB, NB = Z::NB, BM = 32 * MB * Z::WM, BN = 32 * NB * Z::WN;
+    constexpr int PARTS32 = 32 / Core<T>::SIDE; // of the matrix cores' products in 32 rows
+    constexpr int M = PARTS32 * MB, N = PARTS32 * NB;
+    using Sum = typename Core<T>::Sum;
     constexpr int NT = 64 * Z::WM * Z::WN, BK = kStep<T>;
     constexpr bool GATED = KIND == kUp;
     constexpr int TN = GATED ? BN / 2 : BN; // columns of the result a block
@@ -510,7 +532,7 @@ product(const Args p) {
     const int spk = (p.K + BK - 1) / BK; // steps a segment
     const int steps = spk * p.segments, s0 = split * p.split_steps;
     const int s1 = tail < 0 ? steps : min(s0 + p.split_steps, steps);
-    const uint32_t at_a = FA::lane_at(lane), at_b = FB::lane_at(lane);
+    uint32_t at_a = FA::lane_at(lane), at_b = FB::lane_at(lane);
 
     // the tiles' first elements at k = 0, of either segment; gated: of gate and up
     const int64_t off_a = Shape<KIND>::kA ? m0 : m0 * p.a_l, step_a = Shape<KIND>::kA ? p.a_l : 1;
@@ -544,44 +566,38 @@ product(const Args p) {
         fb.load_last(tb, (const char *)pb, (const char *)pu, tid, p.K - k);
     };
 
-    f32x16 acc[NB][MB];
+    Sum acc[N][M];
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int j = 0; j < MB; ++j)
-            acc[i][j] = f32x16{};
-    // operands of two runs of 16 k
-    Operand<T> x0[MB], y0[NB], x1[MB], y1[NB];
-    const auto read = [&](const u32x4 *ta, const u32x4 *tb, int c, Operand<T>(&x)[MB],
-                          Operand<T>(&y)[NB]) {
+        for (int j = 0; j < M; ++j)
+            acc[i][j] = Sum{};
+    // operands of two runs of k
+    Operand<T> x0[M], y0[N], x1[M], y1[N];
+    const auto read = [&](const u32x4 *ta, const u32x4 *tb, int c, Operand<T>(&x)[M],
+                          Operand<T>(&y)[N]) {
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
-            y[i].set(FB::operand(tb, at_b, NB * wn + i, c));
+        for (int i = 0; i < N; ++i)
+            y[i].set(FB::operand(tb, at_b, N * wn + i, c));
 #pragma unroll
-        for (int j = 0; j < MB; ++j)
-            x[j].set(FA::operand(ta, at_a, MB * wm + j, c));
+        for (int j = 0; j < M; ++j)
+            x[j].set(FA::operand(ta, at_a, M * wm + j, c));
     };
-    // One tile: while a run of 16 k is multiplied the next one is read, in the first the last of the
+    // One tile: while a run of k is multiplied the next one is read, in the first the last of the
     // tile before, so that the matrix cores wait neither for LDS nor for the barrier between
-    // tiles.  The next tile is sent for between the products of the first two runs: sent for at
-    // once, its loads would hold up every wave (16 cycles each, of all waves).
-    constexpr int RUNS = BK / 16;
+    // tiles.
+    static_assert(BK == 2 * Core<T>::K);
     const auto tile = [&](const u32x4 *ta, const u32x4 *tb) {
+        asm("" : "+v"(at_a), "+v"(at_b)); // addresses a constant apart are not all held
         read(ta, tb, 0, x0, y0);
         multiply<T>(y1, x1, acc);
         read(ta, tb, 1, x1, y1);
         multiply<T>(y0, x0, acc);
-        if constexpr (RUNS == 4) {
-            read(ta, tb, 2, x0, y0);
-            multiply<T>(y1, x1, acc);
-            read(ta, tb, 3, x1, y1);
-            multiply<T>(y0, x0, acc);
-        }
 #pragma unroll
-        for (int j = 0; j < MB; ++j)
+        for (int j = 0; j < M; ++j)
             x1[j].made_here();
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
+        for (int i = 0; i < N; ++i)
             y1[i].made_here();
     };
     // tile s; its place's neighbour, which is free, takes the last one that is on its way.  Each
@@ -590,17 +606,17 @@ product(const Args p) {
         fetch(s + TILES - 1, next_a, next_b);
         tile(ta, tb);
         if constexpr (sizeof(T) == 2)
-            Order<RUNS, NB * MB, NB * FB::READS + MB * FA::READS, FA::N + FB::N>::runs();
+            Order<2, N * M, N * FB::READS + M * FA::READS, FA::N + FB::N>::runs();
         else
-            OrderParts<RUNS, NB * MB * 6, 2 * (NB + MB), FA::N + FB::N>::runs();
+            OrderParts<2, N * M * 6, 2 * (N + M), FA::N + FB::N>::runs();
         fetch_rest(s + TILES - 1, next_a, next_b);
         meet<(TILES - 2) * LOADS>();
     };
 #pragma unroll
-    for (int j = 0; j < MB; ++j)
+    for (int j = 0; j < M; ++j)
         x1[j] = {};
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+    for (int i = 0; i < N; ++i)
         y1[i] = {};
     if (!JOIN && s0 < s1) {
         const auto first = [&](int s, u32x4 *ta, u32x4 *tb) {
@@ -631,6 +647,8 @@ product(const Args p) {
     }
     if constexpr (!JOIN)
         multiply<T>(y1, x1, acc);
+    // 32 rows are PARTS32 sums of each column, fours of results all told
+    constexpr int PER_SUM = Core<T>::SIDE * Core<T>::SIDE / 256, QUADS = PARTS32 * PER_SUM;
     // where a split tile's sums lie, 16 bytes of each thread in turn
     constexpr int SUMS = 16 * NB * MB * NT * 4; // bytes of a tile's
     const int tails =
@@ -639,19 +657,19 @@ product(const Args p) {
     char *sums = (char *)p.part + ((int64_t)split * tails + tail) * SUMS;
     const int first = JOIN ? (int)blockIdx.x % MB : 0, last = JOIN ? first + 1 : MB;
     if constexpr (JOIN) {
-        sums += first * (4 * NB * 16 * NT);
+        sums += first * (N * QUADS * 16 * NT);
 #pragma unroll 4
         for (int n = 0; n < p.splits; ++n) {
             const char *from = sums + (int64_t)n * tails * SUMS;
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
+            for (int i = 0; i < N; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
+                for (int q = 0; q < QUADS; ++q) {
                     const f32x4 x = *(const f32x4 *)(from + mine);
                     from += 16 * NT;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        acc[i][0][4 * q + e] += x[e];
+                        acc[i][q / PER_SUM][4 * (q % PER_SUM) + e] += x[e];
                 }
         }
     }
@@ -688,23 +706,28 @@ product(const Args p) {
     for (int j = first; j < last; ++j) {
         attn::wave_fence();
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f32x4 x = {acc[i][0][4 * q], acc[i][0][4 * q + 1], acc[i][0][4 * q + 2],
-                                 acc[i][0][4 * q + 3]};
+            for (int q = 0; q < QUADS; ++q) {
+                const Sum &c = acc[i][q / PER_SUM];
+                constexpr int S = Core<T>::SIDE;
+                const int e = 4 * (q % PER_SUM);
+                const f32x4 x = {c[e], c[e + 1], c[e + 2], c[e + 3]};
                 if (leave) {
                     *(f32x4 *)(sums + mine) = x;
                     sums += 16 * NT;
                     continue;
                 }
-                turn[(lane & 31) * ROW + ((8 * i + 2 * q + half) ^ (lane & 15))] = x;
+                // its row, and its four columns
+                const int r = S * (q / PER_SUM) + lane % S;
+                const int unit = S / 4 * i + (S == 16 ? lane >> 4 : 2 * q + half);
+                turn[r * ROW + (unit ^ (r & 15))] = x;
             }
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int k = 0; k + 1 < MB; ++k)
-                acc[i][k] = acc[i][k + 1];
+            for (int k = 0; k + PARTS32 < M; ++k)
+                acc[i][k] = acc[i][k + PARTS32];
         if (leave)
             continue;
         attn::wave_fence();
