@@ -37,10 +37,21 @@ struct Plan {
     int whole, splits, split_steps;
     size_t part; // bytes of partial sums
 };
-// Chosen by the time it takes, in us, as measured on long rows: a step of 128 bytes of k of all the
-// blocks that run at once (16-bit types: 256 large tiles 1.64, 512 small ones 0.91, 256 small ones with four
-// tiles in LDS 0.75; float32 512 small ones 2.85, 256 1.8); 3 for each round's beginning and end;
-// the split tiles' sums are written and read at 3 TB/s, by one launch more, 6.
+// A step of 128 bytes of k of all the blocks that run at once, in us, as measured on 128 to 256 steps with
+// part of the card's places taken: a compute unit that has its block alone is at its own pace, many share
+// the card's clock and its memory.  16-bit types: 128 large tiles 1.20, 176 1.34, 224 1.50, 256
+// 1.57 to 1.73; 256 small ones 0.67, 384 0.80, 512 0.88 to 0.94; 256 small ones with four tiles in
+// LDS 0.52 to 0.57.  float32: 256 small ones 1.8, 512 2.85.
+double step_time(int dtype, int size, int64_t blocks) {
+    const double part = (double)blocks / (size == ff::kSmall ? 512 : 256);
+    if (dtype == TM_F32)
+        return size == ff::kDeep ? 1.8 : std::max(1.8, 0.75 + 2.1 * part);
+    return size == ff::kLarge  ? std::max(1.19, 0.7 + 0.95 * part)
+           : size == ff::kDeep ? 0.49 + 0.07 * part
+                               : std::max(0.67, 0.45 + 0.47 * part);
+}
+// Chosen by these times; 3 for each round's beginning and end; the split tiles' sums are written and
+// read at 3 TB/s, by one launch more, 6.
 Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, int segments,
           int batches) {
     if (M <= ff::kTokens && (kind == ff::kUp || kind == ff::kDown))
@@ -54,10 +65,6 @@ Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, 
         const int64_t t = size == ff::kLarge ? 256 : 128, tn = kind == ff::kUp ? t / 2 : t;
         const int64_t tiles = (M + t - 1) / t * ((N + tn - 1) / tn) * batches;
         const int64_t at_once = size == ff::kSmall ? 512 : 256;
-        const double step = f.dtype == TM_F32 ? (size == ff::kDeep ? 1.8 : 2.85)
-                            : size == ff::kLarge ? 1.64
-                            : size == ff::kDeep  ? 0.75
-                                                 : 0.91;
         const int64_t rounds = tiles / at_once, rest = tiles - rounds * at_once;
         if (size == ff::kDeep && tiles > at_once) // without a second block ends are not hidden either
             continue;
@@ -66,7 +73,8 @@ Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, 
                 break;
             const int64_t split_steps = (steps + splits - 1) / splits;
             const double bytes = splits > 1 ? (double)rest * splits * t * t * 4 : 0.;
-            const double time = step * (rounds * steps + (rest ? split_steps : 0)) +
+            const double time = step_time(f.dtype, size, at_once) * rounds * steps +
+                                step_time(f.dtype, size, rest * splits) * split_steps * (rest > 0) +
                                 3. * (rounds + (rest > 0)) +
                                 (splits > 1 ? 6. + 2. * bytes / 3e6 : 0.);
             if (best.splits == 0 || time < least) {
