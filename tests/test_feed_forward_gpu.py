@@ -81,6 +81,22 @@ def test_split_tiles(device, dtype, rows, c, f, o):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,c,f,o", [(2051, 1032, 140, 1032), (2060, 530, 4200, 260),
+                                        (5000, 264, 130, 1100), (2300, 1160, 2060, 264)])
+def test_tiles_of_more_rows(device, dtype, rows, c, f, o):
+    """More rows than go in small groups: each kind of tile, split and not, in either direction."""
+    _check(*_inputs(dtype, rows, c, f, o, 19, device))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c,f,o", [(136, 250, 72), (256, 683, 256), (1000, 520, 1030)])
+@pytest.mark.parametrize("rows", [66, 113, 515, 1030, 2048])
+def test_groups_of_rows(device, dtype, rows, c, f, o):
+    """Groups of 16 and 32 rows, the last one with a part of its own."""
+    _check(*_inputs(dtype, rows, c, f, o, 20, device))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_few_weights_of_many_rows(device, dtype):
     """The weights' gradients are split over the rows."""
     _check(*_inputs(dtype, (3, 3001), 64, 100, 40, 5, device))

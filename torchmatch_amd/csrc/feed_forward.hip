@@ -41,11 +41,12 @@ struct Plan {
 // part of the card's places taken: a compute unit that has its block alone is at its own pace, many share
 // the card's clock and its memory.  16-bit types: 128 large tiles 1.20, 176 1.34, 224 1.50, 256
 // 1.57 to 1.73; 256 small ones 0.67, 384 0.80, 512 0.88 to 0.94; 256 small ones with four tiles in
-// LDS 0.52 to 0.57.  float32: 256 small ones 1.8, 512 2.85.
+// LDS 0.52 to 0.57.  float32: 128 small ones 1.6, 256 1.77, 384 2.46, 512 2.73 to 2.96; 128 with four
+// 1.6, 256 1.7.
 double step_time(int dtype, int size, int64_t blocks) {
     const double part = (double)blocks / (size == ff::kSmall ? 512 : 256);
     if (dtype == TM_F32)
-        return size == ff::kDeep ? 1.8 : std::max(1.8, 0.75 + 2.1 * part);
+        return size == ff::kDeep ? 1.58 + 0.1 * part : std::max(1.65, 0.9 + 1.9 * part);
     return size == ff::kLarge  ? std::max(1.19, 0.7 + 0.95 * part)
            : size == ff::kDeep ? 0.49 + 0.07 * part
                                : std::max(0.67, 0.45 + 0.47 * part);
@@ -54,8 +55,6 @@ double step_time(int dtype, int size, int64_t blocks) {
 // read at 3 TB/s, by one launch more, 6.
 Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, int segments,
           int batches) {
-    if (M <= ff::kTokens && (kind == ff::kUp || kind == ff::kDown))
-        return {ff::kSmall, true, 0, 1, 0, 0};
     const int64_t k = 128 / size_of(f), steps = (K + k - 1) / k * segments;
     Plan best = {};
     double least = 0.;
@@ -83,6 +82,18 @@ Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, 
                         (int)split_steps, (size_t)bytes};
             }
         }
+    }
+    // product_tokens: 4 for its beginning and end, and on each compute unit its blocks' steps of 4 x 128
+    // bytes of k: up 0.45 with 32 rows a block (float32, at the rate of its own instructions, 0.65),
+    // down 0.35 (0.47), two thirds of that with 16
+    if (M <= ff::kTokens && (kind == ff::kUp || kind == ff::kDown)) {
+        const int rows = ff::tokens_rows(M, N);
+        const double blocks = (double)((M + rows - 1) / rows * ((N + 15) / 16)) / 256.;
+        const double step = (kind == ff::kUp ? (f.dtype == TM_F32 ? 0.65 : 0.45)
+                                             : (f.dtype == TM_F32 ? 0.47 : 0.35)) *
+                            (rows == 16 ? 0.67 : 1.);
+        if (4. + std::max(blocks, 1.) * ((steps + 3) / 4) * step < least)
+            return {ff::kSmall, true, 0, 1, 0, 0};
     }
     return best;
 }

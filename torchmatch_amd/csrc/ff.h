@@ -31,8 +31,13 @@ constexpr int kMostParts = 256;
 enum Kind { kUp, kDown, kHidden, kInput, kWeights };
 enum { kSmall, kDeep, kLarge }; // tiles: 128 x 128, with four in LDS in place of two, 256 x 256
 
-// Products of up to this many rows take product_tokens.
-constexpr int kTokens = 64;
+// Products of more rows than this do not take product_tokens.
+constexpr int kTokens = 2048;
+// Its rows a block: 16 while 32 would give no more than two blocks a compute unit (64 float32 rows of
+// 1024 through 2816: 22 us with 16, 28 with 32; 512 rows 116 and 106).
+inline int tokens_rows(int64_t M, int64_t N) {
+    return M <= 16 || (M + 31) / 32 * ((N + 15) / 16) <= 512 ? 16 : 32;
+}
 
 // Non-zero: a launch failed.
 #define FF_DECLARE(type)                                                                         \

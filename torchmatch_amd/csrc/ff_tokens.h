@@ -1,8 +1,8 @@
-// ff_tokens.h -- the feed-forward block's forward products of few rows, where reading the weights
-// once bounds them.
+// ff_tokens.h -- the feed-forward block's forward products where there are few rows, or so little all
+// told that tiles would leave the card idle: reading the weights bounds them, or a few steps' latency.
 //
-// A block has 16 rows of the weights (of gate and of up), its waves a part of k each, so that a product
-// of few rows of weights still fills the card; their sums meet in LDS, in order.  A wave brings whole
+// A block has 16 rows of the weights (of gate and of up) and 16 or 32 of x, its waves a part of k each, so
+// that a small product still fills the card; their sums meet in LDS, in order.  A wave brings whole
 // lines of 16 rows and of x into its own part of LDS, two or three pieces ahead of its 16 x 16
 // products, and meets the others at the end only.  (Operands straight from memory, 64 bytes of
 // each row a load: 26 and 77 us for the two timed calls of few tokens.)  The contraction
@@ -80,12 +80,12 @@ __global__ __launch_bounds__(64 * WAVES) void product_tokens(const Args p) {
         s2[SLOTS > 2 ? WAVES : 1][SLOTS > 2 ? PER * 128 : 1];
     const int lane = threadIdx.x & 63, quarter = lane >> 4, col = lane & 15;
     const int wave = attn::scalar(threadIdx.x >> 6);
-    const int n0 = blockIdx.x * 16;
+    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * GROUPS, rows = p.M - m0;
     Rows16 w, x[GROUPS];
     w.start(lane, p.b_l * (int)sizeof(T), p.N - n0);
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
-        x[g].start(lane, p.a_l * (int)sizeof(T), max(p.M - 16 * g, 1));
+        x[g].start(lane, p.a_l * (int)sizeof(T), max(rows - 16 * g, 1));
     const int units = (p.K + E - 1) / E, pieces = (units + 7) / 8;
     const int c0 = wave * p.split_steps, c1 = min(pieces, c0 + p.split_steps);
 
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(64 * WAVES) void product_tokens(const Args p) {
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g)
             x[g].load(t + 128 * (MATRICES + g), (const char *)((const T *)p.a[0] +
-                      (int64_t)min(16 * g, p.M - 1) * p.a_l), c, units);
+                      (int64_t)(m0 + min(16 * g, rows - 1)) * p.a_l), c, units);
     };
     f32x4 acc[MATRICES][GROUPS];
 #pragma unroll
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(64 * WAVES) void product_tokens(const Args p) {
     __syncthreads();
     // a wave each group: token 16 g + col, weights' rows n .. n + 3
     for (int g = wave; g < GROUPS; g += WAVES) {
-        const int m = 16 * g + col, n = n0 + 4 * quarter;
+        const int m = m0 + 16 * g + col, n = n0 + 4 * quarter;
         f32x4 s[MATRICES];
 #pragma unroll
         for (int i = 0; i < MATRICES; ++i) {
@@ -185,25 +185,23 @@ __global__ __launch_bounds__(64 * WAVES) void product_tokens(const Args p) {
 
 template <typename T, bool GATED, int GROUPS> void launch_waves(Args p, hipStream_t stream) {
     const unsigned blocks = (unsigned)(((GATED ? p.out_l : (int64_t)p.N) + 15) / 16);
+    const unsigned groups = (unsigned)((p.M + 16 * GROUPS - 1) / (16 * GROUPS));
     const int pieces = (int)(((int64_t)p.K * (int)sizeof(T) + 127) / 128);
-    // few blocks: more waves each, so that enough is on its way (LDS has room for that up to 32 rows)
-    if constexpr (GROUPS <= 2)
-        if (blocks <= 256 && pieces > 4) {
-            p.split_steps = (pieces + 7) / 8;
-            product_tokens<T, GATED, GROUPS, 8><<<dim3(blocks), 512, 0, stream>>>(p);
-            return;
-        }
+    // few blocks: more waves each, so that enough is on its way (LDS has room for that once)
+    if (blocks * groups <= 256 && pieces > 4) {
+        p.split_steps = (pieces + 7) / 8;
+        product_tokens<T, GATED, GROUPS, 8><<<dim3(blocks, groups), 512, 0, stream>>>(p);
+        return;
+    }
     p.split_steps = (pieces + 3) / 4;
-    product_tokens<T, GATED, GROUPS, 4><<<dim3(blocks), 256, 0, stream>>>(p);
+    product_tokens<T, GATED, GROUPS, 4><<<dim3(blocks, groups), 256, 0, stream>>>(p);
 }
 
 template <typename T, bool GATED> int launch_tokens(const Args &p, hipStream_t stream) {
-    if (p.M <= 16)
+    if (tokens_rows(p.M, p.N) == 16)
         launch_waves<T, GATED, 1>(p, stream);
-    else if (p.M <= 32)
-        launch_waves<T, GATED, 2>(p, stream);
     else
-        launch_waves<T, GATED, 4>(p, stream);
+        launch_waves<T, GATED, 2>(p, stream);
     return hipGetLastError() != hipSuccess;
 }
 
