@@ -76,6 +76,11 @@ __device__ inline void activate_all(int kind, F f) {
 
 template <typename T> constexpr int kStep = 128 / (int)sizeof(T); // k a tile: whole lines of memory
 
+// What units of 16 rows of 128 bytes are permuted by, for reads of row lane % 16, unit lane / 16
+__device__ inline int swz16(int row) {
+    return (row >> 1 & 1) << 2 | ((row >> 2 ^ row >> 3) & 1) << 1 | (row >> 3 & 1);
+}
+
 // One operand's tile, ROWS x kStep, brought by NT threads.  STRIDED: a row for each k.  HALF: HALF rows of one
 // matrix, HALF of another, in turn (0: one matrix).
 template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
@@ -89,13 +94,19 @@ template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
 
     uint32_t off[N]; // bytes from the tile's first element, its k aside
 
+    // A row's units are permuted by it.  Rows of 128 bytes: lanes 0-3, 12-15, 20-23, 24-27 of a read take
+    // their 256 bytes at once, so fours of rows at one unit and at its neighbour are to differ.
+    __device__ static inline int swz(int row) {
+        return sizeof(T) == 2 && !STRIDED ? swz16(row) : L::swz(row);
+    }
+
     // left: rows (columns) from the tile's first on
     __device__ inline void start(int tid, int64_t stride, int left) {
         const int row = tid / L::U, pos = tid % L::U;
         const uint32_t bytes = (uint32_t)stride * (uint32_t)sizeof(T);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int r = row + n * STEP, u = pos ^ L::swz(r);
+            const int r = row + n * STEP, u = pos ^ swz(r);
             if constexpr (STRIDED) {
                 off[n] = (uint32_t)r * bytes + 16u * min(u, (left - 1) / E);
             } else {
@@ -130,7 +141,7 @@ template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
         for (int n = 0; n < N; ++n) {
             const char *s = of_second(tid, n) ? second : from;
             const int r = tid / L::U + n * STEP;
-            const bool real = STRIDED ? r < left : (tid % L::U ^ L::swz(r)) * E < left;
+            const bool real = STRIDED ? r < left : (tid % L::U ^ swz(r)) * E < left;
             u32x4 x = {0u, 0u, 0u, 0u};
             if (real)
                 x = *(const u32x4 *)(s + off[n]);
@@ -142,7 +153,7 @@ template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
     // and a constant number of rows.
     __device__ static inline uint32_t lane_at(int lane) {
         if constexpr (sizeof(T) == 2 && !STRIDED) {
-            return 16u * L::at(lane & 15, lane >> 4);
+            return 16u * ((lane & 15) * L::U + ((lane >> 4) ^ swz(lane & 15)));
         } else if constexpr (sizeof(T) == 2) {
             const int d = 4 * (lane & 3);
             return 16u * L::at(8 * (lane >> 4) + ((lane & 15) >> 2), d >> 3) + 2u * (d & 7);

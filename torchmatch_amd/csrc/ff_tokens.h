@@ -45,12 +45,11 @@ template <> struct Unit16<float> {
 struct Rows16 {
     uint32_t off[2]; // bytes from the first row
     int unit[2];
-    __device__ static inline int swz(int row) { return (row >> 1 & 1) << 2 | (row >> 2 & 3); }
     __device__ inline void start(int lane, int64_t row_bytes, int rows) {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const int row = (lane >> 3) + 8 * n;
-            unit[n] = (lane & 7) ^ swz(row);
+            unit[n] = (lane & 7) ^ swz16(row);
             off[n] = (uint32_t)min(row, rows - 1) * (uint32_t)row_bytes;
         }
     }
@@ -66,7 +65,7 @@ struct Rows16 {
     // row lane % 16, unit 4 half + lane / 16
     __device__ static inline u32x4 operand(const u32x4 *t, int lane, int half) {
         const int row = lane & 15;
-        return t[8 * row + ((4 * half + (lane >> 4)) ^ swz(row))];
+        return t[8 * row + ((4 * half + (lane >> 4)) ^ swz16(row))];
     }
 };
 
