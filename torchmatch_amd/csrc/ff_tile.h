@@ -6,10 +6,16 @@
 //     dG = da^T x, dU = db^T x, dD = dy^T h                                (columns by columns)
 //
 // A block has BM x BN of the result.  Tiles of 128 bytes of k go from memory
-// straight into LDS, two buffers, one barrier a tile.  Operands whose rows hold k are read by rows, others
+// straight into LDS, two buffers, one barrier a tile.  (Loads of whole lines run at 133 bytes/ns a compute
+// unit, of half lines, tiles of 64 bytes of k, at 38.)  Operands whose rows hold k are read by rows, others
 // by transposed reads (attn_tile.h has the tiles' layout), so nothing is transposed in memory.  The
 // result's columns lie along a lane's registers; a wave turns them through LDS, 32 rows at a
 // time, and writes whole rows of its tile.
+//
+// Bound by power in long products: 8192 x 2048 x 5632 bfloat16, y 145 us (1.3 PFLOP/s), dG and dU
+// 353 (1.07), where the matrix cores alone reach 2.0 to 2.1; h with what is saved 405 and dh with da and
+// db 250, of which writing 369 and 461 MB is 95 and 100, behind which one block a compute unit hides
+// nothing.  float32 by the vector work of taking numbers apart: 190 TFLOP/s.
 #ifndef TORCHMATCH_AMD_FF_TILE_H
 #define TORCHMATCH_AMD_FF_TILE_H
 

@@ -10,6 +10,9 @@
 // the norm's sum is a few exchanges between neighbouring lanes and nothing is read twice.  The
 // cosines, sines and weights of a block's tokens lie in LDS, shared by the heads.
 //
+// 27306 tokens, 32 heads of 128, bfloat16: 109 us, 4.1 TB/s.  16396 tokens, 20 heads of 128: forward 33,
+// backward 59 (4.3 TB/s) and 4 for the blocks' sums.
+//
 // dw: a block has one row of the weight, so a lane adds what belongs to its own features in
 // registers over all of the block's tokens and heads; a block's lanes are joined in LDS and the
 // blocks by a second kernel, each in a fixed order (no atomics: the same call, the same bits).
