@@ -97,6 +97,14 @@ def test_groups_of_rows(device, dtype, rows, c, f, o):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,c,f,o", [(2049, 72, 137, 140), (3001, 40, 64, 65), (2500, 250, 33, 31),
+                                        (200, 300, 700, 257), (1025, 65, 1030, 90)])
+def test_small_tiles(device, dtype, rows, c, f, o):
+    """Products that would give larger tiles too few blocks."""
+    _check(*_inputs(dtype, rows, c, f, o, 21, device))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_few_weights_of_many_rows(device, dtype):
     """The weights' gradients are split over the rows."""
     _check(*_inputs(dtype, (3, 3001), 64, 100, 40, 5, device))

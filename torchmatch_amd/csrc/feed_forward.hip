@@ -42,28 +42,40 @@ struct Plan {
 // the card's clock and its memory.  16-bit types: 128 large tiles 1.20, 176 1.34, 224 1.50, 256
 // 1.57 to 1.73; 256 small ones 0.67, 384 0.80, 512 0.88 to 0.94; 256 small ones with four tiles in
 // LDS 0.52 to 0.57.  float32: 128 small ones 1.6, 256 1.77, 384 2.46, 512 2.73 to 2.96; 128 with four
-// 1.6, 256 1.7.
+// 1.6, 256 1.7.  64 x 64: up to 176 tiles 0.29 to 0.34, 352 0.46; float32 0.77 and 1.1.
 double step_time(int dtype, int size, int64_t blocks) {
-    const double part = (double)blocks / (size == ff::kSmall ? 512 : 256);
+    const double part = (double)blocks / (size == ff::kSmall || size == ff::kTiny ? 512 : 256);
+    if (size == ff::kTiny)
+        return dtype == TM_F32 ? std::max(0.76, 0.3 + 1.15 * part)
+                               : std::max(0.3, 0.13 + 0.45 * part);
     if (dtype == TM_F32)
         return size == ff::kDeep ? 1.58 + 0.1 * part : std::max(1.65, 0.9 + 1.9 * part);
     return size == ff::kLarge  ? std::max(1.19, 0.7 + 0.95 * part)
            : size == ff::kDeep ? 0.49 + 0.07 * part
                                : std::max(0.67, 0.45 + 0.47 * part);
 }
-// Chosen by these times; 3 for each round's beginning and end; the split tiles' sums are written and
-// read at 3 TB/s, by one launch more, 6.
+// A round's beginning and end, us: what up and hidden read and write after their products is
+// not hidden, 5 with 64 x 64, 9 and 14 with 128 x 128, 16 and 24 with 256 x 256.
+double end_time(Kind kind, int size) {
+    if (kind != ff::kUp && kind != ff::kHidden)
+        return 3.;
+    return size == ff::kTiny     ? 5.
+           : size != ff::kLarge ? (kind == ff::kUp ? 9. : 14.)
+                                : (kind == ff::kUp ? 16. : 24.);
+}
+// Chosen by these times; the split tiles' sums are written and read at 3 TB/s, by one launch more, 6.
 Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, int segments,
           int batches) {
     const int64_t k = 128 / size_of(f), steps = (K + k - 1) / k * segments;
     Plan best = {};
     double least = 0.;
-    for (int size : {ff::kSmall, ff::kDeep, ff::kLarge}) {
+    for (int size : {ff::kSmall, ff::kDeep, ff::kTiny, ff::kLarge}) {
         if (size == ff::kLarge && f.dtype == TM_F32)
             continue;
-        const int64_t t = size == ff::kLarge ? 256 : 128, tn = kind == ff::kUp ? t / 2 : t;
+        const int64_t t = size == ff::kLarge ? 256 : size == ff::kTiny ? 64 : 128;
+        const int64_t tn = kind == ff::kUp ? t / 2 : t;
         const int64_t tiles = (M + t - 1) / t * ((N + tn - 1) / tn) * batches;
-        const int64_t at_once = size == ff::kSmall ? 512 : 256;
+        const int64_t at_once = size == ff::kSmall || size == ff::kTiny ? 512 : 256;
         const int64_t rounds = tiles / at_once, rest = tiles - rounds * at_once;
         if (size == ff::kDeep && tiles > at_once) // without a second block ends are not hidden either
             continue;
@@ -74,7 +86,7 @@ Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, 
             const double bytes = splits > 1 ? (double)rest * splits * t * t * 4 : 0.;
             const double time = step_time(f.dtype, size, at_once) * rounds * steps +
                                 step_time(f.dtype, size, rest * splits) * split_steps * (rest > 0) +
-                                3. * (rounds + (rest > 0)) +
+                                end_time(kind, size) * (rounds + (rest > 0)) +
                                 (splits > 1 ? 6. + 2. * bytes / 3e6 : 0.);
             if (best.splits == 0 || time < least) {
                 least = time;
@@ -84,15 +96,15 @@ Plan plan(const tm_feed_forward &f, Kind kind, int64_t M, int64_t N, int64_t K, 
         }
     }
     // product_tokens: 4 for its beginning and end, and on each compute unit its blocks' steps of 4 x 128
-    // bytes of k: up 0.45 with 32 rows a block (float32, at the rate of its own instructions, 0.65),
-    // down 0.35 (0.47), two thirds of that with 16
+    // bytes of k and one and a half each: up 0.40 with 32 rows a block (float32, at the rate of its own
+    // instructions, 0.56), down 0.30 (0.40), 0.62 of that with 16
     if (M <= ff::kTokens && (kind == ff::kUp || kind == ff::kDown)) {
         const int rows = ff::tokens_rows(M, N);
         const double blocks = (double)((M + rows - 1) / rows * ((N + 15) / 16)) / 256.;
-        const double step = (kind == ff::kUp ? (f.dtype == TM_F32 ? 0.65 : 0.45)
-                                             : (f.dtype == TM_F32 ? 0.47 : 0.35)) *
-                            (rows == 16 ? 0.67 : 1.);
-        if (4. + std::max(blocks, 1.) * ((steps + 3) / 4) * step < least)
+        const double step = (kind == ff::kUp ? (f.dtype == TM_F32 ? 0.56 : 0.40)
+                                             : (f.dtype == TM_F32 ? 0.40 : 0.30)) *
+                            (rows == 16 ? 0.62 : 1.);
+        if (4. + std::max(blocks, 1.) * ((steps + 3) / 4 + 1.5) * step < least)
             return {ff::kSmall, true, 0, 1, 0, 0};
     }
     return best;

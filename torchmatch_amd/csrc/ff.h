@@ -29,7 +29,8 @@ struct Args {
 
 constexpr int kMostParts = 256;
 enum Kind { kUp, kDown, kHidden, kInput, kWeights };
-enum { kSmall, kDeep, kLarge }; // tiles: 128 x 128, with four in LDS in place of two, 256 x 256
+// Tiles: 128 x 128, with four in LDS in place of two, 64 x 64 with four, 256 x 256
+enum { kSmall, kDeep, kTiny, kLarge };
 
 // Products of more rows than this do not take product_tokens.
 constexpr int kTokens = 2048;
