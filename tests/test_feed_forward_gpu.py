@@ -105,6 +105,15 @@ def test_small_tiles(device, dtype, rows, c, f, o):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,c,f,o", [(2204, 2745, 27, 98), (2619, 47, 2591, 19), (733, 47, 5258, 630),
+                                        (1821, 2255, 20, 67), (6264, 161, 16, 1725), (5270, 1484, 101, 309),
+                                        (517, 2477, 1657, 183), (5959, 2805, 705, 1945)])
+def test_long_and_narrow(device, dtype, rows, c, f, o):
+    """One size of three far from the others: tiles of each kind, split ones past whole rounds."""
+    _check(*_inputs(dtype, rows, c, f, o, 22, device))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_few_weights_of_many_rows(device, dtype):
     """The weights' gradients are split over the rows."""
     _check(*_inputs(dtype, (3, 3001), 64, 100, 40, 5, device))
