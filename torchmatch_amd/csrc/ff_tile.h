@@ -48,7 +48,8 @@ template <typename T, int KIND> __device__ inline float2 activate(float a) {
         const float s = over<T>(1.f + exp_of<T>(-a)), v = a * s;
         return make_float2(v, fmaf(v, 1.f - s, s));
     } else if constexpr (KIND == TM_RELU) {
-        return make_float2(fmaxf(a, 0.f), a > 0.f ? 1.f : 0.f);
+        // not a maximum, which loses NaN
+        return make_float2(a < 0.f ? 0.f : a, a > 0.f ? 1.f : 0.f);
     } else if constexpr (KIND == TM_GELU) {
         const float cdf = 0.5f * erfcf(-0.70710678118654752440f * a);
         return make_float2(a * cdf, cdf + a * 0.39894228040143267794f * exp_of<T>(-0.5f * a * a));
