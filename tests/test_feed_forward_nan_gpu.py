@@ -87,3 +87,30 @@ def test_a_float32_infinity_is_seen(device, activation):
     want = _formula(x[:5], gate, up, down, activation, dy[:5])[0]
     assert torch.equal(got.isnan(), want.isnan())
     assert torch.equal(got.isposinf(), want.isposinf())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+@pytest.mark.parametrize("rows", ROWS)
+def test_gates_far_from_zero(device, dtype, activation, rows):
+    """a = 2^70 and its like, whose square float32 does not hold, with b = 0: nothing is infinite.
+    dx is db U alone there (da = dh b act' = 0), db rounded once and dx once."""
+    x, gate, up, down, dy = _inputs(dtype, rows, 4, device)
+    up[:, 0] = 0
+    x[3] = 0
+    x[3, 0] = 2.0**70
+    dy[3] *= 2.0**-40
+    leaves = [v.detach().requires_grad_(True) for v in (x, gate, up, down)]
+    y = att.feed_forward(*leaves, activation=activation)
+    got = (y, *torch.autograd.grad(y, leaves, dy))
+    want = _formula(x, gate, up, down, activation, dy)
+    for name, a, b in zip(("y", "dx", "dgate", "dup", "ddown"), got, want):
+        assert b.isfinite().all() and a.isfinite().all(), name
+    assert not got[0][3].any()
+    # each term of a sum is off by u of itself, and sums of 64 and 80 terms by their float32 roundings
+    u = torch.finfo(dtype).eps / 2
+    dh = dy[3].double() @ down.double()
+    act = _activation(2.0**70 * gate[:, 0].double(), activation)[0]
+    terms = (dy[3].double().abs() @ down.double().abs()) * act.abs() @ up.double().abs()
+    limit = (2 * u + 160 * 2.0**-23) * terms + 2.0**-18 * (dh * act).abs() @ up.double().abs()
+    assert ((got[1][3].double() - want[1][3]).abs() <= limit).all()

@@ -57,8 +57,9 @@ template <typename T, int KIND> __device__ inline float2 activate(float a) {
         const float k = 0.79788456080286535588f;
         const float t = tanhf(k * (a + 0.044715f * a * a * a));
         const float half = 0.5f * (1.f + t);
+        // its square bounded: past it 1 - t^2 is zero, and infinity times that no number
         return make_float2(a * half, half + 0.5f * a * (1.f - t * t) * k *
-                                                (1.f + 3.f * 0.044715f * a * a));
+                                                (1.f + fminf(3.f * 0.044715f * a * a, 1e30f)));
     }
 }
 // f(j, the activation) for j < V, the choice outside the loop
