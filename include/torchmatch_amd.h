@@ -459,8 +459,9 @@ int tm_dropout(const void *x, const void *residual, void *out, int64_t count, in
  * x is (T, C), gate and up are (F, C), down is (O, F), of `dtype`, rows `_l` elements apart; addresses
  * and rows at multiples of 16 bytes, fewer than TM_FF_MAX_ROW_BYTES from row to row; where C (F for
  * down) elements do not fill whole units of 16 bytes, the last unit's rest is zeros.  Sums are float32; the
- * hidden features are rounded to `dtype` once, as are their gradients (float16 holds these
- * times a power of two that brings the largest |dout| to 1 .. 2). */
+ * hidden features are rounded to `dtype` once, as are their gradients.  float16 holds these times a
+ * power of two: what brings the largest finite |dout| to 1 .. 2, if that is up; the largest that keeps
+ * every finite one within its range, if that one does not. */
 enum { TM_SILU = 0, TM_GELU = 1, TM_GELU_TANH = 2, TM_RELU = 3 };
 enum { TM_FF_MAX_ROW_BYTES = 1 << 23, TM_FF_MAX_BLOCKS = 1 << 22 };
 typedef struct tm_feed_forward {

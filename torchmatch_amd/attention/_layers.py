@@ -67,9 +67,12 @@ def feed_forward(
 
     bfloat16, float16 or float32, all of one type.  Products are summed in float32; the hidden
     features are rounded to the type once, as are their gradients.  Half precision's hidden
-    features have its range (65504); their gradients are scaled by the output's, so that no loss
-    scaling is needed but for the results' own range.  Differentiable in all four, with the same
-    bits each time; only the gradients that are asked for are computed.  Reverse mode, once.
+    features have its range (65504).  Their gradients are held times one power of two a call: up
+    where the output's gradient is small, down where one of theirs would pass the range; none is
+    infinite and none loses bits that would not without it.  Those 2^15 times smaller than the
+    output's largest gradient may lose some.  Differentiable in all four, with the same bits each
+    time; only the gradients that are asked for are computed.
+    Reverse mode, once.
     """
     _on_device(x, "feed_forward", "x")
     return _FEED_FORWARD(x, gate, up, down, activation)

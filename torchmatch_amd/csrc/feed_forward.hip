@@ -23,6 +23,7 @@ using ff::Args;
 using ff::Kind;
 
 constexpr int64_t kMaxRows = INT32_MAX - 256;
+constexpr size_t kScaleBytes = ff::kMostParts * sizeof(float) + 256; // most and past, half precision
 
 int size_of(const tm_feed_forward &f) { return f.dtype == TM_F32 ? 4 : 2; }
 int64_t hidden_row(const tm_feed_forward &f) { return ((int64_t)f.F + 7) / 8 * 8; }
@@ -180,19 +181,24 @@ void set_saved(const tm_feed_forward &f, Args &p, const void *saved) {
         p.saved[n] = plane(f, saved, n);
 }
 
-// The largest |x| of what each block takes of (rows, n), half precision.
+// The largest finite |x| of what each block takes of (rows, n), half precision; *past is cleared for
+// the product that follows.
 __global__ __launch_bounds__(256) void ff_most(const _Float16 *x, int64_t l, int rows, int n,
-                                               float *most) {
+                                               float *most, uint32_t *past) {
     typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
     __shared__ float waves[4];
     const int units = (n + 7) / 8; // a row's last unit ends in zeros
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        *past = 0;
     float m = 0.f;
     for (int row = blockIdx.x; row < rows; row += ff::kMostParts)
         for (int u = threadIdx.x; u < units; u += 256) {
             const h16x8 v = *(const h16x8 *)(x + row * l + 8 * u);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                m = fmaxf(m, fabsf((float)v[j]));
+            for (int j = 0; j < 8; ++j) {
+                const float a = fabsf((float)v[j]);
+                m = a < __builtin_inff() ? fmaxf(m, a) : m;
+            }
         }
 #pragma unroll
     for (int k = 1; k < 64; k *= 2)
@@ -289,7 +295,7 @@ extern "C" int tm_feed_forward_forward(const tm_feed_forward *f, void *out, void
 extern "C" size_t tm_feed_forward_backward_workspace_bytes(const tm_feed_forward *f) {
     if (check(f))
         return 0;
-    return ff::kMostParts * sizeof(float) + 2 * hidden_bytes(*f) +
+    return kScaleBytes + 2 * hidden_bytes(*f) +
            std::max({plan_hidden(*f).part, plan_input(*f).part, plan_weights(*f).part,
                      plan_output(*f).part});
 }
@@ -312,7 +318,8 @@ extern "C" int tm_feed_forward_backward(const tm_feed_forward *f, const void *sa
         workspace_bytes < tm_feed_forward_backward_workspace_bytes(f))
         return TM_ERR_WORKSPACE;
     float *most = (float *)workspace;
-    char *da = (char *)workspace + ff::kMostParts * sizeof(float);
+    uint32_t *past = (uint32_t *)(most + ff::kMostParts);
+    char *da = (char *)workspace + kScaleBytes;
     char *db = da + hidden_bytes(*f), *part = db + hidden_bytes(*f);
     Args p;
     const bool scaled = f->dtype == TM_F16 && f->T;
@@ -322,7 +329,7 @@ extern "C" int tm_feed_forward_backward(const tm_feed_forward *f, const void *sa
     if (f->T && (dx || dgate)) { // down's gradient needs h alone, which is saved
         if (scaled) {
             ff_most<<<dim3(ff::kMostParts), 256, 0, stream>>>((const _Float16 *)dout, do_l, f->T,
-                                                             f->O, most);
+                                                             f->O, most, past);
             if (hipGetLastError() != hipSuccess)
                 return TM_ERR_LAUNCH;
         }
@@ -330,17 +337,25 @@ extern "C" int tm_feed_forward_backward(const tm_feed_forward *f, const void *sa
         p.a[0] = dout, p.a_l = do_l;
         p.b[0] = f->down, p.b_l = f->down_l;
         p.da = da, p.db = db, p.out_l = hidden_row(*f);
-        p.most = scaled ? most : nullptr;
         set_saved(*f, p, saved);
-        if (const int rc = product(*f, p, ff::kHidden, plan_hidden(*f), part, stream))
+        if (scaled)
+            p.most = most, p.past_out = past;
+        const Plan how = plan_hidden(*f);
+        if (const int rc = product(*f, p, ff::kHidden, how, part, stream))
             return rc;
+        if (scaled) { // again, if the scale turns out too large; else its blocks end at once
+            p.past = past;
+            if (const int rc = product(*f, p, ff::kHidden, how, part, stream))
+                return rc;
+        }
         if (dx) {
             p = args(f->T, f->C, f->F);
             p.segments = 2;
             p.a[0] = da, p.a[1] = db, p.a_l = hidden_row(*f);
             p.b[0] = f->gate, p.b[1] = f->up, p.b_l = f->w_l;
             p.out[0] = dx, p.out_l = f->C, p.wide = wide(*f, dx, f->C);
-            p.most = scaled ? most : nullptr;
+            if (scaled)
+                p.most = most, p.past = past;
             if (const int rc = product(*f, p, ff::kInput, plan_input(*f), part, stream))
                 return rc;
         }
@@ -352,7 +367,8 @@ extern "C" int tm_feed_forward_backward(const tm_feed_forward *f, const void *sa
         p.b[0] = p.b[1] = f->x, p.b_l = f->x_l;
         p.out[0] = dgate, p.out[1] = dup, p.out_l = f->C;
         p.wide = wide(*f, dgate, f->C) && wide(*f, dup, f->C);
-        p.most = scaled ? most : nullptr;
+        if (scaled)
+            p.most = most, p.past = past;
         if (const int rc = product(*f, p, ff::kWeights, plan_weights(*f), part, stream))
             return rc;
     }

@@ -19,7 +19,12 @@ struct Args {
     // eight bits of each
     void *saved[3];
     void *da, *db;      // hidden: gradients of a and b, rows of out_l
-    const float *most;  // kMostParts maxima of |dy|, or null: no scale
+    // half precision (null: no scale): kMostParts maxima of |dy|; the bits of the largest finite |da|
+    // or |db| that the scale they give brings past half precision's range, or zero: written
+    // (hidden, the first time) or read
+    const float *most;
+    uint32_t *past_out;
+    const uint32_t *past;
     float *part;        // sums of the tiles that are split
     int32_t M, N, K;    // K: of one segment
     int32_t segments, batches;

@@ -352,8 +352,11 @@ template <typename T> struct Saved { // 8 of them, as they lie in memory
     }
 };
 
-// The power of two that brings the largest |dy| to 1 .. 2: half precision holds gradients of the
-// hidden features times this (they are as small as the loss makes them, and lose bits below 2^-14).
+// The power of two that half precision holds gradients of the hidden features times (they are as
+// small as the loss makes them, and lose bits below 2^-14): what brings the largest |dy| to 1 .. 2, if
+// that is up; where it brings a gradient past the range, the largest that does not.  So none is
+// infinite and none loses bits that would not without it.
+constexpr float kMostHalf = 65504.f;
 template <typename T> __device__ inline int grad_up(const Args &p, int lane) {
     if constexpr (__is_same(T, _Float16)) {
         if (!p.most)
@@ -364,7 +367,14 @@ template <typename T> __device__ inline int grad_up(const Args &p, int lane) {
 #pragma unroll
         for (int n = 1; n < 64; n *= 2)
             m = fmaxf(m, __shfl_xor(m, n));
-        return m > 0.f && m < attn::kInf ? 1 - __builtin_amdgcn_frexp_expf(m) : 0;
+        int up = m > 0.f ? max(0, 1 - __builtin_amdgcn_frexp_expf(m)) : 0;
+        const uint32_t past = p.past ? *p.past : 0u;
+        if (past) {
+            const float most = __uint_as_float(past);
+            const int by = __builtin_amdgcn_frexp_expf(most) - 16; // to 2^15 .. 2^16
+            up -= __builtin_ldexpf(most, -by) > kMostHalf ? by + 1 : by;
+        }
+        return up;
     }
     return 0;
 }
@@ -401,10 +411,10 @@ __device__ inline void put_hidden(const Args &p, int64_t m, int n, fv<V> a, fv<V
 }
 
 // The gradients of a and b from that of h (half precision: times 2^up); what was saved past the
-// hidden features is zero, dh there anything.
+// hidden features is zero, dh there anything.  most: raised to the largest finite one.
 template <typename T>
 __device__ inline void put_grads(const Args &p, int64_t m, int n, f32x8 dh, const Saved<T> &kept,
-                                 int up) {
+                                 int up, float &most) {
     const int64_t at = m * p.out_l + n;
     f32x8 a, b, da, db;
     kept.give(a, b);
@@ -420,6 +430,14 @@ __device__ inline void put_grads(const Args &p, int64_t m, int n, f32x8 dh, cons
         for (int j = 0; j < 8; ++j)
             if (n + j >= p.N)
                 da[j] = db[j] = 0.f;
+    }
+    if constexpr (__is_same(T, _Float16)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float u = fabsf(da[j]), v = fabsf(db[j]);
+            most = u < attn::kInf ? fmaxf(most, u) : most;
+            most = v < attn::kInf ? fmaxf(most, v) : most;
+        }
     }
     put<T, 8>((T *)p.da + at, da);
     put<T, 8>((T *)p.db + at, db);
@@ -504,6 +522,10 @@ template <typename T, Kind KIND, int SIZE, bool JOIN>
 __global__ __launch_bounds__((JOIN ? 64 : 64 * Size<KIND, SIZE>::WM * Size<KIND, SIZE>::WN),
                              (SIZE == kDeep || JOIN ? 1 : 2)) void
 product(const Args p) {
+    constexpr bool HALF_GRADS = KIND == kHidden && __is_same(T, _Float16);
+    if constexpr (HALF_GRADS)
+        if (p.past && !*p.past) // a second time only where the first one's scale was too large
+            return;
     using Z = Size<KIND, SIZE>;
     constexpr int MB = Z::MB, NB = Z::NB, BM = 32 * MB * Z::WM, BN = 32 * NB * Z::WN;
     constexpr int PARTS32 = 32 / Core<T>::SIDE; // of the matrix cores' products in 32 rows
@@ -726,6 +748,7 @@ product(const Args p) {
                 kept[k].load(p, m * p.out_l + n);
         }
     }
+    float most = 0.f; // of a lane's da and db
     // one copy of what follows: the sums move up in the registers
 #pragma unroll 1
     for (int j = first; j < last; ++j) {
@@ -768,7 +791,7 @@ product(const Args p) {
                 if constexpr (GATED) {
                     put_hidden<T, 8>(p, m, n, read8(r, col), read8(r, col + HALF));
                 } else if constexpr (KIND == kHidden) {
-                    put_grads<T>(p, m, n, read8(r, col), kept[k], up);
+                    put_grads<T>(p, m, n, read8(r, col), kept[k], up, most);
                     if (j + 1 < last && m + 32 < p.M)
                         kept[k].load(p, (m + 32) * p.out_l + n);
                 } else {
@@ -777,6 +800,9 @@ product(const Args p) {
             }
         }
     }
+    if constexpr (HALF_GRADS)
+        if (most > kMostHalf && !p.past) // a maximum: in any order the same
+            atomicMax(p.past_out, __float_as_uint(most));
 }
 
 template <typename T, Kind KIND, int SIZE> int launch(const Args &p, hipStream_t stream) {
