@@ -9,12 +9,14 @@ from torchmatch_amd._loader import load as _load
 _load()
 
 attend = torch.ops.attention.attend
+attend_forward = torch.ops.attention.attend_forward
 attend_backward = torch.ops.attention.attend_backward
 rotate = torch.ops.attention.rotate
 norm_rotate = torch.ops.attention.norm_rotate
 norm_rotate_backward = torch.ops.attention.norm_rotate_backward
 dropout = torch.ops.attention.dropout
 feed_forward = torch.ops.attention.feed_forward
+feed_forward_save = torch.ops.attention.feed_forward_save
 feed_forward_backward = torch.ops.attention.feed_forward_backward
 
 
@@ -92,5 +94,6 @@ def _feed_forward_backward_fake(dout, x, gate, up, down, saved, activation,  # n
                  ((x, need_x), (gate, need_gate), (up, need_up), (down, need_down)))
 
 
-__all__ = ["attend", "attend_backward", "dropout", "feed_forward", "feed_forward_backward",
-           "norm_rotate", "norm_rotate_backward", "rotate"]
+__all__ = ["attend", "attend_backward", "attend_forward", "dropout", "feed_forward",
+           "feed_forward_backward", "feed_forward_save", "norm_rotate", "norm_rotate_backward",
+           "rotate"]
