@@ -12,10 +12,11 @@
 // result's columns lie along a lane's registers; a wave turns them through LDS, 32 rows at a
 // time, and writes whole rows of its tile.
 //
-// Bound by power in long products: 8192 x 2048 x 5632 bfloat16, y 145 us (1.3 PFLOP/s), dG and dU
-// 353 (1.07), where the matrix cores alone reach 2.0 to 2.1; h with what is saved 405 and dh with da and
-// db 250, of which writing 369 and 461 MB is 95 and 100, behind which one block a compute unit hides
-// nothing.  float32 by the vector work of taking numbers apart: 190 TFLOP/s.
+// Long products, 8192 x 2048 x 5632 bfloat16: y 145 us (1.3 PFLOP/s), dG and dU 353 (1.07), where
+// products without loads reach 2.0 to 2.1; waves wait for a third to a half of their time, and a
+// block alone on its compute unit has nothing beside a wait.  h with what is saved 405 and dh with da and
+// db 250, of which writing 369 and 461 MB is 95 and 100, not hidden either.  float32 is bound by the
+// vector work of taking numbers apart: 105 to 133 TFLOP/s of 32768 rows of 256 through 683.
 #ifndef TORCHMATCH_AMD_FF_TILE_H
 #define TORCHMATCH_AMD_FF_TILE_H
 
@@ -208,8 +209,8 @@ template <typename T, int ROWS, bool STRIDED, int NT, int HALF> struct Feed {
 
 // ---- products ---------------------------------------------------------------------
 
-// The matrix cores' products: SIDE x SIDE of the result over K indices.  Sides of 16 take less power
-// than of 32, which bounds long products: 2000 and 1880 TFLOP/s of products alone.
+// The matrix cores' products: SIDE x SIDE of the result over K indices.  Of products alone, sides of
+// 16 run at 2000 TFLOP/s and of 32 at 1880.
 template <typename T> struct Core {
     static constexpr int SIDE = sizeof(T) == 2 ? 16 : 32, K = sizeof(T) == 2 ? 32 : 16;
     using Sum = float __attribute__((ext_vector_type(SIDE * SIDE / 64)));
